@@ -148,6 +148,7 @@ def prepare(case, seed):
     if own:
         from more4d_amd import ops
         st["plan"] = ops.AdapterPlan(lengths, ids, "cuda")
+        st["scale_dev"] = torch.tensor(scale, device="cuda")
         if case["op"] == "serve":
             st["bank"] = ops.AdapterBank(a, b, scale)
     return st
@@ -230,7 +231,7 @@ def _run_own(st):
     if st["op"] == "serve":
         return ops.linear_adapters(st["x"], st["w"], st["bias"], st["bank"], st["plan"])
     if st["op"] == "train":
-        y = autograd.AdapterLinearFn.apply(st["x"], st["w"], st["bias"], st["a"], st["b"], st["scale"], st["plan"], st["bits"])
+        y = autograd.AdapterLinearFn.apply(st["x"], st["w"], st["bias"], st["a"], st["b"], st["scale_dev"], st["plan"], st["bits"])
         return (y.detach(),) + torch.autograd.grad(y, (st["x"], st["a"], st["b"]), st["dy"])
     kept = ops.act_quant8(st["x"])
     if st["op"] == "store":
