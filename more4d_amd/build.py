@@ -18,7 +18,10 @@ LIB = os.path.join(LIBDIR, "libmore4d_hip.so")
 OBJDIR = os.path.join(HERE, "build")
 
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I", CSRC, "-I", INC,
-         "-Wno-unused-result"]
+         "-Wno-unused-result",
+         # no packed float32 instructions (v_pk_add / mul / fma_f32): hipcc forms them from ordinary float code, and some of their operand
+         # forms have returned wrong values now and then on these machines (the host pass warns that it does not know the feature)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def source_hash():
