@@ -489,6 +489,52 @@ int m4d_groupnorm_cl_bwd(m4d_dtype dt, const void* x, const float* weight, const
                          float* dbias, float* ws, int64_t ws_floats, int F, int64_t HW, int C, int G, float eps, int silu,
                          m4d_stream stream);
 
+/* ------------------------------------------------------------------ activations kept in 8 bits for the backward pass
+ * The reference keeps what its backward needs as it is, or recomputes it (wan_transformer4d.py:1273-1291); this is the form between.  A row of
+ * C channels is nb = ceil(C / 32) blocks of 32 (the last may be shorter); codes int8 [rows, 32 * nb], exps uint8 [rows, nb], both
+ * contiguous.  A block stands for code * 2^(exps - 127), with 2^e the smallest power of two (e >= -126) that max|x| <= 127 * 2^e and
+ * code = round_half_even(x / 2^e); e stops at 121 (codes saturate at +-127), so every code stands for a finite number.  exps = 255: the block
+ * held an infinity or NaN and stands for NaN.  act: 0 none, 1 silu, 2 gelu(tanh), 3 gelu(erf).
+ *   act_quant8      x T [rows, C] -> codes, exps.
+ *   act_dequant8    out T [rows, C] = act(value).
+ *   act_dequant8_t  out T [C, rows_pad] = act(value)^T, columns rows .. rows_pad zero (the operand of a weight gradient).
+ *   act_bwd8        out T [rows, C] = dy * act'(value); out may be dy. */
+int m4d_act_quant8(m4d_dtype dt, const void* x, int64_t ldx, int8_t* codes, uint8_t* exps, int64_t rows, int C, m4d_stream stream);
+int m4d_act_dequant8(m4d_dtype dt, const int8_t* codes, const uint8_t* exps, void* out, int64_t ldo, int64_t rows, int C, int act,
+                     m4d_stream stream);
+int m4d_act_dequant8_t(m4d_dtype dt, const int8_t* codes, const uint8_t* exps, void* out, int64_t ldo, int64_t rows, int64_t rows_pad, int C,
+                       int act, m4d_stream stream);
+int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes, const uint8_t* exps, void* out, int64_t ldo, int64_t rows, int C,
+                 int act, m4d_stream stream);
+
+/* ------------------------------------------------------------------ low-rank adapters of many requests beside a shared projection
+ *   y = x W^T + bias + s_g (x A_g^T) B_g^T,   g the adapter that the row's request names (none: the shared projection alone)
+ * (the reference merges ONE adapter into the weights before it runs, utils/lora_utils.py:368, and trains one in its second stage,
+ * scripts/4D_ViSM_training/train.py:686).  Banks: A T [G, R, K], B T [G, N, R], scale float32 [G]; R = the rank padded with zeros to a multiple
+ * of 16.  The plan describes the rows of a batch, host-built (more4d_amd/ops.py: AdapterPlan), tables on the device:
+ *   row_adapter [rows]           adapter of each row, -1 = none
+ *   slot_row [64 * n_pieces]     rows sorted by adapter, each adapter's list padded with -1 to pieces of 64
+ *   piece_adapter [n_pieces]
+ *   chunks [n_chunks][3]         pieces [first, last) of one adapter: the unit of the row contraction; chunk_off [n_adapters + 1] into it
+ *   tilesT_off, tilesT           the adapters of the rows of each T-row tile, each once (T = 256: the last tile is rows [rows - 256, rows))
+ *   adapter_down     u T [rows, R] and / or ut T [R, 64 * n_pieces] = s_g x A_g^T (rows without an adapter are not written, pad slots are zero)
+ *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once
+ *   adapter_grad     out T [G, rank, C] (transposed: [G, C, rank]) = sum over the rows of g of v^T x, v given as vt T [R, 64 * n_pieces], x as T or as
+ *                    8-bit codes; ws from adapter_grad_workspace floats; partial sums are joined in a fixed order. */
+typedef struct {
+    const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks, *chunk_off, *tiles256_off, *tiles256, *tiles128_off, *tiles128;
+    int64_t rows;
+    int32_t n_pieces, n_chunks, n_adapters, reserved;
+} m4d_adapter_plan;
+int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a, const float* scale, const m4d_adapter_plan* plan, void* u, void* ut,
+                     int64_t K, int R, m4d_stream stream);
+int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* u, const void* b,
+                        const m4d_adapter_plan* plan, void* out, int64_t ldo, int64_t N, int64_t K, int R, m4d_stream stream);
+int64_t m4d_adapter_grad_workspace(const m4d_adapter_plan* plan, int64_t C, int R);
+int m4d_adapter_grad(m4d_dtype dt, const void* vt, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps,
+                     const m4d_adapter_plan* plan, float* ws, int64_t ws_floats, void* out, int transposed, int G, int rank, int64_t C, int R,
+                     m4d_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

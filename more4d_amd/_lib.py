@@ -31,6 +31,12 @@ class AttnBwdArgs(Structure):
                 [("scale", c_float), ("ws", c_void_p), ("ws_elems", c_int64)])
 
 
+class AdapterPlanArgs(Structure):      # m4d_adapter_plan
+    _fields_ = ([(n, c_void_p) for n in ("row_adapter", "slot_row", "piece_adapter", "chunks", "chunk_off", "tiles256_off", "tiles256",
+                                         "tiles128_off", "tiles128")] +
+                [("rows", c_int64), ("n_pieces", c_int32), ("n_chunks", c_int32), ("n_adapters", c_int32), ("reserved", c_int32)])
+
+
 # name -> (restype, argtypes); mirrors include/more4d_hip.h one to one
 SIGNATURES = {
     "m4d_version": (c_int, []),
@@ -139,6 +145,17 @@ SIGNATURES = {
                                 c_float, c_void_p, c_void_p, c_void_p]),
     "m4d_cl_to_ncthw": (c_int, [c_int, c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_int, c_float, c_float,
                                 c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "m4d_act_quant8": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
+    "m4d_act_dequant8": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "m4d_act_dequant8_t": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "m4d_act_bwd8": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "m4d_adapter_down": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, POINTER(AdapterPlanArgs), c_void_p, c_void_p, c_int64, c_int,
+                                 c_void_p]),
+    "m4d_linear_adapters": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, POINTER(AdapterPlanArgs),
+                                    c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "m4d_adapter_grad_workspace": (c_int64, [POINTER(AdapterPlanArgs), c_int64, c_int]),
+    "m4d_adapter_grad": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, POINTER(AdapterPlanArgs), c_void_p, c_int64, c_void_p,
+                                 c_int, c_int, c_int, c_int64, c_int, c_void_p]),
 }
 
 _lib = None

@@ -77,6 +77,68 @@ class LinearFn(Function):
         return dx, dw.view(wshape).to(wdt), db.to(bdt), None, None, None
 
 
+class AdapterLinearFn(Function):
+    """A frozen projection with trained low-rank adapters (ops.linear_adapters): apply(x, weight, bias, a, b, scale, plan, bits).
+    x [..., K]; weight [N, K] and bias are not trained; a [G, r, K], b [G, N, r] are, scale is G numbers.  The gradient of `a` needs the input,
+    that of `b` only u = s x A^T: the forward keeps x as it is (bits = 16) or in 8 bits (bits = 8, half the memory of bf16 and half the bytes that
+    the gradient reads).  The forward's own result comes from x itself either way."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, a, b, scale, plan, bits):
+        if bits not in (8, 16):
+            raise ValueError(f"AdapterLinearFn: bits must be 8 or 16, got {bits}")
+        if weight.requires_grad or (bias is not None and bias.requires_grad):
+            raise ValueError("AdapterLinearFn: the projection is frozen; train it with LinearFn")
+        K = x.shape[-1]
+        x2 = x.detach().reshape(-1, K)
+        bank = ops.AdapterBank(a, b, scale)
+        u, ut = ops.adapter_down(x2, bank, plan, slots=True) if x2.shape[0] else (None, None)
+        y = ops.linear_adapters(x2, weight.detach(), bias, bank, plan, u=u)
+        kept = None
+        if ctx.needs_input_grad[3]:
+            kept = ops.act_quant8(x2) if bits == 8 else x2
+        if isinstance(kept, ops.Act8):
+            ctx.save_for_backward(kept.codes, kept.exps, weight, a, b, ut)
+        else:
+            ctx.save_for_backward(kept, None, weight, a, b, ut)
+        ctx.meta = (scale, plan, bits, x.shape, x.dtype)
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        kept, exps, weight, a, b, ut = ctx.saved_tensors
+        scale, plan, bits, xshape, xdt = ctx.meta
+        N, K = weight.shape
+        need_x, need_a, need_b = (ctx.needs_input_grad[i] for i in (0, 3, 4))
+        dy2 = dy.reshape(-1, N)
+        if dy2.dtype != xdt:
+            dy2 = ops.unary(dy2, xdt)
+        elif dy2.stride(-1) != 1:
+            dy2 = dy2.contiguous()
+        if dy2.shape[0] == 0:
+            return (dy2.new_zeros(xshape) if need_x else None, None, None, torch.zeros_like(a) if need_a else None,
+                    torch.zeros_like(b) if need_b else None, None, None, None)
+        Np = -(-N // 8) * 8                              # the rows of dy become K rows of a GEMM: whole 16-byte chunks
+        if Np != N or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
+            dy2 = torch.nn.functional.pad(dy2, (0, Np - N)).contiguous()
+        bank = ops.AdapterBank(a, b, scale)
+        dx = da = db = None
+        if need_x or need_a:
+            back = bank.transposed(Np)
+            v, vt = ops.adapter_down(dy2, back, plan, rows=need_x, slots=need_a)
+            if need_x:
+                wt = torch.empty((K, Np), device=weight.device, dtype=weight.dtype)
+                if Np != N:
+                    wt[:, N:].zero_()
+                ops.transpose(weight.detach(), out=wt[:, :N])
+                dx = ops.linear_adapters(dy2, wt, None, back, plan, u=v).view(xshape)
+            if need_a:
+                da = ops.adapter_grad(vt, ops.Act8(kept, exps, (kept.shape[0], K), xdt) if bits == 8 else kept, plan, bank)
+        if need_b:
+            db = ops.adapter_grad(ut, dy2[:, :N], plan, bank, transposed=True)
+        return dx, None, None, da, db, None, None, None
+
+
 class ActFn(Function):
     """act(x) -> out_dtype (1 silu, 2 gelu_tanh, 3 gelu_erf)."""
 

@@ -1,6 +1,8 @@
 // Shared pieces of the GEMM kernels (gemm.hip, gemm_packed.hip): argument block, LDS swizzle, XCD-aware tile order,
 // fused epilogue.  See gemm.hip for the design notes.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 #include "more4d_hip.h"
 
@@ -28,6 +30,17 @@ struct GemmArgs {
     float* ws;
     int abl;   // timing ablations (tools only; results wrong when != 0): 1 no DMA, 2 frags once, 4 no barriers, 8 no MFMA
     unsigned* sync;   // persistent wide kernel: 8 arrival counters (one per XCD, 128 bytes apart, zeroed before the launch) or nullptr
+};
+
+// Shared projection with low-rank adapters (adapters.hip): behind the K loop a tile adds, for every adapter that one of its rows names,
+// the product of that adapter's rows of u (= s x A^T, other rows read as zero) with its B.
+struct GemmAdArgs : GemmArgs {
+    const void* u;              // T [M, R]
+    const void* up;             // T [G, N, R]
+    const int* row_adapter;     // [M], -1 = none
+    const int* tile_off;        // [tiles_m + 1] into tile_list
+    const int* tile_list;       // adapters of the rows of each tile, each once
+    int R;                      // multiple of 16
 };
 
 constexpr int ROWB = 128;  // bytes of K per LDS row
@@ -133,6 +146,55 @@ M4D_DEV void epilogue_tile(const GemmArgs& p, const f32x16& acc, int64_t m, int6
             const int64_t nb = nb0 + rq * 8 + hi * 4;
             if (nb >= p.N) continue;
             store4((T*)p.out + m * p.ldc + nb, v[rq]);
+        }
+    }
+}
+
+// The adapters' part of a wave's NI x MI accumulator blocks (32 x 32 each; rows m_base + 32 mi + lane, columns n_base + 32 ni + lane of W):
+// acc += up_g[n, :] . u[m, :] over the rank, for each adapter g of the tile.  The operands come straight from L2 in the MFMA layout (16 bytes
+// per lane and 16 ranks): at rank 64 they are 1 - 2 % of the bytes of the K loop, and through LDS they would need two more barriers.  Rows
+// of u that name another adapter (or none: their u was never written) are replaced by zero before the product, not multiplied by zero.
+template <typename T, int NI, int MI>
+M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], int tile, int64_t m_base, int64_t n_base, int lane) {
+    typedef typename Frag8<T>::type frag_t;
+    const int li = lane & 31, hi = lane >> 5;
+    const int i0 = __builtin_amdgcn_readfirstlane(p.tile_off[tile]), i1 = __builtin_amdgcn_readfirstlane(p.tile_off[tile + 1]);
+    if (i0 == i1) return;
+    int ra[MI];
+    const T* pu[MI];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+        const int64_t m = m_base + mi * 32 + li;
+        ra[mi] = m < p.M ? p.row_adapter[m] : -1;
+        pu[mi] = (const T*)p.u + (m < p.M ? m : 0) * p.R + hi * 8;
+    }
+    bool in[NI];
+    int64_t nr[NI];
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) {
+        const int64_t n = n_base + ni * 32 + li;
+        in[ni] = n < p.N;
+        nr[ni] = in[ni] ? n : 0;
+    }
+    for (int i = i0; i < i1; ++i) {
+        const int g = __builtin_amdgcn_readfirstlane(p.tile_list[i]);
+        const T* b = (const T*)p.up + (int64_t)g * p.N * p.R + hi * 8;
+        for (int k = 0; k < p.R; k += 16) {
+            frag_t fu[MI], fb[NI];
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi) {
+                fu[mi] = frag_t{};
+                if (ra[mi] == g) fu[mi] = *reinterpret_cast<const frag_t*>(pu[mi] + k);
+            }
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+                fb[ni] = frag_t{};
+                if (in[ni]) fb[ni] = *reinterpret_cast<const frag_t*>(b + nr[ni] * p.R + k);
+            }
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi) mma32(fb[ni], fu[mi], acc[ni][mi]);
         }
     }
 }

@@ -240,9 +240,11 @@ M4D_DEV void epilogue_block32(const GemmArgs& p, char* wl, const f32x16& a0, con
 // ring in 32 KiB of extra LDS (8 KiB per wave) and only ISSUES its stores (every tile issues all 32: edge tiles rewrite their
 // neighbour's identical values instead of masking).
 // Requirements (host-checked): K/64 even and >= 4, both operands below 4 GiB, bf16 output (bias along n or along m).
-template <int ABL, int EPI, bool PERSIST = false>
-__global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(GemmArgs p) {
+// AD: the shared projection with low-rank adapters (one tile per workgroup; gemm_common.h: adapters_extend).
+template <int ABL, int EPI, bool PERSIST = false, bool AD = false>
+__global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<AD, GemmAdArgs, GemmArgs> p) {
     typedef bf16_t T;
+    static_assert(!AD || (!PERSIST && ABL == 0 && EPI == M4D_EPI_STORE), "adapters: one tile per workgroup, plain store");
     static_assert(!PERSIST || ((EPI == M4D_EPI_STORE || EPI == M4D_EPI_GELU_TANH) && ABL == 0), "persistent form: bf16 epilogues, no ablations");
     unsigned long long ts[6];
     if constexpr (ABL & 64) { ts[0] = __builtin_readcyclecounter(); ts[5] = __builtin_amdgcn_s_memrealtime(); }
@@ -555,10 +557,19 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(GemmArgs p) {
 #undef W_MMA
 #undef W_READ
     W_LGKM0();
+    if constexpr (AD) {
+        // the fragments read ahead by the last phases are not used: keep their registers taken until the wait above, so that nothing computed
+        // for the extension can be put into one that an LDS read in flight still writes
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) asm volatile("" :: "v"(fa0[h][kk]), "v"(fa1[h][kk]), "v"(fbx[h][kk]), "v"(fby[h][kk]));
+    }
     if constexpr (ABL & 64) ts[2] = __builtin_readcyclecounter();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the redundant tail stagings must land before the LDS is re-used
     __builtin_amdgcn_s_barrier();
     if constexpr (ABL & 64) ts[3] = __builtin_readcyclecounter();
+    if constexpr (AD) adapters_extend<T, 4, 4>(p, acc, tm, m0 + wm * 128, n0 + wn * 128, lane);
     char* wl = dyn_smem + wave * 16384;
     // (the host sends bf16 outputs whose rows are not 16-byte aligned, and the erf-GELU / SiLU epilogues of a few small GEMMs, to
     // gemm_bt256p_kernel)

@@ -1057,3 +1057,292 @@ def adamw_(p, g, m, v, *, lr, beta1, beta2, eps, weight_decay, step, grad_scale=
         raise TypeError("adamw_: dtype mismatch")
     check(_lib.load().m4d_adamw(dt_code(p.dtype), _ptr(p), _ptr(g), dt_code(m.dtype), _ptr(m), _ptr(v), p.numel(), lr, beta1,
                                 beta2, eps, weight_decay, step, _ptr(grad_scale), _stream()), "m4d_adamw")
+
+
+# ------------------------------------------------------------------ activations kept in 8 bits
+def _same_device(name, *ts):
+    """All tensors on one HIP device; returns a guard that makes it current (its current stream is the one launched on)."""
+    _dev(*ts)
+    d = {t.device for t in ts if t is not None}
+    if len(d) != 1:
+        raise ValueError(f"{name}: tensors on different devices {sorted(map(str, d))}")
+    return torch.cuda.device(d.pop())
+
+
+class Act8:
+    """8-bit form of an activation tensor (`act_quant8`): int8 codes [rows, 32*nb] and one power-of-two step per block of 32 channels
+    (uint8 exponents [rows, nb], nb = ceil(C / 32)), plus the shape and dtype of the tensor it stands for.  1.03 bytes per element."""
+    __slots__ = ("codes", "exps", "shape", "dtype")
+
+    def __init__(self, codes, exps, shape, dtype):
+        self.codes, self.exps, self.shape, self.dtype = codes, exps, torch.Size(shape), dtype
+
+    @property
+    def rows(self):
+        return self.exps.shape[0]
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self):
+        return self.codes.numel() + self.exps.numel()
+
+
+def act_quant8(x, *, out=None):
+    """x [..., C] (float32 / bfloat16; leading dims collapse onto one row stride) -> Act8.  out: an Act8 of the same shape to overwrite."""
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"act_quant8: a tensor with channels is needed, got shape {tuple(x.shape)}")
+    dt_code(x.dtype)
+    C = x.shape[-1]
+    rows, ld = (0, C) if x.numel() == 0 else _rows2d(x)
+    nb = (C + 31) // 32
+    if out is None:
+        out = Act8(torch.empty((rows, 32 * nb), device=x.device, dtype=torch.int8), torch.empty((rows, nb), device=x.device, dtype=torch.uint8),
+                   x.shape, x.dtype)
+    elif not isinstance(out, Act8) or out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("act_quant8: out must be an Act8 of x's shape and dtype")
+    with _same_device("act_quant8", x, out.codes):
+        if rows:
+            check(_lib.load().m4d_act_quant8(dt_code(x.dtype), _ptr(x), ld, _ptr(out.codes), _ptr(out.exps), rows, C, _stream()), "m4d_act_quant8")
+    return out
+
+
+def act_dequant8(a8, dtype=None, *, act=0, out=None):
+    """act(value) of an Act8 as a tensor of its shape, in its own dtype or `dtype`; act as in `unary` (0 none, 1 silu, 2 gelu(tanh), 3 gelu(erf)).
+    out: [..., C], rows strided alike."""
+    C = a8.shape[-1]
+    if out is None:
+        out = torch.empty(a8.shape, device=a8.device, dtype=dtype or a8.dtype)
+    elif out.shape != a8.shape or (dtype is not None and out.dtype != dtype):
+        raise ValueError("act_dequant8: out must have the activation's shape and the requested dtype")
+    dt = dt_code(out.dtype)
+    with _same_device("act_dequant8", a8.codes, out):
+        if a8.rows:
+            rows, ld = _rows2d(out)
+            check(_lib.load().m4d_act_dequant8(dt, _ptr(a8.codes), _ptr(a8.exps), _ptr(out), ld, rows, C, act, _stream()), "m4d_act_dequant8")
+    return out
+
+
+def act_dequant8_t(a8, dtype=None, *, act=0):
+    """act(value)^T [C, Rp]: the rows become columns, zero-padded to Rp = a multiple of 64 (8 below 512 rows), the operand of a weight
+    gradient `gemm_bt(dy^T, x^T)`."""
+    C, R = a8.shape[-1], a8.rows
+    if R == 0:
+        raise ValueError("act_dequant8_t: no rows")
+    Rp = -(-R // 64) * 64 if R >= 512 else -(-R // 8) * 8
+    out = torch.empty((C, Rp), device=a8.device, dtype=dtype or a8.dtype)
+    with _same_device("act_dequant8_t", a8.codes):
+        check(_lib.load().m4d_act_dequant8_t(dt_code(out.dtype), _ptr(a8.codes), _ptr(a8.exps), _ptr(out), Rp, R, Rp, C, act, _stream()),
+              "m4d_act_dequant8_t")
+    return out
+
+
+def act_bwd8(dy, a8, act, *, out=None):
+    """dy * act'(value) with the pre-activation kept as an Act8; dy [..., C] of its shape, float32 or bfloat16.  out may be dy itself."""
+    if dy.shape != a8.shape:
+        raise ValueError(f"act_bwd8: dy {tuple(dy.shape)} against an activation of shape {tuple(a8.shape)}")
+    if out is None:
+        out = torch.empty(dy.shape, device=dy.device, dtype=dy.dtype)
+    elif out.shape != dy.shape or out.dtype != dy.dtype:
+        raise ValueError("act_bwd8: out must have dy's shape and dtype")
+    dt = dt_code(dy.dtype)
+    with _same_device("act_bwd8", dy, a8.codes, out):
+        if a8.rows:
+            rows, ldy = _rows2d(dy)
+            _, ldo = _rows2d(out)
+            if out.data_ptr() == dy.data_ptr() and ldo != ldy:
+                raise ValueError("act_bwd8: in place needs equal row strides")
+            check(_lib.load().m4d_act_bwd8(dt, _ptr(dy), ldy, _ptr(a8.codes), _ptr(a8.exps), _ptr(out), ldo, rows, dy.shape[-1], act, _stream()),
+                  "m4d_act_bwd8")
+    return out
+
+
+# ------------------------------------------------------------------ low-rank adapters of many requests beside a shared projection
+class AdapterBank:
+    """The adapters of one projection: a [G, r, K], b [G, N, r] (one dtype), scale: G numbers or a float32 tensor [G].  Laid out once: the rank
+    is padded with zeros to a multiple of 16 (adapters of different ranks: pad the smaller ones with zeros)."""
+    __slots__ = ("a", "b", "scale", "rank", "R")
+
+    def __init__(self, a, b, scale):
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError(f"AdapterBank: a [G, r, K] and b [G, N, r] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
+        G, r, K = a.shape
+        if not (G >= 1 and 1 <= r <= 512):
+            raise ValueError(f"AdapterBank: at least one adapter of rank 1..512, got {G} of rank {r}")
+        if a.dtype != b.dtype:
+            raise TypeError(f"AdapterBank: a {a.dtype} vs b {b.dtype}")
+        dt_code(a.dtype)
+        _dev(a, b)
+        a, b = a.detach(), b.detach()
+        if not isinstance(scale, torch.Tensor):
+            scale = torch.tensor([float(s) for s in scale], dtype=torch.float32)
+        if scale.numel() != G:
+            raise ValueError(f"AdapterBank: {scale.numel()} scales for {G} adapters")
+        self.rank, self.R = r, -(-r // 16) * 16
+        pad = self.R - r
+        self.a = (torch.nn.functional.pad(a, (0, 0, 0, pad)) if pad else a).contiguous()
+        self.b = (torch.nn.functional.pad(b, (0, pad)) if pad else b).contiguous()
+        self.scale = scale.to(device=a.device, dtype=torch.float32).contiguous()
+
+    def transposed(self, n_pad=None):
+        """The bank of the backward pass: v = s dy B, dx = ... + v A — b^T [G, R, N] in the place of a (N zero-padded to n_pad, for a dy whose rows
+        are padded to 16 bytes), a^T [G, K, R] in the place of b."""
+        t = AdapterBank.__new__(AdapterBank)
+        t.a, t.b = self.b.transpose(1, 2).contiguous(), self.a.transpose(1, 2).contiguous()
+        if n_pad is not None and n_pad != t.a.shape[2]:
+            t.a = torch.nn.functional.pad(t.a, (0, n_pad - t.a.shape[2]))
+        t.scale, t.rank, t.R = self.scale, self.rank, self.R
+        return t
+
+
+class AdapterPlan:
+    """Which adapter each row of a batch uses: request j owns the next lengths[j] rows (0 allowed) and names adapter adapters[j] (-1: none).
+    Host numbers; the tables (include/more4d_hip.h: m4d_adapter_plan) are built here and copied to `device` once per batch composition, then
+    shared by every projection of the model."""
+    PIECE = 64
+
+    def __init__(self, lengths, adapters, device):
+        import numpy as np
+        lengths, adapters = [int(v) for v in lengths], [int(v) for v in adapters]
+        if len(lengths) != len(adapters):
+            raise ValueError(f"AdapterPlan: {len(lengths)} lengths for {len(adapters)} adapter numbers")
+        if any(v < 0 for v in lengths) or any(v < -1 for v in adapters):
+            raise ValueError("AdapterPlan: lengths are >= 0, adapter numbers >= -1")
+        if sum(lengths) >= 1 << 31:
+            raise ValueError("AdapterPlan: too many rows")
+        P = self.PIECE
+        self.rows = sum(lengths)
+        row = np.repeat(np.array(adapters, dtype=np.int32), np.array(lengths, dtype=np.int64))
+        used = [int(g) for g in np.unique(row) if g >= 0]
+        self.n_adapters = used[-1] + 1 if used else 0
+        slots, pieces, counts = [], [], []
+        for g in used:
+            r = np.nonzero(row == g)[0].astype(np.int32)
+            n = -(-len(r) // P)
+            slots.append(np.concatenate([r, np.full(n * P - len(r), -1, np.int32)]))
+            pieces += [g] * n
+            counts.append(n)
+        self.n_pieces = len(pieces)
+        # the row contraction: about 24 chunks in all, so that a few hundred column tiles x chunks fill the chip and the partial sums stay small
+        per = max(1, -(-self.n_pieces // 24))
+        chunks, chunk_off, p0 = [], [0], 0
+        it = dict(zip(used, counts))
+        for g in range(self.n_adapters):
+            n = it.get(g, 0)
+            for q in range(0, n, per):
+                chunks += [p0 + q, p0 + min(q + per, n), g]
+            p0 += n
+            chunk_off.append(len(chunks) // 3)
+        self.n_chunks = len(chunks) // 3
+
+        def tiles(T, shifted):
+            off, lst = [0], []
+            for m in range(0, self.rows, T):
+                lo = max(0, min(m, self.rows - T)) if shifted else m
+                lst += [int(g) for g in np.unique(row[lo:m + T]) if g >= 0]
+                off.append(len(lst))
+            return off, lst
+
+        t256, l256 = tiles(256, True)
+        t128, l128 = tiles(128, False)
+        parts = [row, np.concatenate(slots) if slots else [], pieces, chunks, chunk_off, t256, l256, t128, l128]
+        parts = [np.asarray(v, dtype=np.int32) for v in parts]
+        at, offs = 0, []
+        for v in parts:
+            offs.append(at)
+            at += -(-max(len(v), 1) // 16) * 16            # every table at a 64-byte boundary
+        host = np.zeros(at, dtype=np.int32)
+        for o, v in zip(offs, parts):
+            host[o:o + len(v)] = v
+        self.table = torch.from_numpy(host).to(device)
+        base = self.table.data_ptr()
+        self.args = _lib.AdapterPlanArgs(*[base + 4 * o for o in offs], self.rows, self.n_pieces, self.n_chunks, self.n_adapters, 0)
+
+
+def _check_adapters(name, x, bank, plan):
+    rows, ldx = _rows2d(x)
+    if rows != plan.rows:
+        raise ValueError(f"{name}: {rows} rows against a plan of {plan.rows}")
+    if plan.n_adapters > bank.a.shape[0]:
+        raise ValueError(f"{name}: the plan names adapter {plan.n_adapters - 1}, the bank has {bank.a.shape[0]}")
+    if bank.a.dtype != x.dtype:
+        raise TypeError(f"{name}: x {x.dtype} vs adapters {bank.a.dtype}")
+    if bank.a.shape[2] != x.shape[-1]:
+        raise ValueError(f"{name}: x has {x.shape[-1]} channels, the adapters {bank.a.shape[2]}")
+    return rows, ldx
+
+
+def adapter_down(x, bank, plan, *, rows=True, slots=False):
+    """(u [rows, R], u^T [R, slots]) = s_g x A_g^T of each row's adapter (either may be left out: None).  u is written for rows with an adapter
+    only; u^T, the operand of `adapter_grad`, holds the plan's slots (pad slots zero)."""
+    M, ldx = _check_adapters("adapter_down", x, bank, plan)
+    u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype) if rows else None
+    ut = torch.empty((bank.R, plan.n_pieces * plan.PIECE), device=x.device, dtype=x.dtype) if slots else None
+    with _same_device("adapter_down", x, bank.a, plan.table):
+        check(_lib.load().m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, _ptr(bank.a), _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut),
+                                           x.shape[-1], bank.R, _stream()), "m4d_adapter_down")
+    return u, ut
+
+
+def linear_adapters(x, w, bias, bank, plan, *, out=None, u=None):
+    """x w^T + bias + s_g (x A_g^T) B_g^T, g the adapter of each row (plan).  x [..., K] (rows strided), w [N, K] (row-strided), bias [N] or None,
+    bank: AdapterBank, out [..., N].  u: the result of `adapter_down(x, bank, plan)` if it is at hand."""
+    K, N = x.shape[-1], w.shape[0]
+    if w.dim() != 2 or w.shape[1] != K:
+        raise ValueError(f"linear_adapters: w {tuple(w.shape)} for x with {K} channels")
+    if w.dtype != x.dtype:
+        raise TypeError(f"linear_adapters: x {x.dtype} vs w {w.dtype}")
+    if bank.b.shape[1] != N:
+        raise ValueError(f"linear_adapters: w has {N} rows, the adapters {bank.b.shape[1]}")
+    if bias is not None and (bias.dtype != x.dtype or bias.numel() != N or not bias.is_contiguous()):
+        raise ValueError("linear_adapters: bias must be contiguous, of x's dtype, with N elements")
+    if out is None:
+        out = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
+    elif out.dtype != x.dtype or out.shape != (*x.shape[:-1], N):
+        raise ValueError(f"linear_adapters: out must be {(*x.shape[:-1], N)} of x's dtype")
+    if x.numel() == 0:
+        if plan.rows:
+            raise ValueError(f"linear_adapters: no rows against a plan of {plan.rows}")
+        return out
+    M, ldx = _check_adapters("linear_adapters", x, bank, plan)
+    if plan.n_pieces == 0:                  # nobody names an adapter: the shared projection alone
+        gemm_bt(x, w, bias, out=out)
+        return out
+    _, ldw = _rows2d(w)
+    _, ldo = _rows2d(out)
+    if u is None:
+        u, _ = adapter_down(x, bank, plan)
+    elif u.shape != (M, bank.R) or u.dtype != x.dtype or not u.is_contiguous():
+        raise ValueError("linear_adapters: u must be contiguous [rows, R] of x's dtype")
+    with _same_device("linear_adapters", x, w, bias, out, u, bank.b, plan.table):
+        check(_lib.load().m4d_linear_adapters(dt_code(x.dtype), _ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(u), _ptr(bank.b), plan.args,
+                                              _ptr(out), ldo, N, K, bank.R, _stream()), "m4d_linear_adapters")
+    return out
+
+
+def adapter_grad(vt, x, plan, bank, *, transposed=False):
+    """Gradient of the adapters: sum over the rows of each adapter of v^T x, as [G, rank, C] (transposed: [G, C, rank]) in vt's dtype; adapters that
+    no row names get zero.  vt: the [R, slots] result of `adapter_down`; x [rows, C], or its Act8."""
+    G, rank, R = bank.a.shape[0], bank.rank, bank.R
+    x8 = x if isinstance(x, Act8) else None
+    C = x.shape[-1]
+    if plan.n_adapters > G:
+        raise ValueError(f"adapter_grad: the plan names adapter {plan.n_adapters - 1}, the bank has {G}")
+    if vt.shape != (R, plan.n_pieces * plan.PIECE) or not vt.is_contiguous():
+        raise ValueError("adapter_grad: vt must be adapter_down's contiguous [R, slots]")
+    rows, ldx = (x8.rows, 0) if x8 is not None else (0, 0) if x.numel() == 0 else _rows2d(x)
+    if rows != plan.rows:
+        raise ValueError(f"adapter_grad: {rows} rows against a plan of {plan.rows}")
+    if x8 is None and x.dtype != vt.dtype:
+        raise TypeError(f"adapter_grad: x {x.dtype} vs v {vt.dtype}")
+    out = torch.empty((G, C, rank) if transposed else (G, rank, C), device=vt.device, dtype=vt.dtype)
+    if plan.n_pieces == 0:
+        return out.zero_()
+    with _same_device("adapter_grad", vt, x8.codes if x8 is not None else x, plan.table):
+        lib = _lib.load()
+        ws = torch.empty(lib.m4d_adapter_grad_workspace(plan.args, C, R), device=vt.device, dtype=torch.float32)
+        check(lib.m4d_adapter_grad(dt_code(vt.dtype), _ptr(vt), 0 if x8 is not None else _ptr(x), ldx, _ptr(x8.codes) if x8 is not None else 0,
+                                   _ptr(x8.exps) if x8 is not None else 0, plan.args, _ptr(ws), ws.numel(), _ptr(out), int(transposed), G, rank, C,
+                                   R, _stream()), "m4d_adapter_grad")
+    return out

@@ -1,0 +1,77 @@
+"""Host side of the adapters' plan and bank, and the refusals that need no GPU."""
+import random
+
+import pytest
+import torch
+
+from more4d_amd import _lib, ops
+
+
+def tables(p):
+    base, t, a = p.table.data_ptr(), p.table.tolist(), p.args
+
+    def at(ptr, n):
+        o = (ptr - base) // 4
+        assert (ptr - base) % 64 == 0 and o + n <= len(t)
+        return t[o:o + n]
+    return at, a
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_plan_tables_cover_every_row_once(seed):
+    rng = random.Random(seed)
+    n = rng.choice([1, 2, 7, 300])
+    lengths = [rng.choice([0, 1, 1, 5, 63, 64, 65, 300]) for _ in range(n)]
+    ids = [rng.randint(-1, 6) for _ in range(n)]
+    p = ops.AdapterPlan(lengths, ids, "cpu")
+    at, a = tables(p)
+    rows = [i for k, i in zip(lengths, ids) for _ in range(k)]
+    assert p.rows == a.rows == len(rows) and at(a.row_adapter, len(rows)) == rows
+    slots, pieces = at(a.slot_row, 64 * p.n_pieces), at(a.piece_adapter, p.n_pieces)
+    assert sorted(s for s in slots if s >= 0) == [r for r, i in enumerate(rows) if i >= 0]
+    for q, g in enumerate(pieces):
+        own = slots[64 * q:64 * q + 64]
+        assert own[0] >= 0 and all(rows[s] == g for s in own if s >= 0)
+        assert all(s >= 0 for s in own) or q == p.n_pieces - 1 or pieces[q + 1] != g       # only an adapter's last piece is padded
+    off = at(a.chunk_off, p.n_adapters + 1)
+    ch = at(a.chunks, 3 * p.n_chunks)
+    assert off[0] == 0 and off[-1] == p.n_chunks and p.n_adapters == max([i for i in rows], default=-1) + 1
+    covered = []
+    for g in range(p.n_adapters):
+        for c in range(off[g], off[g + 1]):
+            assert ch[3 * c + 2] == g and ch[3 * c] < ch[3 * c + 1]
+            covered += range(ch[3 * c], ch[3 * c + 1])
+            assert all(pieces[q] == g for q in range(ch[3 * c], ch[3 * c + 1]))
+    assert covered == list(range(p.n_pieces))
+    for T, o_, l_ in ((256, a.tiles256_off, a.tiles256), (128, a.tiles128_off, a.tiles128)):
+        nt = -(-p.rows // T)
+        off = at(o_, nt + 1)
+        lst = at(l_, off[-1])
+        for i in range(nt):
+            lo = max(0, min(i * T, p.rows - T)) if T == 256 else i * T
+            assert lst[off[i]:off[i + 1]] == sorted({g for g in rows[lo:i * T + T] if g >= 0})
+
+
+def test_plan_of_nothing():
+    for lengths, ids in (([], []), ([0], [3]), ([5], [-1])):
+        p = ops.AdapterPlan(lengths, ids, "cpu")
+        assert p.n_pieces == p.n_chunks == p.n_adapters == 0 and p.rows == sum(lengths)
+
+
+def test_plan_refusals():
+    for lengths, ids in (([1, 2], [0]), ([-1], [0]), ([1], [-2]), ([1 << 30, 1 << 30], [-1, -1])):
+        with pytest.raises(ValueError):
+            ops.AdapterPlan(lengths, ids, "cpu")
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(4, 64)
+    a, b = torch.randn(1, 4, 64), torch.randn(1, 32, 4)
+    with pytest.raises(_lib.More4DHipError):
+        ops.AdapterBank(a, b, [1.0])
+    with pytest.raises(_lib.More4DHipError):
+        ops.act_quant8(x)
+    with pytest.raises(ValueError):
+        ops.act_quant8(torch.empty(4, 0))
+    with pytest.raises(TypeError):
+        ops.act_quant8(x.half())
