@@ -510,26 +510,37 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
 /* ------------------------------------------------------------------ low-rank adapters of many requests beside a shared projection
  *   y = x W^T + bias + s_g (x A_g^T) B_g^T,   g the adapter that the row's request names (none: the shared projection alone)
  * (the reference merges ONE adapter into the weights before it runs, utils/lora_utils.py:368, and trains one in its second stage,
- * scripts/4D_ViSM_training/train.py:686).  Banks: A T [G, R, K], B T [G, N, R], scale float32 [G]; R = the rank padded with zeros to a multiple
- * of 16.  The plan describes the rows of a batch, host-built (more4d_amd/ops.py: AdapterPlan), tables on the device:
+ * scripts/4D_ViSM_training/train.py:686).  Adapters: a T [G, rank, K], b T [G, N, rank], scale float32 [G]; R = the rank rounded up to a multiple
+ * of 16.  adapter_pack lays them out for the kernels: a_down / b_down T [adapter_down_elems(G, R, K or N)], the operands of the forward's and the
+ * backward's down projection, b_up T [G, N, R] and a_up T [G, K, R], zero beyond the rank (b_down and a_up: backward only, may be NULL).
+ * The plan describes the rows of a batch, host-built (more4d_amd/ops.py: AdapterPlan), tables on the device:
  *   row_adapter [rows]           adapter of each row, -1 = none
  *   slot_row [64 * n_pieces]     rows sorted by adapter, each adapter's list padded with -1 to pieces of 64
  *   piece_adapter [n_pieces]
- *   chunks [n_chunks][3]         pieces [first, last) of one adapter: the unit of the row contraction; chunk_off [n_adapters + 1] into it
- *   tilesT_off, tilesT           the adapters of the rows of each T-row tile, each once (T = 256: the last tile is rows [rows - 256, rows))
- *   adapter_down     u T [rows, R] and / or ut T [R, 64 * n_pieces] = s_g x A_g^T (rows without an adapter are not written, pad slots are zero)
- *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once
+ *   chunks[l] [n_chunks[l]][3]   pieces [first, last), at most 64, of one adapter: the unit of the row contraction, at four granularities from
+ *                                coarse to fine; chunk_off[l] [n_adapters + 1] into it
+ *   tiles_off[i], tiles[i]       the adapters of the rows of each tile, each once, for tiles of 64, 128 and 256 rows and (i = 3) of 256 rows
+ *                                whose last one is rows [rows - 256, rows)
+ *   adapter_down     u T [rows, R] and / or ut T [R, 64 * n_pieces] = s_g x A_g^T (rows without an adapter are not written, pad slots are zero);
+ *                    codes / exps (may be NULL): the 8-bit form of x's rows with an adapter, as act_quant8 writes it
+ *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once.  With a_down, u (and ut, codes, exps if given) are written first, by
+ *                    adapter_down; without, u is an input.  ws: linear_adapters_workspace floats
  *   adapter_grad     out T [G, rank, C] (transposed: [G, C, rank]) = sum over the rows of g of v^T x, v given as vt T [R, 64 * n_pieces], x as T or as
- *                    8-bit codes; ws from adapter_grad_workspace floats; partial sums are joined in a fixed order. */
+ *                    8-bit codes; ws: adapter_grad_workspace floats; partial sums are joined in a fixed order. */
 typedef struct {
-    const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks, *chunk_off, *tiles256_off, *tiles256, *tiles128_off, *tiles128;
+    const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks[4], *chunk_off[4], *tiles_off[4], *tiles[4];
     int64_t rows;
-    int32_t n_pieces, n_chunks, n_adapters, reserved;
+    int32_t n_pieces, n_adapters, n_chunks[4];
 } m4d_adapter_plan;
-int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a, const float* scale, const m4d_adapter_plan* plan, void* u, void* ut,
-                     int64_t K, int R, m4d_stream stream);
-int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* u, const void* b,
-                        const m4d_adapter_plan* plan, void* out, int64_t ldo, int64_t N, int64_t K, int R, m4d_stream stream);
+int64_t m4d_adapter_down_elems(int G, int R, int64_t K);
+int m4d_adapter_pack(m4d_dtype dt, const void* a, const void* b, int G, int rank, int64_t K, int64_t N, int R, void* a_down, void* b_up, void* b_down,
+                     void* a_up, m4d_stream stream);
+int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan, void* u, void* ut,
+                     int8_t* codes, uint8_t* exps, int64_t K, int R, m4d_stream stream);
+int64_t m4d_linear_adapters_workspace(m4d_dtype dt, int64_t M, int64_t N, int64_t K);
+int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* a_down, const float* scale,
+                        const void* b_up, const m4d_adapter_plan* plan, void* u, void* ut, int8_t* codes, uint8_t* exps, void* out, int64_t ldo,
+                        int64_t N, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream);
 int64_t m4d_adapter_grad_workspace(const m4d_adapter_plan* plan, int64_t C, int R);
 int m4d_adapter_grad(m4d_dtype dt, const void* vt, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps,
                      const m4d_adapter_plan* plan, float* ws, int64_t ws_floats, void* out, int transposed, int G, int rank, int64_t C, int R,

@@ -32,9 +32,9 @@ class AttnBwdArgs(Structure):
 
 
 class AdapterPlanArgs(Structure):      # m4d_adapter_plan
-    _fields_ = ([(n, c_void_p) for n in ("row_adapter", "slot_row", "piece_adapter", "chunks", "chunk_off", "tiles256_off", "tiles256",
-                                         "tiles128_off", "tiles128")] +
-                [("rows", c_int64), ("n_pieces", c_int32), ("n_chunks", c_int32), ("n_adapters", c_int32), ("reserved", c_int32)])
+    _fields_ = [("row_adapter", c_void_p), ("slot_row", c_void_p), ("piece_adapter", c_void_p), ("chunks", c_void_p * 4),
+                ("chunk_off", c_void_p * 4), ("tiles_off", c_void_p * 4), ("tiles", c_void_p * 4), ("rows", c_int64), ("n_pieces", c_int32),
+                ("n_adapters", c_int32), ("n_chunks", c_int32 * 4)]
 
 
 # name -> (restype, argtypes); mirrors include/more4d_hip.h one to one
@@ -149,10 +149,13 @@ SIGNATURES = {
     "m4d_act_dequant8": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
     "m4d_act_dequant8_t": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
     "m4d_act_bwd8": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
-    "m4d_adapter_down": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, POINTER(AdapterPlanArgs), c_void_p, c_void_p, c_int64, c_int,
-                                 c_void_p]),
-    "m4d_linear_adapters": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, POINTER(AdapterPlanArgs),
-                                    c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "m4d_adapter_down_elems": (c_int64, [c_int, c_int, c_int64]),
+    "m4d_adapter_pack": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int] + [c_void_p] * 5),
+    "m4d_adapter_down": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, POINTER(AdapterPlanArgs)] + [c_void_p] * 4 +
+                         [c_int64, c_int, c_void_p]),
+    "m4d_linear_adapters_workspace": (c_int64, [c_int, c_int64, c_int64, c_int64]),
+    "m4d_linear_adapters": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    POINTER(AdapterPlanArgs)] + [c_void_p] * 5 + [c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
     "m4d_adapter_grad_workspace": (c_int64, [POINTER(AdapterPlanArgs), c_int64, c_int]),
     "m4d_adapter_grad": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, POINTER(AdapterPlanArgs), c_void_p, c_int64, c_void_p,
                                  c_int, c_int, c_int, c_int64, c_int, c_void_p]),

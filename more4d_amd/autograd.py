@@ -89,51 +89,52 @@ class AdapterLinearFn(Function):
             raise ValueError(f"AdapterLinearFn: bits must be 8 or 16, got {bits}")
         if weight.requires_grad or (bias is not None and bias.requires_grad):
             raise ValueError("AdapterLinearFn: the projection is frozen; train it with LinearFn")
-        K = x.shape[-1]
-        x2 = x.detach().reshape(-1, K)
-        bank = ops.AdapterBank(a, b, scale)
-        u, ut = ops.adapter_down(x2, bank, plan, slots=True) if x2.shape[0] else (None, None)
-        y = ops.linear_adapters(x2, weight.detach(), bias, bank, plan, u=u)
-        kept = None
-        if ctx.needs_input_grad[3]:
-            kept = ops.act_quant8(x2) if bits == 8 else x2
-        if isinstance(kept, ops.Act8):
-            ctx.save_for_backward(kept.codes, kept.exps, weight, a, b, ut)
+        x2 = x.detach().reshape(-1, x.shape[-1])
+        need_a, need_b = ctx.needs_input_grad[3], ctx.needs_input_grad[4]
+        bank = ops.AdapterBank(a, b, scale, backward=any(ctx.needs_input_grad))
+        kept, ut = None, None
+        if need_a and bits == 8:
+            y, ut, kept = ops.linear_adapters(x2, weight.detach(), bias, bank, plan, keep8=True)
+        elif need_b:
+            y, ut = ops.linear_adapters(x2, weight.detach(), bias, bank, plan, slots=True)
         else:
-            ctx.save_for_backward(kept, None, weight, a, b, ut)
-        ctx.meta = (scale, plan, bits, x.shape, x.dtype)
+            y = ops.linear_adapters(x2, weight.detach(), bias, bank, plan)
+        if need_a:
+            kept = (kept.codes, kept.exps) if bits == 8 else (x2, None)
+        else:
+            kept = (None, None)
+        ctx.save_for_backward(*kept, weight, ut if need_b else None)
+        ctx.meta = (bank, plan, x.shape, x.dtype)       # (the bank is this call's own copy of a and b, laid out for both passes)
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     def backward(ctx, dy):
-        kept, exps, weight, a, b, ut = ctx.saved_tensors
-        scale, plan, bits, xshape, xdt = ctx.meta
+        kept, exps, weight, ut = ctx.saved_tensors
+        bank, plan, xshape, xdt = ctx.meta
         N, K = weight.shape
         need_x, need_a, need_b = (ctx.needs_input_grad[i] for i in (0, 3, 4))
         dy2 = dy.reshape(-1, N)
         if dy2.dtype != xdt:
             dy2 = ops.unary(dy2, xdt)
-        elif dy2.stride(-1) != 1:
-            dy2 = dy2.contiguous()
         if dy2.shape[0] == 0:
-            return (dy2.new_zeros(xshape) if need_x else None, None, None, torch.zeros_like(a) if need_a else None,
-                    torch.zeros_like(b) if need_b else None, None, None, None)
+            zero = [dy2.new_zeros(s) if n else None for s, n in ((xshape, need_x), ((bank.G, bank.rank, K), need_a), ((bank.G, N, bank.rank), need_b))]
+            return zero[0], None, None, zero[1], zero[2], None, None, None
         Np = -(-N // 8) * 8                              # the rows of dy become K rows of a GEMM: whole 16-byte chunks
-        if Np != N or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
+        if Np != N or dy2.stride(-1) != 1 or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
             dy2 = torch.nn.functional.pad(dy2, (0, Np - N)).contiguous()
-        bank = ops.AdapterBank(a, b, scale)
-        dx = da = db = None
-        if need_x or need_a:
-            back = bank.transposed(Np)
-            v, vt = ops.adapter_down(dy2, back, plan, rows=need_x, slots=need_a)
-            if need_x:
-                wt = torch.empty((K, Np), device=weight.device, dtype=weight.dtype)
-                if Np != N:
-                    wt[:, N:].zero_()
-                ops.transpose(weight.detach(), out=wt[:, :N])
-                dx = ops.linear_adapters(dy2, wt, None, back, plan, u=v).view(xshape)
-            if need_a:
-                da = ops.adapter_grad(vt, ops.Act8(kept, exps, (kept.shape[0], K), xdt) if bits == 8 else kept, plan, bank)
+        dx = da = db = vt = None
+        back = bank.transposed()
+        if need_x:
+            wt = torch.empty((K, Np), device=weight.device, dtype=weight.dtype)
+            if Np != N:
+                wt[:, N:].zero_()
+            ops.transpose(weight.detach(), out=wt[:, :N])
+            dx, vt = ops.linear_adapters(dy2, wt, None, back, plan, slots=True)
+            dx = dx.view(xshape)
+        elif need_a:
+            vt = ops.adapter_down(dy2, back, plan, rows=False, slots=True)[1]
+        if need_a:
+            da = ops.adapter_grad(vt, ops.Act8(kept, exps, (kept.shape[0], K), xdt) if exps is not None else kept, plan, bank)
         if need_b:
             db = ops.adapter_grad(ut, dy2[:, :N], plan, bank, transposed=True)
         return dx, None, None, da, db, None, None, None

@@ -11,12 +11,10 @@
 // All four kernels are one pass over the data and bound by HBM; a "unit" is 8 channels of a row (16 bytes of bf16, 8 bytes of codes), four
 // units are a block.  Rows of codes are padded to whole blocks, so the code side is always aligned; the other side takes 16-byte accesses
 // where its rows are 16-byte aligned and element accesses otherwise.
-#include "common.h"
+#include "act8.h"
 #include "more4d_hip.h"
 
 namespace {
-
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 struct Act8Args {
     const void* in;       // quant: x;  bwd: dy
@@ -85,13 +83,6 @@ M4D_DEV void store_unit(T* dst, int n, bool vec, const float (&v)[8]) {
     }
 }
 
-M4D_DEV float step_of(unsigned b) { return __builtin_bit_cast(float, b << 23); }      // 2^(b - 127); 255 -> +inf (times code 0: NaN)
-
-M4D_DEV void decode8(const u32x2& c, float step, float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)((int)(c[e >> 2] << (24 - 8 * (e & 3))) >> 24) * step;
-}
-
 template <typename T>
 __global__ __launch_bounds__(256) void act_quant8_kernel(Act8Args p) {
     const int nu = p.nb * 4;
@@ -104,19 +95,15 @@ __global__ __launch_bounds__(256) void act_quant8_kernel(Act8Args p) {
         for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(unsigned, v[e]) & 0x7fffffffu);
         top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));      // the block's four units are four neighbouring lanes
         top = max(top, (unsigned)__shfl_xor((int)top, 2, 64));
-        // max = 1.f * 2^E: e = E - 6, one more if 1.f > 127 / 64 (mantissa above 0x7e0000); e + 127 = biased exponent - 6 (+ 1)
-        unsigned b = (top >> 23) + ((top & 0x7fffffu) > 0x7e0000u ? 1u : 0u);
-        b = min(b > 7 ? b - 6 : 1u, 248u);
-        const bool bad = top >= 0x7f800000u;
-        const float inv = bad ? 0.f : __builtin_bit_cast(float, (254u - b) << 23);      // 2^-e, e in [-126, 121]: a normal number
+        const unsigned b = block_exp(top);
         u32x2 c = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float q = bad ? 0.f : fminf(fmaxf(rintf(v[e] * inv), -127.f), 127.f);
-            c[e >> 2] |= ((unsigned)(int)q & 0xffu) << (8 * (e & 3));
+        if (b != 255u) {
+            const float inv = block_inv(b);
+            c[0] = encode4(v[0], v[1], v[2], v[3], inv, b == 248u);
+            c[1] = encode4(v[4], v[5], v[6], v[7], inv, b == 248u);
         }
         *reinterpret_cast<u32x2*>(p.codes + (w.row * p.nb) * 32 + c0) = c;
-        if ((w.j & 3) == 0) p.exps[w.row * p.nb + (w.j >> 2)] = (uint8_t)(bad ? 255u : b);
+        if ((w.j & 3) == 0) p.exps[w.row * p.nb + (w.j >> 2)] = (uint8_t)b;
     }
 }
 

@@ -12,55 +12,170 @@
 // u is written twice: [row][R], the GEMM's operand, and [R][slot], the operand of the row contraction (its 8 consecutive slots of one
 // rank are one 16-byte load in the MFMA layout; pad slots hold zero).  u and v are rounded to T like every other operand of an MFMA here: the
 // error this puts on an output is the one its own final rounding has, or less.
-#include "gemm_common.h"
+//
+// The operand of a down projection is laid out once (m4d_adapter_pack) in the order in which the MFMA lanes read it: chunks of 64 channels, 32
+// ranks, and within them lane (rank l & 31, channels 32 (l >> 5) + [0, 32) as four 8-element fragments).  With that order of the channels a
+// lane holds a whole 32-channel block of its row, so the same pass that multiplies x by A can write x's 8-bit form (act8.h): a training
+// step that keeps its inputs in 8 bits reads them once.
+#include "act8.h"
+#include "adapters_gemm.h"
 
-extern "C" __attribute__((visibility("hidden"))) void m4d_launch_gemm_generic_adapters(const void* args, int bf16, unsigned nwg, hipStream_t st);
 extern "C" __attribute__((visibility("hidden"))) int m4d_launch_gemm_wide_adapters(const void* args, unsigned nwg, hipStream_t st);
 
 namespace {
 
 constexpr int PIECE = 64;
 
+// ---------------------------------------------------------------- layout of a bank
+struct PackArgs {
+    const void *a, *b;          // [G, rank, K], [G, N, rank]
+    void *a_down, *b_up, *b_down, *a_up;
+    int G, rank, K, N, R;
+};
+M4D_DEV int64_t down_elems(int G, int R, int K) { return (int64_t)G * ((K + 63) / 64) * ((R + 31) / 32) * 2048; }
+
+// one element of the down layout of an operand [rank, K] of adapter g: index -> (rank, channel)
+template <typename T>
+M4D_DEV void pack_down(const PackArgs& p, void* out, int K, bool from_b, int64_t i) {
+    const int e = (int)(i & 7), lane = (int)(i >> 3) & 63, kk = (int)(i >> 9) & 3, rts = (p.R + 31) / 32, nc = (K + 63) / 64;
+    int64_t j = i >> 11;
+    const int rt = (int)(j % rts);
+    j /= rts;
+    const int c = (int)(j % nc);
+    const int64_t g = j / nc;
+    const int r = rt * 32 + (lane & 31), k = c * 64 + (lane >> 5) * 32 + kk * 8 + e;
+    T v = (T)0.f;
+    if (r < p.rank && k < K) v = from_b ? ((const T*)p.b)[(g * K + k) * p.rank + r] : ((const T*)p.a)[(g * p.rank + r) * K + k];
+    ((T*)out)[i] = v;
+}
+// one element of the up layout [rows, R] (rows = N from b, K from a)
+template <typename T>
+M4D_DEV void pack_up(const PackArgs& p, void* out, int rows, bool from_a, int64_t i) {
+    const int r = (int)(i % p.R);
+    const int64_t j = i / p.R, n = j % rows, g = j / rows;
+    T v = (T)0.f;
+    if (r < p.rank) v = from_a ? ((const T*)p.a)[(g * p.rank + r) * rows + n] : ((const T*)p.b)[(g * rows + n) * p.rank + r];
+    ((T*)out)[i] = v;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_pack_kernel(PackArgs p) {
+    const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, st = (int64_t)gridDim.x * 256;
+    if (blockIdx.y == 0 && p.a_down) for (int64_t i = i0; i < down_elems(p.G, p.R, p.K); i += st) pack_down<T>(p, p.a_down, p.K, false, i);
+    if (blockIdx.y == 1 && p.b_up) for (int64_t i = i0; i < (int64_t)p.G * p.N * p.R; i += st) pack_up<T>(p, p.b_up, p.N, false, i);
+    if (blockIdx.y == 2 && p.b_down) for (int64_t i = i0; i < down_elems(p.G, p.R, p.N); i += st) pack_down<T>(p, p.b_down, p.N, true, i);
+    if (blockIdx.y == 3 && p.a_up) for (int64_t i = i0; i < (int64_t)p.G * p.K * p.R; i += st) pack_up<T>(p, p.a_up, p.K, true, i);
+}
+
+// ---------------------------------------------------------------- down projection
 struct DownArgs {
     const void* x; const void* a; const float* scale;
     void* u; void* ut;
+    int8_t* codes; uint8_t* exps;
     const int *slot_row, *piece_adapter;
     int64_t ldx, n_slots;
-    int K, R;
+    int K, R, n_pieces;
 };
 
-// 8 consecutive elements of a row at k, those at or beyond K as zero (rows are whole 16-byte chunks)
-template <typename T> M4D_DEV typename Frag8<T>::type load_k8(const T* row, int k, int K);
-template <> M4D_DEV bf16x8 load_k8<bf16_t>(const bf16_t* row, int k, int K) {
-    bf16x8 v = {};
-    if (k < K) v = *reinterpret_cast<const bf16x8*>(row + k);
-    return v;
-}
-template <> M4D_DEV f32x8 load_k8<float>(const float* row, int k, int K) {
-    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-    if (k < K) a = load4(row + k);
-    if (k + 4 < K) b = load4(row + k + 4);
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+// a row's 32-channel block in its lane's four fragments -> codes and exponent byte
+template <typename T>
+M4D_DEV void quant_block(const typename Frag8<T>::type (&x)[4], int8_t* codes, uint8_t* exps) {
+    unsigned top = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(unsigned, (float)x[k][e]) & 0x7fffffffu);
+    const unsigned b = block_exp(top);
+    const float inv = block_inv(min(b, 248u));
+    u32x4q c[2] = {};
+    if (b != 255u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                c[k >> 1][(k & 1) * 2 + h] = encode4((float)x[k][h * 4], (float)x[k][h * 4 + 1], (float)x[k][h * 4 + 2], (float)x[k][h * 4 + 3], inv, b == 248u);
+    }
+    *reinterpret_cast<u32x4q*>(codes) = c[0];
+    *reinterpret_cast<u32x4q*>(codes + 16) = c[1];
+    *exps = (uint8_t)b;
 }
 
-// u of one piece: 64 slots x RT * 32 ranks, K split over the workgroup's four waves (64 elements each in turn), joined in LDS in wave order
-template <typename T, int RT>
-__global__ __launch_bounds__(256) void adapter_down_kernel(DownArgs p) {
+// u of one piece: 64 slots x RT * 32 ranks; K split over the workgroup's NW waves (64 channels each in turn), joined in LDS in wave order.
+// Rows are requested one chunk ahead of the products (they come from HBM), the packed operand right in front of them (from L2).
+template <typename T, int RT, int NW, int NS, bool QUANT>
+M4D_DEV void down_loop(const DownArgs& p, int g, int rt0, int wave, int lane, const int (&row)[2], const int (&rowc)[2], f32x16 (&acc)[RT][2]) {
     typedef typename Frag8<T>::type frag_t;
-    __shared__ float red[RT * 2 * 16 * 64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 31, hi = lane >> 5;
-    const int piece = blockIdx.x, r0 = blockIdx.y * (RT * 32);
-    const int g = p.piece_adapter[piece];
-    int row[2];
-    const T* px[2];
+    const int hi = lane >> 5, nc = (p.K + 63) >> 6, rts = (p.R + 31) >> 5, nb = (p.K + 31) >> 5;
+    const T* px[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) px[s] = (const T*)p.x + (int64_t)rowc[s] * p.ldx + hi * 32;
     const T* pa[RT];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        row[s] = p.slot_row[(int64_t)piece * PIECE + s * 32 + li];
-        px[s] = (const T*)p.x + (int64_t)max(row[s], 0) * p.ldx;
-    }
+    for (int rt = 0; rt < RT; ++rt) pa[rt] = (const T*)p.a + ((int64_t)g * nc * rts + min(rt0 + rt, rts - 1)) * 2048 + lane * 8;
+    auto load = [&](int c, frag_t (&x)[NS][4]) {
+        if (c * 64 + 64 <= p.K) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) pa[rt] = (const T*)p.a + ((int64_t)g * p.R + min(r0 + rt * 32 + li, p.R - 1)) * p.K;
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) x[s][kk] = *reinterpret_cast<const frag_t*>(px[s] + c * 64 + kk * 8);
+        } else {
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) x[s][kk] = load_k8<T>(px[s], c * 64 + kk * 8, p.K - hi * 32);
+        }
+    };
+    auto use = [&](int c, frag_t (&x)[NS][4]) {
+        frag_t a[RT][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) a[rt][kk] = *reinterpret_cast<const frag_t*>(pa[rt] + (int64_t)c * rts * 2048 + kk * 512);
+        if constexpr (QUANT) {
+            const int blk = c * 2 + hi;
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+                if (row[s] >= 0 && blk < nb) quant_block<T>(x[s], p.codes + ((int64_t)row[s] * nb + blk) * 32, p.exps + (int64_t)row[s] * nb + blk);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int s = 0; s < NS; ++s) mma32(a[rt][kk], x[s][kk], acc[rt][s]);
+    };
+    frag_t x0[NS][4], x1[NS][4];
+    int c = wave;
+    if (c < nc) load(c, x0);
+    while (c < nc) {
+        if (c + NW < nc) load(c + NW, x1);
+        use(c, x0);
+        c += NW;
+        if (c >= nc) break;
+        if (c + NW < nc) load(c + NW, x0);
+        use(c, x1);
+        c += NW;
+    }
+}
+
+template <typename T, int RT, int NW, bool QUANT>
+__global__ __launch_bounds__(64 * NW, 2) void adapter_down_kernel(DownArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char ad_smem[];
+    float* red = reinterpret_cast<float*>(ad_smem);              // [NW][2 * 16][64]
+    const int t = threadIdx.x, lane = t & 63, li = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // more than RT * 32 ranks: ny workgroups read the same rows; numbered so that they run next to each other on one XCD and share them in its L2
+    const int ny = ((p.R + 31) / 32 + RT - 1) / RT, b8 = blockIdx.x >> 3;
+    const int piece = (b8 / ny) * 8 + (blockIdx.x & 7), rt0 = (b8 % ny) * RT;
+    if (piece >= p.n_pieces) return;
+    const int g = __builtin_amdgcn_readfirstlane(p.piece_adapter[piece]);
+    const int* sr = p.slot_row + (int64_t)piece * PIECE;
+    const bool two = __builtin_amdgcn_readfirstlane(sr[32]) >= 0;      // more than 32 rows (slot 0 always holds one)
+    int row[2], rowc[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        row[s] = sr[s * 32 + li];
+        rowc[s] = row[s] >= 0 ? row[s] : sr[0];                  // pad slots compute copies of the first row and store nothing
+    }
     f32x16 acc[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -68,62 +183,48 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(DownArgs p) {
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[rt][s][q] = 0.f;
-    for (int kc = wave * 64; kc < p.K; kc += 256) {
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            const int k = kc + kk * 16 + hi * 8;
-            frag_t fx[2], fa[RT];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                fx[s] = frag_t{};
-                if (row[s] >= 0) fx[s] = load_k8<T>(px[s], k, p.K);
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) fa[rt] = load_k8<T>(pa[rt], k, p.K);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) mma32(fa[rt], fx[s], acc[rt][s]);
-        }
-    }
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        float* d = red + ((rt * 2 + s) * 16 + q) * 64 + lane;
-                        *d = w == 0 ? acc[rt][s][q] : *d + acc[rt][s][q];
-                    }
-        }
-        __syncthreads();
+    if (QUANT && rt0 == 0) {
+        if (two) down_loop<T, RT, NW, 2, QUANT>(p, g, rt0, wave, lane, row, rowc, acc);
+        else down_loop<T, RT, NW, 1, QUANT>(p, g, rt0, wave, lane, row, rowc, acc);
+    } else {
+        if (two) down_loop<T, RT, NW, 2, false>(p, g, rt0, wave, lane, row, rowc, acc);
+        else down_loop<T, RT, NW, 1, false>(p, g, rt0, wave, lane, row, rowc, acc);
     }
     const float sc = p.scale[g];
-    // wave -> (rank quad q4 = wave) of every (rt, s): ranks rt*32 + q4*8 + hi*4 + [0, 4) of slot s*32 + li
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int rt = 0; rt < RT; ++rt) {
+        if (rt) __syncthreads();
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int r = r0 + rt * 32 + wave * 8 + hi * 4;
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) red[((wave * 2 + s) * 16 + q) * 64 + lane] = acc[rt][s][q];
+        __syncthreads();
+        // unit (s, rank quad q4, lane): ranks q4 * 8 + hi * 4 + [0, 4) of slot s * 32 + li
+        for (int i = t; i < 512; i += 64 * NW) {
+            const int l = i & 63, q4 = (i >> 6) & 3, s = i >> 8;
+            const int r = (rt0 + rt) * 32 + q4 * 8 + (l >> 5) * 4;
             if (r >= p.R) continue;
-            f32x4 v;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < NW; ++w)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = sc * red[((rt * 2 + s) * 16 + wave * 4 + e) * 64 + lane];
-            const int64_t slot = (int64_t)piece * PIECE + s * 32 + li;
-            if (p.u && row[s] >= 0) store4((T*)p.u + (int64_t)row[s] * p.R + r, v);
+                for (int e = 0; e < 4; ++e) v[e] += red[((w * 2 + s) * 16 + q4 * 4 + e) * 64 + l];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= sc;
+            const int slot = s * 32 + (l & 31), rw = sr[slot];
+            if (p.u && rw >= 0) store4((T*)p.u + (int64_t)rw * p.R + r, v);
             if (p.ut) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ((T*)p.ut)[(r + e) * p.n_slots + slot] = (T)(row[s] >= 0 ? v[e] : 0.f);
+                for (int e = 0; e < 4; ++e) ((T*)p.ut)[(r + e) * p.n_slots + (int64_t)piece * PIECE + slot] = (T)(rw >= 0 ? v[e] : 0.f);
             }
         }
+    }
 }
 
+// ---------------------------------------------------------------- contraction over the rows
 struct GradArgs {
     const void* vt;                 // T [R, n_slots]
     const void* x;                  // T [rows, C] (row stride ldx), or
-    const int8_t* codes; const uint8_t* exps;      // its 8-bit form (csrc/act8.hip)
+    const int8_t* codes; const uint8_t* exps;      // its 8-bit form (act8.hip)
     float* ws;                      // [n_chunks, R, C]
     void* out;                      // T [G, rank, C], or [G, C, rank]
     const int *slot_row, *chunks, *chunk_off;
@@ -139,21 +240,29 @@ template <> struct Quad<float> { typedef f32x4 type; };
 // ws[chunk][r][c] = sum over the chunk's slots of vt[r][slot] * x[row of slot][c].  A workgroup owns 128 columns of one chunk, its four waves take
 // 16 slots each in turn.  The contraction runs over ROWS, so the MFMA wants 8 rows of one column per lane: a lane loads 4 consecutive columns
 // of 8 rows and regroups them in registers into 4 fragments, fragment f = column 4 * lane + f, so that no LDS transpose is needed and a lane
-// ends with 4 consecutive columns of the result.
+// ends with 4 consecutive columns of the result.  The chunk's row numbers sit in LDS, and PF steps of rows are in flight while one is used.
+constexpr int CHUNK_PIECES = 64;       // most pieces in a chunk (the row numbers in LDS)
 template <typename T, bool CODES, int RT>
-__global__ __launch_bounds__(256) void adapter_grad_kernel(GradArgs p) {
+__global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
     typedef typename Frag8<T>::type frag_t;
     typedef typename Quad<T>::type quad_t;
-    __shared__ float red[RT * 4 * 16 * 64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 31, hi = lane >> 5;
+    constexpr int PF = 2;
+    constexpr int RED = RT * 4 * 16 * 64 * 4;
+    __shared__ __attribute__((aligned(16))) char smem[RED > CHUNK_PIECES * PIECE * 4 ? RED : CHUNK_PIECES * PIECE * 4];
+    int* rows = reinterpret_cast<int*>(smem);
+    float* red = reinterpret_cast<float*>(smem);
+    const int t = threadIdx.x, lane = t & 63, li = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = blockIdx.x * 128 + li * 4, r0 = blockIdx.z * (RT * 32);
     const int* ch = p.chunks + 3 * blockIdx.y;
-    const int s0 = ch[0] * PIECE, s1 = ch[1] * PIECE;
+    const int s0 = ch[0] * PIECE, n = ch[1] * PIECE - s0;
+    for (int i = t; i < n; i += 256) rows[i] = p.slot_row[s0 + i];
     const bool cin = c < p.C;
+    const int cc = cin ? c : 0;                     // (columns beyond C are computed from the first ones and not stored)
     const int nb = (p.C + 31) >> 5;
     const T* pv[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) pv[rt] = (const T*)p.vt + (int64_t)min(r0 + rt * 32 + li, p.R - 1) * p.n_slots + hi * 8;
+    for (int rt = 0; rt < RT; ++rt) pv[rt] = (const T*)p.vt + (int64_t)min(r0 + rt * 32 + li, p.R - 1) * p.n_slots + s0 + hi * 8;
     f32x16 acc[RT][4];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -161,36 +270,67 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(GradArgs p) {
         for (int f = 0; f < 4; ++f)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[rt][f][q] = 0.f;
-    for (int s = s0 + wave * 16; s < s1; s += 64) {
-        quad_t xr[8];
+    __syncthreads();
+    struct Step {
+        frag_t v[RT];
+        quad_t x[8];
+        int code[8];
+        unsigned char ex[8];
+    };
+    // (pad slots, -1, read the chunk's first row: what they read is replaced by zero in use() — their v is zero, but zero times an infinity is not)
+    auto load = [&](int s, Step& b) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) b.v[rt] = *reinterpret_cast<const frag_t*>(pv[rt] + s);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int row = p.slot_row[s + hi * 8 + j];
-            xr[j] = quad_t{};
-            if (row >= 0 && cin) {
-                if constexpr (CODES) {
-                    const int cd = *reinterpret_cast<const int*>(p.codes + ((int64_t)row * nb) * 32 + c);
-                    const float step = __builtin_bit_cast(float, (unsigned)p.exps[(int64_t)row * nb + (c >> 5)] << 23);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) xr[j][e] = (T)((float)((cd << (24 - 8 * e)) >> 24) * step);
-                } else {
-                    xr[j] = *reinterpret_cast<const quad_t*>((const T*)p.x + (int64_t)row * p.ldx + c);
-                }
-            }
+            const int r = rows[s + hi * 8 + j];
+            const int64_t row = r >= 0 ? r : rows[0];
+            if constexpr (CODES) {
+                b.code[j] = *reinterpret_cast<const int*>(p.codes + row * nb * 32 + cc);
+                b.ex[j] = p.exps[row * nb + (cc >> 5)];
+            } else b.x[j] = *reinterpret_cast<const quad_t*>((const T*)p.x + row * p.ldx + cc);
         }
-        frag_t fv[RT];
+    };
+    auto use = [&](int s, Step& b) {
+        if (rows[s + 15] < 0) {                     // (uniform: the adapter's last piece) a step with pad slots
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) fv[rt] = *reinterpret_cast<const frag_t*>(pv[rt] + s);
+            for (int j = 0; j < 8; ++j)
+                if (rows[s + hi * 8 + j] < 0) {
+                    if constexpr (CODES) { b.code[j] = 0; b.ex[j] = 1; }
+                    else b.x[j] = quad_t{};
+                }
+        }
+        if constexpr (CODES) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) b.x[j][e] = (T)decode1((unsigned)b.code[j], e, step_of(b.ex[j]));      // exact in T
+        }
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             frag_t fx;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) fx[j] = xr[j][f];
+            for (int j = 0; j < 8; ++j) fx[j] = b.x[j][f];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) mma32(fv[rt], fx, acc[rt][f]);
+            for (int rt = 0; rt < RT; ++rt) mma32(b.v[rt], fx, acc[rt][f]);
+        }
+    };
+    Step b[PF];
+#pragma unroll
+    for (int i = 0; i < PF; ++i)
+        if ((wave + 4 * i) * 16 < n) load((wave + 4 * i) * 16, b[i]);
+    for (int s = wave * 16; s < n; s += 64 * PF) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            const int si = s + 64 * i;
+            if (si < n) {
+                use(si, b[i]);
+                if (si + 64 * PF < n) load(si + 64 * PF, b[i]);
+            }
         }
     }
     for (int w = 0; w < 4; ++w) {
+        __syncthreads();
         if (wave == w) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -201,8 +341,8 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(GradArgs p) {
                     *d = w == 0 ? v : *d + v;
                 }
         }
-        __syncthreads();
     }
+    __syncthreads();
     if (!cin) return;
     float* out = p.ws + (int64_t)blockIdx.y * p.R * p.C + c;
 #pragma unroll
@@ -245,6 +385,37 @@ __global__ __launch_bounds__(256) void adapter_grad_join_kernel(GradArgs p) {
 
 bool dt_ok(int dt) { return dt == M4D_BF16 || dt == M4D_F32; }
 
+int cus() {
+    static std::atomic<int> n[64] = {};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); return 256; }
+    if (dev < 0 || dev >= 64) return 256;
+    int v = n[dev].load(std::memory_order_relaxed);
+    if (v == 0) {
+        if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) { (void)hipGetLastError(); v = 256; }
+        n[dev].store(v, std::memory_order_relaxed);
+    }
+    return v;
+}
+
+enum { GEMV16 = 0, TILE_64x64, TILE_64x128, TILE_128x128, TILE_256x128, WIDE_256x256 };
+struct Choice { int kind, S; };
+
+Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, int ncu) {
+#ifdef M4D_ABLATIONS
+    { const char* v = getenv("M4D_ADAPTER_GEMM"); if (v) { const int c = atoi(v); if (c / 100 != WIDE_256x256 || wide_ok) return Choice{c / 100, c % 100 ? c % 100 : 1}; } }
+#endif
+    if (M <= 16) return Choice{GEMV16, 1};
+    if (wide_ok && M * N >= (int64_t)ncu * 65536 / 2) return Choice{WIDE_256x256, 1};
+    const int nk = (int)((K * (bf16 ? 2 : 4) + ROWB - 1) / ROWB);
+    const int kind = M <= 64 ? TILE_64x128 : TILE_128x128;
+    const int bm = M <= 64 ? 64 : 128;
+    const int64_t tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
+    int S = 1;
+    while (S < 8 && tiles * S * 2 <= ncu && nk / (S * 2) >= 4) S *= 2;
+    return Choice{kind, S};
+}
+
 }  // namespace
 
 #define PLAN_OK(name)                                                                                                          \
@@ -253,62 +424,170 @@ bool dt_ok(int dt) { return dt == M4D_BF16 || dt == M4D_F32; }
     M4D_CHECK_ARG(R > 0 && R % 16 == 0 && R <= 512, name ": padded rank R=%d must be a multiple of 16, at most 512", R);          \
     const int es = dt == M4D_BF16 ? 2 : 4
 
-extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a, const float* scale, const m4d_adapter_plan* plan,
-                                void* u, void* ut, int64_t K, int R, m4d_stream stream) {
-    PLAN_OK("adapter_down");
-    M4D_CHECK_ARG(x && a && scale && (u || ut), "adapter_down: null pointer");
-    M4D_CHECK_ARG(K > 0 && K < (1 << 30) && (K * es) % 16 == 0 && (ldx * es) % 16 == 0 && (plan->rows == 1 || ldx >= K),
-                  "adapter_down: rows of K=%lld elements (row stride %lld) must be multiples of 16 bytes", (long long)K, (long long)ldx);
-    M4D_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)a % 16) == 0 && ((uintptr_t)u % 16) == 0 && ((uintptr_t)ut % 16) == 0,
-                  "adapter_down: pointers must be 16-byte aligned");
-    if (plan->n_pieces == 0) return 0;
-    M4D_CHECK_ARG(plan->slot_row && plan->piece_adapter, "adapter_down: bad plan");
-    DownArgs p{x, a, scale, u, ut, plan->slot_row, plan->piece_adapter, ldx, (int64_t)plan->n_pieces * PIECE, (int)K, R};
-    hipStream_t st = (hipStream_t)stream;
-#define DOWN(T, RT) hipLaunchKernelGGL((adapter_down_kernel<T, RT>), dim3((unsigned)plan->n_pieces, (unsigned)((R + RT * 32 - 1) / (RT * 32))), dim3(256), 0, st, p)
-    if (dt == M4D_BF16) { if (R <= 32) DOWN(bf16_t, 1); else DOWN(bf16_t, 2); }
-    else { if (R <= 32) DOWN(float, 1); else DOWN(float, 2); }
-#undef DOWN
+extern "C" int64_t m4d_adapter_down_elems(int G, int R, int64_t K) { return (int64_t)G * ((K + 63) / 64) * ((R + 31) / 32) * 2048; }
+
+extern "C" int m4d_adapter_pack(m4d_dtype dt, const void* a, const void* b, int G, int rank, int64_t K, int64_t N, int R, void* a_down, void* b_up,
+                                void* b_down, void* a_up, m4d_stream stream) {
+    M4D_CHECK_ARG(dt_ok(dt), "adapter_pack: bad dtype %d", (int)dt);
+    M4D_CHECK_ARG(a && b && G > 0 && rank > 0 && R >= rank && R % 16 == 0 && R <= 512 && K > 0 && N > 0 && K < (1 << 30) && N < (1 << 30),
+                  "adapter_pack: bad adapters (G=%d rank=%d R=%d K=%lld N=%lld)", G, rank, R, (long long)K, (long long)N);
+    M4D_CHECK_ARG(((uintptr_t)a_down % 16) == 0 && ((uintptr_t)b_up % 16) == 0 && ((uintptr_t)b_down % 16) == 0 && ((uintptr_t)a_up % 16) == 0,
+                  "adapter_pack: pointers must be 16-byte aligned");
+    PackArgs p{a, b, a_down, b_up, b_down, a_up, G, rank, (int)K, (int)N, R};
+    const int64_t most = (int64_t)G * (R + 31) * ((K > N ? K : N) + 63);
+    const int64_t nblk = (most + 1023) / 1024;
+    dim3 grid((unsigned)(nblk < 1024 ? nblk : 1024), b_down || a_up ? 4 : 2);
+    if (dt == M4D_BF16) hipLaunchKernelGGL(adapter_pack_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    else hipLaunchKernelGGL(adapter_pack_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    M4D_CHECK_LAUNCH("adapter_pack");
+    return 0;
+}
+
+template <typename T, int RT, int NW, bool QUANT>
+static int launch_down(const DownArgs& p, int n_pieces, hipStream_t st) {
+    constexpr int LDS = NW * 8192;
+    static PerDeviceOnce configured;
+    if (configured.pending()) {
+        if (hipFuncSetAttribute((const void*)adapter_down_kernel<T, RT, NW, QUANT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
+            (void)hipGetLastError();
+            m4d_set_error("adapter_down: cannot enable %d bytes of LDS", LDS);
+            return -3;
+        }
+        configured.mark();
+    }
+    const int ny = ((p.R + 31) / 32 + RT - 1) / RT;
+    hipLaunchKernelGGL((adapter_down_kernel<T, RT, NW, QUANT>), dim3((unsigned)((n_pieces + 7) / 8 * 8 * ny)), dim3(64 * NW), LDS, st, p);
     M4D_CHECK_LAUNCH("adapter_down");
     return 0;
 }
+template <typename T, int RT>
+static int launch_down_nw(const DownArgs& p, int n_pieces, hipStream_t st) {
+    // few pieces: more waves on each (their K loops are serial trips to memory); many: four, so that all pieces of a long batch are resident
+    if (n_pieces < cus() / 2) return p.codes ? launch_down<T, RT, 8, true>(p, n_pieces, st) : launch_down<T, RT, 8, false>(p, n_pieces, st);
+    return p.codes ? launch_down<T, RT, 4, true>(p, n_pieces, st) : launch_down<T, RT, 4, false>(p, n_pieces, st);
+}
 
-extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* u,
-                                   const void* b, const m4d_adapter_plan* plan, void* out, int64_t ldo, int64_t N, int64_t K, int R,
-                                   m4d_stream stream) {
-    PLAN_OK("linear_adapters");
-    const int64_t M = plan->rows;
-    M4D_CHECK_ARG(x && W && out && u && b, "linear_adapters: null pointer");
-    M4D_CHECK_ARG(N > 0 && K > 0 && K < (1 << 30) && (K * es) % 16 == 0, "linear_adapters: K*sizeof(T) must be a multiple of 16 (K=%lld)", (long long)K);
-    M4D_CHECK_ARG(N % 4 == 0 && ldo % 4 == 0 && (M == 1 || ldo >= N), "linear_adapters: N and the output's row stride must be multiples of 4 (N=%lld ldo=%lld)",
-                  (long long)N, (long long)ldo);
-    M4D_CHECK_ARG((ldx * es) % 16 == 0 && (ldw * es) % 16 == 0 && (M == 1 || ldx >= K) && ldw >= K, "linear_adapters: rows must be 16-byte aligned");
-    M4D_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)W % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)u % 16) == 0 && ((uintptr_t)b % 16) == 0,
-                  "linear_adapters: pointers must be 16-byte aligned");
-    M4D_CHECK_ARG(plan->row_adapter && plan->tiles256_off && plan->tiles256 && plan->tiles128_off && plan->tiles128, "linear_adapters: bad plan");
-    GemmAdArgs p{};
-    p.A = x; p.W = W; p.bias = bias; p.out = out; p.lda = ldx; p.ldw = ldw; p.ldc = ldo; p.M = M; p.N = N; p.K = K;
-    p.rows_per_sample = M; p.epilogue = M4D_EPI_STORE;
-    p.u = u; p.up = b; p.row_adapter = plan->row_adapter; p.R = R;
+extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan,
+                                void* u, void* ut, int8_t* codes, uint8_t* exps, int64_t K, int R, m4d_stream stream) {
+    PLAN_OK("adapter_down");
+    M4D_CHECK_ARG(x && a_down && scale && (u || ut) && (codes == nullptr) == (exps == nullptr), "adapter_down: null pointer");
+    M4D_CHECK_ARG(K > 0 && K < (1 << 30) && (K * es) % 16 == 0 && (ldx * es) % 16 == 0 && (plan->rows == 1 || ldx >= K),
+                  "adapter_down: rows of K=%lld elements (row stride %lld) must be multiples of 16 bytes", (long long)K, (long long)ldx);
+    M4D_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)a_down % 16) == 0 && ((uintptr_t)u % 16) == 0 && ((uintptr_t)ut % 16) == 0 && ((uintptr_t)codes % 16) == 0,
+                  "adapter_down: pointers must be 16-byte aligned");
+    if (plan->n_pieces == 0) return 0;
+    M4D_CHECK_ARG(plan->slot_row && plan->piece_adapter, "adapter_down: bad plan");
+    DownArgs p{x, a_down, scale, u, ut, codes, exps, plan->slot_row, plan->piece_adapter, ldx, (int64_t)plan->n_pieces * PIECE, (int)K, R, plan->n_pieces};
     hipStream_t st = (hipStream_t)stream;
-    // the rule of m4d_gemm_bt: 256 x 256 tiles for big bf16 problems with whole 64-element K tiles and 16-byte output rows
-    const bool wide = dt == M4D_BF16 && K % 64 == 0 && M >= 512 && N >= 512 && ldo % 8 == 0 && ((uintptr_t)out % 32) == 0;
-    const int bt = wide ? 256 : 128;
-    const int64_t tm = (M + bt - 1) / bt, tn = (N + bt - 1) / bt;
+    if (dt == M4D_BF16) return R <= 32 ? launch_down_nw<bf16_t, 1>(p, plan->n_pieces, st) : launch_down_nw<bf16_t, 2>(p, plan->n_pieces, st);
+    return launch_down_nw<float, 1>(p, plan->n_pieces, st);
+}
+
+template <typename T, int MI, int NI, int WM, int WN>
+static int launch_gemm(AdGemmArgs& p, hipStream_t st) {
+    typedef AdGemmShape<T, MI, NI, WM, WN> Sh;
+    static PerDeviceOnce configured;
+    if (configured.pending()) {
+        if (hipFuncSetAttribute((const void*)adapter_gemm_kernel<T, MI, NI, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS) != hipSuccess) {
+            (void)hipGetLastError();
+            m4d_set_error("linear_adapters: cannot enable %d bytes of LDS", Sh::LDS);
+            return -3;
+        }
+        configured.mark();
+    }
+    const int64_t tm = (p.M + Sh::BM - 1) / Sh::BM, tn = (p.N + Sh::BN - 1) / Sh::BN;
     M4D_CHECK_ARG(tm * tn < (1ll << 31), "linear_adapters: too many tiles");
     p.tiles_m = (int)tm; p.tiles_n = (int)tn;
-    p.tile_off = wide ? plan->tiles256_off : plan->tiles128_off;
-    p.tile_list = wide ? plan->tiles256 : plan->tiles128;
-    if (wide) {
-        if (m4d_launch_gemm_wide_adapters(&p, (unsigned)(tm * tn), st) != 0) { m4d_set_error("linear_adapters: cannot enable 128 KiB LDS"); return -3; }
-    } else m4d_launch_gemm_generic_adapters(&p, dt == M4D_BF16, (unsigned)(tm * tn), st);
+    hipLaunchKernelGGL((adapter_gemm_kernel<T, MI, NI, WM, WN>), dim3((unsigned)(tm * tn), (unsigned)p.S), dim3(256), Sh::LDS, st, p);
     M4D_CHECK_LAUNCH("linear_adapters");
-    m4d_count_launch(wide ? M4D_KC_GEMM_WIDE : M4D_KC_GEMM_GENERIC);
+    if (p.S > 1) {
+        const int64_t nblk = (p.M * (p.N / 4) + 255) / 256;
+        hipLaunchKernelGGL(adapter_gemm_join_kernel<T>, dim3((unsigned)(nblk < 4096 ? nblk : 4096)), dim3(256), 0, st, p);
+        M4D_CHECK_LAUNCH("linear_adapters(join)");
+    }
     return 0;
 }
 
+static bool wide_shape(m4d_dtype dt, int64_t M, int64_t N, int64_t K) { return dt == M4D_BF16 && K % 64 == 0 && M >= 512 && N >= 512; }
+
+extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    int64_t most = 0;                    // (whether the wide kernel can run depends on the output's alignment too: room for either choice)
+    for (int w = 0; w < 2; ++w) {
+        const Choice c = choose(dt == M4D_BF16, M, N, K, w && wide_shape(dt, M, N, K), cus());
+        if (c.S > 1 && c.S * M * N > most) most = c.S * M * N;
+    }
+    return most;
+}
+
+extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* a_down,
+                                   const float* scale, const void* b_up, const m4d_adapter_plan* plan, void* u, void* ut, int8_t* codes,
+                                   uint8_t* exps, void* out, int64_t ldo, int64_t N, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream) {
+    PLAN_OK("linear_adapters");
+    const int64_t M = plan->rows;
+    M4D_CHECK_ARG(x && W && out && u && b_up, "linear_adapters: null pointer");
+    M4D_CHECK_ARG(N > 0 && K > 0 && K < (1 << 30) && N < (1ll << 31) && (K * es) % 16 == 0, "linear_adapters: K*sizeof(T) must be a multiple of 16 (K=%lld)", (long long)K);
+    M4D_CHECK_ARG(N % 4 == 0 && ldo % 4 == 0 && (M == 1 || ldo >= N), "linear_adapters: N and the output's row stride must be multiples of 4 (N=%lld ldo=%lld)",
+                  (long long)N, (long long)ldo);
+    M4D_CHECK_ARG((ldx * es) % 16 == 0 && (ldw * es) % 16 == 0 && (M == 1 || ldx >= K) && ldw >= K, "linear_adapters: rows must be 16-byte aligned");
+    M4D_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)W % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)u % 16) == 0 && ((uintptr_t)b_up % 16) == 0,
+                  "linear_adapters: pointers must be 16-byte aligned");
+    M4D_CHECK_ARG(((uintptr_t)bias % (4 * es)) == 0, "linear_adapters: bias must be aligned to four elements");
+    M4D_CHECK_ARG(plan->row_adapter && plan->tiles_off[0] && plan->tiles_off[1] && plan->tiles_off[2] && plan->tiles[0] && plan->tiles[1] && plan->tiles[2],
+                  "linear_adapters: bad plan");
+    const bool bf16 = dt == M4D_BF16;
+    const bool wide_ok = wide_shape(dt, M, N, K) && ldo % 8 == 0 && ((uintptr_t)out % 32) == 0;
+    const Choice c = choose(bf16, M, N, K, wide_ok, cus());
+    M4D_CHECK_ARG(c.S == 1 || (ws && ws_floats >= c.S * M * N && ((uintptr_t)ws % 16) == 0), "linear_adapters: workspace of %lld floats needed", (long long)(c.S * M * N));
+    if (a_down) {
+        const int rc = m4d_adapter_down(dt, x, ldx, a_down, scale, plan, u, ut, codes, exps, K, R, stream);
+        if (rc != 0) return rc;
+    }
+    AdGemmArgs p{};
+    p.A = x; p.W = W; p.bias = bias; p.out = out; p.lda = ldx; p.ldw = ldw; p.ldc = ldo; p.M = M; p.N = N; p.K = K;
+    p.rows_per_sample = M; p.epilogue = M4D_EPI_STORE;
+    p.u = u; p.up = b_up; p.row_adapter = plan->row_adapter; p.R = R; p.S = c.S; p.ws = ws;
+    const int tl = c.kind == GEMV16 || c.kind == TILE_64x64 || c.kind == TILE_64x128 ? 0 : c.kind == TILE_128x128 ? 1 : 2;      // tile heights 64, 128, 256
+    p.tile_off = plan->tiles_off[tl]; p.tile_list = plan->tiles[tl];
+    hipStream_t st = (hipStream_t)stream;
+    m4d_count_launch(c.kind == WIDE_256x256 ? M4D_KC_GEMM_WIDE : M4D_KC_GEMM_GENERIC);
+    switch (c.kind) {
+        case GEMV16: {
+            M4D_CHECK_ARG(M <= 16, "linear_adapters: too many rows");
+            dim3 grid((unsigned)((N + 15) / 16)), block(64 * SKINNY_WAVES);
+            if (bf16) hipLaunchKernelGGL(adapter_gemv_kernel<bf16_t>, grid, block, 0, st, p);
+            else hipLaunchKernelGGL(adapter_gemv_kernel<float>, grid, block, 0, st, p);
+            M4D_CHECK_LAUNCH("linear_adapters");
+            return 0;
+        }
+        case TILE_64x64: return bf16 ? launch_gemm<bf16_t, 1, 1, 2, 2>(p, st) : launch_gemm<float, 1, 1, 2, 2>(p, st);
+        case TILE_64x128: return bf16 ? launch_gemm<bf16_t, 1, 2, 2, 2>(p, st) : launch_gemm<float, 1, 2, 2, 2>(p, st);
+        case TILE_128x128: return bf16 ? launch_gemm<bf16_t, 2, 2, 2, 2>(p, st) : launch_gemm<float, 2, 2, 2, 2>(p, st);
+        case TILE_256x128: return bf16 ? launch_gemm<bf16_t, 4, 2, 2, 2>(p, st) : launch_gemm<float, 4, 2, 2, 2>(p, st);
+        default: break;
+    }
+    p.tile_off = plan->tiles_off[3]; p.tile_list = plan->tiles[3];
+    p.tiles_m = (int)((M + 255) / 256); p.tiles_n = (int)((N + 255) / 256);
+    M4D_CHECK_ARG((int64_t)p.tiles_m * p.tiles_n < (1ll << 31), "linear_adapters: too many tiles");
+    if (m4d_launch_gemm_wide_adapters(static_cast<const GemmAdArgs*>(&p), (unsigned)(p.tiles_m * p.tiles_n), st) != 0) {
+        (void)hipGetLastError();
+        m4d_set_error("linear_adapters: cannot enable 128 KiB LDS");
+        return -3;
+    }
+    M4D_CHECK_LAUNCH("linear_adapters");
+    return 0;
+}
+
+// the coarsest chunks that still give two workgroups per CU (coarser: fewer partial sums to write and join)
+static int chunk_level(const m4d_adapter_plan* plan, int64_t C, int R) {
+    const int64_t blocks = ((C + 127) / 128) * (R <= 64 ? 1 : (R + 63) / 64);
+    for (int l = 0; l < 3; ++l)
+        if (blocks * plan->n_chunks[l] >= 2 * cus()) return l;
+    return 3;
+}
+
 extern "C" int64_t m4d_adapter_grad_workspace(const m4d_adapter_plan* plan, int64_t C, int R) {
-    return plan ? (int64_t)plan->n_chunks * R * C : 0;
+    return plan && C > 0 && R > 0 ? (int64_t)plan->n_chunks[chunk_level(plan, C, R)] * R * C : 0;
 }
 
 extern "C" int m4d_adapter_grad(m4d_dtype dt, const void* vt, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps,
@@ -317,20 +596,20 @@ extern "C" int m4d_adapter_grad(m4d_dtype dt, const void* vt, const void* x, int
     PLAN_OK("adapter_grad");
     M4D_CHECK_ARG(out && G > 0 && G <= 65535 && rank > 0 && rank <= R, "adapter_grad: bad adapters (G=%d rank=%d R=%d)", G, rank, R);
     M4D_CHECK_ARG(C > 0 && C < (1 << 30) && C % 4 == 0, "adapter_grad: C=%lld must be a multiple of 4", (long long)C);
-    M4D_CHECK_ARG(plan->n_adapters <= G && plan->n_chunks <= 65535, "adapter_grad: the plan names adapter %d of %d", plan->n_adapters - 1, G);
+    const int lv = chunk_level(plan, C, R), nch = plan->n_chunks[lv];
+    M4D_CHECK_ARG(plan->n_adapters <= G && nch <= 65535, "adapter_grad: the plan names adapter %d of %d, in %d chunks", plan->n_adapters - 1, G, nch);
     hipStream_t st = (hipStream_t)stream;
-    GradArgs p{vt, x, codes, exps, ws, out, plan->slot_row, plan->chunks, plan->chunk_off, ldx, (int64_t)plan->n_pieces * PIECE,
+    GradArgs p{vt, x, codes, exps, ws, out, plan->slot_row, plan->chunks[lv], plan->chunk_off[lv], ldx, (int64_t)plan->n_pieces * PIECE,
                (int)C, R, rank, plan->n_adapters, transposed};
-    if (plan->n_chunks > 0) {
-        M4D_CHECK_ARG(vt && ws && ws_floats >= (int64_t)plan->n_chunks * R * C, "adapter_grad: workspace of %lld floats needed",
-                      (long long)plan->n_chunks * R * C);
+    if (nch > 0) {
+        M4D_CHECK_ARG(vt && ws && ws_floats >= (int64_t)nch * R * C, "adapter_grad: workspace of %lld floats needed", (long long)nch * R * C);
         M4D_CHECK_ARG((x != nullptr) != (codes != nullptr) && (codes == nullptr) == (exps == nullptr), "adapter_grad: either x or its codes");
         M4D_CHECK_ARG(!x || (ldx * es) % 16 == 0, "adapter_grad: rows must be 16-byte aligned");
         M4D_CHECK_ARG(((uintptr_t)vt % 16) == 0 && ((uintptr_t)x % 16) == 0 && ((uintptr_t)codes % 16) == 0 && ((uintptr_t)ws % 16) == 0,
                       "adapter_grad: pointers must be 16-byte aligned");
-        M4D_CHECK_ARG(plan->slot_row && plan->chunks && plan->chunk_off, "adapter_grad: bad plan");
+        M4D_CHECK_ARG(plan->slot_row && p.chunks && p.chunk_off, "adapter_grad: bad plan");
         const int rt = R <= 32 ? 1 : 2;
-        dim3 grid((unsigned)((C + 127) / 128), (unsigned)plan->n_chunks, (unsigned)((R + rt * 32 - 1) / (rt * 32)));
+        dim3 grid((unsigned)((C + 127) / 128), (unsigned)nch, (unsigned)((R + rt * 32 - 1) / (rt * 32)));
 #define GRAD(T, CD)                                                                                         \
     do {                                                                                                    \
         if (rt == 1) hipLaunchKernelGGL((adapter_grad_kernel<T, CD, 1>), grid, dim3(256), 0, st, p);         \

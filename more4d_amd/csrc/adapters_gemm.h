@@ -1,0 +1,241 @@
+// adapter_gemm_kernel: the shared projection with its adapters for the sizes between one row and the 256 x 256 tiles of gemm_wide.h, bf16 and
+// float32.  out[m, n] = x W^T (+ bias) + u_g up_g^T for a BM x BN tile, BM = 32 MI WM, BN = 32 NI WN, four waves as WM x WN.
+//
+// What bounds these sizes is latency: a tile's K loop is serial, and with few tiles per CU nothing else hides a trip to memory.  So the K tiles
+// (128 bytes of a row) run through a ring of NST LDS stages filled by direct-to-LDS loads, NST - 1 tiles in flight, one barrier per tile; and
+// where the tiles do not fill the chip, K is cut into S slices (gridDim.y) whose float32 partial tiles a second kernel joins in slice order.
+// LDS image and swizzle are those of gemm.hip; rows beyond M and N are staged from the last row and not stored, 16-byte chunks beyond K are
+// staged from a page of zeros.
+#pragma once
+#include "gemm_common.h"
+
+namespace {
+
+struct AdGemmArgs : GemmAdArgs {
+    int S;             // K slices; > 1: float32 partial sums to ws [S, M, N]
+};
+
+__device__ __attribute__((aligned(16))) const unsigned zero_page[4] = {0u, 0u, 0u, 0u};
+
+template <typename T, int MI, int NI, int WM, int WN>
+struct AdGemmShape {
+    static constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN;
+    static constexpr int STAGE = (BM + BN) * ROWB;
+    static constexpr int NST = STAGE * 4 <= 131072 ? 4 : 3;
+    static constexpr int LDS = NST * STAGE;
+};
+
+template <typename T, int MI, int NI, int WM, int WN>
+__global__ __launch_bounds__(256) void adapter_gemm_kernel(AdGemmArgs p) {
+    typedef AdGemmShape<T, MI, NI, WM, WN> Sh;
+    typedef typename Frag8<T>::type frag_t;
+    extern __shared__ __attribute__((aligned(16))) char ad_smem[];
+    constexpr int ES = sizeof(T), KT = ROWB / ES, KSTEPS = KT / 16, NST = Sh::NST, BM = Sh::BM, BN = Sh::BN;
+    constexpr int NU = (BM + BN) / 32;                       // staging instructions per wave and K tile (8 rows x 128 bytes each)
+    static_assert(WM * WN == 4 && (BM + BN) % 32 == 0, "four waves");
+    int tm, tn;
+    tile_coords(p, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int li = lane & 31, hi = lane >> 5, wm = wave / WN, wn = wave % WN;
+    const unsigned lds_base = (unsigned)(uintptr_t)(LDS_AS char*)ad_smem;
+
+    const int nk = (int)((p.K + KT - 1) / KT), per = (nk + p.S - 1) / p.S;
+    const int kt0 = (int)blockIdx.y * per, kt1 = min(nk, kt0 + per);
+    const int tail = (int)(p.K * ES - (int64_t)(nk - 1) * ROWB);      // bytes of the last K tile
+
+    // unit j = wave + 4 i: rows 8 j + (lane >> 3) of the stage (x rows, then W rows), physical chunk lane & 7
+    const char* src[NU];
+    int lc16[NU];
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const int j = wave + 4 * i, r = j * 8 + (lane >> 3);
+        const bool isx = j * 8 < BM;
+        const int rr = isx ? r : r - BM;
+        const int64_t row = isx ? min(m0 + rr, p.M - 1) : min(n0 + rr, p.N - 1);
+        lc16[i] = (((lane & 7) ^ ((rr >> 1) & 7)) << 4);
+        src[i] = (isx ? (const char*)p.A + row * p.lda * ES : (const char*)p.W + row * p.ldw * ES) + lc16[i];
+    }
+    auto stage = [&](int kt) {
+        const unsigned dst = __builtin_amdgcn_readfirstlane(lds_base + (unsigned)((kt - kt0) % NST) * Sh::STAGE + wave * 1024);
+        const bool last = kt == nk - 1 && tail < ROWB;
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const char* s = src[i] + (int64_t)kt * ROWB;
+            if (last && lc16[i] >= tail) s = (const char*)zero_page;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst + i * 4096), "v"(s) : "memory", "m0");
+        }
+    };
+    f32x16 acc[NI][MI];
+#pragma unroll
+    for (int a = 0; a < NI; ++a)
+#pragma unroll
+        for (int b = 0; b < MI; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+    auto compute = [&](int kt) {
+        const char* sA = ad_smem + ((kt - kt0) % NST) * Sh::STAGE;
+        const char* sW = sA + BM * ROWB;
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+            frag_t fa[MI], fw[NI];
+            const int c0 = (kk * 16 + hi * 8) * ES / 16;
+            auto rd = [&](const char* s, int row) {
+                if constexpr (ES == 2) return *reinterpret_cast<const frag_t*>(s + lds_off(row, c0));
+                else {
+                    const f32x4 lo = *reinterpret_cast<const f32x4*>(s + lds_off(row, c0)), h4 = *reinterpret_cast<const f32x4*>(s + lds_off(row, c0 + 1));
+                    return (frag_t)__builtin_shufflevector(lo, h4, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < MI; ++i) fa[i] = rd(sA, (wm * MI + i) * 32 + li);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) fw[i] = rd(sW, (wn * NI + i) * 32 + li);
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi) mma32(fw[ni], fa[mi], acc[ni][mi]);
+        }
+    };
+    // tile kt is complete when at most the NU loads of each younger tile in flight are pending (loads return in order); the barrier behind
+    // that wait also says that every wave has read tile kt - 1 (lgkmcnt), whose stage the next request overwrites
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i)
+        if (kt0 + i < kt1) stage(kt0 + i);
+    for (int kt = kt0; kt < kt1; ++kt) {
+        const int younger = kt1 - 1 - kt;
+        if (younger >= NST - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"((NST - 2) * NU) : "memory");
+        else if (NST == 4 && younger == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(NU) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (kt + NST - 1 < kt1) stage(kt + NST - 1);
+        compute(kt);
+    }
+    adapters_extend<T, NI, MI>(p, acc, tm, m0 + wm * MI * 32, n0 + wn * NI * 32, lane, (int)blockIdx.y, p.S);
+
+    // out of the accumulator layout (lane = row) through LDS: 4 consecutive columns per lane, whole rows per group of lanes
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    constexpr int NCH = NI * 8;                              // 16-byte chunks of a row of the wave's columns
+    char* wl = ad_smem + wave * 32 * NCH * 16;
+    static_assert(4 * 32 * NCH * 16 <= Sh::LDS, "the epilogue's block fits");
+    const T* bias = (const T*)p.bias;
+    const int ch = lane % NCH;
+    const int64_t n = n0 + wn * NI * 32 + ch * 4;
+    f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+    if (p.S == 1 && bias && n < p.N) bv = load4(bias + n);
+    float* part = p.S > 1 ? p.ws + (int64_t)blockIdx.y * p.M * p.N : nullptr;
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+#pragma unroll
+        for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+            for (int rq = 0; rq < 4; ++rq) {
+                const int c = ni * 8 + rq * 2 + hi;
+                const f32x4 v = {acc[ni][mi][rq * 4], acc[ni][mi][rq * 4 + 1], acc[ni][mi][rq * 4 + 2], acc[ni][mi][rq * 4 + 3]};
+                *reinterpret_cast<f32x4*>(wl + li * NCH * 16 + ((c ^ (li & (NCH - 1))) << 4)) = v;
+            }
+        // (wave-private region: program order and the compiler's lgkmcnt waits order the reads behind the writes)
+#pragma unroll
+        for (int it = 0; it < NCH / 2; ++it) {
+            const int r = it * (64 / NCH) + lane / NCH;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(wl + r * NCH * 16 + ((ch ^ (r & (NCH - 1))) << 4));
+            const int64_t m = m0 + (wm * MI + mi) * 32 + r;
+            if (m < p.M && n < p.N) {
+                if (part) store4(part + m * p.N + n, v);
+                else store4((T*)p.out + m * p.ldc + n, v + bv);
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_gemm_join_kernel(AdGemmArgs p) {
+    const int64_t n4 = p.N / 4, total = p.M * n4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / n4, n = (i - m * n4) * 4;
+        f32x4 v = load4(p.ws + m * p.N + n);
+        for (int s = 1; s < p.S; ++s) v += load4(p.ws + ((int64_t)s * p.M + m) * p.N + n);
+        if (p.bias) v += load4((const T*)p.bias + n);
+        store4((T*)p.out + m * p.ldc + n, v);
+    }
+}
+
+// D += A(16 x 32) * B(32 x 16): lane = (i = l & 15, q = l >> 4) holds the 8 consecutive k at 8 q of row i; D: column l & 15, rows 4 q + [0, 4)
+M4D_DEV void mma16(const bf16x8& a, const bf16x8& b, f32x4& c) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+M4D_DEV void mma16(const f32x8& a, const f32x8& b, f32x4& c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+}
+
+// 8 consecutive elements of a row at k, those at or beyond K as zero (rows are whole 16-byte chunks)
+template <typename T> M4D_DEV typename Frag8<T>::type load_k8(const T* row, int k, int K);
+template <> M4D_DEV bf16x8 load_k8<bf16_t>(const bf16_t* row, int k, int K) {
+    bf16x8 v = {};
+    if (k < K) v = *reinterpret_cast<const bf16x8*>(row + k);
+    return v;
+}
+template <> M4D_DEV f32x8 load_k8<float>(const float* row, int k, int K) {
+    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+    if (k < K) a = load4(row + k);
+    if (k + 4 < K) b = load4(row + k + 4);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Up to 16 rows (single tokens, modulation vectors): one pass over W, which is all the traffic there is.  A workgroup owns 16 rows of W, its
+// eight waves take 256 bytes of them each in turn straight into registers (every byte is used once: LDS would only add a trip); the adapters
+// of the batch are dealt to the waves like further K steps, and the waves' sums meet in LDS in wave order.
+constexpr int SKINNY_WAVES = 8;
+template <typename T>
+__global__ __launch_bounds__(64 * SKINNY_WAVES) void adapter_gemv_kernel(AdGemmArgs p) {
+    typedef typename Frag8<T>::type frag_t;
+    __shared__ f32x4 red[SKINNY_WAVES][64];
+    constexpr int U = 4, KS = 32 * U;               // K elements of a wave's step
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, i16 = lane & 15, q = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const T* w = (const T*)p.W + min(n0 + i16, p.N - 1) * p.ldw + q * 8;
+    const int row = min(i16, (int)p.M - 1);         // (lanes beyond the last row compute copies of it and store nothing)
+    const T* x = (const T*)p.A + row * p.lda + q * 8;
+    const int K = (int)p.K;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    int k0 = wave * KS;
+    for (; k0 + KS <= K; k0 += SKINNY_WAVES * KS) {
+        frag_t fw[U], fx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) fw[u] = *reinterpret_cast<const frag_t*>(w + k0 + u * 32);
+#pragma unroll
+        for (int u = 0; u < U; ++u) fx[u] = *reinterpret_cast<const frag_t*>(x + k0 + u * 32);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mma16(fw[u], fx[u], acc);
+    }
+    for (int u = 0; u < U && k0 + u * 32 < K; ++u) {      // the last, partial step of one wave
+        const int k = k0 + u * 32;
+        mma16(load_k8<T>(w, k, K - q * 8), load_k8<T>(x, k, K - q * 8), acc);
+    }
+    const int ra = p.row_adapter[row];
+    for (int i = wave; i < p.tile_off[1]; i += SKINNY_WAVES) {      // (at most 16 rows: one tile)
+        const int g = p.tile_list[i];
+        const T* b = (const T*)p.up + ((int64_t)g * p.N + min(n0 + i16, p.N - 1)) * p.R;
+        const T* u = (const T*)p.u + (int64_t)row * p.R;
+        for (int k = 0; k < p.R; k += 32) {
+            const int kq = k + q * 8, ks = min(kq, p.R - 8);
+            const frag_t fb = *reinterpret_cast<const frag_t*>(b + ks);
+            frag_t fu = *reinterpret_cast<const frag_t*>(u + ks);
+            if (ra != g || kq >= p.R) fu = frag_t{};
+            mma16(fb, fu, acc);
+        }
+    }
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+        const int64_t n = n0 + q * 4;
+        if (i16 < p.M && n < p.N) {
+            f32x4 v = red[0][lane];
+#pragma unroll
+            for (int k = 1; k < SKINNY_WAVES; ++k) v += red[k][lane];
+            if (p.bias) v += load4((const T*)p.bias + n);
+            store4((T*)p.out + (int64_t)i16 * p.ldc + n, v);
+        }
+    }
+}
+
+}  // namespace

@@ -34,8 +34,8 @@ namespace {
 constexpr int BM = 128, BN = 128;
 constexpr int STAGE_BYTES = (BM + BN) * ROWB;  // 32 KiB
 
-template <typename T, bool AD = false>
-__global__ __launch_bounds__(256, 2) void gemm_bt_kernel(std::conditional_t<AD, GemmAdArgs, GemmArgs> p) {
+template <typename T>
+__global__ __launch_bounds__(256, 2) void gemm_bt_kernel(GemmArgs p) {
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE_BYTES];
     constexpr int ES = sizeof(T);
     constexpr int KT = ROWB / ES;        // K elements per tile
@@ -138,7 +138,6 @@ __global__ __launch_bounds__(256, 2) void gemm_bt_kernel(std::conditional_t<AD, 
         if (kt + 1 < nk) swrite((kt + 1) & 1);
         __syncthreads();
     }
-    if constexpr (AD) adapters_extend<T, 2, 2>(p, acc, tm, m0 + wm * 64, n0 + wn * 64, lane);
 
     const T* bias = (const T*)p.bias;
 #pragma unroll
@@ -777,11 +776,4 @@ extern "C" int m4d_gemm_bt_taps(m4d_dtype dt, const void* A, int64_t lda, int64_
     M4D_CHECK_LAUNCH("gemm_bt_taps");
     m4d_count_launch(M4D_KC_GEMM_WIDE);
     return 0;
-}
-
-// the 128 x 128 kernel with the adapters' extension (adapters.hip; GemmAdArgs handed over as an opaque pointer)
-extern "C" __attribute__((visibility("hidden"))) void m4d_launch_gemm_generic_adapters(const void* args, int bf16, unsigned nwg, hipStream_t st) {
-    const GemmAdArgs& p = *(const GemmAdArgs*)args;
-    if (bf16) hipLaunchKernelGGL((gemm_bt_kernel<bf16_t, true>), dim3(nwg), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((gemm_bt_kernel<float, true>), dim3(nwg), dim3(256), 0, st, p);
 }

@@ -151,15 +151,18 @@ M4D_DEV void epilogue_tile(const GemmArgs& p, const f32x16& acc, int64_t m, int6
 }
 
 // The adapters' part of a wave's NI x MI accumulator blocks (32 x 32 each; rows m_base + 32 mi + lane, columns n_base + 32 ni + lane of W):
-// acc += up_g[n, :] . u[m, :] over the rank, for each adapter g of the tile.  The operands come straight from L2 in the MFMA layout (16 bytes
-// per lane and 16 ranks): at rank 64 they are 1 - 2 % of the bytes of the K loop, and through LDS they would need two more barriers.  Rows
-// of u that name another adapter (or none: their u was never written) are replaced by zero before the product, not multiplied by zero.
+// acc += up_g[n, :] . u[m, :] over the rank, for every step-th adapter of the tile from `first` on.  The operands come straight from L2 in the
+// MFMA layout (16 bytes per lane and 16 ranks; a block's 32 rows of R ranks are contiguous memory): through LDS they would need two more
+// barriers.  All loads of 64 ranks are issued before their first product, so a tile pays one L2 latency per 64 ranks and adapter, not four.
+// Rows of u that name another adapter (or none: their u was never written) are replaced by zero before the product, not multiplied by zero.
 template <typename T, int NI, int MI>
-M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], int tile, int64_t m_base, int64_t n_base, int lane) {
+M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], int tile, int64_t m_base, int64_t n_base, int lane, int first = 0,
+                             int step = 1) {
     typedef typename Frag8<T>::type frag_t;
+    constexpr int U = sizeof(T) == 2 ? 4 : 1;         // 16-rank steps in flight (float32 fragments are twice as wide, and MFMA-bound)
     const int li = lane & 31, hi = lane >> 5;
-    const int i0 = __builtin_amdgcn_readfirstlane(p.tile_off[tile]), i1 = __builtin_amdgcn_readfirstlane(p.tile_off[tile + 1]);
-    if (i0 == i1) return;
+    const int i0 = __builtin_amdgcn_readfirstlane(p.tile_off[tile]) + first, i1 = __builtin_amdgcn_readfirstlane(p.tile_off[tile + 1]);
+    if (i0 >= i1) return;
     int ra[MI];
     const T* pu[MI];
 #pragma unroll
@@ -168,33 +171,34 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], int til
         ra[mi] = m < p.M ? p.row_adapter[m] : -1;
         pu[mi] = (const T*)p.u + (m < p.M ? m : 0) * p.R + hi * 8;
     }
-    bool in[NI];
-    int64_t nr[NI];
+    int64_t nr[NI];                                   // (columns beyond N are computed from row N - 1 and not stored)
 #pragma unroll
-    for (int ni = 0; ni < NI; ++ni) {
-        const int64_t n = n_base + ni * 32 + li;
-        in[ni] = n < p.N;
-        nr[ni] = in[ni] ? n : 0;
-    }
-    for (int i = i0; i < i1; ++i) {
+    for (int ni = 0; ni < NI; ++ni) nr[ni] = min(n_base + ni * 32 + li, p.N - 1) * p.R + hi * 8;
+    for (int i = i0; i < i1; i += step) {
         const int g = __builtin_amdgcn_readfirstlane(p.tile_list[i]);
-        const T* b = (const T*)p.up + (int64_t)g * p.N * p.R + hi * 8;
-        for (int k = 0; k < p.R; k += 16) {
-            frag_t fu[MI], fb[NI];
+        const T* b = (const T*)p.up + (int64_t)g * p.N * p.R;
+        for (int k = 0; k < p.R; k += 16 * U) {
+            frag_t fu[U][MI], fb[U][NI];
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi) {
-                fu[mi] = frag_t{};
-                if (ra[mi] == g) fu[mi] = *reinterpret_cast<const frag_t*>(pu[mi] + k);
+            for (int s = 0; s < U; ++s) {
+                // (loads without predicates: what a row or a rank beyond R must not contribute is replaced after the load)
+                const int ks = min(k + s * 16, p.R - 16);
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi) fu[s][mi] = *reinterpret_cast<const frag_t*>(pu[mi] + ks);
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni) fb[s][ni] = *reinterpret_cast<const frag_t*>(b + nr[ni] + ks);
             }
 #pragma unroll
-            for (int ni = 0; ni < NI; ++ni) {
-                fb[ni] = frag_t{};
-                if (in[ni]) fb[ni] = *reinterpret_cast<const frag_t*>(b + nr[ni] * p.R + k);
-            }
+            for (int s = 0; s < U; ++s)
 #pragma unroll
-            for (int ni = 0; ni < NI; ++ni)
+                for (int mi = 0; mi < MI; ++mi)
+                    if (ra[mi] != g || k + s * 16 >= p.R) fu[s][mi] = frag_t{};
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi) mma32(fb[ni], fu[mi], acc[ni][mi]);
+            for (int s = 0; s < U; ++s)
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                    for (int mi = 0; mi < MI; ++mi) mma32(fb[s][ni], fu[s][mi], acc[ni][mi]);
         }
     }
 }

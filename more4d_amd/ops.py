@@ -1,5 +1,6 @@
 """Tensor-level wrappers over the C ABI (include/more4d_hip.h).  torch supplies device memory and the
 current HIP stream; every arithmetic op below runs in a hand-written gfx950 kernel.  No fallback."""
+import contextlib
 import math
 import os
 
@@ -1060,13 +1061,17 @@ def adamw_(p, g, m, v, *, lr, beta1, beta2, eps, weight_decay, step, grad_scale=
 
 
 # ------------------------------------------------------------------ activations kept in 8 bits
+_NO_GUARD = contextlib.nullcontext()
+
+
 def _same_device(name, *ts):
     """All tensors on one HIP device; returns a guard that makes it current (its current stream is the one launched on)."""
     _dev(*ts)
-    d = {t.device for t in ts if t is not None}
-    if len(d) != 1:
-        raise ValueError(f"{name}: tensors on different devices {sorted(map(str, d))}")
-    return torch.cuda.device(d.pop())
+    d = ts[0].device
+    for t in ts:
+        if t is not None and t.device != d:
+            raise ValueError(f"{name}: tensors on different devices {d} and {t.device}")
+    return _NO_GUARD if d.index == torch.cuda.current_device() else torch.cuda.device(d)
 
 
 class Act8:
@@ -1089,6 +1094,14 @@ class Act8:
         return self.codes.numel() + self.exps.numel()
 
 
+def _new_act8(x):
+    C = x.shape[-1]
+    nb = (C + 31) // 32
+    rows = x.numel() // C
+    buf = torch.empty(rows * nb * 33, device=x.device, dtype=torch.uint8)
+    return Act8(buf[:rows * nb * 32].view(torch.int8).view(rows, nb * 32), buf[rows * nb * 32:].view(rows, nb), x.shape, x.dtype)
+
+
 def act_quant8(x, *, out=None):
     """x [..., C] (float32 / bfloat16; leading dims collapse onto one row stride) -> Act8.  out: an Act8 of the same shape to overwrite."""
     if x.dim() < 1 or x.shape[-1] == 0:
@@ -1096,10 +1109,8 @@ def act_quant8(x, *, out=None):
     dt_code(x.dtype)
     C = x.shape[-1]
     rows, ld = (0, C) if x.numel() == 0 else _rows2d(x)
-    nb = (C + 31) // 32
     if out is None:
-        out = Act8(torch.empty((rows, 32 * nb), device=x.device, dtype=torch.int8), torch.empty((rows, nb), device=x.device, dtype=torch.uint8),
-                   x.shape, x.dtype)
+        out = _new_act8(x)
     elif not isinstance(out, Act8) or out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("act_quant8: out must be an Act8 of x's shape and dtype")
     with _same_device("act_quant8", x, out.codes):
@@ -1160,47 +1171,62 @@ def act_bwd8(dy, a8, act, *, out=None):
 
 # ------------------------------------------------------------------ low-rank adapters of many requests beside a shared projection
 class AdapterBank:
-    """The adapters of one projection: a [G, r, K], b [G, N, r] (one dtype), scale: G numbers or a float32 tensor [G].  Laid out once: the rank
-    is padded with zeros to a multiple of 16 (adapters of different ranks: pad the smaller ones with zeros)."""
-    __slots__ = ("a", "b", "scale", "rank", "R")
+    """The adapters of one projection: a [G, r, K], b [G, N, r] (one dtype, contiguous), scale: G numbers or a float32 tensor [G] (adapters of
+    different ranks: pad the smaller ones with zeros).  Laid out for the kernels once, here (m4d_adapter_pack): later changes of a and b are not
+    seen.  backward=True lays out the transposed operands of the backward pass as well (`transposed`)."""
+    __slots__ = ("down", "up", "scale", "G", "rank", "R", "K", "N", "back")
 
-    def __init__(self, a, b, scale):
+    def __init__(self, a, b, scale, *, backward=False):
         if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
             raise ValueError(f"AdapterBank: a [G, r, K] and b [G, N, r] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
         G, r, K = a.shape
-        if not (G >= 1 and 1 <= r <= 512):
+        N = b.shape[1]
+        if not (G >= 1 and 1 <= r <= 512 and K >= 1 and N >= 1):
             raise ValueError(f"AdapterBank: at least one adapter of rank 1..512, got {G} of rank {r}")
         if a.dtype != b.dtype:
             raise TypeError(f"AdapterBank: a {a.dtype} vs b {b.dtype}")
-        dt_code(a.dtype)
-        _dev(a, b)
-        a, b = a.detach(), b.detach()
+        dt = dt_code(a.dtype)
         if not isinstance(scale, torch.Tensor):
             scale = torch.tensor([float(s) for s in scale], dtype=torch.float32)
         if scale.numel() != G:
             raise ValueError(f"AdapterBank: {scale.numel()} scales for {G} adapters")
-        self.rank, self.R = r, -(-r // 16) * 16
-        pad = self.R - r
-        self.a = (torch.nn.functional.pad(a, (0, 0, 0, pad)) if pad else a).contiguous()
-        self.b = (torch.nn.functional.pad(b, (0, pad)) if pad else b).contiguous()
-        self.scale = scale.to(device=a.device, dtype=torch.float32).contiguous()
+        _dev(a, b)
+        a, b = a.detach().contiguous(), b.detach().contiguous()
+        self.G, self.rank, self.R, self.K, self.N = G, r, -(-r // 16) * 16, K, N
+        if scale.device != a.device or scale.dtype != torch.float32 or not scale.is_contiguous():
+            scale = scale.to(device=a.device, dtype=torch.float32).contiguous()
+        self.scale = scale
+        lib = _lib.load()
+        n = [lib.m4d_adapter_down_elems(G, self.R, K), G * N * self.R]
+        if backward:
+            n += [lib.m4d_adapter_down_elems(G, self.R, N), G * K * self.R]
+        at = [0]
+        for v in n:
+            at.append(at[-1] + -(-v // 64) * 64)
+        buf = torch.empty(at[-1], device=a.device, dtype=a.dtype)
+        parts = [buf[o:o + v] for o, v in zip(at, n)]
+        self.down, self.up = parts[0], parts[1].view(G, N, self.R)
+        self.back = None
+        if backward:
+            self.back = AdapterBank.__new__(AdapterBank)
+            self.back.down, self.back.up, self.back.scale, self.back.back = parts[2], parts[3].view(G, K, self.R), scale, None
+            self.back.G, self.back.rank, self.back.R, self.back.K, self.back.N = G, r, self.R, N, K
+        with _same_device("AdapterBank", a, b):
+            check(lib.m4d_adapter_pack(dt, _ptr(a), _ptr(b), G, r, K, N, self.R, _ptr(self.down), _ptr(self.up),
+                                       _ptr(parts[2]) if backward else 0, _ptr(parts[3]) if backward else 0, _stream()), "m4d_adapter_pack")
 
-    def transposed(self, n_pad=None):
-        """The bank of the backward pass: v = s dy B, dx = ... + v A — b^T [G, R, N] in the place of a (N zero-padded to n_pad, for a dy whose rows
-        are padded to 16 bytes), a^T [G, K, R] in the place of b."""
-        t = AdapterBank.__new__(AdapterBank)
-        t.a, t.b = self.b.transpose(1, 2).contiguous(), self.a.transpose(1, 2).contiguous()
-        if n_pad is not None and n_pad != t.a.shape[2]:
-            t.a = torch.nn.functional.pad(t.a, (0, n_pad - t.a.shape[2]))
-        t.scale, t.rank, t.R = self.scale, self.rank, self.R
-        return t
+    def transposed(self):
+        """The bank of the backward pass, v = s dy B and dx = dy W + v A: the down projection maps N channels, the up projection gives K."""
+        if self.back is None:
+            raise ValueError("AdapterBank: built without backward=True")
+        return self.back
 
 
 class AdapterPlan:
     """Which adapter each row of a batch uses: request j owns the next lengths[j] rows (0 allowed) and names adapter adapters[j] (-1: none).
     Host numbers; the tables (include/more4d_hip.h: m4d_adapter_plan) are built here and copied to `device` once per batch composition, then
     shared by every projection of the model."""
-    PIECE = 64
+    PIECE, CHUNK_PIECES = 64, 64
 
     def __init__(self, lengths, adapters, device):
         import numpy as np
@@ -1216,37 +1242,38 @@ class AdapterPlan:
         row = np.repeat(np.array(adapters, dtype=np.int32), np.array(lengths, dtype=np.int64))
         used = [int(g) for g in np.unique(row) if g >= 0]
         self.n_adapters = used[-1] + 1 if used else 0
-        slots, pieces, counts = [], [], []
+        slots, pieces, count = [], [], {}
         for g in used:
             r = np.nonzero(row == g)[0].astype(np.int32)
             n = -(-len(r) // P)
             slots.append(np.concatenate([r, np.full(n * P - len(r), -1, np.int32)]))
             pieces += [g] * n
-            counts.append(n)
+            count[g] = n
         self.n_pieces = len(pieces)
-        # the row contraction: about 24 chunks in all, so that a few hundred column tiles x chunks fill the chip and the partial sums stay small
-        per = max(1, -(-self.n_pieces // 24))
-        chunks, chunk_off, p0 = [], [0], 0
-        it = dict(zip(used, counts))
-        for g in range(self.n_adapters):
-            n = it.get(g, 0)
-            for q in range(0, n, per):
-                chunks += [p0 + q, p0 + min(q + per, n), g]
-            p0 += n
-            chunk_off.append(len(chunks) // 3)
-        self.n_chunks = len(chunks) // 3
 
-        def tiles(T, shifted):
+        def chunks(target):                     # about `target` chunks in all, none beyond CHUNK_PIECES pieces, none of two adapters
+            per = min(self.CHUNK_PIECES, max(1, -(-self.n_pieces // target)))
+            lst, off, p0 = [], [0], 0
+            for g in range(self.n_adapters):
+                n = count.get(g, 0)
+                for q in range(0, n, per):
+                    lst += [p0 + q, p0 + min(q + per, n), g]
+                p0 += n
+                off.append(len(lst) // 3)
+            return lst, off
+
+        def tiles(T, shifted=False):
             off, lst = [0], []
             for m in range(0, self.rows, T):
                 lo = max(0, min(m, self.rows - T)) if shifted else m
                 lst += [int(g) for g in np.unique(row[lo:m + T]) if g >= 0]
                 off.append(len(lst))
-            return off, lst
+            return lst, off
 
-        t256, l256 = tiles(256, True)
-        t128, l128 = tiles(128, False)
-        parts = [row, np.concatenate(slots) if slots else [], pieces, chunks, chunk_off, t256, l256, t128, l128]
+        cs = [chunks(t) for t in (12, 24, 48, 96)]
+        ts = [tiles(64), tiles(128), tiles(256), tiles(256, True)]
+        parts = [row, np.concatenate(slots) if slots else [], pieces]
+        parts += [c[0] for c in cs] + [c[1] for c in cs] + [t[1] for t in ts] + [t[0] for t in ts]
         parts = [np.asarray(v, dtype=np.int32) for v in parts]
         at, offs = 0, []
         for v in parts:
@@ -1256,20 +1283,25 @@ class AdapterPlan:
         for o, v in zip(offs, parts):
             host[o:o + len(v)] = v
         self.table = torch.from_numpy(host).to(device)
-        base = self.table.data_ptr()
-        self.args = _lib.AdapterPlanArgs(*[base + 4 * o for o in offs], self.rows, self.n_pieces, self.n_chunks, self.n_adapters, 0)
+        ptr = [self.table.data_ptr() + 4 * o for o in offs]
+        a = self.args = _lib.AdapterPlanArgs()
+        a.row_adapter, a.slot_row, a.piece_adapter = ptr[:3]
+        for k, name in enumerate(("chunks", "chunk_off", "tiles_off", "tiles")):
+            getattr(a, name)[:] = ptr[3 + 4 * k:7 + 4 * k]
+        a.rows, a.n_pieces, a.n_adapters = self.rows, self.n_pieces, self.n_adapters
+        a.n_chunks[:] = [len(c[0]) // 3 for c in cs]
 
 
 def _check_adapters(name, x, bank, plan):
     rows, ldx = _rows2d(x)
     if rows != plan.rows:
         raise ValueError(f"{name}: {rows} rows against a plan of {plan.rows}")
-    if plan.n_adapters > bank.a.shape[0]:
-        raise ValueError(f"{name}: the plan names adapter {plan.n_adapters - 1}, the bank has {bank.a.shape[0]}")
-    if bank.a.dtype != x.dtype:
-        raise TypeError(f"{name}: x {x.dtype} vs adapters {bank.a.dtype}")
-    if bank.a.shape[2] != x.shape[-1]:
-        raise ValueError(f"{name}: x has {x.shape[-1]} channels, the adapters {bank.a.shape[2]}")
+    if plan.n_adapters > bank.G:
+        raise ValueError(f"{name}: the plan names adapter {plan.n_adapters - 1}, the bank has {bank.G}")
+    if bank.up.dtype != x.dtype:
+        raise TypeError(f"{name}: x {x.dtype} vs adapters {bank.up.dtype}")
+    if -(-bank.K // 8) * 8 < x.shape[-1] or bank.K > x.shape[-1]:       # (rows may be zero-padded to whole 16-byte chunks)
+        raise ValueError(f"{name}: x has {x.shape[-1]} channels, the adapters {bank.K}")
     return rows, ldx
 
 
@@ -1279,52 +1311,59 @@ def adapter_down(x, bank, plan, *, rows=True, slots=False):
     M, ldx = _check_adapters("adapter_down", x, bank, plan)
     u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype) if rows else None
     ut = torch.empty((bank.R, plan.n_pieces * plan.PIECE), device=x.device, dtype=x.dtype) if slots else None
-    with _same_device("adapter_down", x, bank.a, plan.table):
-        check(_lib.load().m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, _ptr(bank.a), _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut),
+    with _same_device("adapter_down", x, bank.up, plan.table):
+        check(_lib.load().m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, _ptr(bank.down), _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut), 0, 0,
                                            x.shape[-1], bank.R, _stream()), "m4d_adapter_down")
     return u, ut
 
 
-def linear_adapters(x, w, bias, bank, plan, *, out=None, u=None):
+def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=False):
     """x w^T + bias + s_g (x A_g^T) B_g^T, g the adapter of each row (plan).  x [..., K] (rows strided), w [N, K] (row-strided), bias [N] or None,
-    bank: AdapterBank, out [..., N].  u: the result of `adapter_down(x, bank, plan)` if it is at hand."""
+    bank: AdapterBank, out [..., N].  For a backward pass: slots=True returns (out, u^T), u^T = (s x A^T)^T for `adapter_grad`; keep8=True
+    returns (out, u^T, Act8 of x) — the 8-bit form of the rows that name an adapter, written in the pass that reads x (the codes of other
+    rows are undefined; no gradient of an adapter reads them)."""
     K, N = x.shape[-1], w.shape[0]
     if w.dim() != 2 or w.shape[1] != K:
         raise ValueError(f"linear_adapters: w {tuple(w.shape)} for x with {K} channels")
     if w.dtype != x.dtype:
         raise TypeError(f"linear_adapters: x {x.dtype} vs w {w.dtype}")
-    if bank.b.shape[1] != N:
-        raise ValueError(f"linear_adapters: w has {N} rows, the adapters {bank.b.shape[1]}")
+    if bank.N != N:
+        raise ValueError(f"linear_adapters: w has {N} rows, the adapters {bank.N}")
     if bias is not None and (bias.dtype != x.dtype or bias.numel() != N or not bias.is_contiguous()):
         raise ValueError("linear_adapters: bias must be contiguous, of x's dtype, with N elements")
     if out is None:
         out = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
     elif out.dtype != x.dtype or out.shape != (*x.shape[:-1], N):
         raise ValueError(f"linear_adapters: out must be {(*x.shape[:-1], N)} of x's dtype")
+    ut = torch.empty((bank.R, plan.n_pieces * plan.PIECE), device=x.device, dtype=x.dtype) if slots or keep8 else None
+    x8 = _new_act8(x) if keep8 else None
+    ret = (out, ut, x8) if keep8 else (out, ut) if slots else out
     if x.numel() == 0:
         if plan.rows:
             raise ValueError(f"linear_adapters: no rows against a plan of {plan.rows}")
-        return out
+        return ret
     M, ldx = _check_adapters("linear_adapters", x, bank, plan)
     if plan.n_pieces == 0:                  # nobody names an adapter: the shared projection alone
         gemm_bt(x, w, bias, out=out)
-        return out
+        return ret
     _, ldw = _rows2d(w)
     _, ldo = _rows2d(out)
-    if u is None:
-        u, _ = adapter_down(x, bank, plan)
-    elif u.shape != (M, bank.R) or u.dtype != x.dtype or not u.is_contiguous():
-        raise ValueError("linear_adapters: u must be contiguous [rows, R] of x's dtype")
-    with _same_device("linear_adapters", x, w, bias, out, u, bank.b, plan.table):
-        check(_lib.load().m4d_linear_adapters(dt_code(x.dtype), _ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(u), _ptr(bank.b), plan.args,
-                                              _ptr(out), ldo, N, K, bank.R, _stream()), "m4d_linear_adapters")
-    return out
+    dt = dt_code(x.dtype)
+    lib = _lib.load()
+    with _same_device("linear_adapters", x, w, bias, out, bank.up, plan.table):
+        u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype)
+        nws = lib.m4d_linear_adapters_workspace(dt, M, N, K)
+        ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
+        check(lib.m4d_linear_adapters(dt, _ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(bank.down), _ptr(bank.scale), _ptr(bank.up), plan.args,
+                                      _ptr(u), _ptr(ut), _ptr(x8.codes) if keep8 else 0, _ptr(x8.exps) if keep8 else 0, _ptr(out), ldo, N, K,
+                                      bank.R, _ptr(ws), nws, _stream()), "m4d_linear_adapters")
+    return ret
 
 
 def adapter_grad(vt, x, plan, bank, *, transposed=False):
     """Gradient of the adapters: sum over the rows of each adapter of v^T x, as [G, rank, C] (transposed: [G, C, rank]) in vt's dtype; adapters that
-    no row names get zero.  vt: the [R, slots] result of `adapter_down`; x [rows, C], or its Act8."""
-    G, rank, R = bank.a.shape[0], bank.rank, bank.R
+    no row names get zero.  vt: the [R, slots] result of `adapter_down` / `linear_adapters`; x [rows, C], or its Act8."""
+    G, rank, R = bank.G, bank.rank, bank.R
     x8 = x if isinstance(x, Act8) else None
     C = x.shape[-1]
     if plan.n_adapters > G:
@@ -1336,13 +1375,14 @@ def adapter_grad(vt, x, plan, bank, *, transposed=False):
         raise ValueError(f"adapter_grad: {rows} rows against a plan of {plan.rows}")
     if x8 is None and x.dtype != vt.dtype:
         raise TypeError(f"adapter_grad: x {x.dtype} vs v {vt.dtype}")
+    dt = dt_code(vt.dtype)
     out = torch.empty((G, C, rank) if transposed else (G, rank, C), device=vt.device, dtype=vt.dtype)
     if plan.n_pieces == 0:
         return out.zero_()
     with _same_device("adapter_grad", vt, x8.codes if x8 is not None else x, plan.table):
         lib = _lib.load()
         ws = torch.empty(lib.m4d_adapter_grad_workspace(plan.args, C, R), device=vt.device, dtype=torch.float32)
-        check(lib.m4d_adapter_grad(dt_code(vt.dtype), _ptr(vt), 0 if x8 is not None else _ptr(x), ldx, _ptr(x8.codes) if x8 is not None else 0,
+        check(lib.m4d_adapter_grad(dt, _ptr(vt), 0 if x8 is not None else _ptr(x), ldx, _ptr(x8.codes) if x8 is not None else 0,
                                    _ptr(x8.exps) if x8 is not None else 0, plan.args, _ptr(ws), ws.numel(), _ptr(out), int(transposed), G, rank, C,
                                    R, _stream()), "m4d_adapter_grad")
     return out

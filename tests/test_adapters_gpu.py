@@ -66,7 +66,14 @@ FORWARD = [
     ([1] * 600, [i % 5 - 1 for i in range(600)], 128, 520, 16, BF),      # every row another request, adapters interleaved
     ([513], [0], 64, 512, 130, BF),
     ([520], [-1], 64, 512, 16, BF),                             # nobody names an adapter
+    ([16], [0], 40, 20, 100, BF),
+    ([7, 9], [1, 0], 4096, 96, 16, BF),                         # at most 16 rows, several steps per wave, a ragged last one
+    ([17, 1], [0, 1], 1000, 200, 16, BF),                       # K in slices
+    ([100], [0], 2056, 260, 16, BF),
+    ([400, 100], [0, 1], 72, 1540, 16, BF),
     ([1], [0], 4, 4, 1, F32),
+    ([9], [0], 516, 36, 5, F32),
+    ([150], [0], 1028, 132, 16, F32),
     ([5, 0, 60, 70], [1, 0, 0, -1], 132, 68, 7, F32),
     ([300, 290], [0, 1], 100, 260, 40, F32),
 ]
@@ -135,6 +142,7 @@ BACKWARD = [
     ([1, 1, 0], [1, 0, 2], 72, 36, 3, BF),
     ([65, 1, 130], [0, -1, 1], 136, 196, 16, BF),
     ([700, 1, 260], [1, 0, 1], 256, 512, 24, BF),
+    ([200, 1100], [-1, 0], 712, 200, 200, BF),
     ([1] * 130, [i % 4 - 1 for i in range(130)], 96, 64, 8, BF),
     ([530], [0], 512, 576, 96, BF),
     ([2000], [0], 128, 64, 16, BF),
@@ -290,18 +298,46 @@ def test_streams_and_graph_replay(M):
         buf = torch.zeros_like(v)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            u, ut = o.adapter_down(buf, bank, plan, slots=True)
-            y = o.linear_adapters(buf, w, bias, bank, plan, u=u)
-            ga = o.adapter_grad(ut, buf, plan, bank)
+            y, ut, b8 = o.linear_adapters(buf, w, bias, bank, plan, keep8=True)
+            ga = o.adapter_grad(ut, b8, plan, bank)
         graphs.append((g, buf, y, ga))
     for i in range(4):
         for k, (g, buf, y, ga) in enumerate(graphs):
             v = xs[(i + k) % 2]
             buf.copy_(v)
             g.replay()
-            eager = o.adapter_grad(o.adapter_down(v, bank, plan, slots=True)[1], v, plan, bank)
+            eager = o.adapter_grad(o.adapter_down(v, bank, plan, slots=True)[1], o.act_quant8(v), plan, bank)
             torch.cuda.synchronize()
             assert torch.equal(y, want[(i + k) % 2]) and torch.equal(ga, eager)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("K", [8, 40, 64, 200, 712])
+def test_the_pass_that_reads_x_writes_the_same_codes(K, dt):
+    """linear_adapters(keep8=True) against act_quant8 on the rows that name an adapter, infinities and NaN among them."""
+    o = ops()
+    lengths, ids = [70, 3, 150, 33], [1, -1, 0, 1]
+    x, w, bias, a, b, scale, row = problem(lengths, ids, K, 64, 8, dt)
+    x = x * torch.exp(3 * torch.randn(1, K, generator=torch.Generator().manual_seed(4))).to(dt)
+    x[5, 3], x[100, 7], x[101, 0] = float("inf"), float("nan"), 3e38
+    xd = x.to(DEV)
+    plan, bank = o.AdapterPlan(lengths, ids, DEV), o.AdapterBank(a.to(DEV), b.to(DEV), scale)
+    y, ut, x8 = o.linear_adapters(xd, w.to(DEV), bias.to(DEV), bank, plan, keep8=True)
+    ref = o.act_quant8(xd)
+    on = (row >= 0).to(DEV)
+    assert torch.equal(x8.codes[on], ref.codes[on]) and torch.equal(x8.exps[on], ref.exps[on])
+    y2, ut2 = o.linear_adapters(xd, w.to(DEV), bias.to(DEV), bank, plan, slots=True)
+    assert torch.equal(y.nan_to_num(0), y2.nan_to_num(0)) and torch.equal(ut.nan_to_num(0), ut2.nan_to_num(0))
+    u, ut3 = o.adapter_down(xd, bank, plan, slots=True)
+    assert torch.equal(ut3.nan_to_num(0), ut.nan_to_num(0))
+    slot = torch.tensor(tables_slot_row(plan))
+    assert (ut.cpu()[:, slot < 0] == 0).all()
+    assert torch.equal(ut.cpu()[:, slot >= 0].t().nan_to_num(0), u.cpu()[slot[slot >= 0].long()].nan_to_num(0))
+
+
+def tables_slot_row(plan):
+    o = (plan.args.slot_row - plan.table.data_ptr()) // 4
+    return plan.table.cpu().tolist()[o:o + 64 * plan.n_pieces]
 
 
 def test_no_rows_and_refusals():
@@ -319,7 +355,7 @@ def test_no_rows_and_refusals():
                 lambda: o.linear_adapters(x, w[:, :32], bias, bank, plan), lambda: o.linear_adapters(x, w[:16], bias[:16], bank, plan),
                 lambda: o.linear_adapters(x, w, bias[:8], bank, plan), lambda: o.linear_adapters(x, w, bias, bank, o.AdapterPlan([8], [1], DEV)),
                 lambda: o.linear_adapters(x, w, bias, bank, plan, out=torch.empty(8, 16, device=DEV, dtype=BF)),
-                lambda: o.linear_adapters(x, w, bias, bank, plan, u=torch.empty(8, 4, device=DEV, dtype=BF)),
+                lambda: bank.transposed(),
                 lambda: o.AdapterBank(a, b[:, :, :2], scale), lambda: o.AdapterBank(a, b, [1.0, 2.0]),
                 lambda: AdapterLinearFn.apply(x, w, bias, a, b, scale, plan, 4),
                 lambda: AdapterLinearFn.apply(x, w.clone().requires_grad_(True), bias, a, b, scale, plan, 8)):

@@ -33,29 +33,32 @@ def test_plan_tables_cover_every_row_once(seed):
         own = slots[64 * q:64 * q + 64]
         assert own[0] >= 0 and all(rows[s] == g for s in own if s >= 0)
         assert all(s >= 0 for s in own) or q == p.n_pieces - 1 or pieces[q + 1] != g       # only an adapter's last piece is padded
-    off = at(a.chunk_off, p.n_adapters + 1)
-    ch = at(a.chunks, 3 * p.n_chunks)
-    assert off[0] == 0 and off[-1] == p.n_chunks and p.n_adapters == max([i for i in rows], default=-1) + 1
-    covered = []
-    for g in range(p.n_adapters):
-        for c in range(off[g], off[g + 1]):
-            assert ch[3 * c + 2] == g and ch[3 * c] < ch[3 * c + 1]
-            covered += range(ch[3 * c], ch[3 * c + 1])
-            assert all(pieces[q] == g for q in range(ch[3 * c], ch[3 * c + 1]))
-    assert covered == list(range(p.n_pieces))
-    for T, o_, l_ in ((256, a.tiles256_off, a.tiles256), (128, a.tiles128_off, a.tiles128)):
+    assert p.n_adapters == max(rows, default=-1) + 1
+    for level in range(4):
+        n = a.n_chunks[level]
+        off = at(a.chunk_off[level], p.n_adapters + 1)
+        ch = at(a.chunks[level], 3 * n)
+        assert off[0] == 0 and off[-1] == n
+        covered = []
+        for g in range(p.n_adapters):
+            for c in range(off[g], off[g + 1]):
+                assert ch[3 * c + 2] == g and 0 < ch[3 * c + 1] - ch[3 * c] <= 64
+                covered += range(ch[3 * c], ch[3 * c + 1])
+                assert all(pieces[q] == g for q in range(ch[3 * c], ch[3 * c + 1]))
+        assert covered == list(range(p.n_pieces))
+    for k, T in enumerate((64, 128, 256, 256)):
         nt = -(-p.rows // T)
-        off = at(o_, nt + 1)
-        lst = at(l_, off[-1])
+        off = at(a.tiles_off[k], nt + 1)
+        lst = at(a.tiles[k], off[-1])
         for i in range(nt):
-            lo = max(0, min(i * T, p.rows - T)) if T == 256 else i * T
+            lo = max(0, min(i * T, p.rows - T)) if k == 3 else i * T
             assert lst[off[i]:off[i + 1]] == sorted({g for g in rows[lo:i * T + T] if g >= 0})
 
 
 def test_plan_of_nothing():
     for lengths, ids in (([], []), ([0], [3]), ([5], [-1])):
         p = ops.AdapterPlan(lengths, ids, "cpu")
-        assert p.n_pieces == p.n_chunks == p.n_adapters == 0 and p.rows == sum(lengths)
+        assert p.n_pieces == p.n_adapters == 0 and list(p.args.n_chunks) == [0] * 4 and p.rows == sum(lengths)
 
 
 def test_plan_refusals():
