@@ -522,7 +522,8 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
  *   tiles_off[i], tiles[i]       the adapters of the rows of each tile, each once, for tiles of 64, 128 and 256 rows and (i = 3) of 256 rows
  *                                whose last one is rows [rows - 256, rows)
  *   adapter_down     u T [rows, R] and / or ut T [R, 64 * n_pieces] = s_g x A_g^T (rows without an adapter are not written, pad slots are zero);
- *                    codes / exps (may be NULL): the 8-bit form of x's rows with an adapter, as act_quant8 writes it
+ *                    codes / exps (may be NULL): the 8-bit form of x's rows with an adapter, as act_quant8 writes it;
+ *                    ws: adapter_down_workspace floats
  *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once.  With a_down, u (and ut, codes, exps if given) are written first, by
  *                    adapter_down; without, u is an input.  ws: linear_adapters_workspace floats
  *   adapter_grad     out T [G, rank, C] (transposed: [G, C, rank]) = sum over the rows of g of v^T x, v given as vt T [R, 64 * n_pieces], x as T or as
@@ -535,9 +536,10 @@ typedef struct {
 int64_t m4d_adapter_down_elems(int G, int R, int64_t K);
 int m4d_adapter_pack(m4d_dtype dt, const void* a, const void* b, int G, int rank, int64_t K, int64_t N, int R, void* a_down, void* b_up, void* b_down,
                      void* a_up, m4d_stream stream);
+int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int64_t K, int R);
 int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan, void* u, void* ut,
-                     int8_t* codes, uint8_t* exps, int64_t K, int R, m4d_stream stream);
-int64_t m4d_linear_adapters_workspace(m4d_dtype dt, int64_t M, int64_t N, int64_t K);
+                     int8_t* codes, uint8_t* exps, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream);
+int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R);
 int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* a_down, const float* scale,
                         const void* b_up, const m4d_adapter_plan* plan, void* u, void* ut, int8_t* codes, uint8_t* exps, void* out, int64_t ldo,
                         int64_t N, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream);

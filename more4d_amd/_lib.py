@@ -151,9 +151,10 @@ SIGNATURES = {
     "m4d_act_bwd8": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
     "m4d_adapter_down_elems": (c_int64, [c_int, c_int, c_int64]),
     "m4d_adapter_pack": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int] + [c_void_p] * 5),
+    "m4d_adapter_down_workspace": (c_int64, [POINTER(AdapterPlanArgs), c_int64, c_int]),
     "m4d_adapter_down": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, POINTER(AdapterPlanArgs)] + [c_void_p] * 4 +
-                         [c_int64, c_int, c_void_p]),
-    "m4d_linear_adapters_workspace": (c_int64, [c_int, c_int64, c_int64, c_int64]),
+                         [c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "m4d_linear_adapters_workspace": (c_int64, [c_int, POINTER(AdapterPlanArgs), c_int64, c_int64, c_int]),
     "m4d_linear_adapters": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                     POINTER(AdapterPlanArgs)] + [c_void_p] * 5 + [c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
     "m4d_adapter_grad_workspace": (c_int64, [POINTER(AdapterPlanArgs), c_int64, c_int]),

@@ -99,18 +99,14 @@ class AdapterLinearFn(Function):
             y, ut = ops.linear_adapters(x2, weight.detach(), bias, bank, plan, slots=True)
         else:
             y = ops.linear_adapters(x2, weight.detach(), bias, bank, plan)
-        if need_a:
-            kept = (kept.codes, kept.exps) if bits == 8 else (x2, None)
-        else:
-            kept = (None, None)
-        ctx.save_for_backward(*kept, weight, ut if need_b else None)
-        ctx.meta = (bank, plan, x.shape, x.dtype)       # (the bank is this call's own copy of a and b, laid out for both passes)
+        ctx.save_for_backward((kept.buf if bits == 8 else x2) if need_a else None, weight, ut if need_b else None)
+        ctx.meta = (bank, plan, bits, x.shape, x.dtype)       # (the bank is this call's own copy of a and b, laid out for both passes)
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     def backward(ctx, dy):
-        kept, exps, weight, ut = ctx.saved_tensors
-        bank, plan, xshape, xdt = ctx.meta
+        kept, weight, ut = ctx.saved_tensors
+        bank, plan, bits, xshape, xdt = ctx.meta
         N, K = weight.shape
         need_x, need_a, need_b = (ctx.needs_input_grad[i] for i in (0, 3, 4))
         dy2 = dy.reshape(-1, N)
@@ -134,7 +130,7 @@ class AdapterLinearFn(Function):
         elif need_a:
             vt = ops.adapter_down(dy2, back, plan, rows=False, slots=True)[1]
         if need_a:
-            da = ops.adapter_grad(vt, ops.Act8(kept, exps, (kept.shape[0], K), xdt) if exps is not None else kept, plan, bank)
+            da = ops.adapter_grad(vt, ops.Act8((dy2.shape[0], K), xdt, buf=kept) if bits == 8 else kept, plan, bank)
         if need_b:
             db = ops.adapter_grad(ut, dy2[:, :N], plan, bank, transposed=True)
         return dx, None, None, da, db, None, None, None

@@ -74,7 +74,22 @@ struct DownArgs {
     const int *slot_row, *piece_adapter;
     int64_t ldx, n_slots;
     int K, R, n_pieces;
+    int KS;                // K slices (gridDim.y); > 1: unscaled float32 sums to part [KS, n_pieces, R, 64]
+    float* part;
 };
+
+// four ranks of one slot to u and / or ut, scaled
+template <typename T>
+M4D_DEV void down_store(const DownArgs& p, int64_t piece, int g, int slot, int row, int r, f32x4 v) {
+    const float sc = p.scale[g];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= sc;
+    if (p.u && row >= 0) store4((T*)p.u + (int64_t)row * p.R + r, v);
+    if (p.ut) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ((T*)p.ut)[(r + e) * p.n_slots + piece * PIECE + slot] = (T)(row >= 0 ? v[e] : 0.f);
+    }
+}
 
 // a row's 32-channel block in its lane's four fragments -> codes and exponent byte
 template <typename T>
@@ -100,9 +115,11 @@ M4D_DEV void quant_block(const typename Frag8<T>::type (&x)[4], int8_t* codes, u
 }
 
 // u of one piece: 64 slots x RT * 32 ranks; K split over the workgroup's NW waves (64 channels each in turn), joined in LDS in wave order.
-// Rows are requested one chunk ahead of the products (they come from HBM), the packed operand right in front of them (from L2).
+// Loads return in order, so each chunk requests its packed operand (from L2) BEFORE the next chunk's rows (from HBM): the other way round the
+// products would wait for both, and nothing would be in flight ahead of them.  c0, c1: the chunks of this K slice.
 template <typename T, int RT, int NW, int NS, bool QUANT>
-M4D_DEV void down_loop(const DownArgs& p, int g, int rt0, int wave, int lane, const int (&row)[2], const int (&rowc)[2], f32x16 (&acc)[RT][2]) {
+M4D_DEV void down_loop(const DownArgs& p, int g, int rt0, int wave, int lane, const int (&row)[2], const int (&rowc)[2], int c0, int c1,
+                       f32x16 (&acc)[RT][2]) {
     typedef typename Frag8<T>::type frag_t;
     const int hi = lane >> 5, nc = (p.K + 63) >> 6, rts = (p.R + 31) >> 5, nb = (p.K + 31) >> 5;
     const T* px[NS];
@@ -124,12 +141,15 @@ M4D_DEV void down_loop(const DownArgs& p, int g, int rt0, int wave, int lane, co
                 for (int kk = 0; kk < 4; ++kk) x[s][kk] = load_k8<T>(px[s], c * 64 + kk * 8, p.K - hi * 32);
         }
     };
-    auto use = [&](int c, frag_t (&x)[NS][4]) {
+    auto step = [&](int c, frag_t (&x)[NS][4], frag_t (&next)[NS][4]) {
         frag_t a[RT][4];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) a[rt][kk] = *reinterpret_cast<const frag_t*>(pa[rt] + (int64_t)c * rts * 2048 + kk * 512);
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + NW < c1) load(c + NW, next);
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (QUANT) {
             const int blk = c * 2 + hi;
 #pragma unroll
@@ -144,15 +164,13 @@ M4D_DEV void down_loop(const DownArgs& p, int g, int rt0, int wave, int lane, co
                 for (int s = 0; s < NS; ++s) mma32(a[rt][kk], x[s][kk], acc[rt][s]);
     };
     frag_t x0[NS][4], x1[NS][4];
-    int c = wave;
-    if (c < nc) load(c, x0);
-    while (c < nc) {
-        if (c + NW < nc) load(c + NW, x1);
-        use(c, x0);
+    int c = c0 + wave;
+    if (c < c1) load(c, x0);
+    while (c < c1) {
+        step(c, x0, x1);
         c += NW;
-        if (c >= nc) break;
-        if (c + NW < nc) load(c + NW, x0);
-        use(c, x1);
+        if (c >= c1) break;
+        step(c, x1, x0);
         c += NW;
     }
 }
@@ -183,14 +201,14 @@ __global__ __launch_bounds__(64 * NW, 2) void adapter_down_kernel(DownArgs p) {
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[rt][s][q] = 0.f;
+    const int nc = (p.K + 63) >> 6, per = (nc + p.KS - 1) / p.KS, c0 = (int)blockIdx.y * per, c1 = min(nc, c0 + per);
     if (QUANT && rt0 == 0) {
-        if (two) down_loop<T, RT, NW, 2, QUANT>(p, g, rt0, wave, lane, row, rowc, acc);
-        else down_loop<T, RT, NW, 1, QUANT>(p, g, rt0, wave, lane, row, rowc, acc);
+        if (two) down_loop<T, RT, NW, 2, QUANT>(p, g, rt0, wave, lane, row, rowc, c0, c1, acc);
+        else down_loop<T, RT, NW, 1, QUANT>(p, g, rt0, wave, lane, row, rowc, c0, c1, acc);
     } else {
-        if (two) down_loop<T, RT, NW, 2, false>(p, g, rt0, wave, lane, row, rowc, acc);
-        else down_loop<T, RT, NW, 1, false>(p, g, rt0, wave, lane, row, rowc, acc);
+        if (two) down_loop<T, RT, NW, 2, false>(p, g, rt0, wave, lane, row, rowc, c0, c1, acc);
+        else down_loop<T, RT, NW, 1, false>(p, g, rt0, wave, lane, row, rowc, c0, c1, acc);
     }
-    const float sc = p.scale[g];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if (rt) __syncthreads();
@@ -208,16 +226,27 @@ __global__ __launch_bounds__(64 * NW, 2) void adapter_down_kernel(DownArgs p) {
             for (int w = 0; w < NW; ++w)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] += red[((w * 2 + s) * 16 + q4 * 4 + e) * 64 + l];
+            const int slot = s * 32 + (l & 31);
+            if (p.part) {
+                float* d = p.part + (((int64_t)blockIdx.y * p.n_pieces + piece) * p.R + r) * PIECE + slot;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= sc;
-            const int slot = s * 32 + (l & 31), rw = sr[slot];
-            if (p.u && rw >= 0) store4((T*)p.u + (int64_t)rw * p.R + r, v);
-            if (p.ut) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) ((T*)p.ut)[(r + e) * p.n_slots + (int64_t)piece * PIECE + slot] = (T)(rw >= 0 ? v[e] : 0.f);
-            }
+                for (int e = 0; e < 4; ++e) d[e * PIECE] = v[e];
+            } else down_store<T>(p, piece, g, slot, sr[slot], r, v);
         }
     }
+}
+
+// the K slices' sums of four ranks of one slot, in slice order
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_down_join_kernel(DownArgs p) {
+    const int t = threadIdx.x, slot = t & 63, r = (blockIdx.y * 4 + (t >> 6)) * 4;
+    const int64_t piece = blockIdx.x;
+    if (r >= p.R) return;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < p.KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += p.part[((k * p.n_pieces + piece) * p.R + r + e) * PIECE + slot];
+    down_store<T>(p, piece, p.piece_adapter[piece], slot, p.slot_row[piece * PIECE + slot], r, v);
 }
 
 // ---------------------------------------------------------------- contraction over the rows
@@ -353,34 +382,38 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
     }
 }
 
-// out[g] = sum of the partial products of g's chunks, in chunk order (no atomics: the same bits every time); 16 ranks x 64 columns a workgroup
+// out[g] = sum of the partial products of g's chunks, in chunk order (no atomics: the same bits every time); 16 ranks x 16 columns a workgroup,
+// one output a thread: at one adapter of rank 16 and 1536 channels that is still 96 workgroups
 template <typename T>
 __global__ __launch_bounds__(256) void adapter_grad_join_kernel(GradArgs p) {
-    __shared__ float tile[64][17];
-    const int t = threadIdx.x, cl = t & 63, c = blockIdx.x * 64 + cl, r0 = blockIdx.y * 16, g = blockIdx.z;
+    const int t = threadIdx.x, g = blockIdx.z;
+    // partial sums are read along the columns; a transposed output is written along the ranks
+    const int cl = t & 15, rl = t >> 4;
+    const int c = blockIdx.x * 16 + cl, r = blockIdx.y * 16 + rl;
     const int i0 = g < p.n_adapters ? p.chunk_off[g] : 0, i1 = g < p.n_adapters ? p.chunk_off[g + 1] : 0;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < p.C)
-        for (int i = i0; i < i1; ++i)
+    float v = 0.f;
+    if (c < p.C) {
+        const float* w = p.ws + (int64_t)r * p.C + c;
+        const int64_t st = (int64_t)p.R * p.C;
+        int i = i0;
+        for (; i + 8 <= i1; i += 8) {
+            float b[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] += p.ws[((int64_t)i * p.R + r0 + j * 4 + (t >> 6)) * p.C + c];
-    if (!p.transposed) {
+            for (int k = 0; k < 8; ++k) b[k] = w[(i + k) * st];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = r0 + j * 4 + (t >> 6);
-            if (c < p.C && r < p.rank) ((T*)p.out)[((int64_t)g * p.rank + r) * p.C + c] = (T)v[j];
+            for (int k = 0; k < 8; ++k) v += b[k];
         }
+        for (; i < i1; ++i) v += w[i * st];
+    }
+    if (!p.transposed) {
+        if (c < p.C && r < p.rank) ((T*)p.out)[((int64_t)g * p.rank + r) * p.C + c] = (T)v;
         return;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) tile[cl][j * 4 + (t >> 6)] = v[j];
+    __shared__ float tile[16][17];
+    tile[cl][rl] = v;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int k = j * 256 + t, cc = k >> 4, r = k & 15;
-        if (blockIdx.x * 64 + cc < (unsigned)p.C && r0 + r < p.rank)
-            ((T*)p.out)[((int64_t)g * p.C + blockIdx.x * 64 + cc) * p.rank + r0 + r] = (T)tile[cc][r];
-    }
+    const int c2 = blockIdx.x * 16 + rl, r2 = blockIdx.y * 16 + cl;
+    if (c2 < p.C && r2 < p.rank) ((T*)p.out)[((int64_t)g * p.C + c2) * p.rank + r2] = (T)tile[rl][cl];
 }
 
 bool dt_ok(int dt) { return dt == M4D_BF16 || dt == M4D_F32; }
@@ -401,19 +434,45 @@ int cus() {
 enum { GEMV16 = 0, TILE_64x64, TILE_64x128, TILE_128x128, TILE_256x128, WIDE_256x256 };
 struct Choice { int kind, S; };
 
+// Which kernel, and into how many slices of K: the least estimated time.  A CU runs its workgroups in rounds; a round costs a fixed part (filling
+// the ring, epilogue) and c per 128-byte K tile.  c is what the tile moves from L2 at the 60 - 80 bytes/ns that a CU gets (fp32: the MFMA
+// rate), so larger tiles are cheaper per product and smaller ones waste less of a round; slices pay for writing and joining float32 partial
+// tiles.  Measured c (us, bf16 / fp32): 64 x 64 0.30 / 0.70 alone on a CU and 0.42 / 1.25 as one of two, 64 x 128 0.36 / 1.16, 128 x 128
+// 0.55 / 2.1, 256 x 128 0.92 / 4.0, 256 x 256 (gemm_wide.h) 1.03.  Measured against each other at 40 shapes (M 2 .. 21840): the choice is within
+// 10 % of the best of all kinds and slices, e.g. 64 x 5120 x 4096: 64 x 64 in 3 slices 14.3 us, whole 21.7, 128 x 128 whole 36; 986 x 5120 x
+// 4096: 256 x 128 65 us, 128 x 128 75, 256 x 256 72.
 Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, int ncu) {
 #ifdef M4D_ABLATIONS
     { const char* v = getenv("M4D_ADAPTER_GEMM"); if (v) { const int c = atoi(v); if (c / 100 != WIDE_256x256 || wide_ok) return Choice{c / 100, c % 100 ? c % 100 : 1}; } }
 #endif
-    if (M <= 16) return Choice{GEMV16, 1};
-    if (wide_ok && M * N >= (int64_t)ncu * 65536 / 2) return Choice{WIDE_256x256, 1};
-    const int nk = (int)((K * (bf16 ? 2 : 4) + ROWB - 1) / ROWB);
-    const int kind = M <= 64 ? TILE_64x128 : TILE_128x128;
-    const int bm = M <= 64 ? 64 : 128;
-    const int64_t tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
-    int S = 1;
-    while (S < 8 && tiles * S * 2 <= ncu && nk / (S * 2) >= 4) S *= 2;
-    return Choice{kind, S};
+    const double es = bf16 ? 2 : 4, wbytes = (double)N * K * es;
+    const int64_t nk = (int64_t)((K * es + ROWB - 1) / ROWB);
+    Choice best{TILE_64x64, 1};
+    double t_best = 1e30;
+    auto offer = [&](double t, int kind, int S) { if (t < t_best) { t_best = t; best = Choice{kind, S}; } };
+    if (M <= 16) offer(4.0 + wbytes * (1.0 + M / 16.0) / 5.0e6, GEMV16, 1);
+    if (wide_ok) {
+        const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
+        offer((double)((tiles + ncu - 1) / ncu) * (nk * 1.03 + 10.0), WIDE_256x256, 1);
+    }
+    static const struct { int kind, bm, bn, occ; double c[2][2], fix; } cfg[4] = {
+        {TILE_64x64, 64, 64, 2, {{0.30, 0.42}, {0.70, 1.25}}, 4.0}, {TILE_64x128, 64, 128, 1, {{0.36, 0.36}, {1.16, 1.16}}, 4.0},
+        {TILE_128x128, 128, 128, 1, {{0.55, 0.55}, {2.1, 2.1}}, 5.0}, {TILE_256x128, 256, 128, 1, {{0.92, 0.92}, {4.0, 4.0}}, 7.0}};
+    for (const auto& f : cfg) {
+        const int64_t tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
+        for (int S = 1; S <= 16; ++S) {
+            const int64_t per = (nk + S - 1) / S;
+            if (S > 1 && (per < 4 || (nk + per - 1) / per != S || tiles * S > 4 * ncu || (double)S * M * N > 6.4e7)) continue;      // (at most 256 MB of slices)
+            const int64_t blocks = tiles * S, rounds = (blocks + (int64_t)ncu * f.occ - 1) / ((int64_t)ncu * f.occ);
+            const int shared = blocks > ncu && f.occ > 1;
+            double t = rounds * (per * f.c[bf16 ? 0 : 1][shared] + f.fix);
+            const double floor = wbytes / 6.0e6;
+            if (t < floor) t = floor;
+            if (S > 1) t += 3.0 + (double)M * N * (8.0 * S + es) / 4.5e6;
+            offer(t, f.kind, S);
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -444,7 +503,7 @@ extern "C" int m4d_adapter_pack(m4d_dtype dt, const void* a, const void* b, int 
 }
 
 template <typename T, int RT, int NW, bool QUANT>
-static int launch_down(const DownArgs& p, int n_pieces, hipStream_t st) {
+static int launch_down(const DownArgs& p, hipStream_t st) {
     constexpr int LDS = NW * 8192;
     static PerDeviceOnce configured;
     if (configured.pending()) {
@@ -456,31 +515,56 @@ static int launch_down(const DownArgs& p, int n_pieces, hipStream_t st) {
         configured.mark();
     }
     const int ny = ((p.R + 31) / 32 + RT - 1) / RT;
-    hipLaunchKernelGGL((adapter_down_kernel<T, RT, NW, QUANT>), dim3((unsigned)((n_pieces + 7) / 8 * 8 * ny)), dim3(64 * NW), LDS, st, p);
+    hipLaunchKernelGGL((adapter_down_kernel<T, RT, NW, QUANT>), dim3((unsigned)((p.n_pieces + 7) / 8 * 8 * ny), (unsigned)p.KS), dim3(64 * NW), LDS, st, p);
     M4D_CHECK_LAUNCH("adapter_down");
+    if (p.part) {
+        hipLaunchKernelGGL(adapter_down_join_kernel<T>, dim3((unsigned)p.n_pieces, (unsigned)((p.R + 15) / 16)), dim3(256), 0, st, p);
+        M4D_CHECK_LAUNCH("adapter_down(join)");
+    }
     return 0;
 }
 template <typename T, int RT>
-static int launch_down_nw(const DownArgs& p, int n_pieces, hipStream_t st) {
-    // few pieces: more waves on each (their K loops are serial trips to memory); many: four, so that all pieces of a long batch are resident
-    if (n_pieces < cus() / 2) return p.codes ? launch_down<T, RT, 8, true>(p, n_pieces, st) : launch_down<T, RT, 8, false>(p, n_pieces, st);
-    return p.codes ? launch_down<T, RT, 4, true>(p, n_pieces, st) : launch_down<T, RT, 4, false>(p, n_pieces, st);
+static int launch_down_nw(const DownArgs& p, hipStream_t st) {
+    // four waves where the pieces fill the chip (all of a long batch resident), eight where a workgroup has a CU to itself
+    if (p.n_pieces * p.KS < cus()) return p.codes ? launch_down<T, RT, 8, true>(p, st) : launch_down<T, RT, 8, false>(p, st);
+    return p.codes ? launch_down<T, RT, 4, true>(p, st) : launch_down<T, RT, 4, false>(p, st);
+}
+
+// K slices of a down projection with few pieces: as many as fill half the chip, each at least one chunk of 64 channels per wave.  (A piece's K
+// loop is serial: 16 pieces of K = 4096 took 20 us on 16 CUs.)
+static int down_slices(int n_pieces, int64_t K) {
+    const int nc = (int)((K + 63) / 64);
+    int ks = n_pieces > 0 ? cus() / 2 / n_pieces : 1;
+    if (ks > (nc + 7) / 8) ks = (nc + 7) / 8;
+    if (ks < 2) return 1;
+    const int per = (nc + ks - 1) / ks;
+    return (nc + per - 1) / per;                 // (no empty slices)
+}
+
+extern "C" int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int64_t K, int R) {
+    if (!plan || K <= 0 || R <= 0) return 0;
+    const int ks = down_slices(plan->n_pieces, K);
+    return ks > 1 ? (int64_t)ks * plan->n_pieces * R * PIECE : 0;
 }
 
 extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan,
-                                void* u, void* ut, int8_t* codes, uint8_t* exps, int64_t K, int R, m4d_stream stream) {
+                                void* u, void* ut, int8_t* codes, uint8_t* exps, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream) {
     PLAN_OK("adapter_down");
     M4D_CHECK_ARG(x && a_down && scale && (u || ut) && (codes == nullptr) == (exps == nullptr), "adapter_down: null pointer");
     M4D_CHECK_ARG(K > 0 && K < (1 << 30) && (K * es) % 16 == 0 && (ldx * es) % 16 == 0 && (plan->rows == 1 || ldx >= K),
                   "adapter_down: rows of K=%lld elements (row stride %lld) must be multiples of 16 bytes", (long long)K, (long long)ldx);
-    M4D_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)a_down % 16) == 0 && ((uintptr_t)u % 16) == 0 && ((uintptr_t)ut % 16) == 0 && ((uintptr_t)codes % 16) == 0,
-                  "adapter_down: pointers must be 16-byte aligned");
+    M4D_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)a_down % 16) == 0 && ((uintptr_t)u % 16) == 0 && ((uintptr_t)ut % 16) == 0 &&
+                  ((uintptr_t)codes % 16) == 0 && ((uintptr_t)ws % 16) == 0, "adapter_down: pointers must be 16-byte aligned");
     if (plan->n_pieces == 0) return 0;
     M4D_CHECK_ARG(plan->slot_row && plan->piece_adapter, "adapter_down: bad plan");
-    DownArgs p{x, a_down, scale, u, ut, codes, exps, plan->slot_row, plan->piece_adapter, ldx, (int64_t)plan->n_pieces * PIECE, (int)K, R, plan->n_pieces};
+    const int ks = down_slices(plan->n_pieces, K);
+    M4D_CHECK_ARG(ks == 1 || (ws && ws_floats >= (int64_t)ks * plan->n_pieces * R * PIECE), "adapter_down: workspace of %lld floats needed",
+                  (long long)ks * plan->n_pieces * R * PIECE);
+    DownArgs p{x, a_down, scale, u, ut, codes, exps, plan->slot_row, plan->piece_adapter, ldx, (int64_t)plan->n_pieces * PIECE, (int)K, R,
+               plan->n_pieces, ks, ks > 1 ? ws : nullptr};
     hipStream_t st = (hipStream_t)stream;
-    if (dt == M4D_BF16) return R <= 32 ? launch_down_nw<bf16_t, 1>(p, plan->n_pieces, st) : launch_down_nw<bf16_t, 2>(p, plan->n_pieces, st);
-    return launch_down_nw<float, 1>(p, plan->n_pieces, st);
+    if (dt == M4D_BF16) return R <= 32 ? launch_down_nw<bf16_t, 1>(p, st) : launch_down_nw<bf16_t, 2>(p, st);
+    return launch_down_nw<float, 1>(p, st);
 }
 
 template <typename T, int MI, int NI, int WM, int WN>
@@ -498,7 +582,7 @@ static int launch_gemm(AdGemmArgs& p, hipStream_t st) {
     const int64_t tm = (p.M + Sh::BM - 1) / Sh::BM, tn = (p.N + Sh::BN - 1) / Sh::BN;
     M4D_CHECK_ARG(tm * tn < (1ll << 31), "linear_adapters: too many tiles");
     p.tiles_m = (int)tm; p.tiles_n = (int)tn;
-    hipLaunchKernelGGL((adapter_gemm_kernel<T, MI, NI, WM, WN>), dim3((unsigned)(tm * tn), (unsigned)p.S), dim3(256), Sh::LDS, st, p);
+    hipLaunchKernelGGL((adapter_gemm_kernel<T, MI, NI, WM, WN>), dim3((unsigned)(tm * tn), (unsigned)p.S), dim3(Sh::THREADS), Sh::LDS, st, p);
     M4D_CHECK_LAUNCH("linear_adapters");
     if (p.S > 1) {
         const int64_t nblk = (p.M * (p.N / 4) + 255) / 256;
@@ -510,9 +594,11 @@ static int launch_gemm(AdGemmArgs& p, hipStream_t st) {
 
 static bool wide_shape(m4d_dtype dt, int64_t M, int64_t N, int64_t K) { return dt == M4D_BF16 && K % 64 == 0 && M >= 512 && N >= 512; }
 
-extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
-    int64_t most = 0;                    // (whether the wide kernel can run depends on the output's alignment too: room for either choice)
+// the down projection's slices and the GEMM's run one after the other: one workspace, the larger of the two
+extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R) {
+    if (!plan || plan->rows <= 0 || N <= 0 || K <= 0) return 0;
+    const int64_t M = plan->rows;
+    int64_t most = m4d_adapter_down_workspace(plan, K, R);      // (whether the wide kernel can run depends on the output's alignment too: room for either choice)
     for (int w = 0; w < 2; ++w) {
         const Choice c = choose(dt == M4D_BF16, M, N, K, w && wide_shape(dt, M, N, K), cus());
         if (c.S > 1 && c.S * M * N > most) most = c.S * M * N;
@@ -540,7 +626,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
     const Choice c = choose(bf16, M, N, K, wide_ok, cus());
     M4D_CHECK_ARG(c.S == 1 || (ws && ws_floats >= c.S * M * N && ((uintptr_t)ws % 16) == 0), "linear_adapters: workspace of %lld floats needed", (long long)(c.S * M * N));
     if (a_down) {
-        const int rc = m4d_adapter_down(dt, x, ldx, a_down, scale, plan, u, ut, codes, exps, K, R, stream);
+        const int rc = m4d_adapter_down(dt, x, ldx, a_down, scale, plan, u, ut, codes, exps, K, R, ws, ws_floats, stream);
         if (rc != 0) return rc;
     }
     AdGemmArgs p{};
@@ -561,9 +647,9 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
             return 0;
         }
         case TILE_64x64: return bf16 ? launch_gemm<bf16_t, 1, 1, 2, 2>(p, st) : launch_gemm<float, 1, 1, 2, 2>(p, st);
-        case TILE_64x128: return bf16 ? launch_gemm<bf16_t, 1, 2, 2, 2>(p, st) : launch_gemm<float, 1, 2, 2, 2>(p, st);
-        case TILE_128x128: return bf16 ? launch_gemm<bf16_t, 2, 2, 2, 2>(p, st) : launch_gemm<float, 2, 2, 2, 2>(p, st);
-        case TILE_256x128: return bf16 ? launch_gemm<bf16_t, 4, 2, 2, 2>(p, st) : launch_gemm<float, 4, 2, 2, 2>(p, st);
+        case TILE_64x128: return bf16 ? launch_gemm<bf16_t, 1, 1, 2, 4>(p, st) : launch_gemm<float, 1, 2, 2, 2>(p, st);
+        case TILE_128x128: return bf16 ? launch_gemm<bf16_t, 1, 2, 4, 2>(p, st) : launch_gemm<float, 2, 2, 2, 2>(p, st);
+        case TILE_256x128: return bf16 ? launch_gemm<bf16_t, 2, 2, 4, 2>(p, st) : launch_gemm<float, 4, 2, 2, 2>(p, st);
         default: break;
     }
     p.tile_off = plan->tiles_off[3]; p.tile_list = plan->tiles[3];
@@ -578,11 +664,11 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
     return 0;
 }
 
-// the coarsest chunks that still give two workgroups per CU (coarser: fewer partial sums to write and join)
+// the coarsest chunks that still give three workgroups for two CUs (two fit on one; coarser: fewer partial sums to write and join)
 static int chunk_level(const m4d_adapter_plan* plan, int64_t C, int R) {
     const int64_t blocks = ((C + 127) / 128) * (R <= 64 ? 1 : (R + 63) / 64);
     for (int l = 0; l < 3; ++l)
-        if (blocks * plan->n_chunks[l] >= 2 * cus()) return l;
+        if (2 * blocks * plan->n_chunks[l] >= 3 * cus()) return l;
     return 3;
 }
 
@@ -620,7 +706,7 @@ extern "C" int m4d_adapter_grad(m4d_dtype dt, const void* vt, const void* x, int
 #undef GRAD
         M4D_CHECK_LAUNCH("adapter_grad");
     }
-    dim3 jg((unsigned)((C + 63) / 64), (unsigned)((rank + 15) / 16), (unsigned)G);
+    dim3 jg((unsigned)((C + 15) / 16), (unsigned)((rank + 15) / 16), (unsigned)G);
     if (dt == M4D_BF16) hipLaunchKernelGGL(adapter_grad_join_kernel<bf16_t>, jg, dim3(256), 0, st, p);
     else hipLaunchKernelGGL(adapter_grad_join_kernel<float>, jg, dim3(256), 0, st, p);
     M4D_CHECK_LAUNCH("adapter_grad(join)");

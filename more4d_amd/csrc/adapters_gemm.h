@@ -1,9 +1,12 @@
 // adapter_gemm_kernel: the shared projection with its adapters for the sizes between one row and the 256 x 256 tiles of gemm_wide.h, bf16 and
 // float32.  out[m, n] = x W^T (+ bias) + u_g up_g^T for a BM x BN tile, BM = 32 MI WM, BN = 32 NI WN, four waves as WM x WN.
 //
-// What bounds these sizes is latency: a tile's K loop is serial, and with few tiles per CU nothing else hides a trip to memory.  So the K tiles
-// (128 bytes of a row) run through a ring of NST LDS stages filled by direct-to-LDS loads, NST - 1 tiles in flight, one barrier per tile; and
-// where the tiles do not fill the chip, K is cut into S slices (gridDim.y) whose float32 partial tiles a second kernel joins in slice order.
+// What bounds these sizes is latency: a tile's K loop is serial, and with one wave per SIMD nothing else hides a trip to memory.  So the K tiles
+// (128 bytes of a row) run through a ring of NST LDS stages filled by direct-to-LDS loads, NST - 1 tiles in flight; the fragments of the next
+// 16 channels are read while the MFMAs of these run, across the one barrier of a tile too; and the requests for the tile NST ahead are issued
+// one by one behind MFMAs.  (Reading a tile's fragments behind its barrier, all requests in front of it: 1.6 times the time at 512 x 5120 x
+// 4096.)  Where the tiles do not fill the chip, K is cut into S slices (gridDim.y) whose float32 partial tiles a second kernel joins in slice
+// order.
 // LDS image and swizzle are those of gemm.hip; rows beyond M and N are staged from the last row and not stored, 16-byte chunks beyond K are
 // staged from a page of zeros.
 #pragma once
@@ -22,17 +25,18 @@ struct AdGemmShape {
     static constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN;
     static constexpr int STAGE = (BM + BN) * ROWB;
     static constexpr int NST = STAGE * 4 <= 131072 ? 4 : 3;
+    static constexpr int THREADS = 64 * WM * WN;
     static constexpr int LDS = NST * STAGE;
 };
 
 template <typename T, int MI, int NI, int WM, int WN>
-__global__ __launch_bounds__(256) void adapter_gemm_kernel(AdGemmArgs p) {
+__global__ __launch_bounds__(64 * WM * WN) void adapter_gemm_kernel(AdGemmArgs p) {
     typedef AdGemmShape<T, MI, NI, WM, WN> Sh;
     typedef typename Frag8<T>::type frag_t;
     extern __shared__ __attribute__((aligned(16))) char ad_smem[];
     constexpr int ES = sizeof(T), KT = ROWB / ES, KSTEPS = KT / 16, NST = Sh::NST, BM = Sh::BM, BN = Sh::BN;
-    constexpr int NU = (BM + BN) / 32;                       // staging instructions per wave and K tile (8 rows x 128 bytes each)
-    static_assert(WM * WN == 4 && (BM + BN) % 32 == 0, "four waves");
+    constexpr int NW = WM * WN, NU = (BM + BN) / (8 * NW);      // staging instructions per wave and K tile (8 rows x 128 bytes each)
+    static_assert((BM + BN) % (8 * NW) == 0, "whole requests");
     int tm, tn;
     tile_coords(p, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
@@ -45,27 +49,32 @@ __global__ __launch_bounds__(256) void adapter_gemm_kernel(AdGemmArgs p) {
     const int kt0 = (int)blockIdx.y * per, kt1 = min(nk, kt0 + per);
     const int tail = (int)(p.K * ES - (int64_t)(nk - 1) * ROWB);      // bytes of the last K tile
 
-    // unit j = wave + 4 i: rows 8 j + (lane >> 3) of the stage (x rows, then W rows), physical chunk lane & 7
+    // unit j = wave + NW i: rows 8 j + (lane >> 3) of the stage (x rows, then W rows), physical chunk lane & 7
     const char* src[NU];
     int lc16[NU];
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-        const int j = wave + 4 * i, r = j * 8 + (lane >> 3);
+        const int j = wave + NW * i, r = j * 8 + (lane >> 3);
         const bool isx = j * 8 < BM;
         const int rr = isx ? r : r - BM;
         const int64_t row = isx ? min(m0 + rr, p.M - 1) : min(n0 + rr, p.N - 1);
         lc16[i] = (((lane & 7) ^ ((rr >> 1) & 7)) << 4);
         src[i] = (isx ? (const char*)p.A + row * p.lda * ES : (const char*)p.W + row * p.ldw * ES) + lc16[i];
     }
-    auto stage = [&](int kt) {
-        const unsigned dst = __builtin_amdgcn_readfirstlane(lds_base + (unsigned)((kt - kt0) % NST) * Sh::STAGE + wave * 1024);
-        const bool last = kt == nk - 1 && tail < ROWB;
-#pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            const char* s = src[i] + (int64_t)kt * ROWB;
-            if (last && lc16[i] >= tail) s = (const char*)zero_page;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst + i * 4096), "v"(s) : "memory", "m0");
-        }
+    // request i of K tile kt into its stage; chunks beyond the end of K come from the page of zeros
+    auto request = [&](int kt, unsigned dst, int i) {
+        const char* s = src[i] + (int64_t)kt * ROWB;
+        if (kt == nk - 1 && lc16[i] >= tail) s = (const char*)zero_page;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst + i * (NW * 1024)), "v"(s) : "memory", "m0");
+    };
+    auto stage_of = [&](int kt) { return (unsigned)((kt - kt0) % NST) * Sh::STAGE; };
+    auto dst_of = [&](int kt) { return __builtin_amdgcn_readfirstlane(lds_base + stage_of(kt) + wave * 1024); };
+    // all but the youngest n tiles' requests (n <= 3) have landed, of this wave; then of all, and nobody reads an older stage any more
+    auto arrive = [&](int n) {
+        if (n >= 3) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(3 * NU) : "memory");
+        else if (n == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(2 * NU) : "memory");
+        else if (n == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(NU) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
     f32x16 acc[NI][MI];
 #pragma unroll
@@ -74,42 +83,77 @@ __global__ __launch_bounds__(256) void adapter_gemm_kernel(AdGemmArgs p) {
         for (int b = 0; b < MI; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
-    auto compute = [&](int kt) {
-        const char* sA = ad_smem + ((kt - kt0) % NST) * Sh::STAGE;
+    frag_t fa[2][MI], fw[2][NI];
+    auto read = [&](unsigned stage, int kk, frag_t (&a)[MI], frag_t (&w)[NI]) {
+        const char* sA = ad_smem + stage;
         const char* sW = sA + BM * ROWB;
+        const int c0 = (kk * 16 + hi * 8) * ES / 16;
+        auto rd = [&](const char* s, int row) {
+            if constexpr (ES == 2) return *reinterpret_cast<const frag_t*>(s + lds_off(row, c0));
+            else {
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(s + lds_off(row, c0)), h4 = *reinterpret_cast<const f32x4*>(s + lds_off(row, c0 + 1));
+                return (frag_t)__builtin_shufflevector(lo, h4, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a[i] = rd(sA, (wm * MI + i) * 32 + li);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) w[i] = rd(sW, (wn * NI + i) * 32 + li);
+    };
+    // K tile kt, its first fragments in set 0.  MORE: requests tile kt - 1 + NST into the stage of tile kt - 1 (request i in phase i * KSTEPS / NU);
+    // NEXT: at the end tile kt + 1 has landed and its first fragments are in set 0.  NQ = requests issued before the last phase.
+    constexpr int NQ = (NU * (KSTEPS - 1) + KSTEPS - 1) / KSTEPS;
+    auto tile = [&](int kt, auto MORE_T, auto NEXT_T, int younger) {
+        constexpr bool MORE = decltype(MORE_T)::value, NEXT = decltype(NEXT_T)::value;
+        const unsigned cur = stage_of(kt), nxt = stage_of(kt + 1);
+        unsigned dst = 0;
+        if constexpr (MORE) dst = dst_of(kt - 1);
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk) {
-            frag_t fa[MI], fw[NI];
-            const int c0 = (kk * 16 + hi * 8) * ES / 16;
-            auto rd = [&](const char* s, int row) {
-                if constexpr (ES == 2) return *reinterpret_cast<const frag_t*>(s + lds_off(row, c0));
-                else {
-                    const f32x4 lo = *reinterpret_cast<const f32x4*>(s + lds_off(row, c0)), h4 = *reinterpret_cast<const f32x4*>(s + lds_off(row, c0 + 1));
-                    return (frag_t)__builtin_shufflevector(lo, h4, 0, 1, 2, 3, 4, 5, 6, 7);
+            constexpr int LASTK = KSTEPS - 1;
+            const int c = kk & 1;
+            if (kk < LASTK) read(cur, kk + 1, fa[c ^ 1], fw[c ^ 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            int q = (NU * kk + KSTEPS - 1) / KSTEPS;                 // the phase's first request (all constants after unrolling)
+            const int q1 = (NU * (kk + 1) + KSTEPS - 1) / KSTEPS;
+#pragma unroll
+            for (int m = 0; m < MI * NI; ++m) {
+                mma32(fw[c][m / MI], fa[c][m % MI], acc[m / MI][m % MI]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (m == 0 && kk == LASTK && NEXT) {
+                    if constexpr (MORE) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"((NST - 3) * NU + NQ) : "memory");
+                    else arrive(younger);
+                    read(nxt, 0, fa[c ^ 1], fw[c ^ 1]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            };
-#pragma unroll
-            for (int i = 0; i < MI; ++i) fa[i] = rd(sA, (wm * MI + i) * 32 + li);
-#pragma unroll
-            for (int i = 0; i < NI; ++i) fw[i] = rd(sW, (wn * NI + i) * 32 + li);
-#pragma unroll
-            for (int ni = 0; ni < NI; ++ni)
-#pragma unroll
-                for (int mi = 0; mi < MI; ++mi) mma32(fw[ni], fa[mi], acc[ni][mi]);
+                if constexpr (MORE) {
+                    if (q < q1) request(kt - 1 + NST, dst, q++);
+                    if (m == MI * NI - 1)
+                        while (q < q1) request(kt - 1 + NST, dst, q++);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
         }
     };
-    // tile kt is complete when at most the NU loads of each younger tile in flight are pending (loads return in order); the barrier behind
-    // that wait also says that every wave has read tile kt - 1 (lgkmcnt), whose stage the next request overwrites
+    const int n_tiles = kt1 - kt0;
+    if (n_tiles > 0) {
 #pragma unroll
-    for (int i = 0; i < NST - 1; ++i)
-        if (kt0 + i < kt1) stage(kt0 + i);
-    for (int kt = kt0; kt < kt1; ++kt) {
-        const int younger = kt1 - 1 - kt;
-        if (younger >= NST - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"((NST - 2) * NU) : "memory");
-        else if (NST == 4 && younger == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(NU) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (kt + NST - 1 < kt1) stage(kt + NST - 1);
-        compute(kt);
+        for (int s = 0; s < NST; ++s)
+            if (s < n_tiles) {
+                const unsigned dst = dst_of(kt0 + s);
+#pragma unroll
+                for (int i = 0; i < NU; ++i) request(kt0 + s, dst, i);
+            }
+        arrive(min(NST, n_tiles) - 1);
+        read(stage_of(kt0), 0, fa[0], fw[0]);
+        int kt = kt0;
+        if (n_tiles > 1) {
+            tile(kt, std::false_type{}, std::true_type{}, min(NST, n_tiles) - 2);
+            ++kt;
+        }
+        for (; kt - 1 + NST < kt1; ++kt) tile(kt, std::true_type{}, std::true_type{}, 0);
+        for (; kt < kt1 - 1; ++kt) tile(kt, std::false_type{}, std::true_type{}, kt1 - 2 - kt);
+        tile(kt, std::false_type{}, std::false_type{}, 0);
     }
     adapters_extend<T, NI, MI>(p, acc, tm, m0 + wm * MI * 32, n0 + wn * NI * 32, lane, (int)blockIdx.y, p.S);
 
@@ -117,7 +161,7 @@ __global__ __launch_bounds__(256) void adapter_gemm_kernel(AdGemmArgs p) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     constexpr int NCH = NI * 8;                              // 16-byte chunks of a row of the wave's columns
     char* wl = ad_smem + wave * 32 * NCH * 16;
-    static_assert(4 * 32 * NCH * 16 <= Sh::LDS, "the epilogue's block fits");
+    static_assert(NW * 32 * NCH * 16 <= Sh::LDS, "the epilogue's block fits");
     const T* bias = (const T*)p.bias;
     const int ch = lane % NCH;
     const int64_t n = n0 + wn * NI * 32 + ch * 4;

@@ -1074,32 +1074,44 @@ def _same_device(name, *ts):
     return _NO_GUARD if d.index == torch.cuda.current_device() else torch.cuda.device(d)
 
 
+def _raw_stream(t):
+    """The current stream of the tensor's device, as _stream() gives it, without the stream object (a microsecond per call)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 class Act8:
     """8-bit form of an activation tensor (`act_quant8`): int8 codes [rows, 32*nb] and one power-of-two step per block of 32 channels
-    (uint8 exponents [rows, nb], nb = ceil(C / 32)), plus the shape and dtype of the tensor it stands for.  1.03 bytes per element."""
-    __slots__ = ("codes", "exps", "shape", "dtype")
+    (uint8 exponents [rows, nb], nb = ceil(C / 32)) in one buffer, plus the shape and dtype of the tensor it stands for.  1.03 bytes per
+    element."""
+    __slots__ = ("buf", "rows", "nb", "shape", "dtype")
 
-    def __init__(self, codes, exps, shape, dtype):
-        self.codes, self.exps, self.shape, self.dtype = codes, exps, torch.Size(shape), dtype
+    def __init__(self, shape, dtype, device=None, *, buf=None):
+        C = shape[-1]
+        self.shape, self.dtype, self.nb = torch.Size(shape), dtype, (C + 31) // 32
+        self.rows = self.shape.numel() // C if C else 0
+        n = self.rows * self.nb * 33
+        if buf is not None and buf.numel() != n:
+            raise ValueError(f"Act8: a buffer of {n} bytes expected, got {buf.numel()}")
+        self.buf = torch.empty(n, device=device, dtype=torch.uint8) if buf is None else buf
 
     @property
-    def rows(self):
-        return self.exps.shape[0]
+    def codes(self):
+        return self.buf[:self.rows * self.nb * 32].view(torch.int8).view(self.rows, self.nb * 32)
+
+    @property
+    def exps(self):
+        return self.buf[self.rows * self.nb * 32:].view(self.rows, self.nb)
+
+    def _ptrs(self):
+        p = self.buf.data_ptr()
+        return p, p + self.rows * self.nb * 32
 
     @property
     def device(self):
-        return self.codes.device
+        return self.buf.device
 
     def nbytes(self):
-        return self.codes.numel() + self.exps.numel()
-
-
-def _new_act8(x):
-    C = x.shape[-1]
-    nb = (C + 31) // 32
-    rows = x.numel() // C
-    buf = torch.empty(rows * nb * 33, device=x.device, dtype=torch.uint8)
-    return Act8(buf[:rows * nb * 32].view(torch.int8).view(rows, nb * 32), buf[rows * nb * 32:].view(rows, nb), x.shape, x.dtype)
+        return self.buf.numel()
 
 
 def act_quant8(x, *, out=None):
@@ -1110,12 +1122,12 @@ def act_quant8(x, *, out=None):
     C = x.shape[-1]
     rows, ld = (0, C) if x.numel() == 0 else _rows2d(x)
     if out is None:
-        out = _new_act8(x)
+        out = Act8(x.shape, x.dtype, x.device)
     elif not isinstance(out, Act8) or out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("act_quant8: out must be an Act8 of x's shape and dtype")
-    with _same_device("act_quant8", x, out.codes):
+    with _same_device("act_quant8", x, out.buf):
         if rows:
-            check(_lib.load().m4d_act_quant8(dt_code(x.dtype), _ptr(x), ld, _ptr(out.codes), _ptr(out.exps), rows, C, _stream()), "m4d_act_quant8")
+            check(_lib.load().m4d_act_quant8(dt_code(x.dtype), _ptr(x), ld, *out._ptrs(), rows, C, _raw_stream(x)), "m4d_act_quant8")
     return out
 
 
@@ -1128,10 +1140,10 @@ def act_dequant8(a8, dtype=None, *, act=0, out=None):
     elif out.shape != a8.shape or (dtype is not None and out.dtype != dtype):
         raise ValueError("act_dequant8: out must have the activation's shape and the requested dtype")
     dt = dt_code(out.dtype)
-    with _same_device("act_dequant8", a8.codes, out):
+    with _same_device("act_dequant8", a8.buf, out):
         if a8.rows:
             rows, ld = _rows2d(out)
-            check(_lib.load().m4d_act_dequant8(dt, _ptr(a8.codes), _ptr(a8.exps), _ptr(out), ld, rows, C, act, _stream()), "m4d_act_dequant8")
+            check(_lib.load().m4d_act_dequant8(dt, *a8._ptrs(), _ptr(out), ld, rows, C, act, _raw_stream(out)), "m4d_act_dequant8")
     return out
 
 
@@ -1143,8 +1155,8 @@ def act_dequant8_t(a8, dtype=None, *, act=0):
         raise ValueError("act_dequant8_t: no rows")
     Rp = -(-R // 64) * 64 if R >= 512 else -(-R // 8) * 8
     out = torch.empty((C, Rp), device=a8.device, dtype=dtype or a8.dtype)
-    with _same_device("act_dequant8_t", a8.codes):
-        check(_lib.load().m4d_act_dequant8_t(dt_code(out.dtype), _ptr(a8.codes), _ptr(a8.exps), _ptr(out), Rp, R, Rp, C, act, _stream()),
+    with _same_device("act_dequant8_t", a8.buf):
+        check(_lib.load().m4d_act_dequant8_t(dt_code(out.dtype), *a8._ptrs(), _ptr(out), Rp, R, Rp, C, act, _raw_stream(out)),
               "m4d_act_dequant8_t")
     return out
 
@@ -1158,13 +1170,13 @@ def act_bwd8(dy, a8, act, *, out=None):
     elif out.shape != dy.shape or out.dtype != dy.dtype:
         raise ValueError("act_bwd8: out must have dy's shape and dtype")
     dt = dt_code(dy.dtype)
-    with _same_device("act_bwd8", dy, a8.codes, out):
+    with _same_device("act_bwd8", dy, a8.buf, out):
         if a8.rows:
             rows, ldy = _rows2d(dy)
             _, ldo = _rows2d(out)
             if out.data_ptr() == dy.data_ptr() and ldo != ldy:
                 raise ValueError("act_bwd8: in place needs equal row strides")
-            check(_lib.load().m4d_act_bwd8(dt, _ptr(dy), ldy, _ptr(a8.codes), _ptr(a8.exps), _ptr(out), ldo, rows, dy.shape[-1], act, _stream()),
+            check(_lib.load().m4d_act_bwd8(dt, _ptr(dy), ldy, *a8._ptrs(), _ptr(out), ldo, rows, dy.shape[-1], act, _raw_stream(dy)),
                   "m4d_act_bwd8")
     return out
 
@@ -1213,7 +1225,7 @@ class AdapterBank:
             self.back.G, self.back.rank, self.back.R, self.back.K, self.back.N = G, r, self.R, N, K
         with _same_device("AdapterBank", a, b):
             check(lib.m4d_adapter_pack(dt, _ptr(a), _ptr(b), G, r, K, N, self.R, _ptr(self.down), _ptr(self.up),
-                                       _ptr(parts[2]) if backward else 0, _ptr(parts[3]) if backward else 0, _stream()), "m4d_adapter_pack")
+                                       _ptr(parts[2]) if backward else 0, _ptr(parts[3]) if backward else 0, _raw_stream(a)), "m4d_adapter_pack")
 
     def transposed(self):
         """The bank of the backward pass, v = s dy B and dx = dy W + v A: the down projection maps N channels, the up projection gives K."""
@@ -1311,9 +1323,12 @@ def adapter_down(x, bank, plan, *, rows=True, slots=False):
     M, ldx = _check_adapters("adapter_down", x, bank, plan)
     u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype) if rows else None
     ut = torch.empty((bank.R, plan.n_pieces * plan.PIECE), device=x.device, dtype=x.dtype) if slots else None
+    lib = _lib.load()
     with _same_device("adapter_down", x, bank.up, plan.table):
-        check(_lib.load().m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, _ptr(bank.down), _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut), 0, 0,
-                                           x.shape[-1], bank.R, _stream()), "m4d_adapter_down")
+        nws = lib.m4d_adapter_down_workspace(plan.args, x.shape[-1], bank.R)
+        ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
+        check(lib.m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, _ptr(bank.down), _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut), 0, 0,
+                                   x.shape[-1], bank.R, _ptr(ws), nws, _raw_stream(x)), "m4d_adapter_down")
     return u, ut
 
 
@@ -1336,7 +1351,7 @@ def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=Fals
     elif out.dtype != x.dtype or out.shape != (*x.shape[:-1], N):
         raise ValueError(f"linear_adapters: out must be {(*x.shape[:-1], N)} of x's dtype")
     ut = torch.empty((bank.R, plan.n_pieces * plan.PIECE), device=x.device, dtype=x.dtype) if slots or keep8 else None
-    x8 = _new_act8(x) if keep8 else None
+    x8 = Act8(x.shape, x.dtype, x.device) if keep8 else None
     ret = (out, ut, x8) if keep8 else (out, ut) if slots else out
     if x.numel() == 0:
         if plan.rows:
@@ -1352,11 +1367,11 @@ def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=Fals
     lib = _lib.load()
     with _same_device("linear_adapters", x, w, bias, out, bank.up, plan.table):
         u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype)
-        nws = lib.m4d_linear_adapters_workspace(dt, M, N, K)
+        nws = lib.m4d_linear_adapters_workspace(dt, plan.args, N, K, bank.R)
         ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
         check(lib.m4d_linear_adapters(dt, _ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(bank.down), _ptr(bank.scale), _ptr(bank.up), plan.args,
-                                      _ptr(u), _ptr(ut), _ptr(x8.codes) if keep8 else 0, _ptr(x8.exps) if keep8 else 0, _ptr(out), ldo, N, K,
-                                      bank.R, _ptr(ws), nws, _stream()), "m4d_linear_adapters")
+                                      _ptr(u), _ptr(ut), *(x8._ptrs() if keep8 else (0, 0)), _ptr(out), ldo, N, K, bank.R, _ptr(ws), nws,
+                                      _raw_stream(x)), "m4d_linear_adapters")
     return ret
 
 
@@ -1379,10 +1394,9 @@ def adapter_grad(vt, x, plan, bank, *, transposed=False):
     out = torch.empty((G, C, rank) if transposed else (G, rank, C), device=vt.device, dtype=vt.dtype)
     if plan.n_pieces == 0:
         return out.zero_()
-    with _same_device("adapter_grad", vt, x8.codes if x8 is not None else x, plan.table):
+    with _same_device("adapter_grad", vt, x8.buf if x8 is not None else x, plan.table):
         lib = _lib.load()
         ws = torch.empty(lib.m4d_adapter_grad_workspace(plan.args, C, R), device=vt.device, dtype=torch.float32)
-        check(lib.m4d_adapter_grad(dt, _ptr(vt), 0 if x8 is not None else _ptr(x), ldx, _ptr(x8.codes) if x8 is not None else 0,
-                                   _ptr(x8.exps) if x8 is not None else 0, plan.args, _ptr(ws), ws.numel(), _ptr(out), int(transposed), G, rank, C,
-                                   R, _stream()), "m4d_adapter_grad")
+        check(lib.m4d_adapter_grad(dt, _ptr(vt), 0 if x8 is not None else _ptr(x), ldx, *(x8._ptrs() if x8 is not None else (0, 0)),
+                                   plan.args, _ptr(ws), ws.numel(), _ptr(out), int(transposed), G, rank, C, R, _raw_stream(vt)), "m4d_adapter_grad")
     return out
