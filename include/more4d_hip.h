@@ -521,12 +521,13 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
  *                                coarse to fine; chunk_off[l] [n_adapters + 1] into it
  *   tiles_off[i], tiles[i]       the adapters of the rows of each tile, each once, for tiles of 64, 128 and 256 rows and (i = 3) of 256 rows
  *                                whose last one is rows [rows - 256, rows)
- *   adapter_down     u T [rows, R] and / or ut T [R, 64 * n_pieces] = s_g x A_g^T (rows without an adapter are not written, pad slots are zero);
+ *   adapter_down     u T [rows, R] and / or ut = s_g x A_g^T (u's rows without an adapter are not written).  ut T [4 * n_pieces][ceil(R / 32)][64][8]:
+ *                    slot s, rank r at [s / 16][r / 32][r % 32 + 32 * (s % 16 / 8)][s % 8], zero for pad slots and ranks beyond R;
  *                    codes / exps (may be NULL): the 8-bit form of x's rows with an adapter, as act_quant8 writes it;
  *                    ws: adapter_down_workspace floats
  *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once.  With a_down, u (and ut, codes, exps if given) are written first, by
  *                    adapter_down; without, u is an input.  ws: linear_adapters_workspace floats
- *   adapter_grad     out T [G, rank, C] (transposed: [G, C, rank]) = sum over the rows of g of v^T x, v given as vt T [R, 64 * n_pieces], x as T or as
+ *   adapter_grad     out T [G, rank, C] (transposed: [G, C, rank]) = sum over the rows of g of v^T x, vt as adapter_down writes ut, x as T or as
  *                    8-bit codes; ws: adapter_grad_workspace floats; partial sums are joined in a fixed order. */
 typedef struct {
     const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks[4], *chunk_off[4], *tiles_off[4], *tiles[4];

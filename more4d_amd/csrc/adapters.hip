@@ -9,8 +9,9 @@
 //
 // Rows are worked on in SLOTS: the plan lists the rows adapter by adapter, each adapter's list padded (slot_row = -1) to whole PIECES of 64
 // slots, so a workgroup never sees two adapters whatever the order of the requests, and one-row requests of one adapter share a piece.
-// u is written twice: [row][R], the GEMM's operand, and [R][slot], the operand of the row contraction (its 8 consecutive slots of one
-// rank are one 16-byte load in the MFMA layout; pad slots hold zero).  u and v are rounded to T like every other operand of an MFMA here: the
+// u is written twice: [row][R], the GEMM's operand, and as the operand of the row contraction in the order in which its MFMA lanes read it,
+// [slot / 16][rank / 32][lane][8] with lane = rank % 32 + 32 * (slot % 16 / 8) (read row by row, 16 bytes of 32 ranks each, these loads cost the
+// address unit as much as x's); pad slots and ranks hold zero.  u and v are rounded to T like every other operand of an MFMA here: the
 // error this puts on an output is the one its own final rounding has, or less.
 //
 // The operand of a down projection is laid out once (m4d_adapter_pack) in the order in which the MFMA lanes read it: chunks of 64 channels, 32
@@ -72,168 +73,191 @@ struct DownArgs {
     void* u; void* ut;
     int8_t* codes; uint8_t* exps;
     const int *slot_row, *piece_adapter;
-    int64_t ldx, n_slots;
+    int64_t ldx;
     int K, R, n_pieces;
-    int KS;                // K slices (gridDim.y); > 1: unscaled float32 sums to part [KS, n_pieces, R, 64]
+    int KS;                // K slices (gridDim.y); > 1: unscaled float32 sums to part [KS, n_pieces, R rounded up to 32, 64]
     float* part;
 };
 
-// four ranks of one slot to u and / or ut, scaled
+// four ranks (r .. r + 3) of one slot to u and / or ut, scaled
 template <typename T>
 M4D_DEV void down_store(const DownArgs& p, int64_t piece, int g, int slot, int row, int r, f32x4 v) {
     const float sc = p.scale[g];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= sc;
-    if (p.u && row >= 0) store4((T*)p.u + (int64_t)row * p.R + r, v);
+    for (int e = 0; e < 4; ++e) v[e] = row >= 0 ? v[e] * sc : 0.f;
+    if (p.u && row >= 0 && r < p.R) store4((T*)p.u + (int64_t)row * p.R + r, v);
     if (p.ut) {
+        const int64_t s = piece * PIECE + slot;
+        T* d = (T*)p.ut + (((s >> 4) * ((p.R + 31) >> 5) + (r >> 5)) * 64 + (r & 31) + ((slot >> 3) & 1) * 32) * 8 + (slot & 7);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ((T*)p.ut)[(r + e) * p.n_slots + piece * PIECE + slot] = (T)(row >= 0 ? v[e] : 0.f);
+        for (int e = 0; e < 4; ++e) d[e * 8] = (T)v[e];
     }
 }
 
-// a row's 32-channel block in its lane's four fragments -> codes and exponent byte
-template <typename T>
-M4D_DEV void quant_block(const typename Frag8<T>::type (&x)[4], int8_t* codes, uint8_t* exps) {
+// 16 channels, half a block, of two neighbouring lanes each -> 16 codes and (from the even lane) the exponent byte
+M4D_DEV void quant_half(const float (&x)[16], int8_t* codes, uint8_t* exps, bool store) {
     unsigned top = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(unsigned, (float)x[k][e]) & 0x7fffffffu);
+    for (int e = 0; e < 16; ++e) top = max(top, __builtin_bit_cast(unsigned, x[e]) & 0x7fffffffu);
+    top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));
     const unsigned b = block_exp(top);
     const float inv = block_inv(min(b, 248u));
-    u32x4q c[2] = {};
+    u32x4q c = {};
     if (b != 255u) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                c[k >> 1][(k & 1) * 2 + h] = encode4((float)x[k][h * 4], (float)x[k][h * 4 + 1], (float)x[k][h * 4 + 2], (float)x[k][h * 4 + 3], inv, b == 248u);
+        for (int k = 0; k < 4; ++k) c[k] = encode4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3], inv, b == 248u);
     }
-    *reinterpret_cast<u32x4q*>(codes) = c[0];
-    *reinterpret_cast<u32x4q*>(codes + 16) = c[1];
-    *exps = (uint8_t)b;
+    if (store) {
+        *reinterpret_cast<u32x4q*>(codes) = c;
+        if ((threadIdx.x & 1) == 0) *exps = (uint8_t)b;
+    }
 }
 
-// u of one piece: 64 slots x RT * 32 ranks; K split over the workgroup's NW waves (64 channels each in turn), joined in LDS in wave order.
-// Loads return in order, so each chunk requests its packed operand (from L2) BEFORE the next chunk's rows (from HBM): the other way round the
-// products would wait for both, and nothing would be in flight ahead of them.  c0, c1: the chunks of this K slice.
-template <typename T, int RT, int NW, int NS, bool QUANT>
-M4D_DEV void down_loop(const DownArgs& p, int g, int rt0, int wave, int lane, const int (&row)[2], const int (&rowc)[2], int c0, int c1,
-                       f32x16 (&acc)[RT][2]) {
+// u of one piece: 64 slots x RT * 32 ranks, a chunk of 64 channels at a time.  Bound by reading x once; the operand comes from L2, as many bytes
+// again at 64 ranks.  Rows and operand go to LDS by direct loads, whole 128-byte lines of a row per request (straight into registers, a lane of
+// the MFMA layout wants 16 bytes of a row of its own, and the address unit then handles 64 lines per request: 85 us for 21840 x 5120 at rank
+// 64, against 46 us of HBM time), NST - 1 chunks in flight, one barrier per chunk, two workgroups per CU.
+// Wave (s, h): slots 32 s + [0, 32) and rank tiles h, h + 2, ...; with one rank tile h takes every other 16 channels instead.  QUANT: each
+// wave also writes the codes of 16 of the piece's rows, two lanes per block of 32 channels, out of the same LDS.
+template <typename T, int RT> struct DownShape {
+    static constexpr int XB = 64 * 64 * sizeof(T), AB = RT * 64 * 32 * sizeof(T), STAGE = XB + AB;
+    static constexpr int NST = STAGE * 4 <= 80 * 1024 ? 4 : STAGE * 3 <= 80 * 1024 ? 3 : 2;
+    static constexpr int LDS = NST * STAGE;
+};
+template <typename T, int RT, bool QUANT>
+__global__ __launch_bounds__(256, 2) void adapter_down_kernel(DownArgs p) {
+    typedef DownShape<T, RT> Sh;
     typedef typename Frag8<T>::type frag_t;
-    const int hi = lane >> 5, nc = (p.K + 63) >> 6, rts = (p.R + 31) >> 5, nb = (p.K + 31) >> 5;
-    const T* px[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) px[s] = (const T*)p.x + (int64_t)rowc[s] * p.ldx + hi * 32;
-    const T* pa[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) pa[rt] = (const T*)p.a + ((int64_t)g * nc * rts + min(rt0 + rt, rts - 1)) * 2048 + lane * 8;
-    auto load = [&](int c, frag_t (&x)[NS][4]) {
-        if (c * 64 + 64 <= p.K) {
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) x[s][kk] = *reinterpret_cast<const frag_t*>(px[s] + c * 64 + kk * 8);
-        } else {
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) x[s][kk] = load_k8<T>(px[s], c * 64 + kk * 8, p.K - hi * 32);
-        }
-    };
-    auto step = [&](int c, frag_t (&x)[NS][4], frag_t (&next)[NS][4]) {
-        frag_t a[RT][4];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) a[rt][kk] = *reinterpret_cast<const frag_t*>(pa[rt] + (int64_t)c * rts * 2048 + kk * 512);
-        __builtin_amdgcn_sched_barrier(0);
-        if (c + NW < c1) load(c + NW, next);
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (QUANT) {
-            const int blk = c * 2 + hi;
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                if (row[s] >= 0 && blk < nb) quant_block<T>(x[s], p.codes + ((int64_t)row[s] * nb + blk) * 32, p.exps + (int64_t)row[s] * nb + blk);
-        }
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int s = 0; s < NS; ++s) mma32(a[rt][kk], x[s][kk], acc[rt][s]);
-    };
-    frag_t x0[NS][4], x1[NS][4];
-    int c = c0 + wave;
-    if (c < c1) load(c, x0);
-    while (c < c1) {
-        step(c, x0, x1);
-        c += NW;
-        if (c >= c1) break;
-        step(c, x1, x0);
-        c += NW;
-    }
-}
-
-template <typename T, int RT, int NW, bool QUANT>
-__global__ __launch_bounds__(64 * NW, 2) void adapter_down_kernel(DownArgs p) {
     extern __shared__ __attribute__((aligned(16))) char ad_smem[];
-    float* red = reinterpret_cast<float*>(ad_smem);              // [NW][2 * 16][64]
-    const int t = threadIdx.x, lane = t & 63, li = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    constexpr int ES = sizeof(T), NST = Sh::NST, RB = 64 * ES, CPR = RB / 16, RPU = 1024 / RB;      // bytes, 16-byte chunks of a row; rows of a request
+    constexpr int NX = 64 / RPU / 4, NA = Sh::AB / 4096, NU = NX + NA;                               // requests of a wave and chunk
+    constexpr int NT = RT == 1 ? 1 : RT / 2;
+    const int t = threadIdx.x, lane = t & 63, li = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), s = wave & 1, h = wave >> 1;
     // more than RT * 32 ranks: ny workgroups read the same rows; numbered so that they run next to each other on one XCD and share them in its L2
-    const int ny = ((p.R + 31) / 32 + RT - 1) / RT, b8 = blockIdx.x >> 3;
+    const int rts = (p.R + 31) / 32, ny = (rts + RT - 1) / RT, b8 = blockIdx.x >> 3;
     const int piece = (b8 / ny) * 8 + (blockIdx.x & 7), rt0 = (b8 % ny) * RT;
     if (piece >= p.n_pieces) return;
     const int g = __builtin_amdgcn_readfirstlane(p.piece_adapter[piece]);
     const int* sr = p.slot_row + (int64_t)piece * PIECE;
-    const bool two = __builtin_amdgcn_readfirstlane(sr[32]) >= 0;      // more than 32 rows (slot 0 always holds one)
-    int row[2], rowc[2];
+    const int nc = (p.K + 63) >> 6, nb = (p.K + 31) >> 5, per = (nc + p.KS - 1) / p.KS, c0 = (int)blockIdx.y * per, c1 = min(nc, c0 + per);
+    const int tail = (p.K - (nc - 1) * 64) * ES;         // bytes of the last chunk of a row
+    const unsigned lds_base = (unsigned)(uintptr_t)(LDS_AS char*)ad_smem;
+    auto swz = [](int r) { return ES == 2 ? (r >> 1) & 7 : r & 15; };      // 16-byte chunk c of row r sits at chunk c ^ swz(r)
+    const char* sx[NX];
+    int cb[NX];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        row[s] = sr[s * 32 + li];
-        rowc[s] = row[s] >= 0 ? row[s] : sr[0];                  // pad slots compute copies of the first row and store nothing
+    for (int i = 0; i < NX; ++i) {
+        const int r = (wave + 4 * i) * RPU + lane / CPR, rw = sr[r];
+        cb[i] = ((lane % CPR) ^ swz(r)) * 16;
+        sx[i] = (const char*)p.x + (int64_t)(rw >= 0 ? rw : sr[0]) * p.ldx * ES + cb[i];      // (pad slots compute copies of the first row)
     }
-    f32x16 acc[RT][2];
+    const char* sa[NA];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) acc[rt][s][q] = 0.f;
-    const int nc = (p.K + 63) >> 6, per = (nc + p.KS - 1) / p.KS, c0 = (int)blockIdx.y * per, c1 = min(nc, c0 + per);
-    if (QUANT && rt0 == 0) {
-        if (two) down_loop<T, RT, NW, 2, QUANT>(p, g, rt0, wave, lane, row, rowc, c0, c1, acc);
-        else down_loop<T, RT, NW, 1, QUANT>(p, g, rt0, wave, lane, row, rowc, c0, c1, acc);
-    } else {
-        if (two) down_loop<T, RT, NW, 2, false>(p, g, rt0, wave, lane, row, rowc, c0, c1, acc);
-        else down_loop<T, RT, NW, 1, false>(p, g, rt0, wave, lane, row, rowc, c0, c1, acc);
+    for (int i = 0; i < NA; ++i) {
+        const int o = (wave + 4 * i) * 1024, rt = o / (2048 * ES), in = o % (2048 * ES);
+        sa[i] = (const char*)p.a + (((int64_t)g * nc * rts + min(rt0 + rt, rts - 1)) * 2048) * ES + in + lane * 16;
     }
+    auto request = [&](int c) {
+        const unsigned dst = __builtin_amdgcn_readfirstlane(lds_base + (unsigned)((c - c0) % NST) * Sh::STAGE + wave * 1024);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        if (rt) __syncthreads();
+        for (int i = 0; i < NX; ++i) {
+            const char* q = sx[i] + (int64_t)c * RB;
+            if (c == nc - 1 && cb[i] >= tail) q = (const char*)zero_page;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst + i * 4096), "v"(q) : "memory", "m0");
+        }
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < NA; ++i) {
+            const char* q = sa[i] + (int64_t)c * rts * 2048 * ES;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst + Sh::XB + i * 4096), "v"(q) : "memory", "m0");
+        }
+    };
+    f32x16 acc[NT];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) red[((wave * 2 + s) * 16 + q) * 64 + lane] = acc[rt][s][q];
-        __syncthreads();
-        // unit (s, rank quad q4, lane): ranks q4 * 8 + hi * 4 + [0, 4) of slot s * 32 + li
-        for (int i = t; i < 512; i += 64 * NW) {
-            const int l = i & 63, q4 = (i >> 6) & 3, s = i >> 8;
-            const int r = (rt0 + rt) * 32 + q4 * 8 + (l >> 5) * 4;
-            if (r >= p.R) continue;
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            for (int w = 0; w < NW; ++w)
+    for (int k = 0; k < NT; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] += red[((w * 2 + s) * 16 + q4 * 4 + e) * 64 + l];
-            const int slot = s * 32 + (l & 31);
-            if (p.part) {
-                float* d = p.part + (((int64_t)blockIdx.y * p.n_pieces + piece) * p.R + r) * PIECE + slot;
+        for (int q = 0; q < 16; ++q) acc[k][q] = 0.f;
+    const int row = sr[s * 32 + li];
+    // (QUANT) this lane's row, and where its codes and exponents go
+    const int qr = wave * 16 + (lane >> 2), qrow = QUANT && rt0 == 0 ? sr[qr] : -1;
+    int8_t* qc = p.codes + (int64_t)max(qrow, 0) * nb * 32 + (lane & 3) * 16;
+    uint8_t* qe = p.exps + (int64_t)max(qrow, 0) * nb;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) d[e * PIECE] = v[e];
-            } else down_store<T>(p, piece, g, slot, sr[slot], r, v);
+    for (int i = 0; i < NST - 1; ++i)
+        if (c0 + i < c1) request(c0 + i);
+    for (int c = c0; c < c1; ++c) {
+        // chunk c has landed when at most the younger chunks' requests are pending (only loads are counted: a store in flight makes the wait
+        // stricter); behind the barrier everybody's has, and nobody reads chunk c - 1 any more, whose stage the next request overwrites
+        const int younger = c1 - 1 - c;
+        if (NST > 2 && younger >= NST - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"((NST - 2) * NU) : "memory");
+        else if (NST == 4 && younger == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(NU) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (c + NST - 1 < c1) request(c + NST - 1);
+        const char* st = ad_smem + ((c - c0) % NST) * Sh::STAGE;
+        auto frag = [&](const char* q, int o0, int o1) {
+            if constexpr (ES == 2) return *reinterpret_cast<const frag_t*>(q + o0);
+            else return (frag_t)__builtin_shufflevector(*reinterpret_cast<const f32x4*>(q + o0), *reinterpret_cast<const f32x4*>(q + o1), 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        frag_t x[4];
+        const int r = s * 32 + li;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            const int ch = (hi * 32 + kk * 8) * ES / 16;
+            x[kk] = frag(st + r * RB, (ch ^ swz(r)) << 4, ((ch + 1) ^ swz(r)) << 4);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            if (RT == 1 && (kk & 1) != h) continue;          // (wave-uniform)
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                const char* q = st + Sh::XB + (((RT == 1 ? 0 : h + 2 * k) * 4 + kk) * 64 + lane) * 8 * ES;
+                mma32(frag(q, 0, 16), x[kk], acc[k]);
+            }
+        }
+        if constexpr (QUANT) {
+            const int blk = c * 2 + ((lane >> 1) & 1);
+            float v[16];
+#pragma unroll
+            for (int k = 0; k < ES; ++k) {
+                const char* q = st + qr * RB + ((((lane & 3) * ES + k) ^ swz(qr)) << 4);
+                if constexpr (ES == 2) {
+                    const bf16x8 b = *reinterpret_cast<const bf16x8*>(q);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[k * 8 + e] = (float)b[e];
+                } else {
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(q);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[k * 4 + e] = b[e];
+                }
+            }
+            quant_half(v, qc + (int64_t)c * 64, qe + blk, qrow >= 0 && blk < nb);
         }
     }
+    if constexpr (RT == 1) {                                 // join the two halves of the channels
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        float* red = reinterpret_cast<float*>(ad_smem) + s * 1024 + lane;
+        if (h == 1) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q) red[q * 64] = acc[0][q];
+        }
+        __syncthreads();
+        if (h == 1) return;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[0][q] += red[q * 64];
+    }
+#pragma unroll
+    for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const int rt = rt0 + (RT == 1 ? 0 : h + 2 * k), r = rt * 32 + q4 * 8 + hi * 4, slot = s * 32 + li;
+            if (rt >= rts) continue;
+            const f32x4 v = {acc[k][q4 * 4], acc[k][q4 * 4 + 1], acc[k][q4 * 4 + 2], acc[k][q4 * 4 + 3]};
+            if (p.part) {
+                float* d = p.part + (((int64_t)blockIdx.y * p.n_pieces + piece) * rts * 32 + r) * PIECE + slot;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e * PIECE] = v[e];
+            } else down_store<T>(p, piece, g, slot, row, r, v);
+        }
 }
 
 // the K slices' sums of four ranks of one slot, in slice order
@@ -241,23 +265,24 @@ template <typename T>
 __global__ __launch_bounds__(256) void adapter_down_join_kernel(DownArgs p) {
     const int t = threadIdx.x, slot = t & 63, r = (blockIdx.y * 4 + (t >> 6)) * 4;
     const int64_t piece = blockIdx.x;
-    if (r >= p.R) return;
+    const int64_t R32 = (p.R + 31) / 32 * 32;
+    if (r >= R32) return;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     for (int k = 0; k < p.KS; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += p.part[((k * p.n_pieces + piece) * p.R + r + e) * PIECE + slot];
+        for (int e = 0; e < 4; ++e) v[e] += p.part[((k * p.n_pieces + piece) * R32 + r + e) * PIECE + slot];
     down_store<T>(p, piece, p.piece_adapter[piece], slot, p.slot_row[piece * PIECE + slot], r, v);
 }
 
 // ---------------------------------------------------------------- contraction over the rows
 struct GradArgs {
-    const void* vt;                 // T [R, n_slots]
+    const void* vt;                 // T, packed: [slot / 16][rank / 32][64][8]
     const void* x;                  // T [rows, C] (row stride ldx), or
     const int8_t* codes; const uint8_t* exps;      // its 8-bit form (act8.hip)
     float* ws;                      // [n_chunks, R, C]
     void* out;                      // T [G, rank, C], or [G, C, rank]
     const int *slot_row, *chunks, *chunk_off;
-    int64_t ldx, n_slots;
+    int64_t ldx;
     int C, R, rank, n_adapters, transposed;
 };
 
@@ -275,7 +300,7 @@ template <typename T, bool CODES, int RT>
 __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
     typedef typename Frag8<T>::type frag_t;
     typedef typename Quad<T>::type quad_t;
-    constexpr int PF = 2;
+    constexpr int PF = CODES ? 3 : 2;
     constexpr int RED = RT * 4 * 16 * 64 * 4;
     __shared__ __attribute__((aligned(16))) char smem[RED > CHUNK_PIECES * PIECE * 4 ? RED : CHUNK_PIECES * PIECE * 4];
     int* rows = reinterpret_cast<int*>(smem);
@@ -288,10 +313,10 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
     for (int i = t; i < n; i += 256) rows[i] = p.slot_row[s0 + i];
     const bool cin = c < p.C;
     const int cc = cin ? c : 0;                     // (columns beyond C are computed from the first ones and not stored)
-    const int nb = (p.C + 31) >> 5;
+    const int nb = (p.C + 31) >> 5, rts = (p.R + 31) >> 5;
     const T* pv[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) pv[rt] = (const T*)p.vt + (int64_t)min(r0 + rt * 32 + li, p.R - 1) * p.n_slots + s0 + hi * 8;
+    for (int rt = 0; rt < RT; ++rt) pv[rt] = (const T*)p.vt + ((int64_t)(s0 >> 4) * rts + min((int)blockIdx.z * RT + rt, rts - 1)) * 512 + lane * 8;
     f32x16 acc[RT][4];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -307,13 +332,14 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
         unsigned char ex[8];
     };
     // (pad slots, -1, read the chunk's first row: what they read is replaced by zero in use() — their v is zero, but zero times an infinity is not)
+    const int row0 = rows[0];
     auto load = [&](int s, Step& b) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) b.v[rt] = *reinterpret_cast<const frag_t*>(pv[rt] + s);
+        for (int rt = 0; rt < RT; ++rt) b.v[rt] = *reinterpret_cast<const frag_t*>(pv[rt] + (int64_t)(s >> 4) * rts * 512);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int r = rows[s + hi * 8 + j];
-            const int64_t row = r >= 0 ? r : rows[0];
+            const int64_t row = r >= 0 ? r : row0;
             if constexpr (CODES) {
                 b.code[j] = *reinterpret_cast<const int*>(p.codes + row * nb * 32 + cc);
                 b.ex[j] = p.exps[row * nb + (cc >> 5)];
@@ -321,7 +347,7 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
         }
     };
     auto use = [&](int s, Step& b) {
-        if (rows[s + 15] < 0) {                     // (uniform: the adapter's last piece) a step with pad slots
+        if (s + PIECE >= n && rows[s + 15] < 0) {   // (uniform: only an adapter's last piece has pad slots)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (rows[s + hi * 8 + j] < 0) {
@@ -344,20 +370,24 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
             for (int rt = 0; rt < RT; ++rt) mma32(b.v[rt], fx, acc[rt][f]);
         }
     };
+    // (n is whole pieces: every wave has n / 64 steps.  Requests beyond the end repeat the last step's rows: a branch around them would make the
+    // compiler wait for everything in flight at its join)
+    const int ns = n >> 6, last = (ns - 1) * 64 + wave * 16;
     Step b[PF];
 #pragma unroll
-    for (int i = 0; i < PF; ++i)
-        if ((wave + 4 * i) * 16 < n) load((wave + 4 * i) * 16, b[i]);
-    for (int s = wave * 16; s < n; s += 64 * PF) {
+    for (int i = 0; i < PF; ++i) load(min(wave * 16 + 64 * i, last), b[i]);
+    int k = 0;
+    for (; k + PF <= ns; k += PF) {
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
-            const int si = s + 64 * i;
-            if (si < n) {
-                use(si, b[i]);
-                if (si + 64 * PF < n) load(si + 64 * PF, b[i]);
-            }
+            const int s = wave * 16 + 64 * (k + i);
+            use(s, b[i]);
+            load(min(s + 64 * PF, last), b[i]);
         }
     }
+#pragma unroll
+    for (int i = 0; i < PF - 1; ++i)
+        if (k + i < ns) use(wave * 16 + 64 * (k + i), b[i]);
     for (int w = 0; w < 4; ++w) {
         __syncthreads();
         if (wave == w) {
@@ -502,12 +532,12 @@ extern "C" int m4d_adapter_pack(m4d_dtype dt, const void* a, const void* b, int 
     return 0;
 }
 
-template <typename T, int RT, int NW, bool QUANT>
-static int launch_down(const DownArgs& p, hipStream_t st) {
-    constexpr int LDS = NW * 8192;
+template <typename T, int RT, bool QUANT>
+static int launch_down_q(const DownArgs& p, hipStream_t st) {
+    constexpr int LDS = DownShape<T, RT>::LDS;
     static PerDeviceOnce configured;
     if (configured.pending()) {
-        if (hipFuncSetAttribute((const void*)adapter_down_kernel<T, RT, NW, QUANT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
+        if (hipFuncSetAttribute((const void*)adapter_down_kernel<T, RT, QUANT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
             (void)hipGetLastError();
             m4d_set_error("adapter_down: cannot enable %d bytes of LDS", LDS);
             return -3;
@@ -515,27 +545,23 @@ static int launch_down(const DownArgs& p, hipStream_t st) {
         configured.mark();
     }
     const int ny = ((p.R + 31) / 32 + RT - 1) / RT;
-    hipLaunchKernelGGL((adapter_down_kernel<T, RT, NW, QUANT>), dim3((unsigned)((p.n_pieces + 7) / 8 * 8 * ny), (unsigned)p.KS), dim3(64 * NW), LDS, st, p);
+    hipLaunchKernelGGL((adapter_down_kernel<T, RT, QUANT>), dim3((unsigned)((p.n_pieces + 7) / 8 * 8 * ny), (unsigned)p.KS), dim3(256), LDS, st, p);
     M4D_CHECK_LAUNCH("adapter_down");
     if (p.part) {
-        hipLaunchKernelGGL(adapter_down_join_kernel<T>, dim3((unsigned)p.n_pieces, (unsigned)((p.R + 15) / 16)), dim3(256), 0, st, p);
+        hipLaunchKernelGGL(adapter_down_join_kernel<T>, dim3((unsigned)p.n_pieces, (unsigned)((p.R + 31) / 32 * 2)), dim3(256), 0, st, p);
         M4D_CHECK_LAUNCH("adapter_down(join)");
     }
     return 0;
 }
 template <typename T, int RT>
-static int launch_down_nw(const DownArgs& p, hipStream_t st) {
-    // four waves where the pieces fill the chip (all of a long batch resident), eight where a workgroup has a CU to itself
-    if (p.n_pieces * p.KS < cus()) return p.codes ? launch_down<T, RT, 8, true>(p, st) : launch_down<T, RT, 8, false>(p, st);
-    return p.codes ? launch_down<T, RT, 4, true>(p, st) : launch_down<T, RT, 4, false>(p, st);
-}
+static int launch_down(const DownArgs& p, hipStream_t st) { return p.codes ? launch_down_q<T, RT, true>(p, st) : launch_down_q<T, RT, false>(p, st); }
 
-// K slices of a down projection with few pieces: as many as fill half the chip, each at least one chunk of 64 channels per wave.  (A piece's K
-// loop is serial: 16 pieces of K = 4096 took 20 us on 16 CUs.)
+// K slices of a down projection with few pieces: as many as fill half the chip, each at least eight chunks of 64 channels.  (A piece's K loop is
+// serial: 16 pieces of K = 4096 took 20 us on 16 CUs, in slices and joined 10.)
 static int down_slices(int n_pieces, int64_t K) {
     const int nc = (int)((K + 63) / 64);
     int ks = n_pieces > 0 ? cus() / 2 / n_pieces : 1;
-    if (ks > (nc + 7) / 8) ks = (nc + 7) / 8;
+    if (ks > nc / 8) ks = nc / 8;
     if (ks < 2) return 1;
     const int per = (nc + ks - 1) / ks;
     return (nc + per - 1) / per;                 // (no empty slices)
@@ -544,7 +570,7 @@ static int down_slices(int n_pieces, int64_t K) {
 extern "C" int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int64_t K, int R) {
     if (!plan || K <= 0 || R <= 0) return 0;
     const int ks = down_slices(plan->n_pieces, K);
-    return ks > 1 ? (int64_t)ks * plan->n_pieces * R * PIECE : 0;
+    return ks > 1 ? (int64_t)ks * plan->n_pieces * ((R + 31) / 32 * 32) * PIECE : 0;
 }
 
 extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan,
@@ -558,13 +584,13 @@ extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const 
     if (plan->n_pieces == 0) return 0;
     M4D_CHECK_ARG(plan->slot_row && plan->piece_adapter, "adapter_down: bad plan");
     const int ks = down_slices(plan->n_pieces, K);
-    M4D_CHECK_ARG(ks == 1 || (ws && ws_floats >= (int64_t)ks * plan->n_pieces * R * PIECE), "adapter_down: workspace of %lld floats needed",
-                  (long long)ks * plan->n_pieces * R * PIECE);
-    DownArgs p{x, a_down, scale, u, ut, codes, exps, plan->slot_row, plan->piece_adapter, ldx, (int64_t)plan->n_pieces * PIECE, (int)K, R,
+    const int64_t need = m4d_adapter_down_workspace(plan, K, R);
+    M4D_CHECK_ARG(need == 0 || (ws && ws_floats >= need), "adapter_down: workspace of %lld floats needed", (long long)need);
+    DownArgs p{x, a_down, scale, u, ut, codes, exps, plan->slot_row, plan->piece_adapter, ldx, (int)K, R,
                plan->n_pieces, ks, ks > 1 ? ws : nullptr};
     hipStream_t st = (hipStream_t)stream;
-    if (dt == M4D_BF16) return R <= 32 ? launch_down_nw<bf16_t, 1>(p, st) : launch_down_nw<bf16_t, 2>(p, st);
-    return launch_down_nw<float, 1>(p, st);
+    if (dt == M4D_BF16) return R <= 32 ? launch_down<bf16_t, 1>(p, st) : R <= 64 ? launch_down<bf16_t, 2>(p, st) : launch_down<bf16_t, 4>(p, st);
+    return R <= 32 ? launch_down<float, 1>(p, st) : launch_down<float, 2>(p, st);
 }
 
 template <typename T, int MI, int NI, int WM, int WN>
@@ -685,7 +711,7 @@ extern "C" int m4d_adapter_grad(m4d_dtype dt, const void* vt, const void* x, int
     const int lv = chunk_level(plan, C, R), nch = plan->n_chunks[lv];
     M4D_CHECK_ARG(plan->n_adapters <= G && nch <= 65535, "adapter_grad: the plan names adapter %d of %d, in %d chunks", plan->n_adapters - 1, G, nch);
     hipStream_t st = (hipStream_t)stream;
-    GradArgs p{vt, x, codes, exps, ws, out, plan->slot_row, plan->chunks[lv], plan->chunk_off[lv], ldx, (int64_t)plan->n_pieces * PIECE,
+    GradArgs p{vt, x, codes, exps, ws, out, plan->slot_row, plan->chunks[lv], plan->chunk_off[lv], ldx,
                (int)C, R, rank, plan->n_adapters, transposed};
     if (nch > 0) {
         M4D_CHECK_ARG(vt && ws && ws_floats >= (int64_t)nch * R * C, "adapter_grad: workspace of %lld floats needed", (long long)nch * R * C);

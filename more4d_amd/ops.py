@@ -1317,12 +1317,16 @@ def _check_adapters(name, x, bank, plan):
     return rows, ldx
 
 
+def _slots_shape(bank, plan):
+    return 4 * plan.n_pieces, (bank.R + 31) // 32, 64, 8
+
+
 def adapter_down(x, bank, plan, *, rows=True, slots=False):
-    """(u [rows, R], u^T [R, slots]) = s_g x A_g^T of each row's adapter (either may be left out: None).  u is written for rows with an adapter
-    only; u^T, the operand of `adapter_grad`, holds the plan's slots (pad slots zero)."""
+    """(u [rows, R], ut) = s_g x A_g^T of each row's adapter (either may be left out: None).  u is written for rows with an adapter only; ut is the
+    same by the plan's slots, in the order in which `adapter_grad` reads it (include/more4d_hip.h: adapter_down)."""
     M, ldx = _check_adapters("adapter_down", x, bank, plan)
     u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype) if rows else None
-    ut = torch.empty((bank.R, plan.n_pieces * plan.PIECE), device=x.device, dtype=x.dtype) if slots else None
+    ut = torch.empty(_slots_shape(bank, plan), device=x.device, dtype=x.dtype) if slots else None
     lib = _lib.load()
     with _same_device("adapter_down", x, bank.up, plan.table):
         nws = lib.m4d_adapter_down_workspace(plan.args, x.shape[-1], bank.R)
@@ -1334,8 +1338,8 @@ def adapter_down(x, bank, plan, *, rows=True, slots=False):
 
 def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=False):
     """x w^T + bias + s_g (x A_g^T) B_g^T, g the adapter of each row (plan).  x [..., K] (rows strided), w [N, K] (row-strided), bias [N] or None,
-    bank: AdapterBank, out [..., N].  For a backward pass: slots=True returns (out, u^T), u^T = (s x A^T)^T for `adapter_grad`; keep8=True
-    returns (out, u^T, Act8 of x) — the 8-bit form of the rows that name an adapter, written in the pass that reads x (the codes of other
+    bank: AdapterBank, out [..., N].  For a backward pass: slots=True returns (out, ut), ut = s x A^T in the slots of `adapter_grad`; keep8=True
+    returns (out, ut, Act8 of x) — the 8-bit form of the rows that name an adapter, written in the pass that reads x (the codes of other
     rows are undefined; no gradient of an adapter reads them)."""
     K, N = x.shape[-1], w.shape[0]
     if w.dim() != 2 or w.shape[1] != K:
@@ -1350,7 +1354,7 @@ def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=Fals
         out = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
     elif out.dtype != x.dtype or out.shape != (*x.shape[:-1], N):
         raise ValueError(f"linear_adapters: out must be {(*x.shape[:-1], N)} of x's dtype")
-    ut = torch.empty((bank.R, plan.n_pieces * plan.PIECE), device=x.device, dtype=x.dtype) if slots or keep8 else None
+    ut = torch.empty(_slots_shape(bank, plan), device=x.device, dtype=x.dtype) if slots or keep8 else None
     x8 = Act8(x.shape, x.dtype, x.device) if keep8 else None
     ret = (out, ut, x8) if keep8 else (out, ut) if slots else out
     if x.numel() == 0:
@@ -1377,14 +1381,14 @@ def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=Fals
 
 def adapter_grad(vt, x, plan, bank, *, transposed=False):
     """Gradient of the adapters: sum over the rows of each adapter of v^T x, as [G, rank, C] (transposed: [G, C, rank]) in vt's dtype; adapters that
-    no row names get zero.  vt: the [R, slots] result of `adapter_down` / `linear_adapters`; x [rows, C], or its Act8."""
+    no row names get zero.  vt: the slots that `adapter_down` / `linear_adapters` return; x [rows, C], or its Act8."""
     G, rank, R = bank.G, bank.rank, bank.R
     x8 = x if isinstance(x, Act8) else None
     C = x.shape[-1]
     if plan.n_adapters > G:
         raise ValueError(f"adapter_grad: the plan names adapter {plan.n_adapters - 1}, the bank has {G}")
-    if vt.shape != (R, plan.n_pieces * plan.PIECE) or not vt.is_contiguous():
-        raise ValueError("adapter_grad: vt must be adapter_down's contiguous [R, slots]")
+    if vt.shape != _slots_shape(bank, plan) or not vt.is_contiguous():
+        raise ValueError("adapter_grad: vt must be adapter_down's slots")
     rows, ldx = (x8.rows, 0) if x8 is not None else (0, 0) if x.numel() == 0 else _rows2d(x)
     if rows != plan.rows:
         raise ValueError(f"adapter_grad: {rows} rows against a plan of {plan.rows}")

@@ -331,8 +331,10 @@ def test_the_pass_that_reads_x_writes_the_same_codes(K, dt):
     u, ut3 = o.adapter_down(xd, bank, plan, slots=True)
     assert torch.equal(ut3.nan_to_num(0), ut.nan_to_num(0))
     slot = torch.tensor(tables_slot_row(plan))
-    assert (ut.cpu()[:, slot < 0] == 0).all()
-    assert torch.equal(ut.cpu()[:, slot >= 0].t().nan_to_num(0), u.cpu()[slot[slot >= 0].long()].nan_to_num(0))
+    # [slot / 16][rank / 32][rank % 32 + 32 * (slot % 16 / 8)][slot % 8] -> [slot][rank]
+    v = ut.cpu().view(len(slot) // 16, ut.shape[1], 2, 32, 8).permute(0, 2, 4, 1, 3).reshape(len(slot), -1)
+    assert (v[slot < 0] == 0).all() and (v[slot >= 0][:, 8:].nan_to_num(0) == 0).all()
+    assert torch.equal(v[slot >= 0][:, :u.shape[1]].nan_to_num(0), u.cpu()[slot[slot >= 0].long()].nan_to_num(0))
 
 
 def tables_slot_row(plan):
