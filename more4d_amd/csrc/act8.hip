@@ -22,7 +22,6 @@ struct Act8Args {
     int8_t* codes; uint8_t* exps;
     int64_t ld_in, ld_out, rows;
     int C, nb;            // channels, blocks per row (codes row stride = 32 * nb)
-    int act;
     int64_t rows_pad;     // transposed output: columns written (rows .. rows_pad are zero)
     int vec;              // 1: the T side has 16-byte aligned rows
 };
@@ -107,20 +106,26 @@ __global__ __launch_bounds__(256) void act_quant8_kernel(Act8Args p) {
     }
 }
 
-M4D_DEV float act_f(float x, int act) {
-    return act == 1 ? silu_f(x) : act == 2 ? gelu_tanh_f(x) : act == 3 ? gelu_erf_f(x) : x;
+// gelu_tanh as x s(2u) with 2u log2 e = x (c0 + c1 x^2) in one multiply-add: the transposed reader evaluates it at the rate of HBM, and common.h's
+// form, which rounds like the forward's, has three instructions more.  (x^2 may overflow: the exponential is then 0 or inf, the result x or -0.)
+M4D_DEV float gelu_f(float x) {
+    const float c0 = -2.3022081981f, c1 = -0.1029432396f;      // -2 log2(e) sqrt(2 / pi), times 0.044715
+    return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * fmaf(c1, x * x, c0)));
+}
+template <int ACT> M4D_DEV float act_f(float x) {
+    return ACT == 1 ? silu_f(x) : ACT == 2 ? gelu_f(x) : ACT == 3 ? gelu_erf_f(x) : x;
 }
 
 // act'(x).  Beyond |x| = 128 the three derivatives are 0 or 1 in float32, and clamping there keeps the polynomials finite; x * 0 brings
 // back the NaN that the clamp would lose.
-M4D_DEV float dact_f(float x0, int act) {
+template <int ACT> M4D_DEV float dact_f(float x0) {
     const float x = fminf(fmaxf(x0, -128.f), 128.f);
     float d;
-    if (act == 2) {      // gelu_tanh = x s(2u), s the logistic function, u = k0 (x + k1 x^3):  s + x s (1 - s) 2 u'
+    if constexpr (ACT == 2) {      // gelu_tanh = x s(2u), s the logistic function, u = k0 (x + k1 x^3):  s + x s (1 - s) 2 u'
         const float k0 = 0.7978845608028654f, k1 = 0.044715f, x2 = x * x;
         const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(k0 * x * (1.0f + k1 * x2) * -2.8853900817779268f));
         d = s + x * s * (1.0f - s) * (2.0f * k0) * (1.0f + 3.0f * k1 * x2);
-    } else if (act == 1) {
+    } else if constexpr (ACT == 1) {
         const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-x));
         d = s * (1.0f + x * (1.0f - s));
     } else {
@@ -129,7 +134,7 @@ M4D_DEV float dact_f(float x0, int act) {
     return fmaf(x0, 0.f, d);
 }
 
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void act_dequant8_kernel(Act8Args p) {
     const int nu = (p.C + 7) >> 3;
     for (UnitWalk w(nu); w.row < p.rows; w.next()) {
@@ -137,15 +142,13 @@ __global__ __launch_bounds__(256) void act_dequant8_kernel(Act8Args p) {
         const u32x2 c = *reinterpret_cast<const u32x2*>(p.codes + (w.row * p.nb) * 32 + c0);
         float v[8];
         decode8(c, step_of(p.exps[w.row * p.nb + (w.j >> 2)]), v);
-        if (p.act) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = act_f(v[e], p.act);
-        }
+        for (int e = 0; e < 8; ++e) v[e] = act_f<ACT>(v[e]);
         store_unit<T>((T*)p.out + w.row * p.ld_out + c0, n, p.vec, v);
     }
 }
 
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void act_bwd8_kernel(Act8Args p) {
     const int nu = (p.C + 7) >> 3;
     for (UnitWalk w(nu); w.row < p.rows; w.next()) {
@@ -155,7 +158,7 @@ __global__ __launch_bounds__(256) void act_bwd8_kernel(Act8Args p) {
         load_unit<T>((const T*)p.in + w.row * p.ld_in + c0, n, p.vec, d);
         decode8(c, step_of(p.exps[w.row * p.nb + (w.j >> 2)]), v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = d[e] * dact_f(v[e], p.act);
+        for (int e = 0; e < 8; ++e) v[e] = d[e] * dact_f<ACT>(v[e]);
         store_unit<T>((T*)p.out + w.row * p.ld_out + c0, n, p.vec, v);
     }
 }
@@ -164,7 +167,7 @@ __global__ __launch_bounds__(256) void act_bwd8_kernel(Act8Args p) {
 // Tile: 128 channels x 64 dwords of rows (bf16: two rows in a dword, fp32: one), in LDS as [channel][dword] with the 16-byte chunks of a
 // channel XORed by channel / 8: the 16 x 4 (unit, dword) pairs that a wave writes per channel land in 64 different banks, and a lane reads its
 // 8 (4) rows of a channel as one 16-byte chunk.
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void act_dequant8_t_kernel(Act8Args p) {
     constexpr int RPD = 4 / sizeof(T);          // rows per dword
     constexpr int TR = 64 * RPD;                // rows of a tile
@@ -184,10 +187,8 @@ __global__ __launch_bounds__(256) void act_dequant8_t_kernel(Act8Args p) {
             if (r < p.rows && col < p.C) {
                 const u32x2 c = *reinterpret_cast<const u32x2*>(p.codes + (r * p.nb) * 32 + col);
                 decode8(c, step_of(p.exps[r * p.nb + (col >> 5)]), v[h]);
-                if (p.act) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[h][e] = act_f(v[h][e], p.act);
-                }
+                for (int e = 0; e < 8; ++e) v[h][e] = act_f<ACT>(v[h][e]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[h][e] = 0.f;
@@ -223,6 +224,18 @@ unsigned grid_of(int64_t units) {
 
 }  // namespace
 
+// the activation as a template parameter: a runtime switch per element was a fifth of the transposed reader's time
+#define ACT8_ONE(KERNEL, ACT)                                                                                           \
+    do {                                                                                                                \
+        if (dt == M4D_BF16) hipLaunchKernelGGL((KERNEL<bf16_t, ACT>), grid, block, 0, (hipStream_t)stream, p);           \
+        else hipLaunchKernelGGL((KERNEL<float, ACT>), grid, block, 0, (hipStream_t)stream, p);                          \
+    } while (0)
+#define ACT8_BY_ACT(KERNEL)                                                                                             \
+    do {                                                                                                                \
+        if (act == 1) ACT8_ONE(KERNEL, 1);                                                                              \
+        else if (act == 2) ACT8_ONE(KERNEL, 2);                                                                         \
+        else ACT8_ONE(KERNEL, 3);                                                                                       \
+    } while (0)
 #define DT_OK(dt) ((dt) == M4D_BF16 || (dt) == M4D_F32)
 #define ACT8_COMMON(name)                                                                                              \
     M4D_CHECK_ARG(DT_OK(dt), name ": bad dtype %d", (int)dt);                                                           \
@@ -252,11 +265,11 @@ extern "C" int m4d_act_dequant8(m4d_dtype dt, const int8_t* codes, const uint8_t
     M4D_CHECK_ARG(act >= 0 && act <= 3, "act_dequant8: bad activation %d", act);
     M4D_CHECK_ARG(out && (rows == 1 || ldo >= C), "act_dequant8: null output or row stride %lld below C=%d", (long long)ldo, C);
     Act8Args p{};
-    p.out = out; p.ld_out = ldo; p.codes = (int8_t*)codes; p.exps = (uint8_t*)exps; p.rows = rows; p.C = C; p.nb = nb; p.act = act;
+    p.out = out; p.ld_out = ldo; p.codes = (int8_t*)codes; p.exps = (uint8_t*)exps; p.rows = rows; p.C = C; p.nb = nb;
     p.vec = ((uintptr_t)out % 16) == 0 && (ldo * es) % 16 == 0;
     dim3 grid(grid_of(rows * ((C + 7) / 8))), block(256);
-    if (dt == M4D_BF16) hipLaunchKernelGGL(act_dequant8_kernel<bf16_t>, grid, block, 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(act_dequant8_kernel<float>, grid, block, 0, (hipStream_t)stream, p);
+    if (act == 0) ACT8_ONE(act_dequant8_kernel, 0);
+    else ACT8_BY_ACT(act_dequant8_kernel);
     M4D_CHECK_LAUNCH("act_dequant8");
     return 0;
 }
@@ -273,11 +286,11 @@ extern "C" int m4d_act_dequant8_t(m4d_dtype dt, const int8_t* codes, const uint8
     const int gy = (C + 127) / 128;
     M4D_CHECK_ARG(gx < (1ll << 31) && gy <= 65535, "act_dequant8_t: too large");
     Act8Args p{};
-    p.out = out; p.ld_out = ldo; p.codes = (int8_t*)codes; p.exps = (uint8_t*)exps; p.rows = rows; p.C = C; p.nb = nb; p.act = act;
+    p.out = out; p.ld_out = ldo; p.codes = (int8_t*)codes; p.exps = (uint8_t*)exps; p.rows = rows; p.C = C; p.nb = nb;
     p.rows_pad = rows_pad;
     dim3 grid((unsigned)gx, (unsigned)gy), block(256);
-    if (dt == M4D_BF16) hipLaunchKernelGGL(act_dequant8_t_kernel<bf16_t>, grid, block, 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(act_dequant8_t_kernel<float>, grid, block, 0, (hipStream_t)stream, p);
+    if (act == 0) ACT8_ONE(act_dequant8_t_kernel, 0);
+    else ACT8_BY_ACT(act_dequant8_t_kernel);
     M4D_CHECK_LAUNCH("act_dequant8_t");
     return 0;
 }
@@ -289,11 +302,10 @@ extern "C" int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int
     M4D_CHECK_ARG(dy && out && (rows == 1 || (ldy >= C && ldo >= C)), "act_bwd8: null pointer or row stride below C=%d", C);
     Act8Args p{};
     p.in = dy; p.ld_in = ldy; p.out = out; p.ld_out = ldo; p.codes = (int8_t*)codes; p.exps = (uint8_t*)exps;
-    p.rows = rows; p.C = C; p.nb = nb; p.act = act;
+    p.rows = rows; p.C = C; p.nb = nb;
     p.vec = ((uintptr_t)dy % 16) == 0 && ((uintptr_t)out % 16) == 0 && (ldy * es) % 16 == 0 && (ldo * es) % 16 == 0;
     dim3 grid(grid_of(rows * ((C + 7) / 8))), block(256);
-    if (dt == M4D_BF16) hipLaunchKernelGGL(act_bwd8_kernel<bf16_t>, grid, block, 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(act_bwd8_kernel<float>, grid, block, 0, (hipStream_t)stream, p);
+    ACT8_BY_ACT(act_bwd8_kernel);
     M4D_CHECK_LAUNCH("act_bwd8");
     return 0;
 }

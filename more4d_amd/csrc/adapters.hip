@@ -119,14 +119,25 @@ M4D_DEV void quant_half(const float (&x)[16], int8_t* codes, uint8_t* exps, bool
 // 64, against 46 us of HBM time), NST - 1 chunks in flight, one barrier per chunk, two workgroups per CU.
 // Wave (s, h): slots 32 s + [0, 32) and rank tiles h, h + 2, ...; with one rank tile h takes every other 16 channels instead.  QUANT: each
 // wave also writes the codes of 16 of the piece's rows, two lanes per block of 32 channels, out of the same LDS.
-template <typename T, int RT> struct DownShape {
+// DEEP: fewer workgroups than CUs, each with the LDS of a whole CU: up to twelve chunks in flight, because alone a workgroup waits for memory (0.5
+// us a chunk with four stages).
+template <typename T, int RT, bool DEEP> struct DownShape {
     static constexpr int XB = 64 * 64 * sizeof(T), AB = RT * 64 * 32 * sizeof(T), STAGE = XB + AB;
-    static constexpr int NST = STAGE * 4 <= 80 * 1024 ? 4 : STAGE * 3 <= 80 * 1024 ? 3 : 2;
+    static constexpr int NST = DEEP ? (STAGE * 12 <= 144 * 1024 ? 12 : 144 * 1024 / STAGE) : STAGE * 4 <= 80 * 1024 ? 4 : STAGE * 3 <= 80 * 1024 ? 3 : 2;
     static constexpr int LDS = NST * STAGE;
 };
-template <typename T, int RT, bool QUANT>
+// s_waitcnt vmcnt(N * NU) lgkmcnt(0); s_barrier  with N = min(n, MAX)
+template <int MAX, int NU>
+M4D_DEV void wait_younger(int n) {
+    if constexpr (MAX > 0) {
+        if (n < MAX) { wait_younger<MAX - 1, NU>(n); return; }
+    }
+    static_assert(MAX * NU < 64, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(MAX * NU) : "memory");
+}
+template <typename T, int RT, bool QUANT, bool DEEP>
 __global__ __launch_bounds__(256, 2) void adapter_down_kernel(DownArgs p) {
-    typedef DownShape<T, RT> Sh;
+    typedef DownShape<T, RT, DEEP> Sh;
     typedef typename Frag8<T>::type frag_t;
     extern __shared__ __attribute__((aligned(16))) char ad_smem[];
     constexpr int ES = sizeof(T), NST = Sh::NST, RB = 64 * ES, CPR = RB / 16, RPU = 1024 / RB;      // bytes, 16-byte chunks of a row; rows of a request
@@ -188,10 +199,7 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(DownArgs p) {
     for (int c = c0; c < c1; ++c) {
         // chunk c has landed when at most the younger chunks' requests are pending (only loads are counted: a store in flight makes the wait
         // stricter); behind the barrier everybody's has, and nobody reads chunk c - 1 any more, whose stage the next request overwrites
-        const int younger = c1 - 1 - c;
-        if (NST > 2 && younger >= NST - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"((NST - 2) * NU) : "memory");
-        else if (NST == 4 && younger == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(NU) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        wait_younger<NST - 2, NU>(c1 - 1 - c);
         if (c + NST - 1 < c1) request(c + NST - 1);
         const char* st = ad_smem + ((c - c0) % NST) * Sh::STAGE;
         auto frag = [&](const char* q, int o0, int o1) {
@@ -268,6 +276,7 @@ __global__ __launch_bounds__(256) void adapter_down_join_kernel(DownArgs p) {
     const int64_t R32 = (p.R + 31) / 32 * 32;
     if (r >= R32) return;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int k = 0; k < p.KS; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += p.part[((k * p.n_pieces + piece) * R32 + r + e) * PIECE + slot];
@@ -480,7 +489,7 @@ Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, int ncu)
     Choice best{TILE_64x64, 1};
     double t_best = 1e30;
     auto offer = [&](double t, int kind, int S) { if (t < t_best) { t_best = t; best = Choice{kind, S}; } };
-    if (M <= 16) offer(4.0 + wbytes * (1.0 + M / 16.0) / 5.0e6, GEMV16, 1);
+    if (M <= 16) offer(4.0 + wbytes * (1.0 + M / 24.0) / 6.0e6, GEMV16, 1);
     if (wide_ok) {
         const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
         offer((double)((tiles + ncu - 1) / ncu) * (nk * 1.03 + 10.0), WIDE_256x256, 1);
@@ -498,7 +507,7 @@ Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, int ncu)
             double t = rounds * (per * f.c[bf16 ? 0 : 1][shared] + f.fix);
             const double floor = wbytes / 6.0e6;
             if (t < floor) t = floor;
-            if (S > 1) t += 3.0 + (double)M * N * (8.0 * S + es) / 4.5e6;
+            if (S > 1) t += 4.5 + (double)M * N * (8.0 * S + es) / 4.5e6;
             offer(t, f.kind, S);
         }
     }
@@ -532,12 +541,12 @@ extern "C" int m4d_adapter_pack(m4d_dtype dt, const void* a, const void* b, int 
     return 0;
 }
 
-template <typename T, int RT, bool QUANT>
+template <typename T, int RT, bool QUANT, bool DEEP>
 static int launch_down_q(const DownArgs& p, hipStream_t st) {
-    constexpr int LDS = DownShape<T, RT>::LDS;
+    constexpr int LDS = DownShape<T, RT, DEEP>::LDS;
     static PerDeviceOnce configured;
     if (configured.pending()) {
-        if (hipFuncSetAttribute((const void*)adapter_down_kernel<T, RT, QUANT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
+        if (hipFuncSetAttribute((const void*)adapter_down_kernel<T, RT, QUANT, DEEP>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
             (void)hipGetLastError();
             m4d_set_error("adapter_down: cannot enable %d bytes of LDS", LDS);
             return -3;
@@ -545,7 +554,7 @@ static int launch_down_q(const DownArgs& p, hipStream_t st) {
         configured.mark();
     }
     const int ny = ((p.R + 31) / 32 + RT - 1) / RT;
-    hipLaunchKernelGGL((adapter_down_kernel<T, RT, QUANT>), dim3((unsigned)((p.n_pieces + 7) / 8 * 8 * ny), (unsigned)p.KS), dim3(256), LDS, st, p);
+    hipLaunchKernelGGL((adapter_down_kernel<T, RT, QUANT, DEEP>), dim3((unsigned)((p.n_pieces + 7) / 8 * 8 * ny), (unsigned)p.KS), dim3(256), LDS, st, p);
     M4D_CHECK_LAUNCH("adapter_down");
     if (p.part) {
         hipLaunchKernelGGL(adapter_down_join_kernel<T>, dim3((unsigned)p.n_pieces, (unsigned)((p.R + 31) / 32 * 2)), dim3(256), 0, st, p);
@@ -554,7 +563,11 @@ static int launch_down_q(const DownArgs& p, hipStream_t st) {
     return 0;
 }
 template <typename T, int RT>
-static int launch_down(const DownArgs& p, hipStream_t st) { return p.codes ? launch_down_q<T, RT, true>(p, st) : launch_down_q<T, RT, false>(p, st); }
+static int launch_down(const DownArgs& p, hipStream_t st) {
+    const int64_t blocks = (int64_t)p.n_pieces * p.KS * (((p.R + 31) / 32 + RT - 1) / RT);
+    if (blocks <= cus()) return p.codes ? launch_down_q<T, RT, true, true>(p, st) : launch_down_q<T, RT, false, true>(p, st);
+    return p.codes ? launch_down_q<T, RT, true, false>(p, st) : launch_down_q<T, RT, false, false>(p, st);
+}
 
 // K slices of a down projection with few pieces: as many as fill half the chip, each at least eight chunks of 64 channels.  (A piece's K loop is
 // serial: 16 pieces of K = 4096 took 20 us on 16 CUs, in slices and joined 10.)
@@ -562,7 +575,7 @@ static int down_slices(int n_pieces, int64_t K) {
     const int nc = (int)((K + 63) / 64);
     int ks = n_pieces > 0 ? cus() / 2 / n_pieces : 1;
     if (ks > nc / 8) ks = nc / 8;
-    if (ks < 2) return 1;
+    if (ks < 2 || nc <= 40) return 1;            // (up to 40 chunks the second launch costs what the slices save)
     const int per = (nc + ks - 1) / ks;
     return (nc + per - 1) / per;                 // (no empty slices)
 }

@@ -135,6 +135,7 @@ __global__ __launch_bounds__(64 * WM * WN) void adapter_gemm_kernel(AdGemmArgs p
             }
         }
     };
+    const AdTile<MI> ad_tile = adapters_tile<MI>(p, tm, m0 + wm * MI * 32, lane, (int)blockIdx.y);      // (a slice takes every S-th adapter)
     const int n_tiles = kt1 - kt0;
     if (n_tiles > 0) {
 #pragma unroll
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(64 * WM * WN) void adapter_gemm_kernel(AdGemmArgs p
         for (; kt < kt1 - 1; ++kt) tile(kt, std::false_type{}, std::true_type{}, kt1 - 2 - kt);
         tile(kt, std::false_type{}, std::false_type{}, 0);
     }
-    adapters_extend<T, NI, MI>(p, acc, tm, m0 + wm * MI * 32, n0 + wn * NI * 32, lane, (int)blockIdx.y, p.S);
+    adapters_extend<T, NI, MI>(p, acc, ad_tile, m0 + wm * MI * 32, n0 + wn * NI * 32, lane, p.S);
 
     // out of the accumulator layout (lane = row) through LDS: 4 consecutive columns per lane, whole rows per group of lanes
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");

@@ -155,50 +155,66 @@ M4D_DEV void epilogue_tile(const GemmArgs& p, const f32x16& acc, int64_t m, int6
 // MFMA layout (16 bytes per lane and 16 ranks; a block's 32 rows of R ranks are contiguous memory): through LDS they would need two more
 // barriers.  All loads of 64 ranks are issued before their first product, so a tile pays one L2 latency per 64 ranks and adapter, not four.
 // Rows of u that name another adapter (or none: their u was never written) are replaced by zero before the product, not multiplied by zero.
+// AdTile: what the extension has to know about its tile, loaded in front of the K loop (behind it these would be three dependent trips to L2).
+template <int MI> struct AdTile { int i0, i1, g0; int ra[MI]; };
+template <int MI>
+M4D_DEV AdTile<MI> adapters_tile(const GemmAdArgs& p, int tile, int64_t m_base, int lane, int first = 0) {
+    AdTile<MI> a;
+    a.i0 = __builtin_amdgcn_readfirstlane(p.tile_off[tile]) + first;
+    a.i1 = __builtin_amdgcn_readfirstlane(p.tile_off[tile + 1]);
+    a.g0 = a.i0 < a.i1 ? __builtin_amdgcn_readfirstlane(p.tile_list[a.i0]) : 0;
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+        const int64_t m = m_base + mi * 32 + (lane & 31);
+        a.ra[mi] = m < p.M ? p.row_adapter[m] : -1;
+    }
+    return a;
+}
 template <typename T, int NI, int MI>
-M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], int tile, int64_t m_base, int64_t n_base, int lane, int first = 0,
-                             int step = 1) {
+M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const AdTile<MI>& a, int64_t m_base, int64_t n_base, int lane, int step = 1) {
     typedef typename Frag8<T>::type frag_t;
     constexpr int U = sizeof(T) == 2 ? 4 : 1;         // 16-rank steps in flight (float32 fragments are twice as wide, and MFMA-bound)
     const int li = lane & 31, hi = lane >> 5;
-    const int i0 = __builtin_amdgcn_readfirstlane(p.tile_off[tile]) + first, i1 = __builtin_amdgcn_readfirstlane(p.tile_off[tile + 1]);
-    if (i0 >= i1) return;
-    int ra[MI];
+    if (a.i0 >= a.i1) return;
     const T* pu[MI];
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
         const int64_t m = m_base + mi * 32 + li;
-        ra[mi] = m < p.M ? p.row_adapter[m] : -1;
         pu[mi] = (const T*)p.u + (m < p.M ? m : 0) * p.R + hi * 8;
     }
     int64_t nr[NI];                                   // (columns beyond N are computed from row N - 1 and not stored)
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) nr[ni] = min(n_base + ni * 32 + li, p.N - 1) * p.R + hi * 8;
-    for (int i = i0; i < i1; i += step) {
-        const int g = __builtin_amdgcn_readfirstlane(p.tile_list[i]);
+    for (int i = a.i0; i < a.i1; i += step) {
+        const int g = i == a.i0 ? a.g0 : __builtin_amdgcn_readfirstlane(p.tile_list[i]);
         const T* b = (const T*)p.up + (int64_t)g * p.N * p.R;
-        for (int k = 0; k < p.R; k += 16 * U) {
-            frag_t fu[U][MI], fb[U][NI];
+        // C steps of 16 ranks: all loads (without predicates: rows of other adapters are replaced after the load), then the products
+        auto chunk = [&](auto C_T, int k) {
+            constexpr int C = decltype(C_T)::value;
+            frag_t fu[C][MI], fb[C][NI];
 #pragma unroll
-            for (int s = 0; s < U; ++s) {
-                // (loads without predicates: what a row or a rank beyond R must not contribute is replaced after the load)
-                const int ks = min(k + s * 16, p.R - 16);
+            for (int s = 0; s < C; ++s) {
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi) fu[s][mi] = *reinterpret_cast<const frag_t*>(pu[mi] + ks);
+                for (int mi = 0; mi < MI; ++mi) fu[s][mi] = *reinterpret_cast<const frag_t*>(pu[mi] + k + s * 16);
 #pragma unroll
-                for (int ni = 0; ni < NI; ++ni) fb[s][ni] = *reinterpret_cast<const frag_t*>(b + nr[ni] + ks);
+                for (int ni = 0; ni < NI; ++ni) fb[s][ni] = *reinterpret_cast<const frag_t*>(b + nr[ni] + k + s * 16);
             }
 #pragma unroll
-            for (int s = 0; s < U; ++s)
+            for (int s = 0; s < C; ++s) {
 #pragma unroll
                 for (int mi = 0; mi < MI; ++mi)
-                    if (ra[mi] != g || k + s * 16 >= p.R) fu[s][mi] = frag_t{};
-#pragma unroll
-            for (int s = 0; s < U; ++s)
+                    if (a.ra[mi] != g) fu[s][mi] = frag_t{};
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
                     for (int mi = 0; mi < MI; ++mi) mma32(fb[s][ni], fu[s][mi], acc[ni][mi]);
+            }
+        };
+        int k = 0;
+        for (; k + 16 * U <= p.R; k += 16 * U) chunk(std::integral_constant<int, U>{}, k);
+        if constexpr (U == 4) {
+            if (k + 32 <= p.R) { chunk(std::integral_constant<int, 2>{}, k); k += 32; }
+            if (k < p.R) chunk(std::integral_constant<int, 1>{}, k);
         }
     }
 }

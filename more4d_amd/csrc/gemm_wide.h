@@ -416,6 +416,8 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
         W_STG_I(R, VOFF, H, G, BUFB, 2); W_STG_I(R, VOFF, H, G, BUFB, 3); W_ADV(VOFF, KC, DLT);                  \
     } while (0)
 
+    AdTile<4> ad_tile;
+    if constexpr (AD) ad_tile = adapters_tile<4>(p, tm, m0 + wm * 128, lane);
     const T* bias = (const T*)p.bias;
     // PERSIST: the bias of the wave's 128 columns travels like the operands — ONE LDS-DMA instruction (4 bytes per lane) at the start of
     // a tile into the wave's epilogue block, which nothing touches before the epilogue — so it retires in order with the stagings under
@@ -564,12 +566,12 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
             for (int h = 0; h < 2; ++h) asm volatile("" :: "v"(fa0[h][kk]), "v"(fa1[h][kk]), "v"(fbx[h][kk]), "v"(fby[h][kk]));
+        adapters_extend<T, 4, 4>(p, acc, ad_tile, m0 + wm * 128, n0 + wn * 128, lane);      // (its loads fly with the last stagings)
     }
     if constexpr (ABL & 64) ts[2] = __builtin_readcyclecounter();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the redundant tail stagings must land before the LDS is re-used
     __builtin_amdgcn_s_barrier();
     if constexpr (ABL & 64) ts[3] = __builtin_readcyclecounter();
-    if constexpr (AD) adapters_extend<T, 4, 4>(p, acc, tm, m0 + wm * 128, n0 + wn * 128, lane);
     char* wl = dyn_smem + wave * 16384;
     // (the host sends bf16 outputs whose rows are not 16-byte aligned, and the erf-GELU / SiLU epilogues of a few small GEMMs, to
     // gemm_bt256p_kernel)

@@ -1064,19 +1064,19 @@ def adamw_(p, g, m, v, *, lr, beta1, beta2, eps, weight_decay, step, grad_scale=
 _NO_GUARD = contextlib.nullcontext()
 
 
-def _same_device(name, *ts):
+def _same_device(name, first, *rest):
     """All tensors on one HIP device; returns a guard that makes it current (its current stream is the one launched on)."""
-    _dev(*ts)
-    d = ts[0].device
-    for t in ts:
-        if t is not None and t.device != d:
-            raise ValueError(f"{name}: tensors on different devices {d} and {t.device}")
-    return _NO_GUARD if d.index == torch.cuda.current_device() else torch.cuda.device(d)
+    _dev(first, *rest)
+    d = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"{name}: tensors on different devices {first.device} and {t.device}")
+    return _NO_GUARD if d == torch._C._cuda_getDevice() else torch.cuda.device(d)
 
 
 def _raw_stream(t):
     """The current stream of the tensor's device, as _stream() gives it, without the stream object (a microsecond per call)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 class Act8:
@@ -1186,7 +1186,7 @@ class AdapterBank:
     """The adapters of one projection: a [G, r, K], b [G, N, r] (one dtype, contiguous), scale: G numbers or a float32 tensor [G] (adapters of
     different ranks: pad the smaller ones with zeros).  Laid out for the kernels once, here (m4d_adapter_pack): later changes of a and b are not
     seen.  backward=True lays out the transposed operands of the backward pass as well (`transposed`)."""
-    __slots__ = ("down", "up", "scale", "G", "rank", "R", "K", "N", "back")
+    __slots__ = ("buf", "scale", "G", "rank", "R", "K", "N", "_down", "_up", "_back")
 
     def __init__(self, a, b, scale, *, backward=False):
         if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
@@ -1215,23 +1215,20 @@ class AdapterBank:
         at = [0]
         for v in n:
             at.append(at[-1] + -(-v // 64) * 64)
-        buf = torch.empty(at[-1], device=a.device, dtype=a.dtype)
-        parts = [buf[o:o + v] for o, v in zip(at, n)]
-        self.down, self.up = parts[0], parts[1].view(G, N, self.R)
-        self.back = None
-        if backward:
-            self.back = AdapterBank.__new__(AdapterBank)
-            self.back.down, self.back.up, self.back.scale, self.back.back = parts[2], parts[3].view(G, K, self.R), scale, None
-            self.back.G, self.back.rank, self.back.R, self.back.K, self.back.N = G, r, self.R, N, K
-        with _same_device("AdapterBank", a, b):
-            check(lib.m4d_adapter_pack(dt, _ptr(a), _ptr(b), G, r, K, N, self.R, _ptr(self.down), _ptr(self.up),
-                                       _ptr(parts[2]) if backward else 0, _ptr(parts[3]) if backward else 0, _raw_stream(a)), "m4d_adapter_pack")
+        self.buf = torch.empty(at[-1], device=a.device, dtype=a.dtype)
+        p = [self.buf.data_ptr() + o * a.element_size() for o in at[:-1]] + [0, 0]
+        self._down, self._up, self._back = p[0], p[1], p[2:4] if backward else None
+        with _same_device("AdapterBank", a, b, self.buf):
+            check(lib.m4d_adapter_pack(dt, _ptr(a), _ptr(b), G, r, K, N, self.R, *p[:4], _raw_stream(a)), "m4d_adapter_pack")
 
     def transposed(self):
         """The bank of the backward pass, v = s dy B and dx = dy W + v A: the down projection maps N channels, the up projection gives K."""
-        if self.back is None:
+        if self._back is None:
             raise ValueError("AdapterBank: built without backward=True")
-        return self.back
+        t = AdapterBank.__new__(AdapterBank)
+        t.buf, t.scale, t.G, t.rank, t.R, t.K, t.N = self.buf, self.scale, self.G, self.rank, self.R, self.N, self.K
+        t._down, t._up, t._back = *self._back, None
+        return t
 
 
 class AdapterPlan:
@@ -1310,8 +1307,8 @@ def _check_adapters(name, x, bank, plan):
         raise ValueError(f"{name}: {rows} rows against a plan of {plan.rows}")
     if plan.n_adapters > bank.G:
         raise ValueError(f"{name}: the plan names adapter {plan.n_adapters - 1}, the bank has {bank.G}")
-    if bank.up.dtype != x.dtype:
-        raise TypeError(f"{name}: x {x.dtype} vs adapters {bank.up.dtype}")
+    if bank.buf.dtype != x.dtype:
+        raise TypeError(f"{name}: x {x.dtype} vs adapters {bank.buf.dtype}")
     if -(-bank.K // 8) * 8 < x.shape[-1] or bank.K > x.shape[-1]:       # (rows may be zero-padded to whole 16-byte chunks)
         raise ValueError(f"{name}: x has {x.shape[-1]} channels, the adapters {bank.K}")
     return rows, ldx
@@ -1328,10 +1325,10 @@ def adapter_down(x, bank, plan, *, rows=True, slots=False):
     u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype) if rows else None
     ut = torch.empty(_slots_shape(bank, plan), device=x.device, dtype=x.dtype) if slots else None
     lib = _lib.load()
-    with _same_device("adapter_down", x, bank.up, plan.table):
+    with _same_device("adapter_down", x, bank.buf, plan.table):
         nws = lib.m4d_adapter_down_workspace(plan.args, x.shape[-1], bank.R)
         ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
-        check(lib.m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, _ptr(bank.down), _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut), 0, 0,
+        check(lib.m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, bank._down, _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut), 0, 0,
                                    x.shape[-1], bank.R, _ptr(ws), nws, _raw_stream(x)), "m4d_adapter_down")
     return u, ut
 
@@ -1369,11 +1366,11 @@ def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=Fals
     _, ldo = _rows2d(out)
     dt = dt_code(x.dtype)
     lib = _lib.load()
-    with _same_device("linear_adapters", x, w, bias, out, bank.up, plan.table):
+    with _same_device("linear_adapters", x, w, bias, out, bank.buf, plan.table):
         u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype)
         nws = lib.m4d_linear_adapters_workspace(dt, plan.args, N, K, bank.R)
         ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
-        check(lib.m4d_linear_adapters(dt, _ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(bank.down), _ptr(bank.scale), _ptr(bank.up), plan.args,
+        check(lib.m4d_linear_adapters(dt, _ptr(x), ldx, _ptr(w), ldw, _ptr(bias), bank._down, _ptr(bank.scale), bank._up, plan.args,
                                       _ptr(u), _ptr(ut), *(x8._ptrs() if keep8 else (0, 0)), _ptr(out), ldo, N, K, bank.R, _ptr(ws), nws,
                                       _raw_stream(x)), "m4d_linear_adapters")
     return ret
