@@ -520,27 +520,27 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
  *   chunks[l] [n_chunks[l]][3]   pieces [first, last), at most 64, of one adapter: the unit of the row contraction, at four granularities from
  *                                coarse to fine; chunk_off[l] [n_adapters + 1] into it
  *   tiles_off[i], tiles[i]       the adapters of the rows of each tile, each once, for tiles of 64, 128 and 256 rows and (i = 3) of 256 rows
- *                                whose last one is rows [rows - 256, rows)
+ *                                whose last one is rows [rows - 256, rows); tile_one: for the latter, the adapter of all of a tile's rows, or -1
  *   adapter_down     u T [rows, R] and / or ut = s_g x A_g^T (u's rows without an adapter are not written).  ut T [4 * n_pieces][ceil(R / 32)][64][8]:
  *                    slot s, rank r at [s / 16][r / 32][r % 32 + 32 * (s % 16 / 8)][s % 8], zero for pad slots and ranks beyond R;
  *                    codes / exps (may be NULL): the 8-bit form of x's rows with an adapter, as act_quant8 writes it;
- *                    ws: adapter_down_workspace floats
+ *                    ws: adapter_down_workspace floats (slots: ut or codes will be asked for)
  *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once.  With a_down, u (and ut, codes, exps if given) are written first, by
  *                    adapter_down; without, u is an input.  ws: linear_adapters_workspace floats
  *   adapter_grad     out T [G, rank, C] (transposed: [G, C, rank]) = sum over the rows of g of v^T x, vt as adapter_down writes ut, x as T or as
  *                    8-bit codes; ws: adapter_grad_workspace floats; partial sums are joined in a fixed order. */
 typedef struct {
-    const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks[4], *chunk_off[4], *tiles_off[4], *tiles[4];
+    const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks[4], *chunk_off[4], *tiles_off[4], *tiles[4], *tile_one;
     int64_t rows;
-    int32_t n_pieces, n_adapters, n_chunks[4];
+    int32_t n_pieces, n_adapters, n_chunks[4], n_listed;      /* n_listed: entries of tiles[0] */
 } m4d_adapter_plan;
 int64_t m4d_adapter_down_elems(int G, int R, int64_t K);
 int m4d_adapter_pack(m4d_dtype dt, const void* a, const void* b, int G, int rank, int64_t K, int64_t N, int R, void* a_down, void* b_up, void* b_down,
                      void* a_up, m4d_stream stream);
-int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int64_t K, int R);
+int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int64_t K, int R, int slots);
 int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan, void* u, void* ut,
                      int8_t* codes, uint8_t* exps, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream);
-int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R);
+int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R, int slots);
 int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, const void* W, int64_t ldw, const void* bias, const void* a_down, const float* scale,
                         const void* b_up, const m4d_adapter_plan* plan, void* u, void* ut, int8_t* codes, uint8_t* exps, void* out, int64_t ldo,
                         int64_t N, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream);

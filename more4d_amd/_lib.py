@@ -33,8 +33,8 @@ class AttnBwdArgs(Structure):
 
 class AdapterPlanArgs(Structure):      # m4d_adapter_plan
     _fields_ = [("row_adapter", c_void_p), ("slot_row", c_void_p), ("piece_adapter", c_void_p), ("chunks", c_void_p * 4),
-                ("chunk_off", c_void_p * 4), ("tiles_off", c_void_p * 4), ("tiles", c_void_p * 4), ("rows", c_int64), ("n_pieces", c_int32),
-                ("n_adapters", c_int32), ("n_chunks", c_int32 * 4)]
+                ("chunk_off", c_void_p * 4), ("tiles_off", c_void_p * 4), ("tiles", c_void_p * 4), ("tile_one", c_void_p), ("rows", c_int64), ("n_pieces", c_int32),
+                ("n_adapters", c_int32), ("n_chunks", c_int32 * 4), ("n_listed", c_int32)]
 
 
 # name -> (restype, argtypes); mirrors include/more4d_hip.h one to one
@@ -151,10 +151,10 @@ SIGNATURES = {
     "m4d_act_bwd8": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
     "m4d_adapter_down_elems": (c_int64, [c_int, c_int, c_int64]),
     "m4d_adapter_pack": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int] + [c_void_p] * 5),
-    "m4d_adapter_down_workspace": (c_int64, [POINTER(AdapterPlanArgs), c_int64, c_int]),
+    "m4d_adapter_down_workspace": (c_int64, [POINTER(AdapterPlanArgs), c_int64, c_int, c_int]),
     "m4d_adapter_down": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_void_p, POINTER(AdapterPlanArgs)] + [c_void_p] * 4 +
                          [c_int64, c_int, c_void_p, c_int64, c_void_p]),
-    "m4d_linear_adapters_workspace": (c_int64, [c_int, POINTER(AdapterPlanArgs), c_int64, c_int64, c_int]),
+    "m4d_linear_adapters_workspace": (c_int64, [c_int, POINTER(AdapterPlanArgs), c_int64, c_int64, c_int, c_int]),
     "m4d_linear_adapters": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                     POINTER(AdapterPlanArgs)] + [c_void_p] * 5 + [c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
     "m4d_adapter_grad_workspace": (c_int64, [POINTER(AdapterPlanArgs), c_int64, c_int]),

@@ -268,6 +268,50 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(DownArgs p) {
         }
 }
 
+// The same for at most 16 rows (single tokens): a workgroup takes 16 ranks of one adapter, its eight waves the chunks of K in turn, straight from
+// memory into the 16 x 16 x 32 MFMA; all rows are multiplied by every adapter and only its own are kept.  One launch instead of slices and
+// their join: K = 5120, six adapters 12 us -> 5.
+template <typename T>
+__global__ __launch_bounds__(64 * SKINNY_WAVES) void adapter_down16_kernel(DownArgs p, const int* row_adapter, const int* adapters, int rows) {
+    typedef typename Frag8<T>::type frag_t;
+    __shared__ f32x4 red[SKINNY_WAVES][64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, i16 = lane & 15, q = lane >> 4;
+    const int g = adapters[blockIdx.x], r0 = blockIdx.y * 16, nc = (p.K + 63) >> 6, rts = (p.R + 31) >> 5;
+    const int row = min(i16, rows - 1);
+    // of a chunk's packed operand (channel 32 hi + 8 kk + e at [rt][kk][rank + 32 hi][e]) quarter q of the wave takes hi = q & 1, kk = 2 j + (q >> 1)
+    const T* a = (const T*)p.a + ((int64_t)g * nc * rts + (r0 >> 5)) * 2048 + (q >> 1) * 512 + ((r0 & 16) + i16 + 32 * (q & 1)) * 8;
+    const T* x = (const T*)p.x + (int64_t)row * p.ldx + (q & 1) * 32 + (q >> 1) * 8;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    int c = wave;
+    constexpr int U = 4;
+    for (; c + (U - 1) * SKINNY_WAVES < nc - 1; c += U * SKINNY_WAVES) {      // whole chunks: all loads first
+        frag_t fa[U][2], fx[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                fa[u][j] = *reinterpret_cast<const frag_t*>(a + (int64_t)(c + u * SKINNY_WAVES) * rts * 2048 + j * 1024);
+                fx[u][j] = *reinterpret_cast<const frag_t*>(x + (c + u * SKINNY_WAVES) * 64 + j * 16);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) mma16(fa[u][j], fx[u][j], acc);
+    }
+    for (; c < nc; c += SKINNY_WAVES)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            mma16(*reinterpret_cast<const frag_t*>(a + (int64_t)c * rts * 2048 + j * 1024), load_k8<T>(x, c * 64 + j * 16, p.K - (q & 1) * 32 - (q >> 1) * 8), acc);
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && i16 < rows && row_adapter[i16] == g) {
+        f32x4 v = red[0][lane];
+#pragma unroll
+        for (int k = 1; k < SKINNY_WAVES; ++k) v += red[k][lane];
+        store4((T*)p.u + (int64_t)i16 * p.R + r0 + q * 4, v * p.scale[g]);
+    }
+}
+
 // the K slices' sums of four ranks of one slot, in slice order
 template <typename T>
 __global__ __launch_bounds__(256) void adapter_down_join_kernel(DownArgs p) {
@@ -570,18 +614,20 @@ static int launch_down(const DownArgs& p, hipStream_t st) {
 }
 
 // K slices of a down projection with few pieces: as many as fill half the chip, each at least eight chunks of 64 channels.  (A piece's K loop is
-// serial: 16 pieces of K = 4096 took 20 us on 16 CUs, in slices and joined 10.)
+// serial, 0.5 us a chunk where a workgroup is alone on its CU: K = 1536 12 us, in three slices and joined 8; K = 4096 32 and 10.)
 static int down_slices(int n_pieces, int64_t K) {
     const int nc = (int)((K + 63) / 64);
     int ks = n_pieces > 0 ? cus() / 2 / n_pieces : 1;
     if (ks > nc / 8) ks = nc / 8;
-    if (ks < 2 || nc <= 40) return 1;            // (up to 40 chunks the second launch costs what the slices save)
+    if (ks < 2) return 1;
     const int per = (nc + ks - 1) / ks;
     return (nc + per - 1) / per;                 // (no empty slices)
 }
+// at most 16 rows, and only u wanted (serving single tokens): adapter_down16_kernel
+static bool down_few(const m4d_adapter_plan* plan, const void* ut, const void* codes) { return plan->rows <= 16 && !ut && !codes; }
 
-extern "C" int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int64_t K, int R) {
-    if (!plan || K <= 0 || R <= 0) return 0;
+extern "C" int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int64_t K, int R, int slots) {
+    if (!plan || K <= 0 || R <= 0 || (plan->rows <= 16 && !slots)) return 0;
     const int ks = down_slices(plan->n_pieces, K);
     return ks > 1 ? (int64_t)ks * plan->n_pieces * ((R + 31) / 32 * 32) * PIECE : 0;
 }
@@ -597,7 +643,16 @@ extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const 
     if (plan->n_pieces == 0) return 0;
     M4D_CHECK_ARG(plan->slot_row && plan->piece_adapter, "adapter_down: bad plan");
     const int ks = down_slices(plan->n_pieces, K);
-    const int64_t need = m4d_adapter_down_workspace(plan, K, R);
+    if (down_few(plan, ut, codes)) {
+        M4D_CHECK_ARG(plan->row_adapter && plan->tiles[0] && plan->n_listed > 0 && plan->n_listed <= 16, "adapter_down: bad plan");
+        DownArgs p{x, a_down, scale, u, nullptr, nullptr, nullptr, nullptr, nullptr, ldx, (int)K, R, plan->n_pieces, 1, nullptr};
+        dim3 grid((unsigned)plan->n_listed, (unsigned)(R / 16)), block(64 * SKINNY_WAVES);
+        if (dt == M4D_BF16) hipLaunchKernelGGL(adapter_down16_kernel<bf16_t>, grid, block, 0, (hipStream_t)stream, p, plan->row_adapter, plan->tiles[0], (int)plan->rows);
+        else hipLaunchKernelGGL(adapter_down16_kernel<float>, grid, block, 0, (hipStream_t)stream, p, plan->row_adapter, plan->tiles[0], (int)plan->rows);
+        M4D_CHECK_LAUNCH("adapter_down");
+        return 0;
+    }
+    const int64_t need = m4d_adapter_down_workspace(plan, K, R, 1);
     M4D_CHECK_ARG(need == 0 || (ws && ws_floats >= need), "adapter_down: workspace of %lld floats needed", (long long)need);
     DownArgs p{x, a_down, scale, u, ut, codes, exps, plan->slot_row, plan->piece_adapter, ldx, (int)K, R,
                plan->n_pieces, ks, ks > 1 ? ws : nullptr};
@@ -634,10 +689,10 @@ static int launch_gemm(AdGemmArgs& p, hipStream_t st) {
 static bool wide_shape(m4d_dtype dt, int64_t M, int64_t N, int64_t K) { return dt == M4D_BF16 && K % 64 == 0 && M >= 512 && N >= 512; }
 
 // the down projection's slices and the GEMM's run one after the other: one workspace, the larger of the two
-extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R) {
+extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R, int slots) {
     if (!plan || plan->rows <= 0 || N <= 0 || K <= 0) return 0;
     const int64_t M = plan->rows;
-    int64_t most = m4d_adapter_down_workspace(plan, K, R);      // (whether the wide kernel can run depends on the output's alignment too: room for either choice)
+    int64_t most = m4d_adapter_down_workspace(plan, K, R, slots);      // (whether the wide kernel can run depends on the output's alignment too: room for either choice)
     for (int w = 0; w < 2; ++w) {
         const Choice c = choose(dt == M4D_BF16, M, N, K, w && wide_shape(dt, M, N, K), cus());
         if (c.S > 1 && c.S * M * N > most) most = c.S * M * N;
@@ -658,7 +713,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
     M4D_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)W % 16) == 0 && ((uintptr_t)out % 16) == 0 && ((uintptr_t)u % 16) == 0 && ((uintptr_t)b_up % 16) == 0,
                   "linear_adapters: pointers must be 16-byte aligned");
     M4D_CHECK_ARG(((uintptr_t)bias % (4 * es)) == 0, "linear_adapters: bias must be aligned to four elements");
-    M4D_CHECK_ARG(plan->row_adapter && plan->tiles_off[0] && plan->tiles_off[1] && plan->tiles_off[2] && plan->tiles[0] && plan->tiles[1] && plan->tiles[2],
+    M4D_CHECK_ARG(plan->row_adapter && plan->tiles_off[0] && plan->tiles_off[1] && plan->tiles_off[2] && plan->tiles[0] && plan->tiles[1] && plan->tiles[2] && plan->tile_one,
                   "linear_adapters: bad plan");
     const bool bf16 = dt == M4D_BF16;
     const bool wide_ok = wide_shape(dt, M, N, K) && ldo % 8 == 0 && ((uintptr_t)out % 32) == 0;
@@ -691,7 +746,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
         case TILE_256x128: return bf16 ? launch_gemm<bf16_t, 2, 2, 4, 2>(p, st) : launch_gemm<float, 4, 2, 2, 2>(p, st);
         default: break;
     }
-    p.tile_off = plan->tiles_off[3]; p.tile_list = plan->tiles[3];
+    p.tile_off = plan->tiles_off[3]; p.tile_list = plan->tiles[3]; p.tile_one = plan->tile_one;
     p.tiles_m = (int)((M + 255) / 256); p.tiles_n = (int)((N + 255) / 256);
     M4D_CHECK_ARG((int64_t)p.tiles_m * p.tiles_n < (1ll << 31), "linear_adapters: too many tiles");
     if (m4d_launch_gemm_wide_adapters(static_cast<const GemmAdArgs*>(&p), (unsigned)(p.tiles_m * p.tiles_n), st) != 0) {

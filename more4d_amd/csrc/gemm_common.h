@@ -40,6 +40,7 @@ struct GemmAdArgs : GemmArgs {
     const int* row_adapter;     // [M], -1 = none
     const int* tile_off;        // [tiles_m + 1] into tile_list
     const int* tile_list;       // adapters of the rows of each tile, each once
+    const int* tile_one;        // [tiles_m] the adapter that ALL rows of the tile name, or -1 (wide kernel only)
     int R;                      // multiple of 16
 };
 
@@ -171,11 +172,12 @@ M4D_DEV AdTile<MI> adapters_tile(const GemmAdArgs& p, int tile, int64_t m_base, 
     return a;
 }
 template <typename T, int NI, int MI>
-M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const AdTile<MI>& a, int64_t m_base, int64_t n_base, int lane, int step = 1) {
+M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const AdTile<MI>& a, int64_t m_base, int64_t n_base, int lane, int step = 1,
+                             int k0 = 0) {      // k0: ranks in front of it are already in
     typedef typename Frag8<T>::type frag_t;
     constexpr int U = sizeof(T) == 2 ? 4 : 1;         // 16-rank steps in flight (float32 fragments are twice as wide, and MFMA-bound)
     const int li = lane & 31, hi = lane >> 5;
-    if (a.i0 >= a.i1) return;
+    if (a.i0 >= a.i1 || k0 >= p.R) return;
     const T* pu[MI];
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
@@ -210,7 +212,7 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
                     for (int mi = 0; mi < MI; ++mi) mma32(fb[s][ni], fu[s][mi], acc[ni][mi]);
             }
         };
-        int k = 0;
+        int k = k0;
         for (; k + 16 * U <= p.R; k += 16 * U) chunk(std::integral_constant<int, U>{}, k);
         if constexpr (U == 4) {
             if (k + 32 <= p.R) { chunk(std::integral_constant<int, 2>{}, k); k += 32; }

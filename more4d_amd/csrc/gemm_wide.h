@@ -325,11 +325,41 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
     if constexpr (!(ABL & 1)) asm volatile("s_add_u32 m0, %0, %3\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(ldsw), "v"(VOFF), "s"(SRC), "i"(DSTOFF) : "memory", "m0", "scc")
     // instruction I (0..3) of the group (operand rows R, half H, group offset G) for the K-tile buffer BUFB (0 / W_BUF)
 #define W_STG_I(R, VOFF, H, G, BUFB, I) W_GLDS(VOFF, R[((I) >> 1) * 4 + (H) * 2 + ((I) & 1)], (BUFB) + (G) + (I) * 4096)
-#define W_ADV(VOFF, KC, DLT)                                                                                 \
+    // AD: a tile whose rows all name one adapter (p.tile_one) appends whole 64-rank K-tiles of u and up_g to its K loop: a group whose staging
+    // reaches K-tile nk goes over to their rows.  (Behind the loop, with the pipe empty, the same ranks cost two to three times as much.)
+    int nkt = nk, ad_one = -1;
+    const char *ad_u = nullptr, *ad_b = nullptr;
+    unsigned ad_off = 0;
+    if constexpr (AD) {
+        ad_one = __builtin_amdgcn_readfirstlane(p.tile_one[tm]);
+        if (ad_one >= 0) {
+            nkt = nk + (p.R >> 6);
+            ad_u = uniform_ptr((const char*)p.u + m0 * p.R * 2);
+            ad_b = uniform_ptr((const char*)p.up + ((int64_t)ad_one * p.N + n0) * p.R * 2);
+            const int u = wave * 8 + lrow;
+            ad_off = (unsigned)((u * p.R + (pc ^ ((u >> 1) & 7)) * 8) * 2);
+        }
+    }
+    auto ad_switch = [&](const char* (&r)[8], const char* base, int h, unsigned& voff) {
+        if constexpr (AD) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int jx = (i >> 1) * 4 + h * 2 + (i & 1), row = (jx >> 2) * 128 + ((jx >> 1) & 1) * 64 + (jx & 1) * 32;
+                r[jx] = uniform_ptr(base + (int64_t)row * p.R * 2);
+            }
+            voff = ad_off;
+        }
+    };
+    constexpr bool W_TAIL = true;      // (AD: false in the part of the K loop that stages nothing at or beyond K-tile nk)
+#define W_ADV(VOFF, KC, DLT, R, H)                                                                           \
     do {                                                                                                     \
         KC += 1;                                                                                             \
         if constexpr (PERSIST) { const bool wrap_ = KC == nk; VOFF += wrap_ ? DLT : 128u; KC = wrap_ ? 0 : KC; }  \
-        else VOFF += (KC < nk) ? 128u : 0u;                                                                  \
+        else if constexpr (AD && !W_TAIL) VOFF += 128u;                                                      \
+        else if constexpr (AD) {                                                                             \
+            if (KC == nk && nkt > nk) ad_switch(R, &R == &ra ? ad_u : ad_b, H, VOFF);                         \
+            else VOFF += (KC < nkt) ? 128u : 0u;                                                             \
+        } else VOFF += (KC < nk) ? 128u : 0u;                                                                \
     } while (0)
     f32x16 acc[4][4];   // [ni][mi]: rows n, column m = lane (W is the MFMA's A operand, see gemm.hip)
 #pragma unroll
@@ -392,7 +422,7 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
         W_MMA(FN, FM, NB, MB, 2, 1, 0); W_PIN(); W_STG_I(SR, SV, SH, SG, SB, 1); W_PIN();                    \
         W_MMA(FN, FM, NB, MB, 2, 1, 1); W_PIN(); W_STG_I(SR, SV, SH, SG, SB, 2); W_PIN();                    \
         W_MMA(FN, FM, NB, MB, 3, 0, 0); W_PIN(); W_STG_I(SR, SV, SH, SG, SB, 3); W_PIN();                    \
-        W_MMA(FN, FM, NB, MB, 3, 0, 1); W_PIN(); W_ADV(SV, SK, SD); W_PIN();                                     \
+        W_MMA(FN, FM, NB, MB, 3, 0, 1); W_PIN(); W_ADV(SV, SK, SD, SR, SH); W_PIN();                                     \
         W_MMA(FN, FM, NB, MB, 3, 1, 0); W_MMA(FN, FM, NB, MB, 3, 1, 1); W_PIN();                            \
     } while (0)
     // K-tile KT in buffer (AMC, ANC) = byte offset BC, next K-tile's buffer (AMN, ANN) = BN; FX holds B0(KT) on entry, FY receives
@@ -413,7 +443,7 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
 #define W_STAGE(R, VOFF, KC, H, G, BUFB, DLT)                                                                   \
     do {                                                                                                   \
         W_STG_I(R, VOFF, H, G, BUFB, 0); W_STG_I(R, VOFF, H, G, BUFB, 1);                                   \
-        W_STG_I(R, VOFF, H, G, BUFB, 2); W_STG_I(R, VOFF, H, G, BUFB, 3); W_ADV(VOFF, KC, DLT);                  \
+        W_STG_I(R, VOFF, H, G, BUFB, 2); W_STG_I(R, VOFF, H, G, BUFB, 3); W_ADV(VOFF, KC, DLT, R, H);                  \
     } while (0)
 
     AdTile<4> ad_tile;
@@ -548,11 +578,18 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
     }
     {
         int kt = 0;
-        for (; kt + 1 < nk; kt += 2) {
+        if constexpr (AD) {      // the test for the switch costs 3 - 4 % in every phase: only the last six K-tiles make it (tile kt stages up to kt + 3)
+            constexpr bool W_TAIL = false;
+            for (; kt + 1 < nk - 4; kt += 2) {
+                W_KTILE(24, 24, fbx, fby, 0, W_BUF);
+                W_KTILE(24, 24, fby, fbx, W_BUF, 0);
+            }
+        }
+        for (; kt + 1 < nkt; kt += 2) {
             W_KTILE(24, 24, fbx, fby, 0, W_BUF);
             W_KTILE(24, 24, fby, fbx, W_BUF, 0);
         }
-        if (kt < nk) W_KTILE(24, 24, fbx, fby, 0, W_BUF);
+        if (kt < nkt) W_KTILE(24, 24, fbx, fby, 0, W_BUF);
     }
 #undef W_KTILE
 #undef W_PHASE
@@ -566,7 +603,7 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
             for (int h = 0; h < 2; ++h) asm volatile("" :: "v"(fa0[h][kk]), "v"(fa1[h][kk]), "v"(fbx[h][kk]), "v"(fby[h][kk]));
-        adapters_extend<T, 4, 4>(p, acc, ad_tile, m0 + wm * 128, n0 + wn * 128, lane);      // (its loads fly with the last stagings)
+        adapters_extend<T, 4, 4>(p, acc, ad_tile, m0 + wm * 128, n0 + wn * 128, lane, 1, (nkt - nk) * 64);      // (its loads fly with the last stagings)
     }
     if constexpr (ABL & 64) ts[2] = __builtin_readcyclecounter();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the redundant tail stagings must land before the LDS is re-used

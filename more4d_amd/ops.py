@@ -1279,10 +1279,14 @@ class AdapterPlan:
                 off.append(len(lst))
             return lst, off
 
+        one = []                                # the adapter of ALL rows of a (shifted) 256-row tile, or -1
+        for m in range(0, self.rows, 256):
+            lo = max(0, min(m, self.rows - 256))
+            one.append(int(row[lo]) if (row[lo:m + 256] == row[lo]).all() else -1)
         cs = [chunks(t) for t in (12, 24, 48, 96)]
         ts = [tiles(64), tiles(128), tiles(256), tiles(256, True)]
         parts = [row, np.concatenate(slots) if slots else [], pieces]
-        parts += [c[0] for c in cs] + [c[1] for c in cs] + [t[1] for t in ts] + [t[0] for t in ts]
+        parts += [c[0] for c in cs] + [c[1] for c in cs] + [t[1] for t in ts] + [t[0] for t in ts] + [one]
         parts = [np.asarray(v, dtype=np.int32) for v in parts]
         at, offs = 0, []
         for v in parts:
@@ -1297,8 +1301,10 @@ class AdapterPlan:
         a.row_adapter, a.slot_row, a.piece_adapter = ptr[:3]
         for k, name in enumerate(("chunks", "chunk_off", "tiles_off", "tiles")):
             getattr(a, name)[:] = ptr[3 + 4 * k:7 + 4 * k]
+        a.tile_one = ptr[19]
         a.rows, a.n_pieces, a.n_adapters = self.rows, self.n_pieces, self.n_adapters
         a.n_chunks[:] = [len(c[0]) // 3 for c in cs]
+        a.n_listed = len(ts[0][0])
 
 
 def _check_adapters(name, x, bank, plan):
@@ -1326,7 +1332,7 @@ def adapter_down(x, bank, plan, *, rows=True, slots=False):
     ut = torch.empty(_slots_shape(bank, plan), device=x.device, dtype=x.dtype) if slots else None
     lib = _lib.load()
     with _same_device("adapter_down", x, bank.buf, plan.table):
-        nws = lib.m4d_adapter_down_workspace(plan.args, x.shape[-1], bank.R)
+        nws = lib.m4d_adapter_down_workspace(plan.args, x.shape[-1], bank.R, int(slots))
         ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
         check(lib.m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, bank._down, _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut), 0, 0,
                                    x.shape[-1], bank.R, _ptr(ws), nws, _raw_stream(x)), "m4d_adapter_down")
@@ -1368,7 +1374,7 @@ def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=Fals
     lib = _lib.load()
     with _same_device("linear_adapters", x, w, bias, out, bank.buf, plan.table):
         u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype)
-        nws = lib.m4d_linear_adapters_workspace(dt, plan.args, N, K, bank.R)
+        nws = lib.m4d_linear_adapters_workspace(dt, plan.args, N, K, bank.R, int(ut is not None))
         ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
         check(lib.m4d_linear_adapters(dt, _ptr(x), ldx, _ptr(w), ldw, _ptr(bias), bank._down, _ptr(bank.scale), bank._up, plan.args,
                                       _ptr(u), _ptr(ut), *(x8._ptrs() if keep8 else (0, 0)), _ptr(out), ldo, N, K, bank.R, _ptr(ws), nws,
