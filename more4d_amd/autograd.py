@@ -29,11 +29,12 @@ def _tpad(x):
     return out
 
 
-def linear_bwd(x, w, dy, need_dx=True):
-    """y = x w^T + b.  x [R, K], w [N, K], dy [R, N] (all T) -> (dx [R, K] | None, dw [N, K], db float32 [N])."""
+def linear_bwd(x, w, dy, need_dx=True, xt=None):
+    """y = x w^T + b.  x [R, K], w [N, K], dy [R, N] (all T) -> (dx [R, K] | None, dw [N, K], db float32 [N]).
+    xt: x^T [K, Rp] padded like _tpad, in the place of x."""
     db = ops.colsum(dy)[0]
     dx = ops.gemm_bt(dy, ops.transpose(w)) if need_dx else None          # dy [R,N] . (w^T)[K,N]^T
-    dw = ops.gemm_bt(_tpad(dy), _tpad(x))                               # dy^T [N,Rp] . (x^T)[K,Rp]^T
+    dw = ops.gemm_bt(_tpad(dy), _tpad(x) if xt is None else xt)         # dy^T [N,Rp] . (x^T)[K,Rp]^T
     return dx, dw, db
 
 
@@ -295,9 +296,16 @@ def block_backward(blk, x0, e0, c, txt, txt_len, img, img_len, dres, saved=None,
 
     `saved` (STORE_KEYS -> tensor): outputs of the six big GEMMs and of the self-attention that the forward kept in
     HBM ("stored" blocks, see BlockFn); they are used instead of being recomputed — only the HBM-bound LayerNorm /
-    RMSNorm / GELU passes and the small cross-attention run again.  forward_only=True runs just the forward half and
+    RMSNorm / GELU passes and the small cross-attention run again.  An entry may be an ops.Act8 (8-bit form, half the memory of bf16):
+    the GELU input is then read as codes by the two passes that use it, the others are expanded when they are needed.  forward_only=True runs just the forward half and
     returns (x3, {STORE_KEYS}) — the same code path produces the stored tensors, so both modes are bit-identical."""
-    saved = saved or {}
+    saved = dict(saved) if saved else {}
+
+    def take(key):
+        """the stored tensor (None: recompute), expanded from its 8-bit form; the stash lets go of it"""
+        t = saved.pop(key, None)
+        return ops.act_dequant8(t) if isinstance(t, ops.Act8) else t
+
     from .models.wan_transformer4d import _f32
     B, Lp, C = x0.shape
     R = B * Lp
@@ -335,7 +343,7 @@ def block_backward(blk, x0, e0, c, txt, txt_len, img, img_len, dres, saved=None,
 
     # ================= recompute (reference :659-684) =================
     xn1 = ops.ln_modulate(x0, T, shift=e[:, 0], scale=e[:, 1], mod_stride=st, rows_per_sample=rps, eps=eps, **g1).view(R, C)
-    qkv_pre = saved.get("qkv_pre")
+    qkv_pre = take("qkv_pre")
     if qkv_pre is None:
         qkv_pre = torch.empty((R, 3 * C), device=dev, dtype=T)
         for j, lin in enumerate((sa.q, sa.k, sa.v)):
@@ -353,13 +361,13 @@ def block_backward(blk, x0, e0, c, txt, txt_len, img, img_len, dres, saved=None,
     wq_self = _folded_norm_weight(sa.norm_q.weight, d, c.f32cache) if fold else nw(sa.norm_q)
     sm = dict(scale=1.0 / LOG2E) if fold else {}
     ops.rmsnorm_rope(q, wq_self, k, nw(sa.norm_k), **rope)
-    o, lse1 = saved.get("o"), saved.get("lse1")
+    o, lse1 = take("o"), take("lse1")
     if o is None:
         vt = ops.transpose(v)                                        # V^T [C, R]
         lse1 = torch.empty((B, n, Lp), device=dev, dtype=torch.float32)
         o = ops.attention(q, [KV(k, vt, Lp * 3 * C, 3 * C, Lp, R, c.key_len)], B=B, Lq=Lp, heads=n, head_dim=d,
                           q_bs=Lp * 3 * C, q_ls=3 * C, lse=lse1, **sm).view(R, C)
-    y1 = saved.get("y1")
+    y1 = take("y1")
     if y1 is None:
         y1 = ops.gemm_bt(o, sa.o.weight, sa.o.bias)
     x1 = ops.resid_gate(x0, y1, gate=e[:, 2], gate_stride=st, rows_per_sample=rps)
@@ -367,7 +375,7 @@ def block_backward(blk, x0, e0, c, txt, txt_len, img, img_len, dres, saved=None,
         xn3 = ops.ln_modulate(x1, T, ln_w=f32(blk.norm3.weight), ln_b=f32(blk.norm3.bias), eps=eps).view(R, C)
     else:
         xn3 = ops.unary(x1, T).view(R, C)
-    qc_pre = saved.get("qc_pre")
+    qc_pre = take("qc_pre")
     if qc_pre is None:
         qc_pre = ops.gemm_bt(xn3, ca.q.weight, ca.q.bias)
     qc = qc_pre.clone()
@@ -392,16 +400,19 @@ def block_backward(blk, x0, e0, c, txt, txt_len, img, img_len, dres, saved=None,
                            q_bs=Lp * C, q_ls=C, lse=lse).view(R, C)
         oc = oo if oc is None else ops.add(oc, oo)
         cross.append((name, s2, Sp, valid, kl, vl, nk, k_pre, kk, vv, oo, lse))
-    yc = saved.get("yc")
+    yc = take("yc")
     if yc is None:
         yc = ops.gemm_bt(oc, ca.o.weight, ca.o.bias)
     x2 = ops.resid_gate(x1, yc)
     xn2 = ops.ln_modulate(x2, T, shift=e[:, 3], scale=e[:, 4], mod_stride=st, rows_per_sample=rps, eps=eps, **g2).view(R, C)
-    pre = saved.get("pre")
+    pre = saved.pop("pre", None)
     if pre is None:
         pre = ops.gemm_bt(xn2, blk.ffn[0].weight, blk.ffn[0].bias)
-    h = ops.unary(pre, T, act=ACT_GELU_TANH)
-    y2 = saved.get("y2")
+    pre8 = pre if isinstance(pre, ops.Act8) else None
+    y2 = take("y2")
+    # (with codes and the ffn output at hand nobody reads h itself: its transpose, the weight gradient's operand, comes from the codes below)
+    h = None if pre8 is not None and y2 is not None else \
+        ops.unary(pre, T, act=ACT_GELU_TANH) if pre8 is None else ops.act_dequant8(pre8, act=ACT_GELU_TANH)
     if y2 is None:
         y2 = ops.gemm_bt(h, blk.ffn[2].weight, blk.ffn[2].bias)
     if forward_only:
@@ -413,10 +424,14 @@ def block_backward(blk, x0, e0, c, txt, txt_len, img, img_len, dres, saved=None,
     de[:, 5].copy_(ops.colsum(dres2, y2, rows_per_group=rps))
     dy2 = ops.scale_cast(dres2, T, gate=e[:, 5], gate_stride=st, rows_per_sample=rps)
     del y2
-    dh, G["ffn.2.weight"], G["ffn.2.bias"] = linear_bwd(h, blk.ffn[2].weight, dy2)
+    dh, G["ffn.2.weight"], G["ffn.2.bias"] = linear_bwd(h, blk.ffn[2].weight, dy2,
+                                                        xt=ops.act_dequant8_t(pre8, act=ACT_GELU_TANH) if h is None else None)
     del h, dy2
-    ops.act_bwd_(dh, pre, ACT_GELU_TANH)
-    del pre
+    if pre8 is not None:
+        ops.act_bwd8(dh, pre8, ACT_GELU_TANH, out=dh)
+    else:
+        ops.act_bwd_(dh, pre, ACT_GELU_TANH)
+    del pre, pre8
     dxn2, G["ffn.0.weight"], G["ffn.0.bias"] = linear_bwd(xn2, blk.ffn[0].weight, dh)
     del dh
     dgf = None
@@ -499,14 +514,17 @@ def _folds_qscale(blk):
 
 
 class BlockFn(Function):
-    """WanAttentionBlock on the tape.  apply(x, e0, txt, img, gfeat, blk, c, txt_len, img_len, store, gmeta, *params);
+    """WanAttentionBlock on the tape.  apply(x, e0, txt, img, gfeat, blk, c, txt_len, img_len, (store, bits), gmeta, *params);
     gfeat = SiLU'd spatial-guidance features T [B, P, 768] (None without guidance), gmeta = (period, length).
 
     store=0: classic per-block gradient checkpointing (keep the block input, recompute everything in backward).
     store=2: the forward additionally keeps the outputs of the six big GEMMs and of the self-attention (STORE_KEYS,
     2.4 GB per block at L = 21 840, C = 5120) and the backward skips their recompute: fwd + bwd instead of fwd +
     recompute + bwd.  store=1 keeps only STORE_LITE (0.45 GB per block: the self-attention and ffn_down outputs, the
-    best recompute time per byte).  `WanTransformer4DModel.activation_budget_gb` decides how many blocks get which."""
+    best recompute time per byte).  `WanTransformer4DModel.activation_budget_gb` decides how many blocks get which.
+    bits=8 (`WanTransformer4DModel.activation_bits`) keeps what is stored in 8 bits (ops.act_quant8; the log-sum-exp stays float32): half the
+    bytes of bf16, so twice the blocks in the same budget; the block's output and its loss are those of bits=16, the gradients come from
+    the rounded activations."""
 
     @staticmethod
     def forward(ctx, x, e0, txt, img, gfeat, blk, c, txt_len, img_len, store, gmeta, *params):
@@ -514,6 +532,7 @@ class BlockFn(Function):
         if c.sp is not None and c.sp.world_size > 1:
             raise NotImplementedError("training uses data parallelism; sequence parallelism is the inference path")
         stash = None
+        store, bits = store if isinstance(store, tuple) else (store, 16)
         guid = (gfeat.detach(), gmeta[0], gmeta[1]) if gfeat is not None else None
         if store:   # 2: every GEMM / attention output, 1: STORE_LITE only
             out, stash = block_backward(blk, x.detach(), e0.detach().contiguous(), c, txt.detach(), txt_len,
@@ -521,6 +540,8 @@ class BlockFn(Function):
                                         guid=guid)
             if store == 1:
                 stash = {k: stash[k] for k in STORE_LITE}
+            if bits == 8:
+                stash = {k: t if k == "lse1" else ops.act_quant8(t) for k, t in stash.items()}
         elif blk.ffn[0].weight.dtype == torch.bfloat16 and not _folds_qscale(blk):
             # bf16 without the folded softmax scale (qk_norm=False, or M4D_FOLD_QSCALE=0): blk.run's self-attention would take attn128q_kernel,
             # which rounds Q * c to bf16 once more, while the backward's recompute (log-sum-exp requested) runs on attn128p_kernel — the loss

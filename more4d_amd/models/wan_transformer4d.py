@@ -697,6 +697,9 @@ class WanTransformer4DModel(nn.Module):
         # training: GB of HBM the forward may spend on stored activations (None = whatever is free minus the head-room
         # below; 0 = plain per-block gradient checkpointing like the reference)
         self.activation_budget_gb = None
+        # 16: stored activations are kept as they are; 8: in 8 bits with a power-of-two step per 32 channels (ops.act_quant8) — about twice the
+        # blocks fit the budget; the forward's results do not change, the gradients see the rounded activations
+        self.activation_bits = 16
         self.activation_headroom_gb = 95.0     # backward workspace + allocator slack (measured: beyond ~230 GB live the step time gets erratic)
         self.last_stored_blocks = 0
         self.last_full_blocks = 0
@@ -1057,6 +1060,10 @@ class WanTransformer4DModel(nn.Module):
         # activation policy (288 GB of HBM3E per GPU): within the budget, every block first keeps its STORE_LITE tensors
         # (self-attention + ffn_down outputs), then blocks are upgraded to keeping all GEMM outputs; the rest recompute
         es = xres.new_empty(0, dtype=T).element_size()
+        if self.activation_bits not in (8, 16):
+            raise ValueError(f"activation_bits must be 8 or 16, got {self.activation_bits}")
+        if self.activation_bits == 8:
+            es = 33 / 32                # a byte per channel and one per block of 32
         lite = B * Lp * 2 * C * es + B * self.num_heads * Lp * 4
         full = B * Lp * (8 * C + self.ffn_dim) * es + B * self.num_heads * Lp * 4
         budget = self.activation_budget_gb
@@ -1085,8 +1092,8 @@ class WanTransformer4DModel(nn.Module):
                 gmeta = (period, glen)
         for i, blk in enumerate(self.blocks):
             store = 2 if i < n_full else (1 if i < n_lite else 0)
-            xres = BlockFn.apply(xres, e0, ctx_txt, ctx_img, gfeat, blk, c, self.text_len, img_len, store, gmeta,
-                                 *blk.parameters())
+            xres = BlockFn.apply(xres, e0, ctx_txt, ctx_img, gfeat, blk, c, self.text_len, img_len, (store, self.activation_bits),
+                                 gmeta, *blk.parameters())
         # ---- head (:708-721) + unpatchify (:1343-1366)
         if per_token:      # (:713-715) [B, Lp, 2, C]
             m = e.unsqueeze(2) + self.head.modulation.float().unsqueeze(0)

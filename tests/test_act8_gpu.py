@@ -220,3 +220,89 @@ def test_refusals():
         o.act_dequant8(a8, act=4)
     with pytest.raises(ValueError):
         o.act_dequant8(a8, out=torch.empty(8, 32, device=DEV))
+
+
+# ------------------------------------------------------------------ the DiT block's stored activations
+def _tiny(dtype):
+    from more4d_amd.models import WanTransformer4DModel
+    from test_dit_gpu import TINY
+    from util import load_keys, load_npz
+    from weights import fill
+    z = load_npz("dit_tiny.npz")
+    m = WanTransformer4DModel(**TINY)
+    m.load_state_dict(fill(load_keys("dit_tiny_keys.json"), 1234))
+    m = m.to(DEV, dtype).train()
+    kw = dict(x=z["x"].to(DEV), t=z["t"].to(DEV), context=[z["ctx0"].to(DEV), z["ctx1"].to(DEV)], seq_len=int(z["seq_len_pad"]),
+              clip_fea=z["clip"].to(DEV), y=z["y"].to(DEV), full_ref=z["full_ref"].to(DEV))
+    return m, kw
+
+
+def _grads(m, kw):
+    m.zero_grad(set_to_none=True)
+    pred = m(**kw)
+    g = torch.Generator(device=DEV).manual_seed(7)
+    (pred.float() * torch.randn(pred.shape, generator=g, device=DEV)).sum().backward()
+    return pred.detach().clone(), {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_block_gradients_from_codes_equal_those_of_the_values_they_stand_for(dtype, monkeypatch):
+    """The backward over a stash of codes against the same backward over a stash of plain tensors holding the codes' values.  All readers but
+    two expand the codes to exactly those tensors; the two that read codes directly (act_dequant8_t, act_bwd8) evaluate GELU and its
+    derivative in float32 like the plain kernels, in another order of operations: within one rounding to the type, eps / 2 relative, of each
+    element of h^T and of the pre-activation's gradient (plus 1e-5 of their size, the float32 bound at the top of this file).  The last block's
+    feed-forward gradients are linear in those two, and its incoming gradient is the same in both runs: eps of their rms.
+    Behind the feed-forward the difference passes softmaxes, whose gradients are sums that cancel (the keys' dS sum to zero), so it can grow
+    relative to what is left of them.  Both runs evaluate one formula on the same values: in float32 each is within 1e-3 of the exact gradient
+    (the bound of the comparisons with the reference's gradients in test_train_gpu.py), so 2e-3 of each other; in bfloat16 the bound of the
+    next test applies."""
+    from more4d_amd import autograd, ops
+    m, kw = _tiny(dtype)
+    m.activation_budget_gb, m.activation_bits = 1e6, 8
+    pred, coded = _grads(m, kw)
+    assert m.last_full_blocks == len(m.blocks)
+    monkeypatch.setattr(autograd.ops, "act_quant8", lambda t: ops.act_dequant8(_quant8(t)))
+    pred2, plain = _grads(m, kw)
+    assert torch.equal(pred, pred2) and coded.keys() == plain.keys()
+    eps = max(torch.finfo(dtype).eps, 1e-5)
+    direct = [f"blocks.{len(m.blocks) - 1}.ffn.{k}.{w}" for k in (0, 2) for w in ("weight", "bias")]
+    assert set(direct) <= coded.keys()
+    for n in coded:
+        a, b = coded[n].double(), plain[n].double()
+        tol = eps if n in direct else 2e-3 if dtype == torch.float32 else 0.05
+        assert float((a - b).norm()) <= tol * float(b.norm()) + 1e-9, (n, float((a - b).norm() / b.norm()))
+
+
+from more4d_amd.ops import act_quant8 as _quant8  # noqa: E402
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("full", [True, False])
+def test_model_with_8_bit_activations(dtype, full):
+    """activation_bits = 8: the same prediction bit for bit; gradients near those of stored tensors; more blocks in the same budget.  A code is off
+    by at most half a step of max / 64 of its block, for normal data a uniform error of rms below (2.5 / 64) / sqrt(12) = 1.2 % of the block's
+    rms; at most eight rounded tensors enter a gradient: sqrt(8) * 1.2 % = 3.4 %, asked for: 5 %.  That is relative to the terms of a gradient's
+    sum.  The key projections (biases, norm weights, and weights for the part of their inputs that all keys share) sum dS over the keys, which for
+    a softmax sums to zero: what the RMSNorm leaves is the spread of the keys' 1 / rms, 1 / sqrt(2 * 128) = 1 / 16 of the terms at 128 channels, so for them the same error is up to 16 times 3.4 % of the
+    result: 54 %."""
+    m, kw = _tiny(dtype)
+    C, F = m.dim, m.ffn_dim
+    m.activation_budget_gb = 1e6
+    if not full:
+        B, _, f, h, w = kw["x"].shape
+        rows = B * (-(-(f + 1) * (h // 2) * (w // 2) // 8) * 8)      # tokens and the reference frame's
+        es = 4 if dtype == torch.float32 else 2
+        m.activation_budget_gb = (rows * (2 * C * es + m.num_heads * 4) * len(m.blocks) + rows * (6 * C + F) * es * 0.6) / 2 ** 30
+    ref = _grads(m, kw)
+    blocks16 = m.last_full_blocks
+    m.activation_bits = 8
+    got = _grads(m, kw)
+    assert torch.equal(ref[0], got[0])
+    assert m.last_full_blocks > blocks16 if not full else m.last_full_blocks == blocks16 == len(m.blocks)
+    for n, b in ref[1].items():
+        a, b = got[1][n].double(), b.double()
+        tol = 0.54 if ".k." in n or ".k_img." in n or ".norm_k" in n else 0.05
+        assert float((a - b).norm()) <= tol * float(b.norm()) + 1e-9, (n, float((a - b).norm() / b.norm()))
+    m.activation_bits = 4
+    with pytest.raises(ValueError):
+        m(**kw)
