@@ -521,8 +521,9 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
  *                                coarse to fine; chunk_off[l] [n_adapters + 1] into it
  *   tiles_off[i], tiles[i]       the adapters of the rows of each tile, each once, for tiles of 64, 128 and 256 rows and (i = 3) of 256 rows
  *                                whose last one is rows [rows - 256, rows); tile_one: for the latter, the adapter of all of a tile's rows, or -1
- *   adapter_down     u T [rows, R] and / or ut = s_g x A_g^T (u's rows without an adapter are not written).  ut T [4 * n_pieces][ceil(R / 32)][64][8]:
- *                    slot s, rank r at [s / 16][r / 32][r % 32 + 32 * (s % 16 / 8)][s % 8], zero for pad slots and ranks beyond R;
+ *   adapter_down     u T [rows, R] and / or ut = s_g x A_g^T (u's rows without an adapter are not written).  ut T [4 * n_pieces][ceil(R / 32)][parts][64][8]:
+ *                    slot s, rank r at [s / 16][r / 32][.][r % 32 + 32 * (s % 16 / 8)][s % 8], zero for pad slots and ranks beyond R; bf16 in two
+ *                    parts whose sum is the value to 16 bits, float32 in one;
  *                    codes / exps (may be NULL): the 8-bit form of x's rows with an adapter, as act_quant8 writes it;
  *                    ws: adapter_down_workspace floats (slots: ut or codes will be asked for)
  *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once.  With a_down, u (and ut, codes, exps if given) are written first, by

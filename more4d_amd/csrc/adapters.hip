@@ -10,9 +10,11 @@
 // Rows are worked on in SLOTS: the plan lists the rows adapter by adapter, each adapter's list padded (slot_row = -1) to whole PIECES of 64
 // slots, so a workgroup never sees two adapters whatever the order of the requests, and one-row requests of one adapter share a piece.
 // u is written twice: [row][R], the GEMM's operand, and as the operand of the row contraction in the order in which its MFMA lanes read it,
-// [slot / 16][rank / 32][lane][8] with lane = rank % 32 + 32 * (slot % 16 / 8) (read row by row, 16 bytes of 32 ranks each, these loads cost the
-// address unit as much as x's); pad slots and ranks hold zero.  u and v are rounded to T like every other operand of an MFMA here: the
-// error this puts on an output is the one its own final rounding has, or less.
+// [slot / 16][rank / 32][part][lane][8] with lane = rank % 32 + 32 * (slot % 16 / 8) (read row by row, 16 bytes of 32 ranks each, these loads
+// cost the address unit as much as x's); pad slots and ranks hold zero.
+// Rounding: the GEMM's u is rounded to T like every other operand of an MFMA here — it is a small part of an output that is rounded to T itself.
+// The row contraction is all u (or v): rounded once it would put an error of the size of the gradient's own rounding on it, so bf16 keeps u
+// there as a sum of two parts, u = hi + lo to 16 bits (part 0, 1), at twice the products, which are not what bounds that pass.
 //
 // The operand of a down projection is laid out once (m4d_adapter_pack) in the order in which the MFMA lanes read it: chunks of 64 channels, 32
 // ranks, and within them lane (rank l & 31, channels 32 (l >> 5) + [0, 32) as four 8-element fragments).  With that order of the channels a
@@ -79,6 +81,8 @@ struct DownArgs {
     float* part;
 };
 
+template <typename T> struct Parts { static constexpr int N = sizeof(T) == 2 ? 2 : 1; };      // of a value in ut
+
 // four ranks (r .. r + 3) of one slot to u and / or ut, scaled
 template <typename T>
 M4D_DEV void down_store(const DownArgs& p, int64_t piece, int g, int slot, int row, int r, f32x4 v) {
@@ -88,9 +92,13 @@ M4D_DEV void down_store(const DownArgs& p, int64_t piece, int g, int slot, int r
     if (p.u && row >= 0 && r < p.R) store4((T*)p.u + (int64_t)row * p.R + r, v);
     if (p.ut) {
         const int64_t s = piece * PIECE + slot;
-        T* d = (T*)p.ut + (((s >> 4) * ((p.R + 31) >> 5) + (r >> 5)) * 64 + (r & 31) + ((slot >> 3) & 1) * 32) * 8 + (slot & 7);
+        T* d = (T*)p.ut + (((s >> 4) * ((p.R + 31) >> 5) + (r >> 5)) * (64 * Parts<T>::N) + (r & 31) + ((slot >> 3) & 1) * 32) * 8 + (slot & 7);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[e * 8] = (T)v[e];
+        for (int e = 0; e < 4; ++e) {
+            const T hi = (T)v[e];
+            d[e * 8] = hi;
+            if constexpr (Parts<T>::N == 2) d[512 + e * 8] = (T)(isfinite((float)hi) ? v[e] - (float)hi : 0.f);      // (inf - inf would be NaN)
+        }
     }
 }
 
@@ -329,7 +337,7 @@ __global__ __launch_bounds__(256) void adapter_down_join_kernel(DownArgs p) {
 
 // ---------------------------------------------------------------- contraction over the rows
 struct GradArgs {
-    const void* vt;                 // T, packed: [slot / 16][rank / 32][64][8]
+    const void* vt;                 // T, packed: [slot / 16][rank / 32][parts][64][8]
     const void* x;                  // T [rows, C] (row stride ldx), or
     const int8_t* codes; const uint8_t* exps;      // its 8-bit form (act8.hip)
     float* ws;                      // [n_chunks, R, C]
@@ -353,7 +361,7 @@ template <typename T, bool CODES, int RT>
 __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
     typedef typename Frag8<T>::type frag_t;
     typedef typename Quad<T>::type quad_t;
-    constexpr int PF = CODES ? 3 : 2;
+    constexpr int PF = 2, NP = Parts<T>::N;
     constexpr int RED = RT * 4 * 16 * 64 * 4;
     __shared__ __attribute__((aligned(16))) char smem[RED > CHUNK_PIECES * PIECE * 4 ? RED : CHUNK_PIECES * PIECE * 4];
     int* rows = reinterpret_cast<int*>(smem);
@@ -369,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
     const int nb = (p.C + 31) >> 5, rts = (p.R + 31) >> 5;
     const T* pv[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) pv[rt] = (const T*)p.vt + ((int64_t)(s0 >> 4) * rts + min((int)blockIdx.z * RT + rt, rts - 1)) * 512 + lane * 8;
+    for (int rt = 0; rt < RT; ++rt) pv[rt] = (const T*)p.vt + ((int64_t)(s0 >> 4) * rts + min((int)blockIdx.z * RT + rt, rts - 1)) * (512 * NP) + lane * 8;
     f32x16 acc[RT][4];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -379,7 +387,7 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
             for (int q = 0; q < 16; ++q) acc[rt][f][q] = 0.f;
     __syncthreads();
     struct Step {
-        frag_t v[RT];
+        frag_t v[RT][NP];
         quad_t x[8];
         int code[8];
         unsigned char ex[8];
@@ -388,7 +396,9 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
     const int row0 = rows[0];
     auto load = [&](int s, Step& b) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) b.v[rt] = *reinterpret_cast<const frag_t*>(pv[rt] + (int64_t)(s >> 4) * rts * 512);
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int q = 0; q < NP; ++q) b.v[rt][q] = *reinterpret_cast<const frag_t*>(pv[rt] + (int64_t)(s >> 4) * rts * (512 * NP) + q * 512);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int r = rows[s + hi * 8 + j];
@@ -420,7 +430,9 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) fx[j] = b.x[j][f];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) mma32(b.v[rt], fx, acc[rt][f]);
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int q = 0; q < NP; ++q) mma32(b.v[rt][q], fx, acc[rt][f]);
         }
     };
     // (n is whole pieces: every wave has n / 64 steps.  Requests beyond the end repeat the last step's rows: a branch around them would make the
@@ -613,22 +625,32 @@ static int launch_down(const DownArgs& p, hipStream_t st) {
     return p.codes ? launch_down_q<T, RT, true, false>(p, st) : launch_down_q<T, RT, false, false>(p, st);
 }
 
-// K slices of a down projection with few pieces: as many as fill half the chip, each at least eight chunks of 64 channels.  (A piece's K loop is
-// serial, 0.5 us a chunk where a workgroup is alone on its CU: K = 1536 12 us, in three slices and joined 8; K = 4096 32 and 10.)
-static int down_slices(int n_pieces, int64_t K) {
-    const int nc = (int)((K + 63) / 64);
-    int ks = n_pieces > 0 ? cus() / 2 / n_pieces : 1;
-    if (ks > nc / 8) ks = nc / 8;
-    if (ks < 2) return 1;
-    const int per = (nc + ks - 1) / ks;
-    return (nc + per - 1) / per;                 // (no empty slices)
+// K slices of a down projection: the least estimated time.  A piece's K loop is serial, 0.5 us a chunk of 64 channels, and a CU works through the
+// pieces it is dealt; slices shorten the loop where pieces are few (16 pieces, K = 4096: whole 32 us, in eight slices and joined 10) and even out
+// the CUs' shares where they are not much more than CUs (341 on 256); writing and joining the float32 sums costs 4 us and their bytes.
+static int down_slices(int n_pieces, int64_t K, int R) {
+    const int nc = (int)((K + 63) / 64), ncu = cus();
+#ifdef M4D_ABLATIONS
+    { const char* v = getenv("M4D_ADAPTER_KS"); if (v && atoi(v) > 0) { const int per = (nc + atoi(v) - 1) / atoi(v); return (nc + per - 1) / per; } }
+#endif
+    int best = 1;
+    double t_best = 1e30;
+    for (int ks = 1; ks <= 16 && (ks == 1 || nc / ks >= 8); ++ks) {
+        const int per = (nc + ks - 1) / ks;
+        if ((nc + per - 1) / per != ks) continue;                  // (no empty slices)
+        const double rounds = (double)(((int64_t)n_pieces * ks + ncu - 1) / ncu);
+        double t = rounds * (per * 0.47 + 2.0);
+        if (ks > 1) t += 4.0 + (double)ks * n_pieces * ((R + 31) / 32) * 32 * PIECE * 8 / 4.5e6;
+        if (t < t_best) { t_best = t; best = ks; }
+    }
+    return best;
 }
 // at most 16 rows, and only u wanted (serving single tokens): adapter_down16_kernel
 static bool down_few(const m4d_adapter_plan* plan, const void* ut, const void* codes) { return plan->rows <= 16 && !ut && !codes; }
 
 extern "C" int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int64_t K, int R, int slots) {
     if (!plan || K <= 0 || R <= 0 || (plan->rows <= 16 && !slots)) return 0;
-    const int ks = down_slices(plan->n_pieces, K);
+    const int ks = down_slices(plan->n_pieces, K, R);
     return ks > 1 ? (int64_t)ks * plan->n_pieces * ((R + 31) / 32 * 32) * PIECE : 0;
 }
 
@@ -642,7 +664,7 @@ extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const 
                   ((uintptr_t)codes % 16) == 0 && ((uintptr_t)ws % 16) == 0, "adapter_down: pointers must be 16-byte aligned");
     if (plan->n_pieces == 0) return 0;
     M4D_CHECK_ARG(plan->slot_row && plan->piece_adapter, "adapter_down: bad plan");
-    const int ks = down_slices(plan->n_pieces, K);
+    const int ks = down_slices(plan->n_pieces, K, R);
     if (down_few(plan, ut, codes)) {
         M4D_CHECK_ARG(plan->row_adapter && plan->tiles[0] && plan->n_listed > 0 && plan->n_listed <= 16, "adapter_down: bad plan");
         DownArgs p{x, a_down, scale, u, nullptr, nullptr, nullptr, nullptr, nullptr, ldx, (int)K, R, plan->n_pieces, 1, nullptr};

@@ -1248,45 +1248,50 @@ class AdapterPlan:
             raise ValueError("AdapterPlan: too many rows")
         P = self.PIECE
         self.rows = sum(lengths)
-        row = np.repeat(np.array(adapters, dtype=np.int32), np.array(lengths, dtype=np.int64))
-        used = [int(g) for g in np.unique(row) if g >= 0]
-        self.n_adapters = used[-1] + 1 if used else 0
-        slots, pieces, count = [], [], {}
-        for g in used:
-            r = np.nonzero(row == g)[0].astype(np.int32)
-            n = -(-len(r) // P)
-            slots.append(np.concatenate([r, np.full(n * P - len(r), -1, np.int32)]))
-            pieces += [g] * n
-            count[g] = n
+        # runs of rows with one adapter (empty requests gone), all tables come from these
+        size, ids = np.array(lengths, dtype=np.int64), np.array(adapters, dtype=np.int64)
+        ids, size = ids[size > 0], size[size > 0]
+        end = np.cumsum(size)
+        start = end - size
+        self.n_adapters = int(ids.max()) + 1 if len(ids) else 0
+        slots, pieces, count = [], [], [0] * self.n_adapters
+        for g in np.unique(ids[ids >= 0]).tolist():
+            s_, n_ = start[ids == g], size[ids == g]
+            before = np.cumsum(n_) - n_
+            n = count[g] = int(n_.sum())
+            slots += [np.repeat(s_ - before, n_) + np.arange(n), np.full(-n % P, -1)]
+            pieces += [g] * (-(-n // P))
         self.n_pieces = len(pieces)
 
         def chunks(target):                     # about `target` chunks in all, none beyond CHUNK_PIECES pieces, none of two adapters
             per = min(self.CHUNK_PIECES, max(1, -(-self.n_pieces // target)))
             lst, off, p0 = [], [0], 0
             for g in range(self.n_adapters):
-                n = count.get(g, 0)
+                n = -(-count[g] // P)
                 for q in range(0, n, per):
                     lst += [p0 + q, p0 + min(q + per, n), g]
                 p0 += n
                 off.append(len(lst) // 3)
             return lst, off
 
-        def tiles(T, shifted=False):
-            off, lst = [0], []
-            for m in range(0, self.rows, T):
-                lo = max(0, min(m, self.rows - T)) if shifted else m
-                lst += [int(g) for g in np.unique(row[lo:m + T]) if g >= 0]
-                off.append(len(lst))
-            return lst, off
+        def tiles(T, shifted=False):            # (tile, adapter) pairs, each once, in order; the adapter of whole tiles
+            nt = -(-self.rows // T)
+            t0 = start // T
+            n_ = (end - 1) // T - t0 + 1
+            tile, who = np.repeat(t0 - (np.cumsum(n_) - n_), n_) + np.arange(int(n_.sum())), np.repeat(ids, n_)
+            if shifted and nt > 1:              # the last tile also holds rows of the one before
+                more = ids[(end > self.rows - T) & (start < (nt - 1) * T)]
+                tile, who = np.concatenate([tile, np.full(len(more), nt - 1)]), np.concatenate([who, more])
+            key = np.unique(tile * (self.n_adapters + 1) + who + 1)
+            tile, who = key // (self.n_adapters + 1), key % (self.n_adapters + 1) - 1
+            distinct = np.bincount(tile, minlength=nt)
+            one = np.where(distinct == 1, who[np.cumsum(distinct) - distinct], -1) if nt else who
+            return who[who >= 0], np.concatenate([[0], np.cumsum(np.bincount(tile[who >= 0], minlength=nt))]), one
 
-        one = []                                # the adapter of ALL rows of a (shifted) 256-row tile, or -1
-        for m in range(0, self.rows, 256):
-            lo = max(0, min(m, self.rows - 256))
-            one.append(int(row[lo]) if (row[lo:m + 256] == row[lo]).all() else -1)
         cs = [chunks(t) for t in (12, 24, 48, 96)]
         ts = [tiles(64), tiles(128), tiles(256), tiles(256, True)]
-        parts = [row, np.concatenate(slots) if slots else [], pieces]
-        parts += [c[0] for c in cs] + [c[1] for c in cs] + [t[1] for t in ts] + [t[0] for t in ts] + [one]
+        parts = [np.repeat(ids, size), np.concatenate(slots) if slots else [], pieces]
+        parts += [c[0] for c in cs] + [c[1] for c in cs] + [t[1] for t in ts] + [t[0] for t in ts] + [ts[3][2]]      # (tile_one)
         parts = [np.asarray(v, dtype=np.int32) for v in parts]
         at, offs = 0, []
         for v in parts:
@@ -1321,7 +1326,7 @@ def _check_adapters(name, x, bank, plan):
 
 
 def _slots_shape(bank, plan):
-    return 4 * plan.n_pieces, (bank.R + 31) // 32, 64, 8
+    return 4 * plan.n_pieces, (bank.R + 31) // 32, 2 if bank.buf.dtype == torch.bfloat16 else 1, 64, 8
 
 
 def adapter_down(x, bank, plan, *, rows=True, slots=False):

@@ -2,9 +2,9 @@
 
 Tolerances, per output element, h = eps / 2 of the type:
   y      h |y|  (its rounding)  +  h sum_r |u_r| |B_r|  (u is rounded to the type)  +  n 2^-23 S  (float32 accumulation of n terms of total size S)
-  dx     likewise with v;   dA:  h |dA| + h sum |v| |x| + n 2^-23 S;   dB:  with |dy| |u|.
-The sums over many rows of independently rounded v bound the worst case only; their typical error is checked besides: the rounding of v and the final
-rounding are both at most h relative, uniform in sign, so the error's rms is below sqrt(2 / 3) h of the result's rms for normal data: < h."""
+  dx     likewise with v;   dA:  h |dA| + h^2 sum |v| |x| + n 2^-23 S (v in two parts: 16 bits in bf16);   dB:  with |dy| |u|.
+The typical error is checked besides: the final rounding is at most h relative, uniform, so the error's rms is below h / sqrt(3) of the result's rms
+for normal data: < 0.75 h."""
 import pytest
 import torch
 
@@ -181,8 +181,8 @@ def test_backward(case, bits):
         va, ua = abs(scale[i]) * (dyd[m].abs() @ b[i].double().abs()), abs(scale[i]) * (x.double()[m].abs() @ a[i].double().abs().t())
         n = int(m.sum())
         wa, wb = v.t() @ xd[m], dyd[m].t() @ u
-        ta = 1.02 * h * (wa.abs() + v.abs().t() @ xd[m].abs()) + (n + N) * 2.0 ** -23 * (va.t() @ xd[m].abs())
-        tb = 1.02 * h * (wb.abs() + dyd[m].abs().t() @ u.abs()) + (n + K) * 2.0 ** -23 * (dyd[m].abs().t() @ ua)
+        ta = 1.02 * h * (wa.abs() + h * v.abs().t() @ xd[m].abs()) + (n + N) * 2.0 ** -23 * (va.t() @ xd[m].abs())
+        tb = 1.02 * h * (wb.abs() + h * dyd[m].abs().t() @ u.abs()) + (n + K) * 2.0 ** -23 * (dyd[m].abs().t() @ ua)
         ea, eb = (da[i].cpu().double() - wa).abs(), (db[i].cpu().double() - wb).abs()
         assert (ea <= ta).all() and (eb <= tb).all(), (i, float((ea / ta).max()), float((eb / tb).max()))
         num["a"] += float(ea.pow(2).sum()); den["a"] += float(wa.pow(2).sum())
@@ -191,7 +191,7 @@ def test_backward(case, bits):
             assert (da[i] == 0).all() and (db[i] == 0).all()
     if dt == BF and M > 100:
         for k in num:
-            assert (num[k] / den[k]) ** 0.5 < h, k
+            assert (num[k] / den[k]) ** 0.5 < 0.75 * h, k
     y2 = AdapterLinearFn.apply(xg, w.to(DEV), bias.to(DEV), ag, bg, scale, plan, bits)
     for p, q in zip(torch.autograd.grad(y2, (xg, ag, bg), dy.to(DEV)), (dx, da, db)):
         assert torch.equal(p, q)                      # the same bits again: no order-dependent sums
@@ -331,10 +331,15 @@ def test_the_pass_that_reads_x_writes_the_same_codes(K, dt):
     u, ut3 = o.adapter_down(xd, bank, plan, slots=True)
     assert torch.equal(ut3.nan_to_num(0), ut.nan_to_num(0))
     slot = torch.tensor(tables_slot_row(plan))
-    # [slot / 16][rank / 32][rank % 32 + 32 * (slot % 16 / 8)][slot % 8] -> [slot][rank]
-    v = ut.cpu().view(len(slot) // 16, ut.shape[1], 2, 32, 8).permute(0, 2, 4, 1, 3).reshape(len(slot), -1)
-    assert (v[slot < 0] == 0).all() and (v[slot >= 0][:, 8:].nan_to_num(0) == 0).all()
-    assert torch.equal(v[slot >= 0][:, :u.shape[1]].nan_to_num(0), u.cpu()[slot[slot >= 0].long()].nan_to_num(0))
+    # [slot / 16][rank / 32][part][rank % 32 + 32 * (slot % 16 / 8)][slot % 8] -> [part][slot][rank]
+    v = ut.cpu().view(len(slot) // 16, ut.shape[1], -1, 2, 32, 8).permute(2, 0, 3, 5, 1, 4).reshape(ut.shape[2], len(slot), -1)
+    assert (v[:, slot < 0] == 0).all() and (v[:, slot >= 0][..., 8:].nan_to_num(0) == 0).all()
+    on_slot = v[:, slot >= 0][..., :u.shape[1]].nan_to_num(0).double()
+    uu = u.cpu()[slot[slot >= 0].long()].nan_to_num(0).double()
+    assert torch.equal(on_slot[0], uu)
+    if dt == BF:                                       # the second part: what the first one's rounding left, at most half of its last bit
+        fin = uu.abs() < 1e38
+        assert (on_slot[1].abs()[fin] <= uu.abs()[fin] * torch.finfo(BF).eps / 2 + 1e-38).all() and on_slot[1].abs().max() > 0
 
 
 def tables_slot_row(plan):

@@ -53,6 +53,10 @@ def test_plan_tables_cover_every_row_once(seed):
         for i in range(nt):
             lo = max(0, min(i * T, p.rows - T)) if k == 3 else i * T
             assert lst[off[i]:off[i + 1]] == sorted({g for g in rows[lo:i * T + T] if g >= 0})
+            if k == 3:
+                here = set(rows[lo:i * T + T])
+                assert at(a.tile_one, nt)[i] == (here.pop() if len(here) == 1 else -1)
+    assert a.n_listed == at(a.tiles_off[0], -(-p.rows // 64) + 1)[-1]
 
 
 def test_plan_of_nothing():
