@@ -32,6 +32,34 @@ M4D_DEV unsigned encode4(float a, float b, float c, float d, float inv, bool cap
     return lo | hi;
 }
 
+// a lane's value and its neighbours' (lane ^ 1, lane ^ 2) within groups of four, largest
+M4D_DEV unsigned max_xor1(unsigned v) { return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true)); }
+M4D_DEV unsigned max_xor2(unsigned v) { return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true)); }
+
+// bits of the largest magnitude of the values in n dwords (bf16: two in a dword, compared as 16-bit integers)
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+template <typename T, int N> M4D_DEV unsigned top_bits(const unsigned (&w)[N]) {
+    if constexpr (sizeof(T) == 2) {
+        u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+        return (unsigned)max(m[0], m[1]) << 16;
+    } else {
+        unsigned m = w[0] & 0x7fffffffu;
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = max(m, w[i] & 0x7fffffffu);
+        return m;
+    }
+}
+template <typename T, int N> M4D_DEV float value_of(const unsigned (&w)[N], int e) {
+    return __builtin_bit_cast(float, sizeof(T) == 2 ? (e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16) : w[e]);
+}
+// values 4 q .. 4 q + 3 -> codes; b: the block's exponent byte (255: zeros)
+template <typename T, int N> M4D_DEV unsigned encode_of(const unsigned (&w)[N], int q, unsigned b, float inv, bool cap) {
+    const unsigned c = encode4(value_of<T>(w, 4 * q), value_of<T>(w, 4 * q + 1), value_of<T>(w, 4 * q + 2), value_of<T>(w, 4 * q + 3), inv, cap);
+    return b == 255u ? 0u : c;
+}
+
 M4D_DEV float decode1(unsigned c, int e, float step) { return (float)((int)(c << (24 - 8 * e)) >> 24) * step; }
 M4D_DEV void decode8(const u32x2& c, float step, float (&v)[8]) {
 #pragma unroll

@@ -87,20 +87,30 @@ __global__ __launch_bounds__(256) void act_quant8_kernel(Act8Args p) {
     const int nu = p.nb * 4;
     for (UnitWalk w(nu); w.row < p.rows; w.next()) {
         const int c0 = w.j * 8, n = min(8, p.C - c0);
-        float v[8];
-        load_unit<T>((const T*)p.in + w.row * p.ld_in + c0, n, p.vec, v);
-        unsigned top = 0;          // as integers: NaN > inf > every finite magnitude
+        constexpr int ND = 2 * sizeof(T);             // dwords of a unit
+        unsigned v[ND];
+        const T* src = (const T*)p.in + w.row * p.ld_in + c0;
+        if (p.vec && n == 8) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(unsigned, v[e]) & 0x7fffffffu);
-        top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));      // the block's four units are four neighbouring lanes
-        top = max(top, (unsigned)__shfl_xor((int)top, 2, 64));
-        const unsigned b = block_exp(top);
-        u32x2 c = {0u, 0u};
-        if (b != 255u) {
-            const float inv = block_inv(b);
-            c[0] = encode4(v[0], v[1], v[2], v[3], inv, b == 248u);
-            c[1] = encode4(v[4], v[5], v[6], v[7], inv, b == 248u);
+            for (int i = 0; i < ND / 4; ++i) {
+                const u32x4q d = reinterpret_cast<const u32x4q*>(src)[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i * 4 + e] = d[e];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                if constexpr (sizeof(T) == 2) {
+                    bf16x2 b = {(bf16_t)0.f, (bf16_t)0.f};
+                    if (2 * i < n) b[0] = src[2 * i];
+                    if (2 * i + 1 < n) b[1] = src[2 * i + 1];
+                    v[i] = __builtin_bit_cast(unsigned, b);
+                } else v[i] = i < n ? __builtin_bit_cast(unsigned, src[i]) : 0u;
+            }
         }
+        const unsigned b = block_exp(max_xor2(max_xor1(top_bits<T>(v))));      // the block's four units are four neighbouring lanes
+        const float inv = block_inv(min(b, 248u));
+        const u32x2 c = {encode_of<T>(v, 0, b, inv, b == 248u), encode_of<T>(v, 1, b, inv, b == 248u)};
         *reinterpret_cast<u32x2*>(p.codes + (w.row * p.nb) * 32 + c0) = c;
         if ((w.j & 3) == 0) p.exps[w.row * p.nb + (w.j >> 2)] = (uint8_t)b;
     }

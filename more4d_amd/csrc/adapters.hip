@@ -102,31 +102,14 @@ M4D_DEV void down_store(const DownArgs& p, int64_t piece, int g, int slot, int r
     }
 }
 
-// 16 channels, half a block, of two neighbouring lanes each -> 16 codes and (from the even lane) the exponent byte
-M4D_DEV void quant_half(const float (&x)[16], int8_t* codes, uint8_t* exps, bool store) {
-    unsigned top = 0;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) top = max(top, __builtin_bit_cast(unsigned, x[e]) & 0x7fffffffu);
-    top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));
-    const unsigned b = block_exp(top);
-    const float inv = block_inv(min(b, 248u));
-    u32x4q c = {};
-    if (b != 255u) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) c[k] = encode4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3], inv, b == 248u);
-    }
-    if (store) {
-        *reinterpret_cast<u32x4q*>(codes) = c;
-        if ((threadIdx.x & 1) == 0) *exps = (uint8_t)b;
-    }
-}
-
 // u of one piece: 64 slots x RT * 32 ranks, a chunk of 64 channels at a time.  Bound by reading x once; the operand comes from L2, as many bytes
 // again at 64 ranks.  Rows and operand go to LDS by direct loads, whole 128-byte lines of a row per request (straight into registers, a lane of
 // the MFMA layout wants 16 bytes of a row of its own, and the address unit then handles 64 lines per request: 85 us for 21840 x 5120 at rank
 // 64, against 46 us of HBM time), NST - 1 chunks in flight, one barrier per chunk, two workgroups per CU.
-// Wave (s, h): slots 32 s + [0, 32) and rank tiles h, h + 2, ...; with one rank tile h takes every other 16 channels instead.  QUANT: each
-// wave also writes the codes of 16 of the piece's rows, two lanes per block of 32 channels, out of the same LDS.
+// Wave (s, h): slots 32 s + [0, 32) and rank tiles h, h + 2, ...; with one rank tile h takes every other 16 channels instead.  QUANT: four
+// more waves write the codes, 16 of the piece's rows each, two lanes per block of 32 channels, out of the same LDS.  (The waves that request
+// chunks cannot also store: loads and stores share one counter, only loads return in order, so a wait that must not pass too early has to
+// wait for the stores as well, and little stays in flight: 128 us instead of 75 + 40 at 21840 x 5120.)
 // DEEP: fewer workgroups than CUs, each with the LDS of a whole CU: up to twelve chunks in flight, because alone a workgroup waits for memory (0.5
 // us a chunk with four stages).
 template <typename T, int RT, bool DEEP> struct DownShape {
@@ -144,7 +127,7 @@ M4D_DEV void wait_younger(int n) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(MAX * NU) : "memory");
 }
 template <typename T, int RT, bool QUANT, bool DEEP>
-__global__ __launch_bounds__(256, 2) void adapter_down_kernel(DownArgs p) {
+__global__ __launch_bounds__(QUANT ? 512 : 256, 2) void adapter_down_kernel(DownArgs p) {
     typedef DownShape<T, RT, DEEP> Sh;
     typedef typename Frag8<T>::type frag_t;
     extern __shared__ __attribute__((aligned(16))) char ad_smem[];
@@ -163,6 +146,55 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(DownArgs p) {
     const int tail = (p.K - (nc - 1) * 64) * ES;         // bytes of the last chunk of a row
     const unsigned lds_base = (unsigned)(uintptr_t)(LDS_AS char*)ad_smem;
     auto swz = [](int r) { return ES == 2 ? (r >> 1) & 7 : r & 15; };      // 16-byte chunk c of row r sits at chunk c ^ swz(r)
+    if constexpr (QUANT) {
+        if (wave >= 4) {
+            if (rt0 == 0) {
+                // this lane's row, and where its codes and exponents go
+                const int qr = (wave - 4) * 16 + (lane >> 2), qrow = sr[qr];
+                int8_t* qc = p.codes + (int64_t)max(qrow, 0) * nb * 32 + (lane & 3) * 16;
+                uint8_t* qe = p.exps + (int64_t)max(qrow, 0) * nb;
+                unsigned even = 0;                           // the exponents of the even chunk before an odd one
+                for (int c = c0; c < c1; ++c) {
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the barrier of chunk c
+                    const char* st = ad_smem + ((c - c0) % NST) * Sh::STAGE;
+                    unsigned v[4 * ES];                               // 16 channels, half a block
+#pragma unroll
+                    for (int k = 0; k < ES; ++k) {
+                        const u32x4q d = *reinterpret_cast<const u32x4q*>(st + qr * RB + ((((lane & 3) * ES + k) ^ swz(qr)) << 4));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[k * 4 + e] = d[e];
+                    }
+                    const unsigned b = block_exp(max_xor1(top_bits<T>(v)));
+                    const float inv = block_inv(min(b, 248u));
+                    u32x4q q4;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) q4[k] = encode_of<T>(v, k, b, inv, b == 248u);
+                    const int blk = c * 2 + ((lane >> 1) & 1);
+                    if (qrow >= 0 && blk < nb) *reinterpret_cast<u32x4q*>(qc + (int64_t)c * 64) = q4;
+                    // exponents: the row's two bytes meet in its first lane, and where rows of bytes are 4-byte aligned two chunks' go out as one dword
+                    // (bytes one at a time are 32 cache lines a store)
+                    const unsigned both = b | ((unsigned)__builtin_amdgcn_mov_dpp((int)b, 0x4E, 0xF, 0xF, true) << 8);
+                    if ((lane & 3) == 0 && qrow >= 0) {
+                        if (nb & 3) {
+                            qe[c * 2] = (uint8_t)both;
+                            if (c * 2 + 1 < nb) qe[c * 2 + 1] = (uint8_t)(both >> 8);
+                        } else if (c & 1) {
+                            if (c == c0) *reinterpret_cast<uint16_t*>(qe + c * 2) = (uint16_t)both;
+                            else *reinterpret_cast<unsigned*>(qe + c * 2 - 2) = (both << 16) | even;
+                        } else if (c == c1 - 1) *reinterpret_cast<uint16_t*>(qe + c * 2) = (uint16_t)both;
+                    }
+                    even = both;
+                }
+            } else {
+                for (int c = c0; c < c1; ++c) asm volatile("s_barrier" ::: "memory");
+            }
+            if constexpr (RT == 1) {                         // (the barriers of the join below)
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                __syncthreads();
+            }
+            return;
+        }
+    }
     const char* sx[NX];
     int cb[NX];
 #pragma unroll
@@ -197,10 +229,6 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(DownArgs p) {
 #pragma unroll
         for (int q = 0; q < 16; ++q) acc[k][q] = 0.f;
     const int row = sr[s * 32 + li];
-    // (QUANT) this lane's row, and where its codes and exponents go
-    const int qr = wave * 16 + (lane >> 2), qrow = QUANT && rt0 == 0 ? sr[qr] : -1;
-    int8_t* qc = p.codes + (int64_t)max(qrow, 0) * nb * 32 + (lane & 3) * 16;
-    uint8_t* qe = p.exps + (int64_t)max(qrow, 0) * nb;
 #pragma unroll
     for (int i = 0; i < NST - 1; ++i)
         if (c0 + i < c1) request(c0 + i);
@@ -229,24 +257,6 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(DownArgs p) {
                 const char* q = st + Sh::XB + (((RT == 1 ? 0 : h + 2 * k) * 4 + kk) * 64 + lane) * 8 * ES;
                 mma32(frag(q, 0, 16), x[kk], acc[k]);
             }
-        }
-        if constexpr (QUANT) {
-            const int blk = c * 2 + ((lane >> 1) & 1);
-            float v[16];
-#pragma unroll
-            for (int k = 0; k < ES; ++k) {
-                const char* q = st + qr * RB + ((((lane & 3) * ES + k) ^ swz(qr)) << 4);
-                if constexpr (ES == 2) {
-                    const bf16x8 b = *reinterpret_cast<const bf16x8*>(q);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[k * 8 + e] = (float)b[e];
-                } else {
-                    const f32x4 b = *reinterpret_cast<const f32x4*>(q);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[k * 4 + e] = b[e];
-                }
-            }
-            quant_half(v, qc + (int64_t)c * 64, qe + blk, qrow >= 0 && blk < nb);
         }
     }
     if constexpr (RT == 1) {                                 // join the two halves of the channels
@@ -610,7 +620,7 @@ static int launch_down_q(const DownArgs& p, hipStream_t st) {
         configured.mark();
     }
     const int ny = ((p.R + 31) / 32 + RT - 1) / RT;
-    hipLaunchKernelGGL((adapter_down_kernel<T, RT, QUANT, DEEP>), dim3((unsigned)((p.n_pieces + 7) / 8 * 8 * ny), (unsigned)p.KS), dim3(256), LDS, st, p);
+    hipLaunchKernelGGL((adapter_down_kernel<T, RT, QUANT, DEEP>), dim3((unsigned)((p.n_pieces + 7) / 8 * 8 * ny), (unsigned)p.KS), dim3(QUANT ? 512 : 256), LDS, st, p);
     M4D_CHECK_LAUNCH("adapter_down");
     if (p.part) {
         hipLaunchKernelGGL(adapter_down_join_kernel<T>, dim3((unsigned)p.n_pieces, (unsigned)((p.R + 31) / 32 * 2)), dim3(256), 0, st, p);
@@ -661,7 +671,7 @@ extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const 
     M4D_CHECK_ARG(K > 0 && K < (1 << 30) && (K * es) % 16 == 0 && (ldx * es) % 16 == 0 && (plan->rows == 1 || ldx >= K),
                   "adapter_down: rows of K=%lld elements (row stride %lld) must be multiples of 16 bytes", (long long)K, (long long)ldx);
     M4D_CHECK_ARG(((uintptr_t)x % 16) == 0 && ((uintptr_t)a_down % 16) == 0 && ((uintptr_t)u % 16) == 0 && ((uintptr_t)ut % 16) == 0 &&
-                  ((uintptr_t)codes % 16) == 0 && ((uintptr_t)ws % 16) == 0, "adapter_down: pointers must be 16-byte aligned");
+                  ((uintptr_t)codes % 16) == 0 && ((uintptr_t)exps % 4) == 0 && ((uintptr_t)ws % 16) == 0, "adapter_down: pointers must be 16-byte aligned");
     if (plan->n_pieces == 0) return 0;
     M4D_CHECK_ARG(plan->slot_row && plan->piece_adapter, "adapter_down: bad plan");
     const int ks = down_slices(plan->n_pieces, K, R);
