@@ -529,7 +529,9 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
  *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once.  With a_down, u (and ut, codes, exps if given) are written first, by
  *                    adapter_down; without, u is an input.  ws: linear_adapters_workspace floats
  *   adapter_grad     out T [G, rank, C] (transposed: [G, C, rank]) = sum over the rows of g of v^T x, vt as adapter_down writes ut, x as T or as
- *                    8-bit codes; ws: adapter_grad_workspace floats; partial sums are joined in a fixed order. */
+ *                    8-bit codes; ws: adapter_grad_workspace floats; partial sums are joined in a fixed order
+ *   linear_adapters_bwd  the backward of linear_adapters with W [N, K] frozen, in one call: dx T [rows, K] = dy W + v A (NULL: not wanted), da (needs
+ *                    x or its codes), db (needs the forward's ut); N a multiple of 8 (bf16) or 4; ws: linear_adapters_bwd_workspace floats. */
 typedef struct {
     const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks[4], *chunk_off[4], *tiles_off[4], *tiles[4], *tile_one;
     int64_t rows;
@@ -549,6 +551,11 @@ int64_t m4d_adapter_grad_workspace(const m4d_adapter_plan* plan, int64_t C, int 
 int m4d_adapter_grad(m4d_dtype dt, const void* vt, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps,
                      const m4d_adapter_plan* plan, float* ws, int64_t ws_floats, void* out, int transposed, int G, int rank, int64_t C, int R,
                      m4d_stream stream);
+int64_t m4d_linear_adapters_bwd_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R, int need_dx, int need_da, int need_db);
+int m4d_linear_adapters_bwd(m4d_dtype dt, const void* dy, int64_t ldy, const void* W, int64_t ldw, const void* b_down, const float* scale,
+                            const void* a_up, const m4d_adapter_plan* plan, const void* x, int64_t ldx, const int8_t* codes, const uint8_t* exps,
+                            const void* ut, void* dx, void* da, void* db, int G, int rank, int64_t N, int64_t K, int R, float* ws, int64_t ws_floats,
+                            m4d_stream stream);
 
 #ifdef __cplusplus
 }

@@ -160,6 +160,9 @@ SIGNATURES = {
     "m4d_adapter_grad_workspace": (c_int64, [POINTER(AdapterPlanArgs), c_int64, c_int]),
     "m4d_adapter_grad": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, POINTER(AdapterPlanArgs), c_void_p, c_int64, c_void_p,
                                  c_int, c_int, c_int, c_int64, c_int, c_void_p]),
+    "m4d_linear_adapters_bwd_workspace": (c_int64, [c_int, POINTER(AdapterPlanArgs), c_int64, c_int64] + [c_int] * 4),
+    "m4d_linear_adapters_bwd": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, POINTER(AdapterPlanArgs), c_void_p,
+                                        c_int64] + [c_void_p] * 6 + [c_int, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
 }
 
 _lib = None

@@ -116,15 +116,19 @@ class AdapterLinearFn(Function):
         if dy2.shape[0] == 0:
             zero = [dy2.new_zeros(s) if n else None for s, n in ((xshape, need_x), ((bank.G, bank.rank, K), need_a), ((bank.G, N, bank.rank), need_b))]
             return zero[0], None, None, zero[1], zero[2], None, None, None
-        Np = -(-N // 8) * 8                              # the rows of dy become K rows of a GEMM: whole 16-byte chunks
-        if Np != N or dy2.stride(-1) != 1 or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
-            dy2 = torch.nn.functional.pad(dy2, (0, Np - N)).contiguous()
+        if dy2.stride(-1) != 1 or dy2.stride(0) < N or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
+            dy2 = dy2.contiguous()
+        Np = -(-N // 8) * 8
+        if Np == N:
+            x = None if not need_a else ops.Act8((dy2.shape[0], K), xdt, buf=kept) if bits == 8 else kept
+            dx, da, db = ops.linear_adapters_bwd(dy2, weight.detach(), bank, plan, x=x, ut=ut if need_b else None, need_x=need_x)
+            return dx.view(xshape) if need_x else None, None, None, da, db, None, None, None
+        # N that is not whole 16-byte chunks: dy's rows become rows of K of a GEMM and are padded with zeros, W^T and the adapters likewise
+        dy2 = torch.nn.functional.pad(dy2, (0, Np - N))
         dx = da = db = vt = None
         back = bank.transposed()
         if need_x:
-            wt = torch.empty((K, Np), device=weight.device, dtype=weight.dtype)
-            if Np != N:
-                wt[:, N:].zero_()
+            wt = torch.zeros((K, Np), device=weight.device, dtype=weight.dtype)
             ops.transpose(weight.detach(), out=wt[:, :N])
             dx, vt = ops.linear_adapters(dy2, wt, None, back, plan, slots=True)
             dx = dx.view(xshape)

@@ -838,3 +838,58 @@ extern "C" int m4d_adapter_grad(m4d_dtype dt, const void* vt, const void* x, int
     M4D_CHECK_LAUNCH("adapter_grad(join)");
     return 0;
 }
+
+// The whole backward of a frozen projection with adapters in one call: W^T, v = s dy B (with its slots), dx = dy W + v A, dA, dB.  Workspace: W^T, v,
+// its slots, then the largest of what the passes need, which run one after the other.
+namespace {
+struct BwdSpace { int64_t wt, v, vt, rest, total; };
+int64_t up64(int64_t n) { return (n + 63) / 64 * 64; }
+BwdSpace bwd_space(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R, bool dx, bool da, bool db) {
+    const int64_t per = dt == M4D_BF16 ? 2 : 1;                  // elements of T in a float
+    BwdSpace b{};
+    int64_t at = 0;
+    b.wt = at; if (dx) at += up64((K * N + per - 1) / per);
+    b.v = at; if (dx) at += up64((plan->rows * R + per - 1) / per);
+    b.vt = at; if (da) at += up64((int64_t)plan->n_pieces * 4 * ((R + 31) / 32) * 512 * (dt == M4D_BF16 ? 2 : 1) / per);
+    b.rest = at;
+    int64_t most = 0;
+    auto take = [&](int64_t n) { if (n > most) most = n; };
+    if (dx) take(m4d_linear_adapters_workspace(dt, plan, K, N, R, da));
+    else if (da) take(m4d_adapter_down_workspace(plan, N, R, 1));
+    if (da) take(m4d_adapter_grad_workspace(plan, K, R));
+    if (db) take(m4d_adapter_grad_workspace(plan, N, R));
+    b.total = at + most;
+    return b;
+}
+}  // namespace
+
+extern "C" int64_t m4d_linear_adapters_bwd_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R, int need_dx, int need_da,
+                                                     int need_db) {
+    if (!plan || plan->rows <= 0 || N <= 0 || K <= 0 || R <= 0) return 0;
+    return bwd_space(dt, plan, N, K, R, need_dx, need_da, need_db).total;
+}
+
+extern "C" int m4d_linear_adapters_bwd(m4d_dtype dt, const void* dy, int64_t ldy, const void* W, int64_t ldw, const void* b_down, const float* scale,
+                                       const void* a_up, const m4d_adapter_plan* plan, const void* x, int64_t ldx, const int8_t* codes,
+                                       const uint8_t* exps, const void* ut, void* dx, void* da, void* db, int G, int rank, int64_t N, int64_t K, int R,
+                                       float* ws, int64_t ws_floats, m4d_stream stream) {
+    PLAN_OK("linear_adapters_bwd");
+    M4D_CHECK_ARG(dx || da || db, "linear_adapters_bwd: nothing to compute");
+    M4D_CHECK_ARG((N * es) % 16 == 0, "linear_adapters_bwd: rows of dy (N=%lld) must be whole 16-byte chunks", (long long)N);
+    const BwdSpace s = bwd_space(dt, plan, N, K, R, dx, da, db);
+    M4D_CHECK_ARG(s.total == 0 || (ws && ws_floats >= s.total && ((uintptr_t)ws % 16) == 0), "linear_adapters_bwd: workspace of %lld floats needed", (long long)s.total);
+    float* rest = ws + s.rest;
+    const int64_t nrest = s.total - s.rest;
+    int rc = 0;
+    void* vt = da ? (void*)(ws + s.vt) : nullptr;
+    if (dx) {
+        rc = m4d_transpose(dt, W, ldw, ws + s.wt, N, N, K, stream);
+        if (rc == 0) {
+            if (plan->n_pieces == 0) rc = m4d_gemm_bt(dt, dy, ldy, ws + s.wt, N, nullptr, 0, dx, K, plan->rows, K, N, M4D_EPI_STORE, nullptr, 0, 0, stream);
+            else rc = m4d_linear_adapters(dt, dy, ldy, ws + s.wt, N, nullptr, b_down, scale, a_up, plan, ws + s.v, vt, nullptr, nullptr, dx, K, K, N, R, rest, nrest, stream);
+        }
+    } else if (da) rc = m4d_adapter_down(dt, dy, ldy, b_down, scale, plan, nullptr, vt, nullptr, nullptr, N, R, rest, nrest, stream);
+    if (rc == 0 && da) rc = m4d_adapter_grad(dt, vt, x, ldx, codes, exps, plan, rest, nrest, da, 0, G, rank, K, R, stream);
+    if (rc == 0 && db) rc = m4d_adapter_grad(dt, ut, dy, ldy, nullptr, nullptr, plan, rest, nrest, db, 1, G, rank, N, R, stream);
+    return rc;
+}

@@ -1,6 +1,5 @@
 """Tensor-level wrappers over the C ABI (include/more4d_hip.h).  torch supplies device memory and the
 current HIP stream; every arithmetic op below runs in a hand-written gfx950 kernel.  No fallback."""
-import contextlib
 import math
 import os
 
@@ -1061,22 +1060,27 @@ def adamw_(p, g, m, v, *, lr, beta1, beta2, eps, weight_decay, step, grad_scale=
 
 
 # ------------------------------------------------------------------ activations kept in 8 bits
-_NO_GUARD = contextlib.nullcontext()
-
-
-def _same_device(name, first, *rest):
-    """All tensors on one HIP device; returns a guard that makes it current (its current stream is the one launched on)."""
-    _dev(first, *rest)
-    d = first.get_device()
-    for t in rest:
+def _same_device(name, *ts):
+    """Index of the one HIP device that all the tensors are on."""
+    d = ts[0].get_device()
+    for t in ts:
         if t is not None and t.get_device() != d:
-            raise ValueError(f"{name}: tensors on different devices {first.device} and {t.device}")
-    return _NO_GUARD if d == torch._C._cuda_getDevice() else torch.cuda.device(d)
+            _dev(*ts)
+            raise ValueError(f"{name}: tensors on different devices {[str(t.device) for t in ts if t is not None]}")
+    if d < 0:
+        _dev(*ts)
+    return d
 
 
-def _raw_stream(t):
-    """The current stream of the tensor's device, as _stream() gives it, without the stream object (a microsecond per call)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+def _launch(name, device, fn, *args):
+    """fn(*args, stream) with the device current, on its current stream (found without the stream object: a microsecond per call)."""
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        check(rc, name)
 
 
 class Act8:
@@ -1114,36 +1118,45 @@ class Act8:
         return self.buf.numel()
 
 
+def _rows_of(x, C):
+    """(rows, row stride) of [..., C]; anything goes when there are none"""
+    if x.is_contiguous():
+        return x.numel() // C, C
+    return _rows2d(x) if x.numel() else (0, C)
+
+
 def act_quant8(x, *, out=None):
     """x [..., C] (float32 / bfloat16; leading dims collapse onto one row stride) -> Act8.  out: an Act8 of the same shape to overwrite."""
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"act_quant8: a tensor with channels is needed, got shape {tuple(x.shape)}")
-    dt_code(x.dtype)
-    C = x.shape[-1]
-    rows, ld = (0, C) if x.numel() == 0 else _rows2d(x)
+    shape, dtype = x.shape, x.dtype
+    if len(shape) < 1 or shape[-1] == 0:
+        raise ValueError(f"act_quant8: a tensor with channels is needed, got shape {tuple(shape)}")
+    dt, C = dt_code(dtype), shape[-1]
+    rows, ld = _rows_of(x, C)
     if out is None:
-        out = Act8(x.shape, x.dtype, x.device)
-    elif not isinstance(out, Act8) or out.shape != x.shape or out.dtype != x.dtype:
+        out = Act8(shape, dtype, x.device)
+    elif not isinstance(out, Act8) or out.shape != shape or out.dtype != dtype:
         raise ValueError("act_quant8: out must be an Act8 of x's shape and dtype")
-    with _same_device("act_quant8", x, out.buf):
-        if rows:
-            check(_lib.load().m4d_act_quant8(dt_code(x.dtype), _ptr(x), ld, *out._ptrs(), rows, C, _raw_stream(x)), "m4d_act_quant8")
+    d = _same_device("act_quant8", x, out.buf)
+    if rows:
+        codes, exps = out._ptrs()
+        _launch("m4d_act_quant8", d, _lib.load().m4d_act_quant8, dt, x.data_ptr(), ld, codes, exps, rows, C)
     return out
 
 
 def act_dequant8(a8, dtype=None, *, act=0, out=None):
     """act(value) of an Act8 as a tensor of its shape, in its own dtype or `dtype`; act as in `unary` (0 none, 1 silu, 2 gelu(tanh), 3 gelu(erf)).
     out: [..., C], rows strided alike."""
-    C = a8.shape[-1]
+    shape = a8.shape
     if out is None:
-        out = torch.empty(a8.shape, device=a8.device, dtype=dtype or a8.dtype)
-    elif out.shape != a8.shape or (dtype is not None and out.dtype != dtype):
+        out = torch.empty(shape, device=a8.buf.device, dtype=dtype or a8.dtype)
+    elif out.shape != shape or (dtype is not None and out.dtype != dtype):
         raise ValueError("act_dequant8: out must have the activation's shape and the requested dtype")
-    dt = dt_code(out.dtype)
-    with _same_device("act_dequant8", a8.buf, out):
-        if a8.rows:
-            rows, ld = _rows2d(out)
-            check(_lib.load().m4d_act_dequant8(dt, *a8._ptrs(), _ptr(out), ld, rows, C, act, _raw_stream(out)), "m4d_act_dequant8")
+    dt, C = dt_code(out.dtype), shape[-1]
+    d = _same_device("act_dequant8", a8.buf, out)
+    rows, ld = _rows_of(out, C)
+    if rows:
+        codes, exps = a8._ptrs()
+        _launch("m4d_act_dequant8", d, _lib.load().m4d_act_dequant8, dt, codes, exps, out.data_ptr(), ld, rows, C, act)
     return out
 
 
@@ -1154,30 +1167,31 @@ def act_dequant8_t(a8, dtype=None, *, act=0):
     if R == 0:
         raise ValueError("act_dequant8_t: no rows")
     Rp = -(-R // 64) * 64 if R >= 512 else -(-R // 8) * 8
-    out = torch.empty((C, Rp), device=a8.device, dtype=dtype or a8.dtype)
-    with _same_device("act_dequant8_t", a8.buf):
-        check(_lib.load().m4d_act_dequant8_t(dt_code(out.dtype), *a8._ptrs(), _ptr(out), Rp, R, Rp, C, act, _raw_stream(out)),
-              "m4d_act_dequant8_t")
+    out = torch.empty((C, Rp), device=a8.buf.device, dtype=dtype or a8.dtype)
+    codes, exps = a8._ptrs()
+    _launch("m4d_act_dequant8_t", _same_device("act_dequant8_t", a8.buf), _lib.load().m4d_act_dequant8_t, dt_code(out.dtype), codes, exps,
+            out.data_ptr(), Rp, R, Rp, C, act)
     return out
 
 
 def act_bwd8(dy, a8, act, *, out=None):
     """dy * act'(value) with the pre-activation kept as an Act8; dy [..., C] of its shape, float32 or bfloat16.  out may be dy itself."""
-    if dy.shape != a8.shape:
-        raise ValueError(f"act_bwd8: dy {tuple(dy.shape)} against an activation of shape {tuple(a8.shape)}")
+    shape = dy.shape
+    if shape != a8.shape:
+        raise ValueError(f"act_bwd8: dy {tuple(shape)} against an activation of shape {tuple(a8.shape)}")
     if out is None:
-        out = torch.empty(dy.shape, device=dy.device, dtype=dy.dtype)
-    elif out.shape != dy.shape or out.dtype != dy.dtype:
+        out = torch.empty(shape, device=dy.device, dtype=dy.dtype)
+    elif out.shape != shape or out.dtype != dy.dtype:
         raise ValueError("act_bwd8: out must have dy's shape and dtype")
-    dt = dt_code(dy.dtype)
-    with _same_device("act_bwd8", dy, a8.buf, out):
-        if a8.rows:
-            rows, ldy = _rows2d(dy)
-            _, ldo = _rows2d(out)
-            if out.data_ptr() == dy.data_ptr() and ldo != ldy:
-                raise ValueError("act_bwd8: in place needs equal row strides")
-            check(_lib.load().m4d_act_bwd8(dt, _ptr(dy), ldy, *a8._ptrs(), _ptr(out), ldo, rows, dy.shape[-1], act, _raw_stream(dy)),
-                  "m4d_act_bwd8")
+    dt, C = dt_code(dy.dtype), shape[-1]
+    d = _same_device("act_bwd8", dy, a8.buf, out)
+    rows, ldy = _rows_of(dy, C)
+    _, ldo = _rows_of(out, C)
+    if rows:
+        if out.data_ptr() == dy.data_ptr() and ldo != ldy:
+            raise ValueError("act_bwd8: in place needs equal row strides")
+        codes, exps = a8._ptrs()
+        _launch("m4d_act_bwd8", d, _lib.load().m4d_act_bwd8, dt, dy.data_ptr(), ldy, codes, exps, out.data_ptr(), ldo, rows, C, act)
     return out
 
 
@@ -1218,8 +1232,8 @@ class AdapterBank:
         self.buf = torch.empty(at[-1], device=a.device, dtype=a.dtype)
         p = [self.buf.data_ptr() + o * a.element_size() for o in at[:-1]] + [0, 0]
         self._down, self._up, self._back = p[0], p[1], p[2:4] if backward else None
-        with _same_device("AdapterBank", a, b, self.buf):
-            check(lib.m4d_adapter_pack(dt, _ptr(a), _ptr(b), G, r, K, N, self.R, *p[:4], _raw_stream(a)), "m4d_adapter_pack")
+        _launch("m4d_adapter_pack", _same_device("AdapterBank", a, b, self.buf), lib.m4d_adapter_pack, dt, a.data_ptr(), b.data_ptr(), G, r, K, N,
+                self.R, *p[:4])
 
     def transposed(self):
         """The bank of the backward pass, v = s dy B and dx = dy W + v A: the down projection maps N channels, the up projection gives K."""
@@ -1310,18 +1324,20 @@ class AdapterPlan:
         a.rows, a.n_pieces, a.n_adapters = self.rows, self.n_pieces, self.n_adapters
         a.n_chunks[:] = [len(c[0]) // 3 for c in cs]
         a.n_listed = len(ts[0][0])
+        self.sizes = {}                         # workspace sizes by shape (_workspace)
 
 
 def _check_adapters(name, x, bank, plan):
-    rows, ldx = _rows2d(x)
+    K = x.shape[-1]
+    rows, ldx = _rows_of(x, K)
     if rows != plan.rows:
         raise ValueError(f"{name}: {rows} rows against a plan of {plan.rows}")
     if plan.n_adapters > bank.G:
         raise ValueError(f"{name}: the plan names adapter {plan.n_adapters - 1}, the bank has {bank.G}")
     if bank.buf.dtype != x.dtype:
         raise TypeError(f"{name}: x {x.dtype} vs adapters {bank.buf.dtype}")
-    if -(-bank.K // 8) * 8 < x.shape[-1] or bank.K > x.shape[-1]:       # (rows may be zero-padded to whole 16-byte chunks)
-        raise ValueError(f"{name}: x has {x.shape[-1]} channels, the adapters {bank.K}")
+    if not bank.K <= K < bank.K + 8:                # (rows may be zero-padded to whole 16-byte chunks)
+        raise ValueError(f"{name}: x has {K} channels, the adapters {bank.K}")
     return rows, ldx
 
 
@@ -1329,18 +1345,28 @@ def _slots_shape(bank, plan):
     return 4 * plan.n_pieces, (bank.R + 31) // 32, 2 if bank.buf.dtype == torch.bfloat16 else 1, 64, 8
 
 
+def _workspace(plan, key, device, fn, *args):
+    """(tensor or None, elements): the workspace of `fn`, its size kept with the plan (it depends on shapes only)."""
+    n = plan.sizes.get(key)
+    if n is None:
+        n = plan.sizes[key] = fn(*args)
+    return (torch.empty(n, device=device, dtype=torch.float32) if n else None), n
+
+
 def adapter_down(x, bank, plan, *, rows=True, slots=False):
     """(u [rows, R], ut) = s_g x A_g^T of each row's adapter (either may be left out: None).  u is written for rows with an adapter only; ut is the
     same by the plan's slots, in the order in which `adapter_grad` reads it (include/more4d_hip.h: adapter_down)."""
     M, ldx = _check_adapters("adapter_down", x, bank, plan)
-    u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype) if rows else None
+    K, R = x.shape[-1], bank.R
+    u = torch.empty((M, R), device=x.device, dtype=x.dtype) if rows else None
     ut = torch.empty(_slots_shape(bank, plan), device=x.device, dtype=x.dtype) if slots else None
+    if plan.n_pieces == 0 or not (rows or slots):
+        return u, ut
+    d = _same_device("adapter_down", x, bank.buf, plan.table)
     lib = _lib.load()
-    with _same_device("adapter_down", x, bank.buf, plan.table):
-        nws = lib.m4d_adapter_down_workspace(plan.args, x.shape[-1], bank.R, int(slots))
-        ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
-        check(lib.m4d_adapter_down(dt_code(x.dtype), _ptr(x), ldx, bank._down, _ptr(bank.scale), plan.args, _ptr(u), _ptr(ut), 0, 0,
-                                   x.shape[-1], bank.R, _ptr(ws), nws, _raw_stream(x)), "m4d_adapter_down")
+    ws, nws = _workspace(plan, ("down", d, K, R, slots), x.device, lib.m4d_adapter_down_workspace, plan.args, K, R, int(slots))
+    _launch("m4d_adapter_down", d, lib.m4d_adapter_down, dt_code(x.dtype), x.data_ptr(), ldx, bank._down, bank.scale.data_ptr(), plan.args, _ptr(u),
+            _ptr(ut), 0, 0, K, R, _ptr(ws), nws)
     return u, ut
 
 
@@ -1349,66 +1375,98 @@ def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=Fals
     bank: AdapterBank, out [..., N].  For a backward pass: slots=True returns (out, ut), ut = s x A^T in the slots of `adapter_grad`; keep8=True
     returns (out, ut, Act8 of x) — the 8-bit form of the rows that name an adapter, written in the pass that reads x (the codes of other
     rows are undefined; no gradient of an adapter reads them)."""
-    K, N = x.shape[-1], w.shape[0]
+    shape, dtype, device = x.shape, x.dtype, x.device
+    K, N, R = shape[-1], w.shape[0], bank.R
     if w.dim() != 2 or w.shape[1] != K:
         raise ValueError(f"linear_adapters: w {tuple(w.shape)} for x with {K} channels")
-    if w.dtype != x.dtype:
-        raise TypeError(f"linear_adapters: x {x.dtype} vs w {w.dtype}")
+    if w.dtype != dtype:
+        raise TypeError(f"linear_adapters: x {dtype} vs w {w.dtype}")
     if bank.N != N:
         raise ValueError(f"linear_adapters: w has {N} rows, the adapters {bank.N}")
-    if bias is not None and (bias.dtype != x.dtype or bias.numel() != N or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype != dtype or bias.numel() != N or not bias.is_contiguous()):
         raise ValueError("linear_adapters: bias must be contiguous, of x's dtype, with N elements")
     if out is None:
-        out = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
-    elif out.dtype != x.dtype or out.shape != (*x.shape[:-1], N):
-        raise ValueError(f"linear_adapters: out must be {(*x.shape[:-1], N)} of x's dtype")
-    ut = torch.empty(_slots_shape(bank, plan), device=x.device, dtype=x.dtype) if slots or keep8 else None
-    x8 = Act8(x.shape, x.dtype, x.device) if keep8 else None
+        out = torch.empty((*shape[:-1], N), device=device, dtype=dtype)
+    elif out.dtype != dtype or out.shape != (*shape[:-1], N):
+        raise ValueError(f"linear_adapters: out must be {(*shape[:-1], N)} of x's dtype")
+    slots = slots or keep8
+    ut = torch.empty(_slots_shape(bank, plan), device=device, dtype=dtype) if slots else None
+    x8 = Act8(shape, dtype, device) if keep8 else None
     ret = (out, ut, x8) if keep8 else (out, ut) if slots else out
-    if x.numel() == 0:
-        if plan.rows:
-            raise ValueError(f"linear_adapters: no rows against a plan of {plan.rows}")
-        return ret
     M, ldx = _check_adapters("linear_adapters", x, bank, plan)
-    if plan.n_pieces == 0:                  # nobody names an adapter: the shared projection alone
-        gemm_bt(x, w, bias, out=out)
+    if M == 0:
         return ret
-    _, ldw = _rows2d(w)
-    _, ldo = _rows2d(out)
-    dt = dt_code(x.dtype)
+    d = _same_device("linear_adapters", x, w, bias, out, bank.buf, plan.table)
+    if plan.n_pieces == 0:                  # nobody names an adapter: the shared projection alone
+        with torch.cuda.device(d):
+            gemm_bt(x, w, bias, out=out)
+        return ret
+    dt, ldw = dt_code(dtype), _rows_of(w, K)[1]
+    ldo = _rows_of(out, N)[1]
     lib = _lib.load()
-    with _same_device("linear_adapters", x, w, bias, out, bank.buf, plan.table):
-        u = torch.empty((M, bank.R), device=x.device, dtype=x.dtype)
-        nws = lib.m4d_linear_adapters_workspace(dt, plan.args, N, K, bank.R, int(ut is not None))
-        ws = torch.empty(nws, device=x.device, dtype=torch.float32) if nws else None
-        check(lib.m4d_linear_adapters(dt, _ptr(x), ldx, _ptr(w), ldw, _ptr(bias), bank._down, _ptr(bank.scale), bank._up, plan.args,
-                                      _ptr(u), _ptr(ut), *(x8._ptrs() if keep8 else (0, 0)), _ptr(out), ldo, N, K, bank.R, _ptr(ws), nws,
-                                      _raw_stream(x)), "m4d_linear_adapters")
+    u = torch.empty((M, R), device=device, dtype=dtype)
+    ws, nws = _workspace(plan, ("linear", d, dt, N, K, R, slots), device, lib.m4d_linear_adapters_workspace, dt, plan.args, N, K, R, int(slots))
+    codes, exps = x8._ptrs() if keep8 else (0, 0)
+    _launch("m4d_linear_adapters", d, lib.m4d_linear_adapters, dt, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(bias), bank._down, bank.scale.data_ptr(),
+            bank._up, plan.args, u.data_ptr(), _ptr(ut), codes, exps, out.data_ptr(), ldo, N, K, R, _ptr(ws), nws)
     return ret
 
 
 def adapter_grad(vt, x, plan, bank, *, transposed=False):
     """Gradient of the adapters: sum over the rows of each adapter of v^T x, as [G, rank, C] (transposed: [G, C, rank]) in vt's dtype; adapters that
     no row names get zero.  vt: the slots that `adapter_down` / `linear_adapters` return; x [rows, C], or its Act8."""
-    G, rank, R = bank.G, bank.rank, bank.R
-    x8 = x if isinstance(x, Act8) else None
-    C = x.shape[-1]
+    G, rank, R, C = bank.G, bank.rank, bank.R, x.shape[-1]
+    x8 = isinstance(x, Act8)
     if plan.n_adapters > G:
         raise ValueError(f"adapter_grad: the plan names adapter {plan.n_adapters - 1}, the bank has {G}")
     if vt.shape != _slots_shape(bank, plan) or not vt.is_contiguous():
         raise ValueError("adapter_grad: vt must be adapter_down's slots")
-    rows, ldx = (x8.rows, 0) if x8 is not None else (0, 0) if x.numel() == 0 else _rows2d(x)
+    rows, ldx = (x.rows, 0) if x8 else _rows_of(x, C)
     if rows != plan.rows:
         raise ValueError(f"adapter_grad: {rows} rows against a plan of {plan.rows}")
-    if x8 is None and x.dtype != vt.dtype:
+    if not x8 and x.dtype != vt.dtype:
         raise TypeError(f"adapter_grad: x {x.dtype} vs v {vt.dtype}")
     dt = dt_code(vt.dtype)
     out = torch.empty((G, C, rank) if transposed else (G, rank, C), device=vt.device, dtype=vt.dtype)
+    d = _same_device("adapter_grad", vt, x.buf if x8 else x, plan.table)
     if plan.n_pieces == 0:
         return out.zero_()
-    with _same_device("adapter_grad", vt, x8.buf if x8 is not None else x, plan.table):
-        lib = _lib.load()
-        ws = torch.empty(lib.m4d_adapter_grad_workspace(plan.args, C, R), device=vt.device, dtype=torch.float32)
-        check(lib.m4d_adapter_grad(dt, _ptr(vt), 0 if x8 is not None else _ptr(x), ldx, *(x8._ptrs() if x8 is not None else (0, 0)),
-                                   plan.args, _ptr(ws), ws.numel(), _ptr(out), int(transposed), G, rank, C, R, _raw_stream(vt)), "m4d_adapter_grad")
+    lib = _lib.load()
+    ws, nws = _workspace(plan, ("grad", d, C, R), vt.device, lib.m4d_adapter_grad_workspace, plan.args, C, R)
+    codes, exps = x._ptrs() if x8 else (0, 0)
+    _launch("m4d_adapter_grad", d, lib.m4d_adapter_grad, dt, vt.data_ptr(), 0 if x8 else x.data_ptr(), ldx, codes, exps, plan.args, ws.data_ptr(), nws,
+            out.data_ptr(), int(transposed), G, rank, C, R)
     return out
+
+
+def linear_adapters_bwd(dy, w, bank, plan, *, x=None, ut=None, need_x=True):
+    """Backward of `linear_adapters` for a frozen w: (dx, da, db), None for what is not asked for.  dy [rows, N] (rows of whole 16-byte chunks), w
+    [N, K], bank: the forward's, built with backward=True; da if the kept input x ([rows, K] or its Act8) is given, db if the forward's ut is."""
+    N, K = w.shape
+    back = bank.transposed()
+    M, ldy = _check_adapters("linear_adapters_bwd", dy, back, plan)
+    if N != dy.shape[-1] or bank.K != K or w.dtype != dy.dtype:
+        raise ValueError(f"linear_adapters_bwd: dy {tuple(dy.shape)}, w {tuple(w.shape)} and adapters {bank.N} x {bank.K} do not fit")
+    G, rank, R, dtype, device = bank.G, bank.rank, bank.R, dy.dtype, dy.device
+    x8 = isinstance(x, Act8)
+    if x is not None:
+        rows, ldx = (x.rows, 0) if x8 else _rows_of(x, K)
+        if rows != M or x.shape[-1] != K or (not x8 and x.dtype != dtype):
+            raise ValueError("linear_adapters_bwd: x must be the forward's input, [rows, K] of dy's dtype, or its Act8")
+    if ut is not None and (ut.shape != _slots_shape(bank, plan) or ut.dtype != dtype or not ut.is_contiguous()):
+        raise ValueError("linear_adapters_bwd: ut must be the forward's slots")
+    dx = torch.empty((M, K), device=device, dtype=dtype) if need_x else None
+    da = torch.empty((G, rank, K), device=device, dtype=dtype) if x is not None else None
+    db = torch.empty((G, N, rank), device=device, dtype=dtype) if ut is not None else None
+    d = _same_device("linear_adapters_bwd", dy, w, bank.buf, plan.table, ut, x.buf if x8 else x)
+    dt, lib = dt_code(dtype), _lib.load()
+    if M == 0 or not (need_x or x is not None or ut is not None):
+        return dx, da.zero_() if da is not None else None, db.zero_() if db is not None else None
+    ldw = _rows_of(w, K)[1]
+    need = (need_x, x is not None, ut is not None)
+    ws, nws = _workspace(plan, ("bwd", d, dt, N, K, R, need), device, lib.m4d_linear_adapters_bwd_workspace, dt, plan.args, N, K, R, *map(int, need))
+    codes, exps = x._ptrs() if x8 else (0, 0)
+    _launch("m4d_linear_adapters_bwd", d, lib.m4d_linear_adapters_bwd, dt, dy.data_ptr(), ldy, w.data_ptr(), ldw, back._down, back.scale.data_ptr(),
+            back._up, plan.args, 0 if x8 or x is None else x.data_ptr(), ldx if x is not None else 0, codes, exps, _ptr(ut), _ptr(dx), _ptr(da),
+            _ptr(db), G, rank, N, K, R, _ptr(ws), nws)
+    return dx, da, db
