@@ -261,13 +261,14 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void adapter_gemv_kernel(AdGemmA
         const int g = p.tile_list[i];
         const T* b = (const T*)p.up + ((int64_t)g * p.N + min(n0 + i16, p.N - 1)) * p.R;
         const T* u = (const T*)p.u + (int64_t)row * p.R;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < p.R; k += 32) {
             const int kq = k + q * 8, ks = min(kq, p.R - 8);
-            const frag_t fb = *reinterpret_cast<const frag_t*>(b + ks);
-            frag_t fu = *reinterpret_cast<const frag_t*>(u + ks);
-            if (ra != g || kq >= p.R) fu = frag_t{};
-            mma16(fb, fu, acc);
+            frag_t fb = *reinterpret_cast<const frag_t*>(b + ks), fu = *reinterpret_cast<const frag_t*>(u + ks);
+            if (kq >= p.R) fb = fu = frag_t{};
+            mma16(fb, fu, sum);
         }
+        if (ra == g) acc += sum;                    // (see adapters_extend: rows of other adapters see nothing of this one)
     }
     red[wave][lane] = acc;
     __syncthreads();

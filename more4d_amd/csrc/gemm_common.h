@@ -155,7 +155,10 @@ M4D_DEV void epilogue_tile(const GemmArgs& p, const f32x16& acc, int64_t m, int6
 // acc += up_g[n, :] . u[m, :] over the rank, for every step-th adapter of the tile from `first` on.  The operands come straight from L2 in the
 // MFMA layout (16 bytes per lane and 16 ranks; a block's 32 rows of R ranks are contiguous memory): through LDS they would need two more
 // barriers.  All loads of 64 ranks are issued before their first product, so a tile pays one L2 latency per 64 ranks and adapter, not four.
-// Rows of u that name another adapter (or none: their u was never written) are replaced by zero before the product, not multiplied by zero.
+// Rows of u that name another adapter (or none: their u was never written) are replaced by zero before the product, not multiplied by zero; and
+// where a wave's rows do not all name the adapter, an infinity or NaN in its B must not meet those zeros: float32 then takes sums of their own that
+// only the adapter's rows add, bf16 bad_parts (a VALU instruction on its accumulators takes them out of the AGPRs: 200 spilled registers in the
+// 256 x 256 kernel).
 // AdTile: what the extension has to know about its tile, loaded in front of the K loop (behind it these would be three dependent trips to L2).
 template <int MI> struct AdTile { int i0, i1, g0; int ra[MI]; };
 template <int MI>
@@ -171,11 +174,50 @@ M4D_DEV AdTile<MI> adapters_tile(const GemmAdArgs& p, int tile, int64_t m_base, 
     }
     return a;
 }
+// bits of a fragment's largest magnitude as a float32 (integers order like magnitudes, NaN on top)
+M4D_DEV unsigned frag_top(const bf16x8& f) {
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    const u16x8 v = __builtin_bit_cast(u16x8, f) & (unsigned short)0x7fff;
+    const u16x2 a = __builtin_elementwise_max(u16x2{v[0], v[1]}, u16x2{v[2], v[3]}), b = __builtin_elementwise_max(u16x2{v[4], v[5]}, u16x2{v[6], v[7]});
+    const u16x2 m = __builtin_elementwise_max(a, b);
+    return (unsigned)max(m[0], m[1]) << 16;
+}
+M4D_DEV unsigned frag_top(const f32x8& f) {
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, __builtin_bit_cast(unsigned, f[e]) & 0x7fffffffu);
+    return m;
+}
+// A fragment of B that is not finite as a sum of three: b keeps the finite values, `inf` has +-big for every other, `nan` the opposite for NaNs.  u's
+// fragment becomes +-big as well, zero in rows of other adapters (big_signs): big * big overflows to the infinity that the adapter's own rows
+// have to get, inf - inf is the NaN, and the others get 0 * big = 0.  (bf16 only: float32's MFMA does not round the product, inf - big * big is inf.)
+M4D_DEV void bad_parts(bf16x8& b, bf16x8& inf, bf16x8& nan) {
+    const float big = 3.3e38f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float v = (float)b[e];
+        const unsigned u = __builtin_bit_cast(unsigned, v), m = u & 0x7fffffffu;
+        const float s = m >= 0x7f800000u ? (u >> 31 ? -big : big) : 0.f;
+        inf[e] = (bf16_t)s;
+        nan[e] = (bf16_t)(m > 0x7f800000u ? -s : 0.f);
+        b[e] = (bf16_t)(m >= 0x7f800000u ? 0.f : v);
+    }
+}
+M4D_DEV bf16x8 big_signs(const bf16x8& u) {
+    bf16x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float v = (float)u[e];
+        r[e] = (bf16_t)(v > 0.f ? 3.3e38f : v < 0.f ? -3.3e38f : 0.f);
+    }
+    return r;
+}
 template <typename T, int NI, int MI>
 M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const AdTile<MI>& a, int64_t m_base, int64_t n_base, int lane, int step = 1,
                              int k0 = 0) {      // k0: ranks in front of it are already in
     typedef typename Frag8<T>::type frag_t;
-    constexpr int U = sizeof(T) == 2 ? 4 : 1;         // 16-rank steps in flight (float32 fragments are twice as wide, and MFMA-bound)
+    constexpr int U = sizeof(T) != 2 ? 1 : NI * MI < 16 ? 4 : 2;      // 16-rank steps in flight, as registers allow (float32 is MFMA-bound)
     const int li = lane & 31, hi = lane >> 5;
     if (a.i0 >= a.i1 || k0 >= p.R) return;
     const T* pu[MI];
@@ -189,6 +231,11 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
     for (int ni = 0; ni < NI; ++ni) nr[ni] = min(n_base + ni * 32 + li, p.N - 1) * p.R + hi * 8;
     for (int i = a.i0; i < a.i1; i += step) {
         const int g = i == a.i0 ? a.g0 : __builtin_amdgcn_readfirstlane(p.tile_list[i]);
+        bool mine = false, all = true;
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) { mine |= a.ra[mi] == g; all &= a.ra[mi] == g; }
+        if (!__any(mine)) continue;                   // none of this wave's rows
+        const bool mixed = !__all(all);
         const T* b = (const T*)p.up + (int64_t)g * p.N * p.R;
         // C steps of 16 ranks: all loads (without predicates: rows of other adapters are replaced after the load), then the products
         auto chunk = [&](auto C_T, int k) {
@@ -201,11 +248,48 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni) fb[s][ni] = *reinterpret_cast<const frag_t*>(b + nr[ni] + k + s * 16);
             }
+            if (mixed) {
+                unsigned top = 0;
+#pragma unroll
+                for (int s = 0; s < C; ++s) {
+#pragma unroll
+                    for (int mi = 0; mi < MI; ++mi)
+                        if (a.ra[mi] != g) fu[s][mi] = frag_t{};
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni) top = max(top, frag_top(fb[s][ni]));
+                }
+                if (__any(top >= 0x7f800000u)) {
+#pragma unroll
+                    for (int s = 0; s < C; ++s)
+#pragma unroll
+                        for (int ni = 0; ni < NI; ++ni) {
+                            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                                for (int mi = 0; mi < MI; ++mi) {
+                                    f32x16 sum;
+#pragma unroll
+                                    for (int q = 0; q < 16; ++q) sum[q] = 0.f;
+                                    mma32(fb[s][ni], fu[s][mi], sum);
+#pragma unroll
+                                    for (int q = 0; q < 16; ++q) acc[ni][mi][q] += a.ra[mi] == g ? sum[q] : 0.f;
+                                    __builtin_amdgcn_sched_barrier(0);
+                                }
+                                fb[s][ni] = frag_t{};
+                            } else {
+                                frag_t inf, nan;
+                                bad_parts(fb[s][ni], inf, nan);
+#pragma unroll
+                                for (int mi = 0; mi < MI; ++mi) {
+                                    const frag_t us = big_signs(fu[s][mi]);
+                                    mma32(inf, us, acc[ni][mi]);
+                                    mma32(nan, us, acc[ni][mi]);
+                                }
+                            }
+                        }
+                }
+            }
 #pragma unroll
             for (int s = 0; s < C; ++s) {
-#pragma unroll
-                for (int mi = 0; mi < MI; ++mi)
-                    if (a.ra[mi] != g) fu[s][mi] = frag_t{};
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
@@ -214,10 +298,10 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
         };
         int k = k0;
         for (; k + 16 * U <= p.R; k += 16 * U) chunk(std::integral_constant<int, U>{}, k);
-        if constexpr (U == 4) {
+        if constexpr (U == 4)
             if (k + 32 <= p.R) { chunk(std::integral_constant<int, 2>{}, k); k += 32; }
+        if constexpr (U > 1)
             if (k < p.R) chunk(std::integral_constant<int, 1>{}, k);
-        }
     }
 }
 
