@@ -116,9 +116,10 @@ class AdapterLinearFn(Function):
         if dy2.shape[0] == 0:
             zero = [dy2.new_zeros(s) if n else None for s, n in ((xshape, need_x), ((bank.G, bank.rank, K), need_a), ((bank.G, N, bank.rank), need_b))]
             return zero[0], None, None, zero[1], zero[2], None, None, None
-        if dy2.stride(-1) != 1 or dy2.stride(0) < N or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
+        per = 16 // dy2.element_size()
+        if dy2.stride(-1) != 1 or dy2.stride(0) < N or dy2.stride(0) % per or dy2.data_ptr() % 16:
             dy2 = dy2.contiguous()
-        Np = -(-N // 8) * 8
+        Np = -(-N // per) * per
         if Np == N:
             x = None if not need_a else ops.Act8((dy2.shape[0], K), xdt, buf=kept) if bits == 8 else kept
             dx, da, db = ops.linear_adapters_bwd(dy2, weight.detach(), bank, plan, x=x, ut=ut if need_b else None, need_x=need_x)

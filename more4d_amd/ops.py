@@ -1336,7 +1336,7 @@ def _check_adapters(name, x, bank, plan):
         raise ValueError(f"{name}: the plan names adapter {plan.n_adapters - 1}, the bank has {bank.G}")
     if bank.buf.dtype != x.dtype:
         raise TypeError(f"{name}: x {x.dtype} vs adapters {bank.buf.dtype}")
-    if not bank.K <= K < bank.K + 8:                # (rows may be zero-padded to whole 16-byte chunks)
+    if K != bank.K and K != bank.K + -bank.K % (16 // bank.buf.element_size()):      # (rows may be zero-padded to whole 16-byte chunks)
         raise ValueError(f"{name}: x has {K} channels, the adapters {bank.K}")
     return rows, ldx
 

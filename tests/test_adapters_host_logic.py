@@ -82,3 +82,17 @@ def test_cpu_tensors_are_refused():
         ops.act_quant8(torch.empty(4, 0))
     with pytest.raises(TypeError):
         ops.act_quant8(x.half())
+
+
+@pytest.mark.parametrize("dtype,K,fits,too_wide", [(torch.float32, 64, (64,), (68, 72)), (torch.float32, 61, (61, 64), (60, 68)), (torch.bfloat16, 64, (64,), (72,)),
+                                                   (torch.bfloat16, 60, (60, 64), (56, 68, 72))])
+def test_rows_padded_by_more_than_one_chunk_are_refused(dtype, K, fits, too_wide):
+    """The bank is laid out in chunks of 64 channels: a row that reaches into one more would read the next adapter's, or behind the bank."""
+    bank = ops.AdapterBank.__new__(ops.AdapterBank)
+    bank.buf, bank.K, bank.G = torch.empty(0, dtype=dtype), K, 1
+    plan = ops.AdapterPlan([3], [0], "cpu")
+    for k in fits:
+        assert ops._check_adapters("test", torch.zeros(3, k, dtype=dtype), bank, plan) == (3, k)
+    for k in too_wide:
+        with pytest.raises(ValueError):
+            ops._check_adapters("test", torch.zeros(3, k, dtype=dtype), bank, plan)
