@@ -1197,9 +1197,10 @@ def act_bwd8(dy, a8, act, *, out=None):
 
 # ------------------------------------------------------------------ low-rank adapters of many requests beside a shared projection
 class AdapterBank:
-    """The adapters of one projection: a [G, r, K], b [G, N, r] (one dtype, contiguous), scale: G numbers or a float32 tensor [G] (adapters of
-    different ranks: pad the smaller ones with zeros).  Laid out for the kernels once, here (m4d_adapter_pack): later changes of a and b are not
-    seen.  backward=True lays out the transposed operands of the backward pass as well (`transposed`)."""
+    """The adapters of one projection: a [G, r, K], b [G, N, r] (one dtype, G <= 65535, r <= 512), scale: G numbers or a float32 tensor [G]
+    (adapters of different ranks: pad the smaller ones with zeros).  Laid out for the kernels once, here (m4d_adapter_pack): later changes of a
+    and b are not seen; a float32 scale tensor on their device is used as it stands, later changes included (a captured step takes this
+    form: numbers are copied from the host).  backward=True lays out the transposed operands of the backward pass as well (`transposed`)."""
     __slots__ = ("buf", "scale", "G", "rank", "R", "K", "N", "_down", "_up", "_back")
 
     def __init__(self, a, b, scale, *, backward=False):
@@ -1207,8 +1208,8 @@ class AdapterBank:
             raise ValueError(f"AdapterBank: a [G, r, K] and b [G, N, r] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
         G, r, K = a.shape
         N = b.shape[1]
-        if not (G >= 1 and 1 <= r <= 512 and K >= 1 and N >= 1):
-            raise ValueError(f"AdapterBank: at least one adapter of rank 1..512, got {G} of rank {r}")
+        if not (1 <= G <= AdapterPlan.MAX_ADAPTERS and 1 <= r <= 512 and K >= 1 and N >= 1):
+            raise ValueError(f"AdapterBank: 1..{AdapterPlan.MAX_ADAPTERS} adapters of rank 1..512, got {G} of rank {r}")
         if a.dtype != b.dtype:
             raise TypeError(f"AdapterBank: a {a.dtype} vs b {b.dtype}")
         dt = dt_code(a.dtype)
@@ -1248,8 +1249,10 @@ class AdapterBank:
 class AdapterPlan:
     """Which adapter each row of a batch uses: request j owns the next lengths[j] rows (0 allowed) and names adapter adapters[j] (-1: none).
     Host numbers; the tables (include/more4d_hip.h: m4d_adapter_plan) are built here and copied to `device` once per batch composition, then
-    shared by every projection of the model."""
-    PIECE, CHUNK_PIECES = 64, 64
+    shared by every projection of the model (not inside a graph capture).  Any order of the requests is right; requests of one adapter side
+    by side are fastest, because a tile of the projection adds the adapters of all its rows: 1024 one-row requests of 64 adapters, rank 16 / 64,
+    5120 x 5120: 88 / 100 us in order of adapters, 120 / 346 us interleaved."""
+    PIECE, CHUNK_PIECES, MAX_ADAPTERS = 64, 64, 65535
 
     def __init__(self, lengths, adapters, device):
         import numpy as np
@@ -1258,6 +1261,8 @@ class AdapterPlan:
             raise ValueError(f"AdapterPlan: {len(lengths)} lengths for {len(adapters)} adapter numbers")
         if any(v < 0 for v in lengths) or any(v < -1 for v in adapters):
             raise ValueError("AdapterPlan: lengths are >= 0, adapter numbers >= -1")
+        if max(adapters, default=-1) >= self.MAX_ADAPTERS:
+            raise ValueError(f"AdapterPlan: adapter numbers below {self.MAX_ADAPTERS}, got {max(adapters)}")
         if sum(lengths) >= 1 << 31:
             raise ValueError("AdapterPlan: too many rows")
         P = self.PIECE
@@ -1372,7 +1377,7 @@ def adapter_down(x, bank, plan, *, rows=True, slots=False):
 
 def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=False):
     """x w^T + bias + s_g (x A_g^T) B_g^T, g the adapter of each row (plan).  x [..., K] (rows strided), w [N, K] (row-strided), bias [N] or None,
-    bank: AdapterBank, out [..., N].  For a backward pass: slots=True returns (out, ut), ut = s x A^T in the slots of `adapter_grad`; keep8=True
+    bank: AdapterBank, out [..., N], none of the inputs.  Rows of x and w are whole 16-byte chunks, 16-byte aligned; N is a multiple of 4.  For a backward pass: slots=True returns (out, ut), ut = s x A^T in the slots of `adapter_grad`; keep8=True
     returns (out, ut, Act8 of x) — the 8-bit form of the rows that name an adapter, written in the pass that reads x (the codes of other
     rows are undefined; no gradient of an adapter reads them)."""
     shape, dtype, device = x.shape, x.dtype, x.device

@@ -96,3 +96,14 @@ def test_rows_padded_by_more_than_one_chunk_are_refused(dtype, K, fits, too_wide
     for k in too_wide:
         with pytest.raises(ValueError):
             ops._check_adapters("test", torch.zeros(3, k, dtype=dtype), bank, plan)
+
+
+def test_adapter_numbers_have_a_limit():
+    """(the tables hold an entry per adapter number: a stray one would ask for all the memory there is)"""
+    assert ops.AdapterPlan([1], [65534], "cpu").n_adapters == 65535
+    for i in (65535, 1 << 31, 1 << 40):
+        with pytest.raises(ValueError):
+            ops.AdapterPlan([0], [i], "cpu")
+    a, b = torch.empty(1).expand(65536, 1, 1), torch.empty(1).expand(65536, 1, 1)
+    with pytest.raises(ValueError):
+        ops.AdapterBank(a, b, [1.0] * 65536)
