@@ -80,9 +80,10 @@ class LinearFn(Function):
 
 class AdapterLinearFn(Function):
     """A frozen projection with trained low-rank adapters (ops.linear_adapters): apply(x, weight, bias, a, b, scale, plan, bits).
-    x [..., K]; weight [N, K] and bias are not trained; a [G, r, K], b [G, N, r] are, scale is G numbers.  The gradient of `a` needs the input,
-    that of `b` only u = s x A^T: the forward keeps x as it is (bits = 16) or in 8 bits (bits = 8, half the memory of bf16 and half the bytes that
-    the gradient reads).  The forward's own result comes from x itself either way."""
+    x [..., K]; weight [N, K] and bias are not trained; a [G, r, K], b [G, N, r] are, scale is G numbers or a tensor (AdapterBank).  The gradient
+    of `a` needs the input, that of `b` only u = s x A^T: the forward keeps x as it is (bits = 16) or in 8 bits (bits = 8, half the memory of
+    bf16 and half the bytes that the gradient reads).  The forward's own result comes from x itself either way.
+    In a captured step forward and backward belong into one capture, with scale on the device, and no eager graph of the same leaves may be alive."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, a, b, scale, plan, bits):
@@ -90,6 +91,10 @@ class AdapterLinearFn(Function):
             raise ValueError(f"AdapterLinearFn: bits must be 8 or 16, got {bits}")
         if weight.requires_grad or (bias is not None and bias.requires_grad):
             raise ValueError("AdapterLinearFn: the projection is frozen; train it with LinearFn")
+        if isinstance(scale, torch.Tensor) and scale.requires_grad:
+            raise ValueError("AdapterLinearFn: scale gets no gradient")
+        if a.dim() != 3 or a.shape[2] != x.shape[-1]:
+            raise ValueError(f"AdapterLinearFn: a {tuple(a.shape)} for x with {x.shape[-1]} channels")
         x2 = x.detach().reshape(-1, x.shape[-1])
         need_a, need_b = ctx.needs_input_grad[3], ctx.needs_input_grad[4]
         bank = ops.AdapterBank(a, b, scale, backward=any(ctx.needs_input_grad))
@@ -100,13 +105,14 @@ class AdapterLinearFn(Function):
             y, ut = ops.linear_adapters(x2, weight.detach(), bias, bank, plan, slots=True)
         else:
             y = ops.linear_adapters(x2, weight.detach(), bias, bank, plan)
-        ctx.save_for_backward((kept.buf if bits == 8 else x2) if need_a else None, weight, ut if need_b else None)
+        ctx.save_for_backward((kept.buf if bits == 8 else x2) if need_a else None, weight, ut if need_b else None,
+                              scale if bank.scale is scale else None)       # (only kept so that a change in between is noticed)
         ctx.meta = (bank, plan, bits, x.shape, x.dtype)       # (the bank is this call's own copy of a and b, laid out for both passes)
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     def backward(ctx, dy):
-        kept, weight, ut = ctx.saved_tensors
+        kept, weight, ut, _ = ctx.saved_tensors
         bank, plan, bits, xshape, xdt = ctx.meta
         N, K = weight.shape
         need_x, need_a, need_b = (ctx.needs_input_grad[i] for i in (0, 3, 4))

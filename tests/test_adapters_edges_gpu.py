@@ -39,3 +39,32 @@ def test_an_adapter_that_is_not_finite_stays_with_its_rows(dt, M, N, K, r):
     ok[mine, 9] = y[mine, 9] == -float("inf") * u[mine, 4].double()
     assert (u[mine][:, [2, 4]] != 0).all()
     assert ok.all(), (~ok).nonzero()[:8].tolist()
+
+
+def test_changes_between_forward_and_backward():
+    """A scale tensor that wants a gradient is refused; x, W or scale changed in place between the passes raises; a and b may change (laid out)."""
+    from more4d_amd.autograd import AdapterLinearFn
+    o = ops()
+    lengths, ids = [30, 3, 40], [1, -1, 0]
+    x, w, bias, a, b, scale, _ = on_gpu(*problem(lengths, ids, 64, 72, 4, BF))
+    plan, s = o.AdapterPlan(lengths, ids, DEV), torch.tensor(scale, device=DEV)
+    dy = torch.randn(73, 72, device=DEV).to(BF)
+    with pytest.raises(ValueError):
+        AdapterLinearFn.apply(x, w, bias, a, b, s.clone().requires_grad_(True), plan, 8)
+    with pytest.raises(ValueError):                       # rows padded beyond the adapters' K: serving only
+        AdapterLinearFn.apply(x, w, bias, a[:, :, :60], b, s, plan, 8)
+
+    def run(change):
+        xx, ww, ss, aa, bb = x.clone(), w.clone(), s.clone(), a.clone().requires_grad_(True), b.clone().requires_grad_(True)
+        y = AdapterLinearFn.apply(xx, ww, bias, aa, bb, ss, plan, 16)
+        with torch.no_grad():
+            change(xx, ww, ss, aa, bb)
+        return torch.autograd.grad(y, (aa, bb), dy)
+
+    want = run(lambda *t: None)
+    for i in range(3):
+        with pytest.raises(RuntimeError):
+            run(lambda *t: t[i].mul_(2))
+    for i in (3, 4):
+        for p, q in zip(run(lambda *t: t[i].mul_(2)), want):
+            assert torch.equal(p, q)
