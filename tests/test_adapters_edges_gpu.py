@@ -68,3 +68,203 @@ def test_changes_between_forward_and_backward():
     for i in (3, 4):
         for p, q in zip(run(lambda *t: t[i].mul_(2)), want):
             assert torch.equal(p, q)
+
+
+def check(y, want, tol):
+    err = (y.double() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("lengths,ids,r", [
+    ([4100], [0], 16),                                      # one adapter, ranks behind the K loop
+    ([4100], [0], 64),                                      # ... as one more K tile
+    ([4100], [0], 144),                                     # ... as two and a remainder
+    ([256, 2048, 1796], [2, 0, 1], 72),                     # whole tiles of each, the shifted last one of one adapter
+    ([1000, 1, 2000, 0, 1099], [1, 0, -1, 2, 1], 64),       # tiles of several, tiles of none
+    ([1] * 300 + [3800], [i % 7 - 1 for i in range(300)] + [0], 8),
+])
+@pytest.mark.parametrize("K", [1984, 2048])
+def test_the_largest_tiles(lengths, ids, r, K):
+    o = ops()
+    M, N, _ = WIDE
+    x, w, bias, a, b, scale, row = on_gpu(*problem(lengths, ids, K, N, r, BF))
+    plan, bank = o.AdapterPlan(lengths, ids, DEV), o.AdapterBank(a, b, scale)
+    out = torch.full((M + 1, N + 4), float("nan"), device=DEV, dtype=BF)
+    o.launch_counts(reset=True)
+    y = o.linear_adapters(x, w, bias, bank, plan, out=out[:M, :N])
+    assert o.launch_counts()["gemm_wide"] == 1
+    check(y, *oracle(x, w, bias, a, b, scale, row))
+    assert torch.isnan(out[M]).all() and torch.isnan(out[:, N:]).all()
+    assert torch.equal(y, o.linear_adapters(x, w, bias, bank, plan))
+
+
+def test_offsets_beyond_32_bits():
+    """x of 2^31 + elements: its last rows, which alone name adapters with those at the front, in every pass that addresses rows."""
+    o = ops()
+    K, N, r, M = 4096, 64, 16, (1 << 19) + 700
+    lengths, ids = [200, M - 500, 300], [0, -1, 1]
+    _, w, bias, a, b, scale, _ = on_gpu(*problem([1, 1], [0, 1], K, N, r, BF))
+    x = torch.zeros(M, K, device=DEV, dtype=BF)
+    x[:200].normal_()
+    x[-300:].normal_()
+    plan, bank = o.AdapterPlan(lengths, ids, DEV), o.AdapterBank(a, b, scale)
+    y, ut, x8 = o.linear_adapters(x, w, bias, bank, plan, keep8=True)
+    ends = torch.cat([torch.arange(200), torch.arange(M - 300, M)]).to(DEV)
+    rows, xe = torch.cat([torch.zeros(200), torch.ones(300)]).long().to(DEV), x[ends]
+    check(y[ends], *oracle(xe, w, bias, a, b, scale, rows))
+    assert torch.equal(y[200:-300], bias.expand(M - 500, N))
+    small = o.AdapterPlan([200, 300], [0, 1], DEV)
+    ref8 = o.act_quant8(xe)
+    assert torch.equal(x8.codes[ends], ref8.codes) and torch.equal(x8.exps[ends], ref8.exps)
+    big, few = o.adapter_grad(ut, x8, plan, bank), o.adapter_grad(o.adapter_down(xe, bank, small, slots=True)[1], xe, small, bank)
+    assert torch.equal(o.adapter_grad(ut, x, plan, bank), few)
+    h = torch.finfo(BF).eps / 2
+    v8 = o.act_dequant8(ref8).double()
+    u = o.adapter_down(xe, bank, small)[0].double()[:, :r]
+    for g in range(2):                                     # (u rounded to bf16 once instead of kept to 16 bits: h of every term more)
+        want = u[rows == g].t() @ v8[rows == g]
+        tol = h * want.abs() + (2 * h + 500 * 2.0 ** -23) * (u[rows == g].abs().t() @ v8[rows == g].abs())
+        check(big[g], want, tol)
+    q = o.act_quant8(x)
+    assert torch.equal(q.codes[ends], ref8.codes) and not q.codes[200:-300].any()
+    assert torch.equal(o.act_dequant8(q)[ends], o.act_dequant8(ref8))
+    t = o.act_dequant8_t(q, act=1)
+    assert t.shape[1] >= M and torch.equal(t[:, ends], o.act_dequant8(ref8, act=1).t().contiguous()) and not t[:, M:].any()
+    del t, q
+    x.fill_(1.0)
+    assert torch.equal(o.act_bwd8(x, x8, 2, out=x)[ends], o.act_bwd8(torch.ones_like(xe), ref8, 2))
+
+
+def test_a_long_output():
+    """out of 2^31 + elements: the tiles' stores at its end."""
+    o = ops()
+    K, r, N, M = 64, 16, 32768, 65536 + 300
+    lengths, ids = [M - 300, 300], [0, 1]
+    x, w, bias, a, b, scale, row = on_gpu(*problem(lengths, ids, K, N, r, BF))
+    y = o.linear_adapters(x, w, bias, o.AdapterBank(a, b, scale), o.AdapterPlan(lengths, ids, DEV))
+    for sl in (slice(0, 300), slice(M // 2, M // 2 + 300), slice(M - 600, M)):
+        check(y[sl], *oracle(x[sl], w, bias, a, b, scale, row[sl]))
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("wants", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)])
+@pytest.mark.parametrize("N", [64, 68])
+def test_some_of_the_gradients(wants, dt, N):
+    """Any of x, A, B may not be trained, bias may be missing, dy may be an expanded scalar or a column range."""
+    from more4d_amd.autograd import AdapterLinearFn
+    o = ops()
+    lengths, ids = [70, 2, 40], [1, -1, 0]
+    x, w, _, a, b, scale, _ = on_gpu(*problem(lengths, ids, 72, N, 6, dt))
+    plan = o.AdapterPlan(lengths, ids, DEV)
+    wide = torch.randn(112, 3 * N, device=DEV).to(dt)
+    for bits in (8, 16):
+        for dy in (wide[:, N:2 * N], torch.ones(1, device=DEV, dtype=dt).expand(112, N)):
+            t = [v.clone().requires_grad_(True) for v in (x, a, b)]
+            full = torch.autograd.grad(AdapterLinearFn.apply(t[0], w, None, t[1], t[2], scale, plan, bits), t, dy.contiguous())
+            t = [v.clone().requires_grad_(bool(k)) for v, k in zip((x, a, b), wants)]
+            some = torch.autograd.grad(AdapterLinearFn.apply(t[0], w, None, t[1], t[2], scale, plan, bits), [v for v in t if v.requires_grad], dy)
+            for p, q in zip(some, [f for f, k in zip(full, wants) if k]):
+                assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_nobody_names_an_adapter(dt):
+    from more4d_amd.autograd import AdapterLinearFn
+    o = ops()
+    x, w, bias, a, b, scale, row = on_gpu(*problem([90], [-1], 64, 68, 6, dt))
+    plan = o.AdapterPlan([90], [-1], DEV)
+    t = [v.requires_grad_(True) for v in (x, a, b)]
+    y = AdapterLinearFn.apply(*t[:1], w, bias, *t[1:], scale, plan, 8)
+    dy = torch.randn(90, 68, device=DEV).to(dt)
+    dx, da, db = torch.autograd.grad(y, t, dy)
+    check(y.detach(), *oracle(x.detach(), w, bias, a.detach(), b.detach(), scale, row))
+    check(dx, *oracle(dy, w.t(), None, b.detach().transpose(1, 2), a.detach().transpose(1, 2), scale, row))
+    assert not da.any() and not db.any()
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("M", [9, 333])
+def test_the_largest_rank(dt, M):
+    from more4d_amd.autograd import AdapterLinearFn
+    o = ops()
+    lengths, ids = [M - 3, 3], [1, 0]
+    x, w, bias, a, b, scale, row = on_gpu(*problem(lengths, ids, 520, 264, 512, dt))
+    plan = o.AdapterPlan(lengths, ids, DEV)
+    t = [v.requires_grad_(True) for v in (x, a, b)]
+    y = AdapterLinearFn.apply(*t[:1], w, bias, *t[1:], scale, plan, 16)
+    dy = torch.randn(M, 264, device=DEV).to(dt)
+    dx, da, db = (g.double() for g in torch.autograd.grad(y, t, dy))
+    x, a, b = (v.detach() for v in t)
+    check(y.detach(), *oracle(x, w, bias, a, b, scale, row))
+    check(dx, *oracle(dy, w.t(), None, b.transpose(1, 2), a.transpose(1, 2), scale, row))
+    h = torch.finfo(dt).eps / 2
+    for g in range(2):
+        m = row == g
+        v, u = scale[g] * dy[m].double() @ b[g].double(), scale[g] * x[m].double() @ a[g].double().t()
+        va, ua = scale[g] * dy[m].double().abs() @ b[g].double().abs(), scale[g] * x[m].double().abs() @ a[g].double().abs().t()
+        for got, p, q, s, n in ((da[g], v, x[m].double(), va, 264), (db[g].t(), u, dy[m].double(), ua, 520)):
+            want = p.t() @ q
+            check(got, want, 1.02 * h * (want.abs() + h * p.abs().t() @ q.abs()) + (M + n) * 2.0 ** -23 * (s.t() @ q.abs()))
+
+
+def test_a_captured_training_step():
+    """Forward and backward of two layers in one graph, replayed with other inputs and eager steps of the same leaves between."""
+    from more4d_amd.autograd import AdapterLinearFn
+    o = ops()
+    lengths, ids = [200, 1, 99], [1, -1, 0]
+    x, w1, _, a1, b1, scale, _ = on_gpu(*problem(lengths, ids, 128, 256, 8, BF))
+    _, w2, _, a2, b2, _, _ = on_gpu(*problem(lengths, ids, 256, 128, 8, BF, seed=1))
+    plan, s = o.AdapterPlan(lengths, ids, DEV), torch.tensor(scale, device=DEV)
+    leaves = [v.requires_grad_(True) for v in (a1, b1, a2, b2)]
+
+    def step(xx, dy):
+        xx = xx.detach().requires_grad_(True)
+        y = AdapterLinearFn.apply(AdapterLinearFn.apply(xx, w1, None, a1, b1, s, plan, 8), w2, None, a2, b2, s, plan, 16)
+        return torch.autograd.grad(y, [xx] + leaves, dy)
+
+    gen = torch.Generator().manual_seed(1)
+    data = [(torch.randn(300, 128, generator=gen).to(BF).to(DEV), torch.randn(300, 128, generator=gen).to(BF).to(DEV)) for _ in range(3)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*data[0])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    xs, ds = (torch.zeros_like(v) for v in data[0])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(xs, ds)
+    for i in range(5):
+        xs.copy_(data[i % 3][0])
+        ds.copy_(data[i % 3][1])
+        g.replay()
+        eager = step(*data[i % 3])
+        torch.cuda.synchronize()
+        for p, q in zip(out, eager):
+            assert torch.equal(p, q)
+
+
+def test_two_streams_at_once():
+    """Calls that share plan and bank, on two streams without waiting for each other."""
+    o = ops()
+    lengths, ids = [700, 1, 300], [1, -1, 0]
+    x, w, bias, a, b, scale, _ = on_gpu(*problem(lengths, ids, 512, 512, 16, BF))
+    plan, bank = o.AdapterPlan(lengths, ids, DEV), o.AdapterBank(a, b, scale, backward=True)
+    xs = [x, x.flip(0).contiguous()]
+
+    def run(v):
+        y, ut, x8 = o.linear_adapters(v, w, bias, bank, plan, keep8=True)
+        return (y,) + o.linear_adapters_bwd(y, w, bank, plan, x=x8, ut=ut)
+
+    want = [run(v) for v in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(run(xs[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for r in got[k]:
+            for p, q in zip(r, want[k]):
+                assert torch.equal(p, q)
