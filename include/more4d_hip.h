@@ -515,6 +515,8 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
  * backward's down projection, b_up T [G, N, R] and a_up T [G, K, R], zero beyond the rank (b_down and a_up: backward only, may be NULL).
  * The plan describes the rows of a batch, host-built (more4d_amd/ops.py: AdapterPlan), tables on the device:
  *   row_adapter [rows]           adapter of each row, -1 = none
+ *   row_order [rows] or NULL     the rows in order of their adapters, for batches that interleave them (a tile adds the adapters of all its
+ *                                rows): tiles[0..2] are then of rows in this order
  *   slot_row [64 * n_pieces]     rows sorted by adapter, each adapter's list padded with -1 to pieces of 64
  *   piece_adapter [n_pieces]
  *   chunks[l] [n_chunks[l]][3]   pieces [first, last), at most 64, of one adapter: the unit of the row contraction, at four granularities from
@@ -533,9 +535,9 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
  *   linear_adapters_bwd  the backward of linear_adapters with W [N, K] frozen, in one call: dx T [rows, K] = dy W + v A (NULL: not wanted), da (needs
  *                    x or its codes), db (needs the forward's ut); N a multiple of 8 (bf16) or 4; ws: linear_adapters_bwd_workspace floats. */
 typedef struct {
-    const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks[4], *chunk_off[4], *tiles_off[4], *tiles[4], *tile_one;
+    const int32_t *row_adapter, *slot_row, *piece_adapter, *chunks[4], *chunk_off[4], *tiles_off[4], *tiles[4], *tile_one, *row_order;
     int64_t rows;
-    int32_t n_pieces, n_adapters, n_chunks[4], n_listed;      /* n_listed: entries of tiles[0] */
+    int32_t n_pieces, n_adapters, n_chunks[4], n_listed, n_wide;      /* n_listed, n_wide: entries of tiles[0], tiles[3] */
 } m4d_adapter_plan;
 int64_t m4d_adapter_down_elems(int G, int R, int64_t K);
 int m4d_adapter_pack(m4d_dtype dt, const void* a, const void* b, int G, int rank, int64_t K, int64_t N, int R, void* a_down, void* b_up, void* b_down,

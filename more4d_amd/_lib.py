@@ -33,8 +33,8 @@ class AttnBwdArgs(Structure):
 
 class AdapterPlanArgs(Structure):      # m4d_adapter_plan
     _fields_ = [("row_adapter", c_void_p), ("slot_row", c_void_p), ("piece_adapter", c_void_p), ("chunks", c_void_p * 4),
-                ("chunk_off", c_void_p * 4), ("tiles_off", c_void_p * 4), ("tiles", c_void_p * 4), ("tile_one", c_void_p), ("rows", c_int64), ("n_pieces", c_int32),
-                ("n_adapters", c_int32), ("n_chunks", c_int32 * 4), ("n_listed", c_int32)]
+                ("chunk_off", c_void_p * 4), ("tiles_off", c_void_p * 4), ("tiles", c_void_p * 4), ("tile_one", c_void_p), ("row_order", c_void_p),
+                ("rows", c_int64), ("n_pieces", c_int32), ("n_adapters", c_int32), ("n_chunks", c_int32 * 4), ("n_listed", c_int32), ("n_wide", c_int32)]
 
 
 # name -> (restype, argtypes); mirrors include/more4d_hip.h one to one

@@ -546,7 +546,7 @@ struct Choice { int kind, S; };
 // 0.55 / 2.1, 256 x 128 0.92 / 4.0, 256 x 256 (gemm_wide.h) 1.03.  Measured against each other at 40 shapes (M 2 .. 21840): the choice is within
 // 10 % of the best of all kinds and slices, e.g. 64 x 5120 x 4096: 64 x 64 in 3 slices 14.3 us, whole 21.7, 128 x 128 whole 36; 986 x 5120 x
 // 4096: 256 x 128 65 us, 128 x 128 75, 256 x 256 72.
-Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, int ncu) {
+Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, double wide_ad, int ncu) {
 #ifdef M4D_ABLATIONS
     { const char* v = getenv("M4D_ADAPTER_GEMM"); if (v) { const int c = atoi(v); if (c / 100 != WIDE_256x256 || wide_ok) return Choice{c / 100, c % 100 ? c % 100 : 1}; } }
 #endif
@@ -558,7 +558,7 @@ Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, int ncu)
     if (M <= 16) offer(4.0 + wbytes * (1.0 + M / 24.0) / 6.0e6, GEMV16, 1);
     if (wide_ok) {
         const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
-        offer((double)((tiles + ncu - 1) / ncu) * (nk * 1.03 + 10.0), WIDE_256x256, 1);
+        offer((double)((tiles + ncu - 1) / ncu) * (nk * 1.03 + 10.0 + wide_ad), WIDE_256x256, 1);
     }
     static const struct { int kind, bm, bn, occ; double c[2][2], fix; } cfg[4] = {
         {TILE_64x64, 64, 64, 2, {{0.30, 0.42}, {0.70, 1.25}}, 4.0}, {TILE_64x128, 64, 128, 1, {{0.36, 0.36}, {1.16, 1.16}}, 4.0},
@@ -719,6 +719,9 @@ static int launch_gemm(AdGemmArgs& p, hipStream_t st) {
 }
 
 static bool wide_shape(m4d_dtype dt, int64_t M, int64_t N, int64_t K) { return dt == M4D_BF16 && K % 64 == 0 && M >= 512 && N >= 512; }
+// what the adapters of a 256 x 256 tile add to its time, us (its direct loads take 32 consecutive rows each: it does not see row_order).  Measured
+// per adapter: rank 16 0.8, rank 64 3.8.  The other tiles take interleaved rows in order and have one or two adapters each.
+static double wide_adapters_us(const m4d_adapter_plan* plan, int R) { return plan->row_order ? 0.06 * R * plan->n_wide / (double)((plan->rows + 255) / 256) : 0.0; }
 
 // the down projection's slices and the GEMM's run one after the other: one workspace, the larger of the two
 extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R, int slots) {
@@ -726,7 +729,7 @@ extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter
     const int64_t M = plan->rows;
     int64_t most = m4d_adapter_down_workspace(plan, K, R, slots);      // (whether the wide kernel can run depends on the output's alignment too: room for either choice)
     for (int w = 0; w < 2; ++w) {
-        const Choice c = choose(dt == M4D_BF16, M, N, K, w && wide_shape(dt, M, N, K), cus());
+        const Choice c = choose(dt == M4D_BF16, M, N, K, w && wide_shape(dt, M, N, K), wide_adapters_us(plan, R), cus());
         if (c.S > 1 && c.S * M * N > most) most = c.S * M * N;
     }
     return most;
@@ -749,7 +752,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
                   "linear_adapters: bad plan");
     const bool bf16 = dt == M4D_BF16;
     const bool wide_ok = wide_shape(dt, M, N, K) && ldo % 8 == 0 && ((uintptr_t)out % 32) == 0;
-    const Choice c = choose(bf16, M, N, K, wide_ok, cus());
+    const Choice c = choose(bf16, M, N, K, wide_ok, wide_adapters_us(plan, R), cus());
     M4D_CHECK_ARG(c.S == 1 || (ws && ws_floats >= c.S * M * N && ((uintptr_t)ws % 16) == 0), "linear_adapters: workspace of %lld floats needed", (long long)(c.S * M * N));
     if (a_down) {
         const int rc = m4d_adapter_down(dt, x, ldx, a_down, scale, plan, u, ut, codes, exps, K, R, ws, ws_floats, stream);
@@ -758,7 +761,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
     AdGemmArgs p{};
     p.A = x; p.W = W; p.bias = bias; p.out = out; p.lda = ldx; p.ldw = ldw; p.ldc = ldo; p.M = M; p.N = N; p.K = K;
     p.rows_per_sample = M; p.epilogue = M4D_EPI_STORE;
-    p.u = u; p.up = b_up; p.row_adapter = plan->row_adapter; p.R = R; p.S = c.S; p.ws = ws;
+    p.u = u; p.up = b_up; p.row_adapter = plan->row_adapter; p.order = plan->row_order; p.R = R; p.S = c.S; p.ws = ws;
     const int tl = c.kind == GEMV16 || c.kind == TILE_64x64 || c.kind == TILE_64x128 ? 0 : c.kind == TILE_128x128 ? 1 : 2;      // tile heights 64, 128, 256
     p.tile_off = plan->tiles_off[tl]; p.tile_list = plan->tiles[tl];
     hipStream_t st = (hipStream_t)stream;

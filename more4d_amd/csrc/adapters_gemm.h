@@ -16,6 +16,7 @@ namespace {
 
 struct AdGemmArgs : GemmAdArgs {
     int S;             // K slices; > 1: float32 partial sums to ws [S, M, N]
+    const int* order;  // [M] the row of x, u and out behind each row of the tiles, or nullptr: the same
 };
 
 __device__ __attribute__((aligned(16))) const unsigned zero_page[4] = {0u, 0u, 0u, 0u};
@@ -57,7 +58,8 @@ __global__ __launch_bounds__(64 * WM * WN) void adapter_gemm_kernel(AdGemmArgs p
         const int j = wave + NW * i, r = j * 8 + (lane >> 3);
         const bool isx = j * 8 < BM;
         const int rr = isx ? r : r - BM;
-        const int64_t row = isx ? min(m0 + rr, p.M - 1) : min(n0 + rr, p.N - 1);
+        int64_t row = isx ? min(m0 + rr, p.M - 1) : min(n0 + rr, p.N - 1);
+        if (isx && p.order) row = p.order[row];
         lc16[i] = (((lane & 7) ^ ((rr >> 1) & 7)) << 4);
         src[i] = (isx ? (const char*)p.A + row * p.lda * ES : (const char*)p.W + row * p.ldw * ES) + lc16[i];
     }
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(64 * WM * WN) void adapter_gemm_kernel(AdGemmArgs p
             }
         }
     };
-    const AdTile<MI> ad_tile = adapters_tile<MI>(p, tm, m0 + wm * MI * 32, lane, (int)blockIdx.y);      // (a slice takes every S-th adapter)
+    const AdTile<MI> ad_tile = adapters_tile<MI>(p, tm, m0 + wm * MI * 32, lane, (int)blockIdx.y, p.order);      // (a slice takes every S-th adapter)
     const int n_tiles = kt1 - kt0;
     if (n_tiles > 0) {
 #pragma unroll
@@ -156,7 +158,7 @@ __global__ __launch_bounds__(64 * WM * WN) void adapter_gemm_kernel(AdGemmArgs p
         for (; kt < kt1 - 1; ++kt) tile(kt, std::false_type{}, std::true_type{}, kt1 - 2 - kt);
         tile(kt, std::false_type{}, std::false_type{}, 0);
     }
-    adapters_extend<T, NI, MI>(p, acc, ad_tile, m0 + wm * MI * 32, n0 + wn * NI * 32, lane, p.S);
+    adapters_extend<T, NI, MI>(p, acc, ad_tile, n0 + wn * NI * 32, lane, p.S);
 
     // out of the accumulator layout (lane = row) through LDS: 4 consecutive columns per lane, whole rows per group of lanes
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(64 * WM * WN) void adapter_gemm_kernel(AdGemmArgs p
             const int64_t m = m0 + (wm * MI + mi) * 32 + r;
             if (m < p.M && n < p.N) {
                 if (part) store4(part + m * p.N + n, v);
-                else store4((T*)p.out + m * p.ldc + n, v + bv);
+                else store4((T*)p.out + (p.order ? p.order[m] : m) * p.ldc + n, v + bv);
             }
         }
     }
@@ -201,7 +203,7 @@ __global__ __launch_bounds__(256) void adapter_gemm_join_kernel(AdGemmArgs p) {
         f32x4 v = load4(p.ws + m * p.N + n);
         for (int s = 1; s < p.S; ++s) v += load4(p.ws + ((int64_t)s * p.M + m) * p.N + n);
         if (p.bias) v += load4((const T*)p.bias + n);
-        store4((T*)p.out + m * p.ldc + n, v);
+        store4((T*)p.out + (p.order ? p.order[m] : m) * p.ldc + n, v);
     }
 }
 

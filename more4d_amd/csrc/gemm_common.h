@@ -160,9 +160,10 @@ M4D_DEV void epilogue_tile(const GemmArgs& p, const f32x16& acc, int64_t m, int6
 // only the adapter's rows add, bf16 bad_parts (a VALU instruction on its accumulators takes them out of the AGPRs: 200 spilled registers in the
 // 256 x 256 kernel).
 // AdTile: what the extension has to know about its tile, loaded in front of the K loop (behind it these would be three dependent trips to L2).
-template <int MI> struct AdTile { int i0, i1, g0; int ra[MI]; };
+// order (or nullptr): the row behind each row of the tiles.
+template <int MI> struct AdTile { int i0, i1, g0; int ra[MI], row[MI]; };
 template <int MI>
-M4D_DEV AdTile<MI> adapters_tile(const GemmAdArgs& p, int tile, int64_t m_base, int lane, int first = 0) {
+M4D_DEV AdTile<MI> adapters_tile(const GemmAdArgs& p, int tile, int64_t m_base, int lane, int first = 0, const int* order = nullptr) {
     AdTile<MI> a;
     a.i0 = __builtin_amdgcn_readfirstlane(p.tile_off[tile]) + first;
     a.i1 = __builtin_amdgcn_readfirstlane(p.tile_off[tile + 1]);
@@ -170,7 +171,8 @@ M4D_DEV AdTile<MI> adapters_tile(const GemmAdArgs& p, int tile, int64_t m_base, 
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
         const int64_t m = m_base + mi * 32 + (lane & 31);
-        a.ra[mi] = m < p.M ? p.row_adapter[m] : -1;
+        a.row[mi] = m >= p.M ? 0 : order ? order[m] : (int)m;
+        a.ra[mi] = m < p.M ? p.row_adapter[a.row[mi]] : -1;
     }
     return a;
 }
@@ -214,18 +216,14 @@ M4D_DEV bf16x8 big_signs(const bf16x8& u) {
     return r;
 }
 template <typename T, int NI, int MI>
-M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const AdTile<MI>& a, int64_t m_base, int64_t n_base, int lane, int step = 1,
-                             int k0 = 0) {      // k0: ranks in front of it are already in
+M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const AdTile<MI>& a, int64_t n_base, int lane, int step = 1, int k0 = 0) {      // k0: ranks in front of it are already in
     typedef typename Frag8<T>::type frag_t;
     constexpr int U = sizeof(T) != 2 ? 1 : NI * MI < 16 ? 4 : 2;      // 16-rank steps in flight, as registers allow (float32 is MFMA-bound)
     const int li = lane & 31, hi = lane >> 5;
     if (a.i0 >= a.i1 || k0 >= p.R) return;
     const T* pu[MI];
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-        const int64_t m = m_base + mi * 32 + li;
-        pu[mi] = (const T*)p.u + (m < p.M ? m : 0) * p.R + hi * 8;
-    }
+    for (int mi = 0; mi < MI; ++mi) pu[mi] = (const T*)p.u + (int64_t)a.row[mi] * p.R + hi * 8;
     int64_t nr[NI];                                   // (columns beyond N are computed from row N - 1 and not stored)
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) nr[ni] = min(n_base + ni * 32 + li, p.N - 1) * p.R + hi * 8;

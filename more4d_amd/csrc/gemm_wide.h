@@ -603,7 +603,7 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
             for (int h = 0; h < 2; ++h) asm volatile("" :: "v"(fa0[h][kk]), "v"(fa1[h][kk]), "v"(fbx[h][kk]), "v"(fby[h][kk]));
-        adapters_extend<T, 4, 4>(p, acc, ad_tile, m0 + wm * 128, n0 + wn * 128, lane, 1, (nkt - nk) * 64);      // (its loads fly with the last stagings)
+        adapters_extend<T, 4, 4>(p, acc, ad_tile, n0 + wn * 128, lane, 1, (nkt - nk) * 64);      // (its loads fly with the last stagings)
     }
     if constexpr (ABL & 64) ts[2] = __builtin_readcyclecounter();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the redundant tail stagings must land before the LDS is re-used

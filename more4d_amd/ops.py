@@ -1249,9 +1249,10 @@ class AdapterBank:
 class AdapterPlan:
     """Which adapter each row of a batch uses: request j owns the next lengths[j] rows (0 allowed) and names adapter adapters[j] (-1: none).
     Host numbers; the tables (include/more4d_hip.h: m4d_adapter_plan) are built here and copied to `device` once per batch composition, then
-    shared by every projection of the model (not inside a graph capture).  Any order of the requests is right; requests of one adapter side
-    by side are fastest, because a tile of the projection adds the adapters of all its rows: 1024 one-row requests of 64 adapters, rank 16 / 64,
-    5120 x 5120: 88 / 100 us in order of adapters, 120 / 346 us interleaved."""
+    shared by every projection of the model (not inside a graph capture).  Any order of the requests is right, requests of one adapter side
+    by side are a little faster: a tile of the projection adds the adapters of all its rows, so where requests interleave them (twice the
+    (tile, adapter) pairs or more) the smaller tiles take the rows in order of their adapters (row_order).  1024 one-row requests of 64 adapters,
+    rank 16 / 64, 5120 x 5120: 95 / 108 us, 90 / 103 sorted by the caller (120 / 346 without row_order)."""
     PIECE, CHUNK_PIECES, MAX_ADAPTERS = 64, 64, 65535
 
     def __init__(self, lengths, adapters, device):
@@ -1274,8 +1275,11 @@ class AdapterPlan:
         start = end - size
         self.n_adapters = int(ids.max()) + 1 if len(ids) else 0
         slots, pieces, count = [], [], [0] * self.n_adapters
-        for g in np.unique(ids[ids >= 0]).tolist():
-            s_, n_ = start[ids == g], size[ids == g]
+        by_id = np.argsort(ids, kind="stable")
+        for run in np.split(by_id, np.flatnonzero(np.diff(ids[by_id])) + 1):
+            if not len(run) or ids[run[0]] < 0:
+                continue
+            g, s_, n_ = int(ids[run[0]]), start[run], size[run]
             before = np.cumsum(n_) - n_
             n = count[g] = int(n_.sum())
             slots += [np.repeat(s_ - before, n_) + np.arange(n), np.full(-n % P, -1)]
@@ -1293,8 +1297,9 @@ class AdapterPlan:
                 off.append(len(lst) // 3)
             return lst, off
 
-        def tiles(T, shifted=False):            # (tile, adapter) pairs, each once, in order; the adapter of whole tiles
+        def tiles(ids, size, end, T, shifted=False):   # (tile, adapter) pairs of runs of rows, each once, in order; the adapter of whole tiles
             nt = -(-self.rows // T)
+            start = end - size
             t0 = start // T
             n_ = (end - 1) // T - t0 + 1
             tile, who = np.repeat(t0 - (np.cumsum(n_) - n_), n_) + np.arange(int(n_.sum())), np.repeat(ids, n_)
@@ -1307,10 +1312,18 @@ class AdapterPlan:
             one = np.where(distinct == 1, who[np.cumsum(distinct) - distinct], -1) if nt else who
             return who[who >= 0], np.concatenate([[0], np.cumsum(np.bincount(tile[who >= 0], minlength=nt))]), one
 
+        row_adapter, runs, order = np.repeat(ids, size), (ids, size, end), []
+        small = [tiles(*runs, T) for T in (64, 128, 256)]
+        if self.n_pieces and len(ids) > 1:      # requests that interleave adapters: tiles of rows in order of their adapters
+            total = np.bincount(row_adapter + 1, minlength=self.n_adapters + 1)
+            who = np.flatnonzero(total)
+            by_adapter = (who - 1, total[who], np.cumsum(total[who]))
+            if len(small[0][0]) >= 2 * len(tiles(*by_adapter, 64)[0]):
+                order, small = np.argsort(row_adapter, kind="stable"), [tiles(*by_adapter, T) for T in (64, 128, 256)]
         cs = [chunks(t) for t in (12, 24, 48, 96)]
-        ts = [tiles(64), tiles(128), tiles(256), tiles(256, True)]
-        parts = [np.repeat(ids, size), np.concatenate(slots) if slots else [], pieces]
-        parts += [c[0] for c in cs] + [c[1] for c in cs] + [t[1] for t in ts] + [t[0] for t in ts] + [ts[3][2]]      # (tile_one)
+        ts = small + [tiles(*runs, 256, True)]
+        parts = [row_adapter, np.concatenate(slots) if slots else [], pieces]
+        parts += [c[0] for c in cs] + [c[1] for c in cs] + [t[1] for t in ts] + [t[0] for t in ts] + [ts[3][2], order]      # (tile_one, row_order)
         parts = [np.asarray(v, dtype=np.int32) for v in parts]
         at, offs = 0, []
         for v in parts:
@@ -1325,10 +1338,10 @@ class AdapterPlan:
         a.row_adapter, a.slot_row, a.piece_adapter = ptr[:3]
         for k, name in enumerate(("chunks", "chunk_off", "tiles_off", "tiles")):
             getattr(a, name)[:] = ptr[3 + 4 * k:7 + 4 * k]
-        a.tile_one = ptr[19]
+        a.tile_one, a.row_order = ptr[19], ptr[20] if len(order) else None
         a.rows, a.n_pieces, a.n_adapters = self.rows, self.n_pieces, self.n_adapters
         a.n_chunks[:] = [len(c[0]) // 3 for c in cs]
-        a.n_listed = len(ts[0][0])
+        a.n_listed, a.n_wide = len(ts[0][0]), len(ts[3][0])
         self.sizes = {}                         # workspace sizes by shape (_workspace)
 
 

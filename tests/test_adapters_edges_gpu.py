@@ -268,3 +268,30 @@ def test_two_streams_at_once():
         for r in got[k]:
             for p, q in zip(r, want[k]):
                 assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dt,M,N,K,r", [(BF, 200, 260, 1000, 16), (BF, 700, 1540, 200, 40), (BF, 1500, 2052, 256, 64), (F32, 300, 516, 260, 20), (F32, 1200, 1028, 64, 8)])
+def test_interleaved_requests(dt, M, N, K, r):
+    """One-row requests of 24 adapters, some of none: tiles of rows in order of their adapters, K slices among them; rows of a wider tensor."""
+    from more4d_amd.autograd import AdapterLinearFn
+    o = ops()
+    ids = [(i * 7) % 25 - 1 for i in range(M)]
+    x, w, bias, a, b, scale, row = on_gpu(*problem([1] * M, ids, K, N, r, dt))
+    plan, bank = o.AdapterPlan([1] * M, ids, DEV), o.AdapterBank(a, b, scale)
+    assert plan.args.row_order
+    out = torch.full((M, N + 8), float("nan"), device=DEV, dtype=dt)
+    y = o.linear_adapters(x, w, bias, bank, plan, out=out[:, :N])
+    check(y, *oracle(x, w, bias, a, b, scale, row))
+    assert torch.isnan(out[:, N:]).all()
+    t = [v.requires_grad_(True) for v in (x, a, b)]
+    y = AdapterLinearFn.apply(t[0], w, None, t[1], t[2], scale, plan, 16)
+    dy = torch.randn(M, N, device=DEV).to(dt)
+    dx, da, db = torch.autograd.grad(y, t, dy)
+    x, a, b = (v.detach() for v in t)
+    check(dx, *oracle(dy, w.t(), None, b.transpose(1, 2), a.transpose(1, 2), scale, row))
+    by = sorted(range(M), key=lambda i: (ids[i], i))
+    srt = o.AdapterPlan([1] * M, [ids[i] for i in by], DEV)
+    t = [v.clone().requires_grad_(True) for v in (x[by], a, b)]
+    ys = AdapterLinearFn.apply(t[0], w, None, t[1], t[2], scale, srt, 16)
+    _, da2, db2 = torch.autograd.grad(ys, t, dy[by])
+    assert torch.equal(da, da2) and torch.equal(db, db2)              # the same slots, so the same sums

@@ -46,17 +46,29 @@ def test_plan_tables_cover_every_row_once(seed):
                 covered += range(ch[3 * c], ch[3 * c + 1])
                 assert all(pieces[q] == g for q in range(ch[3 * c], ch[3 * c + 1]))
         assert covered == list(range(p.n_pieces))
+    order = at(a.row_order, len(rows)) if a.row_order else list(range(len(rows)))
+    assert sorted(order) == list(range(len(rows))) and (not a.row_order or [rows[r] for r in order] == sorted(rows))
+    in_order = [rows[r] for r in order]
     for k, T in enumerate((64, 128, 256, 256)):
+        of_tiles = rows if k == 3 else in_order
         nt = -(-p.rows // T)
         off = at(a.tiles_off[k], nt + 1)
         lst = at(a.tiles[k], off[-1])
         for i in range(nt):
             lo = max(0, min(i * T, p.rows - T)) if k == 3 else i * T
-            assert lst[off[i]:off[i + 1]] == sorted({g for g in rows[lo:i * T + T] if g >= 0})
+            assert lst[off[i]:off[i + 1]] == sorted({g for g in of_tiles[lo:i * T + T] if g >= 0})
             if k == 3:
                 here = set(rows[lo:i * T + T])
                 assert at(a.tile_one, nt)[i] == (here.pop() if len(here) == 1 else -1)
-    assert a.n_listed == at(a.tiles_off[0], -(-p.rows // 64) + 1)[-1]
+    assert a.n_listed == at(a.tiles_off[0], -(-p.rows // 64) + 1)[-1] and a.n_wide == at(a.tiles_off[3], -(-p.rows // 256) + 1)[-1]
+
+
+def test_interleaved_requests_are_tiled_in_order_of_their_adapters():
+    p = ops.AdapterPlan([1] * 256, [i % 8 for i in range(256)], "cpu")
+    at, a = tables(p)
+    assert at(a.row_order, 256) == sorted(range(256), key=lambda r: r % 8) and a.n_listed == 8 and a.n_wide == 8
+    assert ops.AdapterPlan([32] * 8, list(range(8)), "cpu").args.row_order is None
+    assert ops.AdapterPlan([1] * 64, [i % 8 for i in range(64)], "cpu").args.row_order is None       # one tile either way
 
 
 def test_plan_of_nothing():
