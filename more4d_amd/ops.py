@@ -1314,7 +1314,8 @@ class AdapterPlan:
 
         row_adapter, runs, order = np.repeat(ids, size), (ids, size, end), []
         small = [tiles(*runs, T) for T in (64, 128, 256)]
-        if self.n_pieces and len(ids) > 1:      # requests that interleave adapters: tiles of rows in order of their adapters
+        fewest = max(-(-int(size[ids >= 0].sum()) // 64), sum(1 for n in count if n))
+        if self.n_pieces and len(small[0][0]) >= 2 * fewest:      # requests that interleave adapters: tiles of rows in order of their adapters
             total = np.bincount(row_adapter + 1, minlength=self.n_adapters + 1)
             who = np.flatnonzero(total)
             by_adapter = (who - 1, total[who], np.cumsum(total[who]))
