@@ -537,8 +537,9 @@ int cus() {
 }
 
 enum { GEMV16 = 0, TILE_64x64, TILE_64x128, TILE_128x128, TILE_256x128, WIDE_256x256 };
-struct Choice { int kind, S; };
+struct Choice { int kind, S; int64_t head; };      // head rows on the 256 x 256 kernel, the others on `kind` in S slices of K
 
+double wide_round_us(int64_t K, double wide_ad) { return (double)(K / 64) * 1.03 + 10.0 + wide_ad; }
 // Which kernel, and into how many slices of K: the least estimated time.  A CU runs its workgroups in rounds; a round costs a fixed part (filling
 // the ring, epilogue) and c per 128-byte K tile.  c is what the tile moves from L2 at the 60 - 80 bytes/ns that a CU gets (fp32: the MFMA
 // rate), so larger tiles are cheaper per product and smaller ones waste less of a round; slices pay for writing and joining float32 partial
@@ -546,19 +547,19 @@ struct Choice { int kind, S; };
 // 0.55 / 2.1, 256 x 128 0.92 / 4.0, 256 x 256 (gemm_wide.h) 1.03.  Measured against each other at 40 shapes (M 2 .. 21840): the choice is within
 // 10 % of the best of all kinds and slices, e.g. 64 x 5120 x 4096: 64 x 64 in 3 slices 14.3 us, whole 21.7, 128 x 128 whole 36; 986 x 5120 x
 // 4096: 256 x 128 65 us, 128 x 128 75, 256 x 256 72.
-Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, double wide_ad, int ncu) {
+Choice choose_whole(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, double wide_ad, int ncu, double& t_best) {
+    t_best = 1e30;
 #ifdef M4D_ABLATIONS
-    { const char* v = getenv("M4D_ADAPTER_GEMM"); if (v) { const int c = atoi(v); if (c / 100 != WIDE_256x256 || wide_ok) return Choice{c / 100, c % 100 ? c % 100 : 1}; } }
+    { const char* v = getenv("M4D_ADAPTER_GEMM"); if (v) { const int c = atoi(v); if (c / 100 != WIDE_256x256 || wide_ok) return Choice{c / 100, c % 100 ? c % 100 : 1, 0}; } }
 #endif
     const double es = bf16 ? 2 : 4, wbytes = (double)N * K * es;
     const int64_t nk = (int64_t)((K * es + ROWB - 1) / ROWB);
-    Choice best{TILE_64x64, 1};
-    double t_best = 1e30;
-    auto offer = [&](double t, int kind, int S) { if (t < t_best) { t_best = t; best = Choice{kind, S}; } };
+    Choice best{TILE_64x64, 1, 0};
+    auto offer = [&](double t, int kind, int S) { if (t < t_best) { t_best = t; best = Choice{kind, S, 0}; } };
     if (M <= 16) offer(4.0 + wbytes * (1.0 + M / 24.0) / 6.0e6, GEMV16, 1);
     if (wide_ok) {
         const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
-        offer((double)((tiles + ncu - 1) / ncu) * (nk * 1.03 + 10.0 + wide_ad), WIDE_256x256, 1);
+        offer((double)((tiles + ncu - 1) / ncu) * wide_round_us(K, wide_ad), WIDE_256x256, 1);
     }
     static const struct { int kind, bm, bn, occ; double c[2][2], fix; } cfg[4] = {
         {TILE_64x64, 64, 64, 2, {{0.30, 0.42}, {0.70, 1.25}}, 4.0}, {TILE_64x128, 64, 128, 1, {{0.36, 0.36}, {1.16, 1.16}}, 4.0},
@@ -576,6 +577,20 @@ Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, double w
             if (S > 1) t += 4.5 + (double)M * N * (8.0 * S + es) / 4.5e6;
             offer(t, f.kind, S);
         }
+    }
+    return best;
+}
+// The 256 x 256 kernel's last round may leave most CUs idle (11776 x 1536 x 8960: 276 tiles on 256 CUs).  Whole rounds of it for the rows in
+// front and the remaining rows on whatever is fastest for them, 8 us for one more launch: 11776 x 1536 x 8960 392 us -> 338, 21840 x 1536 x 1536
+// 130 -> 112, 3584 x 5120 x 5120 217 -> 184; 4400 x 4100 x 1024 70 -> 72, and nothing (under 2 % by the estimate) at many rounds.
+Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, bool split_ok, double wide_ad, int ncu) {
+    double t;
+    Choice best = choose_whole(bf16, M, N, K, wide_ok, wide_ad, ncu, t);
+    const int64_t tn = (N + 255) / 256, rounds = ((M + 255) / 256) * tn / ncu, head = rounds * ncu / tn * 256;
+    if (best.kind == WIDE_256x256 && split_ok && head > 0 && head < M) {
+        double t2;
+        Choice rest = choose_whole(bf16, M - head, N, K, false, wide_ad, ncu, t2);
+        if (rounds * wide_round_us(K, wide_ad) + t2 + 8.0 < 0.98 * t) { best = rest; best.head = head; }
     }
     return best;
 }
@@ -729,8 +744,8 @@ extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter
     const int64_t M = plan->rows;
     int64_t most = m4d_adapter_down_workspace(plan, K, R, slots);      // (whether the wide kernel can run depends on the output's alignment too: room for either choice)
     for (int w = 0; w < 2; ++w) {
-        const Choice c = choose(dt == M4D_BF16, M, N, K, w && wide_shape(dt, M, N, K), wide_adapters_us(plan, R), cus());
-        if (c.S > 1 && c.S * M * N > most) most = c.S * M * N;
+        const Choice c = choose(dt == M4D_BF16, M, N, K, w && wide_shape(dt, M, N, K), !plan->row_order, wide_adapters_us(plan, R), cus());
+        if (c.S > 1 && c.S * (M - c.head) * N > most) most = c.S * (M - c.head) * N;
     }
     return most;
 }
@@ -752,8 +767,9 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
                   "linear_adapters: bad plan");
     const bool bf16 = dt == M4D_BF16;
     const bool wide_ok = wide_shape(dt, M, N, K) && ldo % 8 == 0 && ((uintptr_t)out % 32) == 0;
-    const Choice c = choose(bf16, M, N, K, wide_ok, wide_adapters_us(plan, R), cus());
-    M4D_CHECK_ARG(c.S == 1 || (ws && ws_floats >= c.S * M * N && ((uintptr_t)ws % 16) == 0), "linear_adapters: workspace of %lld floats needed", (long long)(c.S * M * N));
+    const Choice c = choose(bf16, M, N, K, wide_ok, !plan->row_order, wide_adapters_us(plan, R), cus());
+    M4D_CHECK_ARG(c.S == 1 || (ws && ws_floats >= c.S * (M - c.head) * N && ((uintptr_t)ws % 16) == 0), "linear_adapters: workspace of %lld floats needed",
+                  (long long)(c.S * (M - c.head) * N));
     if (a_down) {
         const int rc = m4d_adapter_down(dt, x, ldx, a_down, scale, plan, u, ut, codes, exps, K, R, ws, ws_floats, stream);
         if (rc != 0) return rc;
@@ -762,13 +778,31 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
     p.A = x; p.W = W; p.bias = bias; p.out = out; p.lda = ldx; p.ldw = ldw; p.ldc = ldo; p.M = M; p.N = N; p.K = K;
     p.rows_per_sample = M; p.epilogue = M4D_EPI_STORE;
     p.u = u; p.up = b_up; p.row_adapter = plan->row_adapter; p.order = plan->row_order; p.R = R; p.S = c.S; p.ws = ws;
-    const int tl = c.kind == GEMV16 || c.kind == TILE_64x64 || c.kind == TILE_64x128 ? 0 : c.kind == TILE_128x128 ? 1 : 2;      // tile heights 64, 128, 256
-    p.tile_off = plan->tiles_off[tl]; p.tile_list = plan->tiles[tl];
     hipStream_t st = (hipStream_t)stream;
-    m4d_count_launch(c.kind == WIDE_256x256 ? M4D_KC_GEMM_WIDE : M4D_KC_GEMM_GENERIC);
+    const int64_t rows_wide = c.kind == WIDE_256x256 ? M : c.head;
+    if (rows_wide > 0) {
+        p.M = rows_wide;
+        p.tile_off = plan->tiles_off[3]; p.tile_list = plan->tiles[3]; p.tile_one = plan->tile_one;
+        p.tiles_m = (int)((rows_wide + 255) / 256); p.tiles_n = (int)((N + 255) / 256);
+        M4D_CHECK_ARG((int64_t)p.tiles_m * p.tiles_n < (1ll << 31), "linear_adapters: too many tiles");
+        m4d_count_launch(M4D_KC_GEMM_WIDE);
+        if (m4d_launch_gemm_wide_adapters(static_cast<const GemmAdArgs*>(&p), (unsigned)(p.tiles_m * p.tiles_n), st) != 0) {
+            (void)hipGetLastError();
+            m4d_set_error("linear_adapters: cannot enable 128 KiB LDS");
+            return -3;
+        }
+        M4D_CHECK_LAUNCH("linear_adapters");
+        if (rows_wide == M) return 0;
+        // the rows behind it (whole tiles of 256 in front, so every tile table goes on at its own row)
+        p.A = (const char*)x + rows_wide * ldx * es; p.u = (const char*)u + rows_wide * R * es; p.out = (char*)out + rows_wide * ldo * es;
+        p.row_adapter = plan->row_adapter + rows_wide; p.M = p.rows_per_sample = M - rows_wide;
+    }
+    const int tl = c.kind == GEMV16 || c.kind == TILE_64x64 || c.kind == TILE_64x128 ? 0 : c.kind == TILE_128x128 ? 1 : 2;      // tile heights 64, 128, 256
+    p.tile_off = plan->tiles_off[tl] + (rows_wide >> (6 + tl)); p.tile_list = plan->tiles[tl];
+    m4d_count_launch(M4D_KC_GEMM_GENERIC);
     switch (c.kind) {
         case GEMV16: {
-            M4D_CHECK_ARG(M <= 16, "linear_adapters: too many rows");
+            M4D_CHECK_ARG(p.M <= 16, "linear_adapters: too many rows");
             dim3 grid((unsigned)((N + 15) / 16)), block(64 * SKINNY_WAVES);
             if (bf16) hipLaunchKernelGGL(adapter_gemv_kernel<bf16_t>, grid, block, 0, st, p);
             else hipLaunchKernelGGL(adapter_gemv_kernel<float>, grid, block, 0, st, p);
@@ -778,19 +812,8 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
         case TILE_64x64: return bf16 ? launch_gemm<bf16_t, 1, 1, 2, 2>(p, st) : launch_gemm<float, 1, 1, 2, 2>(p, st);
         case TILE_64x128: return bf16 ? launch_gemm<bf16_t, 1, 1, 2, 4>(p, st) : launch_gemm<float, 1, 2, 2, 2>(p, st);
         case TILE_128x128: return bf16 ? launch_gemm<bf16_t, 1, 2, 4, 2>(p, st) : launch_gemm<float, 2, 2, 2, 2>(p, st);
-        case TILE_256x128: return bf16 ? launch_gemm<bf16_t, 2, 2, 4, 2>(p, st) : launch_gemm<float, 4, 2, 2, 2>(p, st);
-        default: break;
+        default: return bf16 ? launch_gemm<bf16_t, 2, 2, 4, 2>(p, st) : launch_gemm<float, 4, 2, 2, 2>(p, st);
     }
-    p.tile_off = plan->tiles_off[3]; p.tile_list = plan->tiles[3]; p.tile_one = plan->tile_one;
-    p.tiles_m = (int)((M + 255) / 256); p.tiles_n = (int)((N + 255) / 256);
-    M4D_CHECK_ARG((int64_t)p.tiles_m * p.tiles_n < (1ll << 31), "linear_adapters: too many tiles");
-    if (m4d_launch_gemm_wide_adapters(static_cast<const GemmAdArgs*>(&p), (unsigned)(p.tiles_m * p.tiles_n), st) != 0) {
-        (void)hipGetLastError();
-        m4d_set_error("linear_adapters: cannot enable 128 KiB LDS");
-        return -3;
-    }
-    M4D_CHECK_LAUNCH("linear_adapters");
-    return 0;
 }
 
 // the coarsest chunks that still give three workgroups for two CUs (two fit on one; coarser: fewer partial sums to write and join)

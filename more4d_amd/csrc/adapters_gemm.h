@@ -259,7 +259,7 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void adapter_gemv_kernel(AdGemmA
         mma16(load_k8<T>(w, k, K - q * 8), load_k8<T>(x, k, K - q * 8), acc);
     }
     const int ra = p.row_adapter[row];
-    for (int i = wave; i < p.tile_off[1]; i += SKINNY_WAVES) {      // (at most 16 rows: one tile)
+    for (int i = p.tile_off[0] + wave; i < p.tile_off[1]; i += SKINNY_WAVES) {      // (at most 16 rows: one tile)
         const int g = p.tile_list[i];
         const T* b = (const T*)p.up + ((int64_t)g * p.N + min(n0 + i16, p.N - 1)) * p.R;
         const T* u = (const T*)p.u + (int64_t)row * p.R;

@@ -295,3 +295,21 @@ def test_interleaved_requests(dt, M, N, K, r):
     ys = AdapterLinearFn.apply(t[0], w, None, t[1], t[2], scale, srt, 16)
     _, da2, db2 = torch.autograd.grad(ys, t, dy[by])
     assert torch.equal(da, da2) and torch.equal(db, db2)              # the same slots, so the same sums
+
+
+@pytest.mark.parametrize("M,lengths,ids", [(4400, [4400], [0]), (4400, [3000, 1, 900, 0, 400, 99], [1, 0, -1, 0, 2, 1]), (3850, [3838, 1, 6, 5], [0, 1, -1, 2]),
+                                           (3841, [3841], [-1]), (4000, [3840, 160], [-1, 0])])
+@pytest.mark.parametrize("r", [16, 64])
+def test_whole_rounds_of_the_largest_tiles_and_the_rows_behind(M, lengths, ids, r):
+    o = ops()
+    N, K = 4100, 1024
+    x, w, bias, a, b, scale, row = on_gpu(*problem(lengths, ids, K, N, r, BF))
+    plan, bank = o.AdapterPlan(lengths, ids, DEV), o.AdapterBank(a, b, scale) if max(ids) >= 0 else o.AdapterBank(a[:1], b[:1], scale[:1])
+    out = torch.full((M + 1, N + 4), float("nan"), device=DEV, dtype=BF)
+    o.launch_counts(reset=True)
+    y = o.linear_adapters(x, w, bias, bank, plan, out=out[:M, :N])
+    n = o.launch_counts()
+    if max(ids) >= 0:
+        assert n["gemm_wide"] == 1 and n["gemm_generic"] == 1
+    check(y, *oracle(x, w, bias, a, b, scale, row))
+    assert torch.isnan(out[M]).all() and torch.isnan(out[:, N:]).all()
