@@ -536,7 +536,7 @@ int cus() {
     return v;
 }
 
-enum { GEMV16 = 0, TILE_64x64, TILE_64x128, TILE_128x128, TILE_256x128, WIDE_256x256 };
+enum { GEMV16 = 0, TILE_64x64, TILE_64x128, TILE_128x128, TILE_256x128, WIDE_256x256, TILE_128x192 };
 struct Choice { int kind, S; int64_t head; };      // head rows on the 256 x 256 kernel, the others on `kind` in S slices of K
 
 double wide_round_us(int64_t K, double wide_ad) { return (double)(K / 64) * 1.03 + 10.0 + wide_ad; }
@@ -544,9 +544,9 @@ double wide_round_us(int64_t K, double wide_ad) { return (double)(K / 64) * 1.03
 // the ring, epilogue) and c per 128-byte K tile.  c is what the tile moves from L2 at the 60 - 80 bytes/ns that a CU gets (fp32: the MFMA
 // rate), so larger tiles are cheaper per product and smaller ones waste less of a round; slices pay for writing and joining float32 partial
 // tiles.  Measured c (us, bf16 / fp32): 64 x 64 0.30 / 0.70 alone on a CU and 0.42 / 1.25 as one of two, 64 x 128 0.36 / 1.16, 128 x 128
-// 0.55 / 2.1, 256 x 128 0.92 / 4.0, 256 x 256 (gemm_wide.h) 1.03.  Measured against each other at 40 shapes (M 2 .. 21840): the choice is within
-// 10 % of the best of all kinds and slices, e.g. 64 x 5120 x 4096: 64 x 64 in 3 slices 14.3 us, whole 21.7, 128 x 128 whole 36; 986 x 5120 x
-// 4096: 256 x 128 65 us, 128 x 128 75, 256 x 256 72.
+// 0.55 / 2.1, 128 x 192 0.66 / -, 256 x 128 0.78 / 4.0, 256 x 256 (gemm_wide.h) 1.03.  Measured against each other at 40 shapes (M 2 .. 21840): the
+// choice is within 10 % of the best of all kinds and slices, e.g. 64 x 5120 x 4096: 64 x 64 in 3 slices 14.2 us, whole 21.4, 128 x 128 whole 32;
+// 986 x 5120 x 4096: 128 x 192 47 us, 256 x 128 54, 256 x 256 67, 128 x 128 72.
 Choice choose_whole(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, double wide_ad, int ncu, double& t_best) {
     t_best = 1e30;
 #ifdef M4D_ABLATIONS
@@ -561,9 +561,10 @@ Choice choose_whole(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, do
         const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
         offer((double)((tiles + ncu - 1) / ncu) * wide_round_us(K, wide_ad), WIDE_256x256, 1);
     }
-    static const struct { int kind, bm, bn, occ; double c[2][2], fix; } cfg[4] = {
+    static const struct { int kind, bm, bn, occ; double c[2][2], fix; } cfg[5] = {
         {TILE_64x64, 64, 64, 2, {{0.30, 0.42}, {0.70, 1.25}}, 4.0}, {TILE_64x128, 64, 128, 1, {{0.36, 0.36}, {1.16, 1.16}}, 4.0},
-        {TILE_128x128, 128, 128, 1, {{0.55, 0.55}, {2.1, 2.1}}, 5.0}, {TILE_256x128, 256, 128, 1, {{0.92, 0.92}, {4.0, 4.0}}, 7.0}};
+        {TILE_128x128, 128, 128, 1, {{0.55, 0.55}, {2.1, 2.1}}, 5.0}, {TILE_256x128, 256, 128, 1, {{0.78, 0.78}, {4.0, 4.0}}, 7.0},
+        {TILE_128x192, 128, 192, 1, {{0.66, 0.66}, {1e6, 1e6}}, 6.0}};      // (bf16 only)
     for (const auto& f : cfg) {
         const int64_t tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
         for (int S = 1; S <= 16; ++S) {
@@ -574,7 +575,7 @@ Choice choose_whole(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, do
             double t = rounds * (per * f.c[bf16 ? 0 : 1][shared] + f.fix);
             const double floor = wbytes / 6.0e6;
             if (t < floor) t = floor;
-            if (S > 1) t += 4.5 + (double)M * N * (8.0 * S + es) / 4.5e6;
+            if (S > 1) t += 4.5 + (double)M * N * (8.0 * S + es) / 7.0e6;
             offer(t, f.kind, S);
         }
     }
@@ -587,7 +588,7 @@ Choice choose(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, bool spl
     double t;
     Choice best = choose_whole(bf16, M, N, K, wide_ok, wide_ad, ncu, t);
     const int64_t tn = (N + 255) / 256, rounds = ((M + 255) / 256) * tn / ncu, head = rounds * ncu / tn * 256;
-    if (best.kind == WIDE_256x256 && split_ok && head > 0 && head < M) {
+    if (wide_ok && split_ok && head > 0 && head < M) {
         double t2;
         Choice rest = choose_whole(bf16, M - head, N, K, false, wide_ad, ncu, t2);
         if (rounds * wide_round_us(K, wide_ad) + t2 + 8.0 < 0.98 * t) { best = rest; best.head = head; }
@@ -797,7 +798,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
         p.A = (const char*)x + rows_wide * ldx * es; p.u = (const char*)u + rows_wide * R * es; p.out = (char*)out + rows_wide * ldo * es;
         p.row_adapter = plan->row_adapter + rows_wide; p.M = p.rows_per_sample = M - rows_wide;
     }
-    const int tl = c.kind == GEMV16 || c.kind == TILE_64x64 || c.kind == TILE_64x128 ? 0 : c.kind == TILE_128x128 ? 1 : 2;      // tile heights 64, 128, 256
+    const int tl = c.kind == GEMV16 || c.kind == TILE_64x64 || c.kind == TILE_64x128 ? 0 : c.kind == TILE_128x128 || c.kind == TILE_128x192 ? 1 : 2;      // tile heights 64, 128, 256
     p.tile_off = plan->tiles_off[tl] + (rows_wide >> (6 + tl)); p.tile_list = plan->tiles[tl];
     m4d_count_launch(M4D_KC_GEMM_GENERIC);
     switch (c.kind) {
@@ -812,6 +813,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
         case TILE_64x64: return bf16 ? launch_gemm<bf16_t, 1, 1, 2, 2>(p, st) : launch_gemm<float, 1, 1, 2, 2>(p, st);
         case TILE_64x128: return bf16 ? launch_gemm<bf16_t, 1, 1, 2, 4>(p, st) : launch_gemm<float, 1, 2, 2, 2>(p, st);
         case TILE_128x128: return bf16 ? launch_gemm<bf16_t, 1, 2, 4, 2>(p, st) : launch_gemm<float, 2, 2, 2, 2>(p, st);
+        case TILE_128x192: return launch_gemm<bf16_t, 1, 3, 4, 2>(p, st);
         default: return bf16 ? launch_gemm<bf16_t, 2, 2, 4, 2>(p, st) : launch_gemm<float, 4, 2, 2, 2>(p, st);
     }
 }

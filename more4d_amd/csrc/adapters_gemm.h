@@ -162,34 +162,39 @@ __global__ __launch_bounds__(64 * WM * WN) void adapter_gemm_kernel(AdGemmArgs p
 
     // out of the accumulator layout (lane = row) through LDS: 4 consecutive columns per lane, whole rows per group of lanes
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    constexpr int NCH = NI * 8;                              // 16-byte chunks of a row of the wave's columns
+    constexpr int EN = NI % 2 ? 1 : NI;                      // column blocks of 32 in one trip (three: one after the other)
+    constexpr int NCH = EN * 8;                              // 16-byte chunks of a row of them
     char* wl = ad_smem + wave * 32 * NCH * 16;
     static_assert(NW * 32 * NCH * 16 <= Sh::LDS, "the epilogue's block fits");
     const T* bias = (const T*)p.bias;
     const int ch = lane % NCH;
-    const int64_t n = n0 + wn * NI * 32 + ch * 4;
-    f32x4 bv = {0.f, 0.f, 0.f, 0.f};
-    if (p.S == 1 && bias && n < p.N) bv = load4(bias + n);
     float* part = p.S > 1 ? p.ws + (int64_t)blockIdx.y * p.M * p.N : nullptr;
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
+    for (int nb = 0; nb < NI; nb += EN) {
+        const int64_t n = n0 + (wn * NI + nb) * 32 + ch * 4;
+        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+        if (p.S == 1 && bias && n < p.N) bv = load4(bias + n);
 #pragma unroll
-        for (int ni = 0; ni < NI; ++ni)
+        for (int mi = 0; mi < MI; ++mi) {
 #pragma unroll
-            for (int rq = 0; rq < 4; ++rq) {
-                const int c = ni * 8 + rq * 2 + hi;
-                const f32x4 v = {acc[ni][mi][rq * 4], acc[ni][mi][rq * 4 + 1], acc[ni][mi][rq * 4 + 2], acc[ni][mi][rq * 4 + 3]};
-                *reinterpret_cast<f32x4*>(wl + li * NCH * 16 + ((c ^ (li & (NCH - 1))) << 4)) = v;
-            }
-        // (wave-private region: program order and the compiler's lgkmcnt waits order the reads behind the writes)
+            for (int ni = 0; ni < EN; ++ni)
 #pragma unroll
-        for (int it = 0; it < NCH / 2; ++it) {
-            const int r = it * (64 / NCH) + lane / NCH;
-            const f32x4 v = *reinterpret_cast<const f32x4*>(wl + r * NCH * 16 + ((ch ^ (r & (NCH - 1))) << 4));
-            const int64_t m = m0 + (wm * MI + mi) * 32 + r;
-            if (m < p.M && n < p.N) {
-                if (part) store4(part + m * p.N + n, v);
-                else store4((T*)p.out + (p.order ? p.order[m] : m) * p.ldc + n, v + bv);
+                for (int rq = 0; rq < 4; ++rq) {
+                    const int c = ni * 8 + rq * 2 + hi;
+                    const f32x16& a = acc[nb + ni][mi];
+                    const f32x4 v = {a[rq * 4], a[rq * 4 + 1], a[rq * 4 + 2], a[rq * 4 + 3]};
+                    *reinterpret_cast<f32x4*>(wl + li * NCH * 16 + ((c ^ (li & (NCH - 1))) << 4)) = v;
+                }
+            // (wave-private region: program order and the compiler's lgkmcnt waits order the reads behind the writes)
+#pragma unroll
+            for (int it = 0; it < NCH / 2; ++it) {
+                const int r = it * (64 / NCH) + lane / NCH;
+                const f32x4 v = *reinterpret_cast<const f32x4*>(wl + r * NCH * 16 + ((ch ^ (r & (NCH - 1))) << 4));
+                const int64_t m = m0 + (wm * MI + mi) * 32 + r;
+                if (m < p.M && n < p.N) {
+                    if (part) store4(part + m * p.N + n, v);
+                    else store4((T*)p.out + (p.order ? p.order[m] : m) * p.ldc + n, v + bv);
+                }
             }
         }
     }

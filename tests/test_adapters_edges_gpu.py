@@ -313,3 +313,18 @@ def test_whole_rounds_of_the_largest_tiles_and_the_rows_behind(M, lengths, ids, 
         assert n["gemm_wide"] == 1 and n["gemm_generic"] == 1
     check(y, *oracle(x, w, bias, a, b, scale, row))
     assert torch.isnan(out[M]).all() and torch.isnan(out[:, N:]).all()
+
+
+@pytest.mark.parametrize("lengths,ids,K,N", [([512, 77, 1, 0, 226, 131, 39], [0, 2, 1, 1, -1, 2, 3], 4096, 5124), ([300], [0], 4096, 5120),
+                                             ([1] * 986, [i % 9 - 1 for i in range(986)], 1024, 5120), ([2900, 100], [1, 0], 8960, 1540)])
+def test_tiles_of_192_columns(lengths, ids, K, N):
+    """Shapes that the size rule sends to the 128 x 192 tiles: whole K, slices of K, rows in order of their adapters, a ragged last column tile."""
+    o = ops()
+    x, w, bias, a, b, scale, row = on_gpu(*problem(lengths, ids, K, N, 12, BF))
+    M = x.shape[0]
+    plan, bank = o.AdapterPlan(lengths, ids, DEV), o.AdapterBank(a, b, scale)
+    out = torch.full((M + 1, N + 8), float("nan"), device=DEV, dtype=BF)
+    y = o.linear_adapters(x, w, bias, bank, plan, out=out[:M, :N])
+    check(y, *oracle(x, w, bias, a, b, scale, row))
+    assert torch.isnan(out[M]).all() and torch.isnan(out[:, N:]).all()
+    assert torch.equal(y, o.linear_adapters(x, w, bias, bank, plan))
