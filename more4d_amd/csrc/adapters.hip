@@ -767,7 +767,8 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
     M4D_CHECK_ARG(plan->row_adapter && plan->tiles_off[0] && plan->tiles_off[1] && plan->tiles_off[2] && plan->tiles[0] && plan->tiles[1] && plan->tiles[2] && plan->tile_one,
                   "linear_adapters: bad plan");
     const bool bf16 = dt == M4D_BF16;
-    const bool wide_ok = wide_shape(dt, M, N, K) && ldo % 8 == 0 && ((uintptr_t)out % 32) == 0;
+    // (the wide kernel's lanes hold the offsets of 32 rows in 32 bits)
+    const bool wide_ok = wide_shape(dt, M, N, K) && ldo % 8 == 0 && ((uintptr_t)out % 32) == 0 && ldx <= (1 << 25) && ldw <= (1 << 25);
     const Choice c = choose(bf16, M, N, K, wide_ok, !plan->row_order, wide_adapters_us(plan, R), cus());
     M4D_CHECK_ARG(c.S == 1 || (ws && ws_floats >= c.S * (M - c.head) * N && ((uintptr_t)ws % 16) == 0), "linear_adapters: workspace of %lld floats needed",
                   (long long)(c.S * (M - c.head) * N));

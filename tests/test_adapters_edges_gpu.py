@@ -328,3 +328,27 @@ def test_tiles_of_192_columns(lengths, ids, K, N):
     check(y, *oracle(x, w, bias, a, b, scale, row))
     assert torch.isnan(out[M]).all() and torch.isnan(out[:, N:]).all()
     assert torch.equal(y, o.linear_adapters(x, w, bias, bank, plan))
+
+
+def test_rows_far_apart():
+    """Row strides whose 31-fold passes 32 bits in bytes: not for the 256 x 256 tiles, which the shape would go to otherwise."""
+    o = ops()
+    M, N, K, ld = 512, 30720, 1024, 70_000_000
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 72 GB")
+    lengths, ids = [300, 212], [1, 0]
+    x, w, bias, a, b, scale, row = on_gpu(*problem(lengths, ids, K, N, 16, BF))
+    far = torch.empty((M - 1) * ld + K, device=DEV, dtype=BF).as_strided((M, K), (ld, 1))
+    far.copy_(x)
+    plan, bank = o.AdapterPlan(lengths, ids, DEV), o.AdapterBank(a, b, scale)
+    o.launch_counts(reset=True)
+    y = o.linear_adapters(far, w, bias, bank, plan)
+    assert o.launch_counts()["gemm_wide"] == 0
+    check(y, *oracle(x, w, bias, a, b, scale, row))
+    o.launch_counts(reset=True)
+    check(o.linear_adapters(x, w, bias, bank, plan), *oracle(x, w, bias, a, b, scale, row))
+    assert o.launch_counts()["gemm_wide"] == 1
+    del far
+    torch.cuda.empty_cache()
