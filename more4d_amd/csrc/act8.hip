@@ -10,7 +10,8 @@
 //
 // All four kernels are one pass over the data and bound by HBM; a "unit" is 8 channels of a row (16 bytes of bf16, 8 bytes of codes), four
 // units are a block.  Rows of codes are padded to whole blocks, so the code side is always aligned; the other side takes 16-byte accesses
-// where its rows are 16-byte aligned and element accesses otherwise.
+// where its rows are 16-byte aligned and element accesses otherwise.  21840 x 13824 bf16 (a copy of 2 GiB runs at 4.9 TB/s): act_quant8 183 us = 5.0
+// TB/s, act_bwd8 302 us = 5.0, act_dequant8_t with GELU 245 us = 3.7 (its activation's instructions); 21840 x 5120 float32: act_quant8 112 us, act_dequant8 138.
 #include "act8.h"
 #include "more4d_hip.h"
 
