@@ -154,7 +154,8 @@ M4D_DEV void epilogue_tile(const GemmArgs& p, const f32x16& acc, int64_t m, int6
 // The adapters' part of a wave's NI x MI accumulator blocks (32 x 32 each; rows m_base + 32 mi + lane, columns n_base + 32 ni + lane of W):
 // acc += up_g[n, :] . u[m, :] over the rank, for every step-th adapter of the tile from `first` on.  The operands come straight from L2 in the
 // MFMA layout (16 bytes per lane and 16 ranks; a block's 32 rows of R ranks are contiguous memory): through LDS they would need two more
-// barriers.  All loads of 64 ranks are issued before their first product, so a tile pays one L2 latency per 64 ranks and adapter, not four.
+// barriers.  All loads of 64 ranks (32 with 256 accumulators) are issued before their first product, so a tile pays one L2
+// latency for them and adapter, not four (two).
 // Rows of u that name another adapter (or none: their u was never written) are replaced by zero before the product, not multiplied by zero; and
 // where a wave's rows do not all name the adapter, an infinity or NaN in its B must not meet those zeros: float32 then takes sums of their own that
 // only the adapter's rows add, bf16 bad_parts (a VALU instruction on its accumulators takes them out of the AGPRs: 200 spilled registers in the
@@ -216,7 +217,8 @@ M4D_DEV bf16x8 big_signs(const bf16x8& u) {
     return r;
 }
 template <typename T, int NI, int MI>
-M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const AdTile<MI>& a, int64_t n_base, int lane, int step = 1, int k0 = 0) {      // k0: ranks in front of it are already in
+M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const AdTile<MI>& a, int64_t n_base, int lane, int step = 1,
+                             int k0 = 0) {      // k0: ranks in front of it are already in
     typedef typename Frag8<T>::type frag_t;
     constexpr int U = sizeof(T) != 2 ? 1 : NI * MI < 16 ? 4 : 2;      // 16-rank steps in flight, as registers allow (float32 is MFMA-bound)
     const int li = lane & 31, hi = lane >> 5;
