@@ -528,8 +528,9 @@ int m4d_act_bwd8(m4d_dtype dt, const void* dy, int64_t ldy, const int8_t* codes,
  *                    parts whose sum is the value to 16 bits, float32 in one;
  *                    codes / exps (may be NULL): the 8-bit form of x's rows with an adapter, as act_quant8 writes it;
  *                    ws: adapter_down_workspace floats (slots: ut or codes will be asked for)
- *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once.  With a_down, u (and ut, codes, exps if given) are written first, by
- *                    adapter_down; without, u is an input.  ws: linear_adapters_workspace floats
+ *   linear_adapters  out T [rows, N] = x W^T + bias + u B_g^T, rounded once.  u (and ut, codes, exps if given) are written first, as by adapter_down;
+ *                    u is scratch here: bf16 [rows, 2 R], u in two parts whose sum is the value to 16 bits, float32 [rows, R].
+ *                    ws: linear_adapters_workspace floats
  *   adapter_grad     out T [G, rank, C] (transposed: [G, C, rank]) = sum over the rows of g of v^T x, vt as adapter_down writes ut, x as T or as
  *                    8-bit codes; ws: adapter_grad_workspace floats; partial sums are joined in a fixed order
  *   linear_adapters_bwd  the backward of linear_adapters with W [N, K] frozen, in one call: dx T [rows, K] = dy W + v A (NULL: not wanted), da (needs

@@ -9,12 +9,12 @@
 //
 // Rows are worked on in SLOTS: the plan lists the rows adapter by adapter, each adapter's list padded (slot_row = -1) to whole PIECES of 64
 // slots, so a workgroup never sees two adapters whatever the order of the requests, and one-row requests of one adapter share a piece.
-// u is written twice: [row][R], the GEMM's operand, and as the operand of the row contraction in the order in which its MFMA lanes read it,
-// [slot / 16][rank / 32][part][lane][8] with lane = rank % 32 + 32 * (slot % 16 / 8) (read row by row, 16 bytes of 32 ranks each, these loads
-// cost the address unit as much as x's); pad slots and ranks hold zero.
-// Rounding: the GEMM's u is rounded to T like every other operand of an MFMA here — it is a small part of an output that is rounded to T itself.
-// The row contraction is all u (or v): rounded once it would put an error of the size of the gradient's own rounding on it, so bf16 keeps u
-// there as a sum of two parts, u = hi + lo to 16 bits (part 0, 1), at twice the products, which are not what bounds that pass.
+// u is written twice: by rows, the GEMM's operand (gemm_common.h: u_hi), and as the operand of the row contraction in the order in which its MFMA
+// lanes read it, [slot / 16][rank / 32][part][lane][8] with lane = rank % 32 + 32 * (slot % 16 / 8) (read row by row, 16 bytes of 32 ranks each,
+// these loads cost the address unit as much as x's); pad slots and ranks hold zero.
+// Rounding: u (or v) is nowhere rounded to bf16 once, which would put an error of the size of the result's own rounding on it (gradients: 0.0024 of
+// their size instead of 0.0017; y and dx more with every rank, 0.0019 at 128): it is kept as a sum of two parts, u = hi + lo to 16 bits, at
+// twice the products, which are not what bounds the row contraction and 32 more of K = 1536 .. 5120 per 32 ranks in the GEMM.
 //
 // The operand of a down projection is laid out once (m4d_adapter_pack) in the order in which the MFMA lanes read it: chunks of 64 channels, 32
 // ranks, and within them lane (rank l & 31, channels 32 (l >> 5) + [0, 32) as four 8-element fragments).  With that order of the channels a
@@ -79,9 +79,29 @@ struct DownArgs {
     int K, R, n_pieces;
     int KS;                // K slices (gridDim.y); > 1: unscaled float32 sums to part [KS, n_pieces, R rounded up to 32, 64]
     float* part;
+    int split;             // u as the projection's operand (gemm_common.h: u_hi); 0: [rows, R], rounded once
 };
 
-template <typename T> struct Parts { static constexpr int N = sizeof(T) == 2 ? 2 : 1; };      // of a value in ut
+// bf16, the projection's operand: v = hi + lo to 16 bits, hi being v cut off towards zero (its predecessor where v is a bf16 number itself), so that
+// both parts have v's sign: hi * b + lo * b is then what v * b is for an infinite b or v too (parts of v rounded to nearest give inf - inf or 0 * inf).
+M4D_DEV void split2(float v, bf16_t& hi, bf16_t& lo) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    if (!isfinite(v)) { hi = lo = (bf16_t)v; return; }
+    const float h = __builtin_bit_cast(float, (u & 0x7fffffffu) != 0u && (u & 0xffffu) == 0u ? u - 0x10000u : u & 0xffff0000u);
+    hi = (bf16_t)h; lo = (bf16_t)(v - h);
+}
+M4D_DEV void split2(float v, float& hi, float&) { hi = v; }
+
+// four ranks (r .. r + 3, r a multiple of 4) of a row of u
+template <typename T>
+M4D_DEV void store_u(T* row, int r, int R, const f32x4& v) {
+    T hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split2(v[e], hi[e], lo[e]);
+    T* d = row + u_hi<T>(r);
+    store4(d, f32x4{(float)hi[0], (float)hi[1], (float)hi[2], (float)hi[3]});
+    if constexpr (Parts<T>::N == 2) store4(d + min(32, R - (r & ~31)), f32x4{(float)lo[0], (float)lo[1], (float)lo[2], (float)lo[3]});
+}
 
 // four ranks (r .. r + 3) of one slot to u and / or ut, scaled
 template <typename T>
@@ -89,7 +109,10 @@ M4D_DEV void down_store(const DownArgs& p, int64_t piece, int g, int slot, int r
     const float sc = p.scale[g];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = row >= 0 ? v[e] * sc : 0.f;
-    if (p.u && row >= 0 && r < p.R) store4((T*)p.u + (int64_t)row * p.R + r, v);
+    if (p.u && row >= 0 && r < p.R) {
+        if (p.split) store_u((T*)p.u + (int64_t)row * u_stride<T>(p.R), r, p.R, v);
+        else store4((T*)p.u + (int64_t)row * p.R + r, v);
+    }
     if (p.ut) {
         const int64_t s = piece * PIECE + slot;
         T* d = (T*)p.ut + (((s >> 4) * ((p.R + 31) >> 5) + (r >> 5)) * (64 * Parts<T>::N) + (r & 31) + ((slot >> 3) & 1) * 32) * 8 + (slot & 7);
@@ -326,7 +349,9 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void adapter_down16_kernel(DownA
         f32x4 v = red[0][lane];
 #pragma unroll
         for (int k = 1; k < SKINNY_WAVES; ++k) v += red[k][lane];
-        store4((T*)p.u + (int64_t)i16 * p.R + r0 + q * 4, v * p.scale[g]);
+        const f32x4 w = v * p.scale[g];
+        if (p.split) store_u((T*)p.u + (int64_t)i16 * u_stride<T>(p.R), r0 + q * 4, p.R, w);
+        else store4((T*)p.u + (int64_t)i16 * p.R + r0 + q * 4, w);
     }
 }
 
@@ -682,8 +707,8 @@ extern "C" int64_t m4d_adapter_down_workspace(const m4d_adapter_plan* plan, int6
     return ks > 1 ? (int64_t)ks * plan->n_pieces * ((R + 31) / 32 * 32) * PIECE : 0;
 }
 
-extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan,
-                                void* u, void* ut, int8_t* codes, uint8_t* exps, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream) {
+static int down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan, void* u, int split,
+                void* ut, int8_t* codes, uint8_t* exps, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream) {
     PLAN_OK("adapter_down");
     M4D_CHECK_ARG(x && a_down && scale && (u || ut) && (codes == nullptr) == (exps == nullptr), "adapter_down: null pointer");
     M4D_CHECK_ARG(K > 0 && K < (1 << 30) && (K * es) % 16 == 0 && (ldx * es) % 16 == 0 && (plan->rows == 1 || ldx >= K),
@@ -695,7 +720,7 @@ extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const 
     const int ks = down_slices(plan->n_pieces, K, R);
     if (down_few(plan, ut, codes)) {
         M4D_CHECK_ARG(plan->row_adapter && plan->tiles[0] && plan->n_listed > 0 && plan->n_listed <= 16, "adapter_down: bad plan");
-        DownArgs p{x, a_down, scale, u, nullptr, nullptr, nullptr, nullptr, nullptr, ldx, (int)K, R, plan->n_pieces, 1, nullptr};
+        DownArgs p{x, a_down, scale, u, nullptr, nullptr, nullptr, nullptr, nullptr, ldx, (int)K, R, plan->n_pieces, 1, nullptr, split};
         dim3 grid((unsigned)plan->n_listed, (unsigned)(R / 16)), block(64 * SKINNY_WAVES);
         if (dt == M4D_BF16) hipLaunchKernelGGL(adapter_down16_kernel<bf16_t>, grid, block, 0, (hipStream_t)stream, p, plan->row_adapter, plan->tiles[0], (int)plan->rows);
         else hipLaunchKernelGGL(adapter_down16_kernel<float>, grid, block, 0, (hipStream_t)stream, p, plan->row_adapter, plan->tiles[0], (int)plan->rows);
@@ -705,10 +730,14 @@ extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const 
     const int64_t need = m4d_adapter_down_workspace(plan, K, R, 1);
     M4D_CHECK_ARG(need == 0 || (ws && ws_floats >= need), "adapter_down: workspace of %lld floats needed", (long long)need);
     DownArgs p{x, a_down, scale, u, ut, codes, exps, plan->slot_row, plan->piece_adapter, ldx, (int)K, R,
-               plan->n_pieces, ks, ks > 1 ? ws : nullptr};
+               plan->n_pieces, ks, ks > 1 ? ws : nullptr, split};
     hipStream_t st = (hipStream_t)stream;
     if (dt == M4D_BF16) return R <= 32 ? launch_down<bf16_t, 1>(p, st) : R <= 64 ? launch_down<bf16_t, 2>(p, st) : launch_down<bf16_t, 4>(p, st);
     return R <= 32 ? launch_down<float, 1>(p, st) : launch_down<float, 2>(p, st);
+}
+extern "C" int m4d_adapter_down(m4d_dtype dt, const void* x, int64_t ldx, const void* a_down, const float* scale, const m4d_adapter_plan* plan,
+                                void* u, void* ut, int8_t* codes, uint8_t* exps, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream) {
+    return down(dt, x, ldx, a_down, scale, plan, u, 0, ut, codes, exps, K, R, ws, ws_floats, stream);
 }
 
 template <typename T, int MI, int NI, int WM, int WN>
@@ -741,6 +770,7 @@ static bool wide_shape(m4d_dtype dt, int64_t M, int64_t N, int64_t K) { return d
 // per adapter: rank 16 0.8, rank 64 3.8.  The other tiles take interleaved rows in order and have one or two adapters each.
 static double wide_adapters_us(const m4d_adapter_plan* plan, int R) { return plan->row_order ? 0.06 * R * plan->n_wide / (double)((plan->rows + 255) / 256) : 0.0; }
 
+static int u_parts(m4d_dtype dt) { return dt == M4D_BF16 ? Parts<bf16_t>::N : Parts<float>::N; }
 // the down projection's slices and the GEMM's run one after the other: one workspace, the larger of the two
 extern "C" int64_t m4d_linear_adapters_workspace(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_t K, int R, int slots) {
     if (!plan || plan->rows <= 0 || N <= 0 || K <= 0) return 0;
@@ -758,7 +788,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
                                    uint8_t* exps, void* out, int64_t ldo, int64_t N, int64_t K, int R, float* ws, int64_t ws_floats, m4d_stream stream) {
     PLAN_OK("linear_adapters");
     const int64_t M = plan->rows;
-    M4D_CHECK_ARG(x && W && out && u && b_up, "linear_adapters: null pointer");
+    M4D_CHECK_ARG(x && W && out && a_down && u && b_up, "linear_adapters: null pointer");
     M4D_CHECK_ARG(N > 0 && K > 0 && K < (1 << 30) && N < (1ll << 31) && (K * es) % 16 == 0, "linear_adapters: K*sizeof(T) must be a multiple of 16 (K=%lld)", (long long)K);
     M4D_CHECK_ARG(N % 4 == 0 && ldo % 4 == 0 && (M == 1 || ldo >= N), "linear_adapters: N and the output's row stride must be multiples of 4 (N=%lld ldo=%lld)",
                   (long long)N, (long long)ldo);
@@ -774,10 +804,8 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
     const Choice c = choose(bf16, M, N, K, wide_ok, !plan->row_order, wide_adapters_us(plan, R), cus());
     M4D_CHECK_ARG(c.S == 1 || (ws && ws_floats >= c.S * (M - c.head) * N && ((uintptr_t)ws % 16) == 0), "linear_adapters: workspace of %lld floats needed",
                   (long long)(c.S * (M - c.head) * N));
-    if (a_down) {
-        const int rc = m4d_adapter_down(dt, x, ldx, a_down, scale, plan, u, ut, codes, exps, K, R, ws, ws_floats, stream);
-        if (rc != 0) return rc;
-    }
+    const int rc = down(dt, x, ldx, a_down, scale, plan, u, 1, ut, codes, exps, K, R, ws, ws_floats, stream);
+    if (rc != 0) return rc;
     AdGemmArgs p{};
     p.A = x; p.W = W; p.bias = bias; p.out = out; p.lda = ldx; p.ldw = ldw; p.ldc = ldo; p.M = M; p.N = N; p.K = K;
     p.rows_per_sample = M; p.epilogue = M4D_EPI_STORE;
@@ -798,7 +826,7 @@ extern "C" int m4d_linear_adapters(m4d_dtype dt, const void* x, int64_t ldx, con
         M4D_CHECK_LAUNCH("linear_adapters");
         if (rows_wide == M) return 0;
         // the rows behind it (whole tiles of 256 in front, so every tile table goes on at its own row)
-        p.A = (const char*)x + rows_wide * ldx * es; p.u = (const char*)u + rows_wide * R * es; p.out = (char*)out + rows_wide * ldo * es;
+        p.A = (const char*)x + rows_wide * ldx * es; p.u = (const char*)u + rows_wide * R * u_parts(dt) * es; p.out = (char*)out + rows_wide * ldo * es;
         p.row_adapter = plan->row_adapter + rows_wide; p.M = p.rows_per_sample = M - rows_wide;
     }
     const int tl = c.kind == GEMV16 || c.kind == TILE_64x64 || c.kind == TILE_64x128 ? 0 : c.kind == TILE_128x128 || c.kind == TILE_128x192 ? 1 : 2;      // tile heights 64, 128, 256
@@ -880,8 +908,8 @@ BwdSpace bwd_space(m4d_dtype dt, const m4d_adapter_plan* plan, int64_t N, int64_
     BwdSpace b{};
     int64_t at = 0;
     b.wt = at; if (dx) at += up64((K * N + per - 1) / per);
-    b.v = at; if (dx) at += up64((plan->rows * R + per - 1) / per);
-    b.vt = at; if (da) at += up64((int64_t)plan->n_pieces * 4 * ((R + 31) / 32) * 512 * (dt == M4D_BF16 ? 2 : 1) / per);
+    b.v = at; if (dx) at += up64((plan->rows * R * u_parts(dt) + per - 1) / per);
+    b.vt = at; if (da) at += up64((int64_t)plan->n_pieces * 4 * ((R + 31) / 32) * 512 * u_parts(dt) / per);
     b.rest = at;
     int64_t most = 0;
     auto take = [&](int64_t n) { if (n > most) most = n; };

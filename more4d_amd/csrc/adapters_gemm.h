@@ -268,13 +268,18 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void adapter_gemv_kernel(AdGemmA
     for (int i = p.tile_off[0] + wave; i < p.tile_off[1]; i += SKINNY_WAVES) {      // (at most 16 rows: one tile)
         const int g = p.tile_list[i];
         const T* b = (const T*)p.up + ((int64_t)g * p.N + min(n0 + i16, p.N - 1)) * p.R;
-        const T* u = (const T*)p.u + (int64_t)row * p.R;
+        const T* u = (const T*)p.u + (int64_t)row * u_stride<T>(p.R);
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < p.R; k += 32) {
-            const int kq = k + q * 8, ks = min(kq, p.R - 8);
-            frag_t fb = *reinterpret_cast<const frag_t*>(b + ks), fu = *reinterpret_cast<const frag_t*>(u + ks);
-            if (kq >= p.R) fb = fu = frag_t{};
-            mma16(fb, fu, sum);
+            const int w = min(32, p.R - k), ks = min(q * 8, w - 8);
+            const frag_t zero = {};
+            frag_t fb = *reinterpret_cast<const frag_t*>(b + k + ks);
+            if (q * 8 >= w) fb = zero;
+#pragma unroll
+            for (int h = 0; h < Parts<T>::N; ++h) {
+                const frag_t fu = *reinterpret_cast<const frag_t*>(u + u_hi<T>(k) + h * w + ks);
+                mma16(fb, q * 8 >= w ? zero : fu, sum);
+            }
         }
         if (ra == g) acc += sum;                    // (see adapters_extend: rows of other adapters see nothing of this one)
     }

@@ -35,7 +35,7 @@ struct GemmArgs {
 // Shared projection with low-rank adapters (adapters.hip): behind the K loop a tile adds, for every adapter that one of its rows names,
 // the product of that adapter's rows of u (= s x A^T, other rows read as zero) with its B.
 struct GemmAdArgs : GemmArgs {
-    const void* u;              // T [M, R]
+    const void* u;              // T [M, u_stride(R)] (u_hi)
     const void* up;             // T [G, N, R]
     const int* row_adapter;     // [M], -1 = none
     const int* tile_off;        // [tiles_m + 1] into tile_list
@@ -43,6 +43,13 @@ struct GemmAdArgs : GemmArgs {
     const int* tile_one;        // [tiles_m] the adapter that ALL rows of the tile name, or -1 (wide kernel only)
     int R;                      // multiple of 16
 };
+
+// A row of u holds float32 ranks in one piece, bf16 as hi + lo of 16 bits (split2) in blocks of 32 ranks, the last may have 16: [hi | lo] of each.  One
+// rounding to bf16 here would put an error of up to 2^-8 of the adapter's part on an output that is itself rounded once; 32 ranks of both parts
+// are one 64-element K-tile of the 256 x 256 kernel.
+template <typename T> struct Parts { static constexpr int N = sizeof(T) == 2 ? 2 : 1; };
+template <typename T> M4D_DEV int u_stride(int R) { return R * Parts<T>::N; }
+template <typename T> M4D_DEV int u_hi(int r) { return Parts<T>::N == 2 ? 2 * (r & ~31) + (r & 31) : r; }      // lo: min(32, R - (r & ~31)) further
 
 constexpr int ROWB = 128;  // bytes of K per LDS row
 
@@ -225,7 +232,7 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
     if (a.i0 >= a.i1 || k0 >= p.R) return;
     const T* pu[MI];
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) pu[mi] = (const T*)p.u + (int64_t)a.row[mi] * p.R + hi * 8;
+    for (int mi = 0; mi < MI; ++mi) pu[mi] = (const T*)p.u + (int64_t)a.row[mi] * u_stride<T>(p.R) + hi * 8;
     int64_t nr[NI];                                   // (columns beyond N are computed from row N - 1 and not stored)
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) nr[ni] = min(n_base + ni * 32 + li, p.N - 1) * p.R + hi * 8;
@@ -237,14 +244,19 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
         if (!__any(mine)) continue;                   // none of this wave's rows
         const bool mixed = !__all(all);
         const T* b = (const T*)p.up + (int64_t)g * p.N * p.R;
-        // C steps of 16 ranks: all loads (without predicates: rows of other adapters are replaced after the load), then the products
+        // C steps of 16 ranks: all loads (without predicates: rows of other adapters are replaced after the load), then the products.  u's parts as they
+        // lie in a block of 32 ranks, in the order in which the 256 x 256 kernel's K loop takes them: a row that two of its tiles write (the last one
+        // is shifted inwards) has to get the same bits from both.
         auto chunk = [&](auto C_T, int k) {
-            constexpr int C = decltype(C_T)::value;
-            frag_t fu[C][MI], fb[C][NI];
+            constexpr int C = decltype(C_T)::value, NP = Parts<T>::N, W = C == 1 ? 16 : 32;      // (bf16: C = 1 is the last block of 16)
+            frag_t fu[C][NP][MI], fb[C][NI];
 #pragma unroll
             for (int s = 0; s < C; ++s) {
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi) fu[s][mi] = *reinterpret_cast<const frag_t*>(pu[mi] + k + s * 16);
+                for (int q = 0; q < NP; ++q)
+#pragma unroll
+                    for (int mi = 0; mi < MI; ++mi)
+                        fu[s][q][mi] = *reinterpret_cast<const frag_t*>(pu[mi] + (NP == 2 ? 2 * k + (s >> 1) * 64 + (s & 1) * 16 + q * W : k + s * 16));
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni) fb[s][ni] = *reinterpret_cast<const frag_t*>(b + nr[ni] + k + s * 16);
             }
@@ -253,8 +265,10 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
 #pragma unroll
                 for (int s = 0; s < C; ++s) {
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
-                        if (a.ra[mi] != g) fu[s][mi] = frag_t{};
+                    for (int q = 0; q < NP; ++q)
+#pragma unroll
+                        for (int mi = 0; mi < MI; ++mi)
+                            if (a.ra[mi] != g) fu[s][q][mi] = frag_t{};
 #pragma unroll
                     for (int ni = 0; ni < NI; ++ni) top = max(top, frag_top(fb[s][ni]));
                 }
@@ -269,7 +283,7 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
                                     f32x16 sum;
 #pragma unroll
                                     for (int q = 0; q < 16; ++q) sum[q] = 0.f;
-                                    mma32(fb[s][ni], fu[s][mi], sum);
+                                    mma32(fb[s][ni], fu[s][0][mi], sum);
 #pragma unroll
                                     for (int q = 0; q < 16; ++q) acc[ni][mi][q] += a.ra[mi] == g ? sum[q] : 0.f;
                                     __builtin_amdgcn_sched_barrier(0);
@@ -280,7 +294,7 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
                                 bad_parts(fb[s][ni], inf, nan);
 #pragma unroll
                                 for (int mi = 0; mi < MI; ++mi) {
-                                    const frag_t us = big_signs(fu[s][mi]);
+                                    const frag_t us = big_signs(fu[s][0][mi]);
                                     mma32(inf, us, acc[ni][mi]);
                                     mma32(nan, us, acc[ni][mi]);
                                 }
@@ -289,12 +303,15 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
                 }
             }
 #pragma unroll
-            for (int s = 0; s < C; ++s) {
+            for (int s2 = 0; s2 < C; s2 += 2)
 #pragma unroll
-                for (int ni = 0; ni < NI; ++ni)
+                for (int q = 0; q < NP; ++q)
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi) mma32(fb[s][ni], fu[s][mi], acc[ni][mi]);
-            }
+                    for (int s = s2; s < s2 + 2 && s < C; ++s)
+#pragma unroll
+                        for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                            for (int mi = 0; mi < MI; ++mi) mma32(fb[s][ni], fu[s][q][mi], acc[ni][mi]);
         };
         int k = k0;
         for (; k + 16 * U <= p.R; k += 16 * U) chunk(std::integral_constant<int, U>{}, k);

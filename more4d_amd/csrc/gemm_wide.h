@@ -325,29 +325,31 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
     if constexpr (!(ABL & 1)) asm volatile("s_add_u32 m0, %0, %3\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(ldsw), "v"(VOFF), "s"(SRC), "i"(DSTOFF) : "memory", "m0", "scc")
     // instruction I (0..3) of the group (operand rows R, half H, group offset G) for the K-tile buffer BUFB (0 / W_BUF)
 #define W_STG_I(R, VOFF, H, G, BUFB, I) W_GLDS(VOFF, R[((I) >> 1) * 4 + (H) * 2 + ((I) & 1)], (BUFB) + (G) + (I) * 4096)
-    // AD: a tile whose rows all name one adapter (p.tile_one) appends whole 64-rank K-tiles of u and up_g to its K loop: a group whose staging
-    // reaches K-tile nk goes over to their rows.  (Behind the loop, with the pipe empty, the same ranks cost two to three times as much.)
+    // AD: a tile whose rows all name one adapter (p.tile_one) appends the ranks to its K loop, 32 of them a K-tile: u's block of 32 ranks is 64
+    // elements, hi and lo, and up_g's 32 are staged twice beside it (chunk c & 3).  A group whose staging reaches K-tile nk goes over to these
+    // rows.  (Behind the loop, with the pipe empty, the same ranks cost two to three times as much.)
     int nkt = nk, ad_one = -1;
     const char *ad_u = nullptr, *ad_b = nullptr;
-    unsigned ad_off = 0;
+    unsigned ad_ou = 0, ad_ob = 0;
     if constexpr (AD) {
         ad_one = __builtin_amdgcn_readfirstlane(p.tile_one[tm]);
         if (ad_one >= 0) {
-            nkt = nk + (p.R >> 6);
-            ad_u = uniform_ptr((const char*)p.u + m0 * p.R * 2);
+            nkt = nk + (p.R >> 5);
+            ad_u = uniform_ptr((const char*)p.u + m0 * u_stride<T>(p.R) * 2);
             ad_b = uniform_ptr((const char*)p.up + ((int64_t)ad_one * p.N + n0) * p.R * 2);
-            const int u = wave * 8 + lrow;
-            ad_off = (unsigned)((u * p.R + (pc ^ ((u >> 1) & 7)) * 8) * 2);
+            const int u = wave * 8 + lrow, c = pc ^ ((u >> 1) & 7);
+            ad_ou = (unsigned)((u * u_stride<T>(p.R) + c * 8) * 2);
+            ad_ob = (unsigned)((u * p.R + (c & 3) * 8) * 2);
         }
     }
-    auto ad_switch = [&](const char* (&r)[8], const char* base, int h, unsigned& voff) {
+    auto ad_switch = [&](const char* (&r)[8], bool is_u, int h, unsigned& voff) {
         if constexpr (AD) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int jx = (i >> 1) * 4 + h * 2 + (i & 1), row = (jx >> 2) * 128 + ((jx >> 1) & 1) * 64 + (jx & 1) * 32;
-                r[jx] = uniform_ptr(base + (int64_t)row * p.R * 2);
+                r[jx] = uniform_ptr((is_u ? ad_u : ad_b) + (int64_t)row * (is_u ? u_stride<T>(p.R) : p.R) * 2);
             }
-            voff = ad_off;
+            voff = is_u ? ad_ou : ad_ob;
         }
     };
     constexpr bool W_TAIL = true;      // (AD: false in the part of the K loop that stages nothing at or beyond K-tile nk)
@@ -357,8 +359,8 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
         if constexpr (PERSIST) { const bool wrap_ = KC == nk; VOFF += wrap_ ? DLT : 128u; KC = wrap_ ? 0 : KC; }  \
         else if constexpr (AD && !W_TAIL) VOFF += 128u;                                                      \
         else if constexpr (AD) {                                                                             \
-            if (KC == nk && nkt > nk) ad_switch(R, &R == &ra ? ad_u : ad_b, H, VOFF);                         \
-            else VOFF += (KC < nkt) ? 128u : 0u;                                                             \
+            if (KC == nk && nkt > nk) ad_switch(R, &R == &ra, H, VOFF);                                       \
+            else VOFF += KC < nkt ? (KC > nk && &R != &ra ? 64u : 128u) : 0u;                                \
         } else VOFF += (KC < nk) ? 128u : 0u;                                                                \
     } while (0)
     f32x16 acc[4][4];   // [ni][mi]: rows n, column m = lane (W is the MFMA's A operand, see gemm.hip)
@@ -603,7 +605,7 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
             for (int h = 0; h < 2; ++h) asm volatile("" :: "v"(fa0[h][kk]), "v"(fa1[h][kk]), "v"(fbx[h][kk]), "v"(fby[h][kk]));
-        adapters_extend<T, 4, 4>(p, acc, ad_tile, n0 + wn * 128, lane, 1, (nkt - nk) * 64);      // (its loads fly with the last stagings)
+        adapters_extend<T, 4, 4>(p, acc, ad_tile, n0 + wn * 128, lane, 1, (nkt - nk) * 32);      // (its loads fly with the last stagings)
     }
     if constexpr (ABL & 64) ts[2] = __builtin_readcyclecounter();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the redundant tail stagings must land before the LDS is re-used

@@ -1423,7 +1423,7 @@ def linear_adapters(x, w, bias, bank, plan, *, out=None, slots=False, keep8=Fals
     dt, ldw = dt_code(dtype), _rows_of(w, K)[1]
     ldo = _rows_of(out, N)[1]
     lib = _lib.load()
-    u = torch.empty((M, R), device=device, dtype=dtype)
+    u = torch.empty((M, R * (2 if dtype == torch.bfloat16 else 1)), device=device, dtype=dtype)
     ws, nws = _workspace(plan, ("linear", d, dt, N, K, R, slots), device, lib.m4d_linear_adapters_workspace, dt, plan.args, N, K, R, int(slots))
     codes, exps = x8._ptrs() if keep8 else (0, 0)
     _launch("m4d_linear_adapters", d, lib.m4d_linear_adapters, dt, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(bias), bank._down, bank.scale.data_ptr(),
