@@ -164,9 +164,9 @@ M4D_DEV void epilogue_tile(const GemmArgs& p, const f32x16& acc, int64_t m, int6
 // barriers.  All loads of 64 ranks (32 with 256 accumulators) are issued before their first product, so a tile pays one L2
 // latency for them and adapter, not four (two).
 // Rows of u that name another adapter (or none: their u was never written) are replaced by zero before the product, not multiplied by zero; and
-// where a wave's rows do not all name the adapter, an infinity or NaN in its B must not meet those zeros: float32 then takes sums of their own that
-// only the adapter's rows add, bf16 bad_parts (a VALU instruction on its accumulators takes them out of the AGPRs: 200 spilled registers in the
-// 256 x 256 kernel).
+// where a wave's rows do not all name the adapter, an infinity or NaN in its B must not meet those zeros, nor be left out where a row's own u is
+// zero or infinite.  float32 then forms the products apart and adds them in the adapter's rows only; bf16 adds what is not finite by add_bad (a VALU
+// instruction on its accumulators takes them out of the AGPRs: 200 spilled registers in the 256 x 256 kernel).
 // AdTile: what the extension has to know about its tile, loaded in front of the K loop (behind it these would be three dependent trips to L2).
 // order (or nullptr): the row behind each row of the tiles.
 template <int MI> struct AdTile { int i0, i1, g0; int ra[MI], row[MI]; };
@@ -199,27 +199,44 @@ M4D_DEV unsigned frag_top(const f32x8& f) {
     for (int e = 0; e < 8; ++e) m = max(m, __builtin_bit_cast(unsigned, f[e]) & 0x7fffffffu);
     return m;
 }
-// A fragment of B that is not finite as a sum of three: b keeps the finite values, `inf` has +-big for every other, `nan` the opposite for NaNs.  u's
-// fragment becomes +-big as well, zero in rows of other adapters (big_signs): big * big overflows to the infinity that the adapter's own rows
-// have to get, inf - inf is the NaN, and the others get 0 * big = 0.  (bf16 only: float32's MFMA does not round the product, inf - big * big is inf.)
-M4D_DEV void bad_parts(bf16x8& b, bf16x8& inf, bf16x8& nan) {
-    const float big = 3.3e38f;
+// bf16, 16 ranks of a block: what an infinity or NaN in B adds to the columns of acc that are its adapter's, as products of +-3.3e38 with +-3.3e38
+// (they overflow to the infinity that is wanted; zeros everywhere else), those of one sign together.  u: the part that has its sign.
+//   b = +-inf, u not 0: sign(b) sign(u) inf;   b = +-inf, u = 0, or b = NaN: inf, then -inf;   (u = NaN: the product itself)
+template <int MI>
+M4D_DEV void add_bad(const bf16x8& b, const bf16x8 (&u)[MI], const bool (&own)[MI], f32x16 (&acc)[MI]) {
+    const bf16_t big = (bf16_t)3.3e38f, none = (bf16_t)0.f;
+    auto pick = [&](const bf16x8& f, bf16_t v, auto which) {
+        bf16x8 r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = which((float)f[e]) ? v : none;
+        return r;
+    };
+    const float inf = __builtin_inff();
+    const bf16x8 bp = pick(b, big, [&](float v) { return v == inf; }), bm = pick(b, -big, [&](float v) { return v == -inf; });
+    const bf16x8 bi = pick(b, big, [&](float v) { return fabsf(v) == inf; }), bn = pick(b, big, [&](float v) { return v != v; });
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+        const bool o = own[mi];
+        const bf16x8 up = pick(u[mi], big, [&](float v) { return o && v > 0.f; }), um = pick(u[mi], -big, [&](float v) { return o && v < 0.f; });
+        mma32(bp, up, acc[mi]);
+        mma32(bm, um, acc[mi]);
+        mma32(bp, um, acc[mi]);
+        mma32(bm, up, acc[mi]);
+#pragma unroll
+        for (int sign = 0; sign < 2; ++sign) {
+            mma32(bi, pick(u[mi], sign ? -big : big, [&](float v) { return o && v == 0.f; }), acc[mi]);
+            mma32(bn, pick(u[mi], sign ? -big : big, [&](float) { return o; }), acc[mi]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// B's fragment for the product itself: 1 with its sign in the place of an infinity (an infinite u is to meet no zero there), 1 of a NaN
+M4D_DEV bf16x8 without_bad(const bf16x8& b) {
+    bf16x8 r = b;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float v = (float)b[e];
-        const unsigned u = __builtin_bit_cast(unsigned, v), m = u & 0x7fffffffu;
-        const float s = m >= 0x7f800000u ? (u >> 31 ? -big : big) : 0.f;
-        inf[e] = (bf16_t)s;
-        nan[e] = (bf16_t)(m > 0x7f800000u ? -s : 0.f);
-        b[e] = (bf16_t)(m >= 0x7f800000u ? 0.f : v);
-    }
-}
-M4D_DEV bf16x8 big_signs(const bf16x8& u) {
-    bf16x8 r;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float v = (float)u[e];
-        r[e] = (bf16_t)(v > 0.f ? 3.3e38f : v < 0.f ? -3.3e38f : 0.f);
+        if (!(fabsf(v) < __builtin_inff())) r[e] = (bf16_t)(v < 0.f ? -1.f : 1.f);
     }
     return r;
 }
@@ -250,15 +267,16 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
         auto chunk = [&](auto C_T, int k) {
             constexpr int C = decltype(C_T)::value, NP = Parts<T>::N, W = C == 1 ? 16 : 32;      // (bf16: C = 1 is the last block of 16)
             frag_t fu[C][NP][MI], fb[C][NI];
+            auto load_u = [&](int s, int q, int mi) { return *reinterpret_cast<const frag_t*>(pu[mi] + (NP == 2 ? 2 * k + (s >> 1) * 64 + (s & 1) * 16 + q * W : k + s * 16)); };
+            auto load_b = [&](int s, int ni) { return *reinterpret_cast<const frag_t*>(b + nr[ni] + k + s * 16); };
 #pragma unroll
             for (int s = 0; s < C; ++s) {
 #pragma unroll
                 for (int q = 0; q < NP; ++q)
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
-                        fu[s][q][mi] = *reinterpret_cast<const frag_t*>(pu[mi] + (NP == 2 ? 2 * k + (s >> 1) * 64 + (s & 1) * 16 + q * W : k + s * 16));
+                    for (int mi = 0; mi < MI; ++mi) fu[s][q][mi] = load_u(s, q, mi);
 #pragma unroll
-                for (int ni = 0; ni < NI; ++ni) fb[s][ni] = *reinterpret_cast<const frag_t*>(b + nr[ni] + k + s * 16);
+                for (int ni = 0; ni < NI; ++ni) fb[s][ni] = load_b(s, ni);
             }
             if (mixed) {
                 unsigned top = 0;
@@ -273,33 +291,45 @@ M4D_DEV void adapters_extend(const GemmAdArgs& p, f32x16 (&acc)[NI][MI], const A
                     for (int ni = 0; ni < NI; ++ni) top = max(top, frag_top(fb[s][ni]));
                 }
                 if (__any(top >= 0x7f800000u)) {
+                    if constexpr (sizeof(T) == 2) {
+                        bool own[MI];
 #pragma unroll
-                    for (int s = 0; s < C; ++s)
+                        for (int mi = 0; mi < MI; ++mi) own[mi] = a.ra[mi] == g;
+#pragma unroll 1
+                        for (int s = 0; s < C; ++s) {      // (rolled up and from memory again: it must not add to the registers of the rest)
+                            frag_t us[MI];
+#pragma unroll
+                            for (int mi = 0; mi < MI; ++mi) us[mi] = load_u(s, 0, mi);
+#pragma unroll
+                            for (int ni = 0; ni < NI; ++ni) add_bad<MI>(load_b(s, ni), us, own, acc[ni]);
+                        }
+#pragma unroll
+                        for (int s = 0; s < C; ++s) {
+#pragma unroll
+                            for (int q = 0; q < NP; ++q)
+#pragma unroll
+                                for (int mi = 0; mi < MI; ++mi) fu[s][q][mi] = own[mi] ? load_u(s, q, mi) : frag_t{};
+#pragma unroll
+                            for (int ni = 0; ni < NI; ++ni) fb[s][ni] = without_bad(load_b(s, ni));
+                        }
+                    } else {
 #pragma unroll
                         for (int ni = 0; ni < NI; ++ni) {
-                            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                                for (int mi = 0; mi < MI; ++mi) {
-                                    f32x16 sum;
+                            for (int mi = 0; mi < MI; ++mi) {
+                                f32x16 sum;
 #pragma unroll
-                                    for (int q = 0; q < 16; ++q) sum[q] = 0.f;
-                                    mma32(fb[s][ni], fu[s][0][mi], sum);
+                                for (int q = 0; q < 16; ++q) sum[q] = 0.f;
+                                mma32(fb[0][ni], fu[0][0][mi], sum);
 #pragma unroll
-                                    for (int q = 0; q < 16; ++q) acc[ni][mi][q] += a.ra[mi] == g ? sum[q] : 0.f;
-                                    __builtin_amdgcn_sched_barrier(0);
-                                }
-                                fb[s][ni] = frag_t{};
-                            } else {
-                                frag_t inf, nan;
-                                bad_parts(fb[s][ni], inf, nan);
-#pragma unroll
-                                for (int mi = 0; mi < MI; ++mi) {
-                                    const frag_t us = big_signs(fu[s][0][mi]);
-                                    mma32(inf, us, acc[ni][mi]);
-                                    mma32(nan, us, acc[ni][mi]);
-                                }
+                                for (int q = 0; q < 16; ++q) acc[ni][mi][q] += a.ra[mi] == g ? sum[q] : 0.f;
+                                __builtin_amdgcn_sched_barrier(0);
                             }
+                            fb[0][ni] = frag_t{};
                         }
+#pragma unroll
+                        for (int mi = 0; mi < MI; ++mi) fu[0][0][mi] = frag_t{};
+                    }
                 }
             }
 #pragma unroll
