@@ -461,15 +461,32 @@ __global__ __launch_bounds__(256, 2) void adapter_grad_kernel(GradArgs p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) b.x[j][e] = (T)decode1((unsigned)b.code[j], e, step_of(b.ex[j]));      // exact in T
         }
+        // two parts of v have signs of their own: an infinity of x meets the first one only (inf - inf would be NaN where v inf is an infinity)
+        bool bad = false;
+        if constexpr (NP == 2 && !CODES) {
+            unsigned top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const u32x2 w = __builtin_bit_cast(u32x2, b.x[j]);
+                const unsigned d[2] = {w[0], w[1]};
+                top = max(top, top_bits<T>(d));
+            }
+            bad = __any(top >= 0x7f800000u);
+        }
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             frag_t fx;
 #pragma unroll
             for (int j = 0; j < 8; ++j) fx[j] = b.x[j][f];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+            for (int q = 0; q < NP; ++q) {
+                if (q == 1 && bad)
 #pragma unroll
-                for (int q = 0; q < NP; ++q) mma32(b.v[rt][q], fx, acc[rt][f]);
+                    for (int j = 0; j < 8; ++j)
+                        if (!isfinite((float)fx[j])) fx[j] = (T)0.f;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) mma32(b.v[rt][q], fx, acc[rt][f]);
+            }
         }
     };
     // (n is whole pieces: every wave has n / 64 steps.  Requests beyond the end repeat the last step's rows: a branch around them would make the

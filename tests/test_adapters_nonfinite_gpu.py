@@ -42,3 +42,31 @@ def test_rows_without_and_beyond_all_bounds_meet_an_adapter_that_is_not_finite(d
     assert same[special].all(), (special & ~same).nonzero()[:8].tolist()
     ok = ((y - want).abs() <= tol)[~special]
     assert ok.all(), int((~ok).sum())
+
+
+def test_an_infinite_input_gives_infinite_gradients():
+    """dA of an adapter whose kept input holds an infinity, dB where dy holds one: v inf is an infinity, not the NaN of two parts of different signs."""
+    o = ops()
+    lengths, ids = [100, 1, 60], [1, -1, 0]
+    for dt in (BF, F32):
+        x, w, _, a, b, scale, _ = (t.to(DEV) if isinstance(t, torch.Tensor) else t for t in problem(lengths, ids, 64, 72, 6, dt))
+        plan = o.AdapterPlan(lengths, ids, DEV)
+        bank = o.AdapterBank(a, b, scale, backward=True)
+        dy = torch.randn(161, 72, generator=torch.Generator().manual_seed(4)).to(dt).to(DEV)
+        _, ut = o.linear_adapters(x, w, None, bank, plan, slots=True)
+        x[3, 5], dy[130, 9], dy[40, 2] = INF, -INF, NAN
+        _, da, db = o.linear_adapters_bwd(dy, w, bank, plan, x=x, ut=ut)
+        u = scale[0] * (x[101:].double() @ a[0].double().t())
+        # row 3's v is finite and not zero: +-inf in channel 5 of its adapter's dA; row 130's and row 40's v are not finite: all of their dA
+        v = scale[1] * (dy[:100].double() @ b[1].double())
+        assert torch.isnan(v[40]).all() and torch.isnan(da[1]).all() and not torch.isfinite(da[0]).any()
+        assert torch.equal(db[0, 9], -torch.sign(u[29]).to(dt) * INF) and torch.isnan(db[1, 2]).all()
+        ok = torch.ones(2, 72, dtype=torch.bool, device=DEV)
+        ok[0, 9] = ok[1, 2] = False
+        assert torch.isfinite(db[ok]).all()
+        dy[40, 2] = 0.5
+        _, da, _ = o.linear_adapters_bwd(dy, w, bank, plan, x=x, ut=ut)
+        v3 = scale[1] * (dy[3].double() @ b[1].double())
+        assert torch.equal(da[1, :, 5], torch.sign(v3).to(dt) * INF)
+        da[1, :, 5] = 0
+        assert torch.isfinite(da[1]).all()
