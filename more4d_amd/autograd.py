@@ -283,6 +283,10 @@ def _block_param_names(blk):
 
 STORE_KEYS = ("qkv_pre", "o", "lse1", "y1", "qc_pre", "yc", "pre", "y2")
 STORE_LITE = ("o", "lse1", "y2")     # best recompute time saved per stored byte: self-attention output + ffn_down output
+# kept as they are with bits = 8 as well (qkv_pre: or not at all): the attention backward's P = exp(S - lse1) and delta = rowsum(dO o) are a softmax's
+# gradient only if lse1 and o are those of the q, k, v at hand (rounded apart, rows of P do not sum to 1 and those of dS not to 0: at scores of
+# standard deviation 4 dV is off by 5 - 17 % instead of 3 %), and to have them of rounded q, k, v would be the whole attention again
+STORE_EXACT = ("qkv_pre", "o", "lse1")
 
 
 def _guidance_site_bwd(x, dz, shift, scale, st, Lp, eps, g, mod, gfeat2, G, prefix, mod_rows=0):
@@ -533,9 +537,9 @@ class BlockFn(Function):
     2.4 GB per block at L = 21 840, C = 5120) and the backward skips their recompute: fwd + bwd instead of fwd +
     recompute + bwd.  store=1 keeps only STORE_LITE (0.45 GB per block: the self-attention and ffn_down outputs, the
     best recompute time per byte).  `WanTransformer4DModel.activation_budget_gb` decides how many blocks get which.
-    bits=8 (`WanTransformer4DModel.activation_bits`) keeps what is stored in 8 bits (ops.act_quant8; the log-sum-exp stays float32): half the
-    bytes of bf16, so twice the blocks in the same budget; the block's output and its loss are those of bits=16, the gradients come from
-    the rounded activations."""
+    bits=8 (`WanTransformer4DModel.activation_bits`) keeps what is stored in 8 bits (ops.act_quant8), but for what the self-attention's backward
+    works on (STORE_EXACT); store=2 then recomputes q, k, v, which save the least time per byte now (1.0 GB per block instead of 2.4), store=3 keeps
+    them too (1.7 GB).  The block's output and its loss are those of bits=16, the gradients come from the rounded activations."""
 
     @staticmethod
     def forward(ctx, x, e0, txt, img, gfeat, blk, c, txt_len, img_len, store, gmeta, *params):
@@ -545,14 +549,16 @@ class BlockFn(Function):
         stash = None
         store, bits = store if isinstance(store, tuple) else (store, 16)
         guid = (gfeat.detach(), gmeta[0], gmeta[1]) if gfeat is not None else None
-        if store:   # 2: every GEMM / attention output, 1: STORE_LITE only
+        if store:   # 2 (8 bits: 3): every GEMM / attention output, 1: STORE_LITE only
             out, stash = block_backward(blk, x.detach(), e0.detach().contiguous(), c, txt.detach(), txt_len,
                                         img.detach() if img is not None else None, img_len, None, forward_only=True,
                                         guid=guid)
             if store == 1:
                 stash = {k: stash[k] for k in STORE_LITE}
+            if bits == 8 and store == 2:
+                del stash["qkv_pre"]
             if bits == 8:
-                stash = {k: t if k == "lse1" else ops.act_quant8(t) for k, t in stash.items()}
+                stash = {k: t if k in STORE_EXACT else ops.act_quant8(t) for k, t in stash.items()}
         elif blk.ffn[0].weight.dtype == torch.bfloat16 and not _folds_qscale(blk):
             # bf16 without the folded softmax scale (qk_norm=False, or M4D_FOLD_QSCALE=0): blk.run's self-attention would take attn128q_kernel,
             # which rounds Q * c to bf16 once more, while the backward's recompute (log-sum-exp requested) runs on attn128p_kernel — the loss

@@ -697,8 +697,9 @@ class WanTransformer4DModel(nn.Module):
         # training: GB of HBM the forward may spend on stored activations (None = whatever is free minus the head-room
         # below; 0 = plain per-block gradient checkpointing like the reference)
         self.activation_budget_gb = None
-        # 16: stored activations are kept as they are; 8: in 8 bits with a power-of-two step per 32 channels (ops.act_quant8) — about twice the
-        # blocks fit the budget; the forward's results do not change, the gradients see the rounded activations
+        # 16: stored activations are kept as they are; 8: in 8 bits with a power-of-two step per 32 channels (ops.act_quant8), but for the
+        # self-attention's output and q, k, v (kept as they are, the latter last) — about twice the blocks fit the budget; the forward's results do
+        # not change, the gradients see the rounded activations
         self.activation_bits = 16
         self.activation_headroom_gb = 95.0     # backward workspace + allocator slack (measured: beyond ~230 GB live the step time gets erratic)
         self.last_stored_blocks = 0
@@ -1062,10 +1063,10 @@ class WanTransformer4DModel(nn.Module):
         es = xres.new_empty(0, dtype=T).element_size()
         if self.activation_bits not in (8, 16):
             raise ValueError(f"activation_bits must be 8 or 16, got {self.activation_bits}")
-        if self.activation_bits == 8:
-            es = 33 / 32                # a byte per channel and one per block of 32
-        lite = B * Lp * 2 * C * es + B * self.num_heads * Lp * 4
-        full = B * Lp * (8 * C + self.ffn_dim) * es + B * self.num_heads * Lp * 4
+        # (8 bits: a byte per channel and one per block of 32; the attention's output stays as it is, and q, k, v come last: autograd.STORE_EXACT)
+        es8, qkv = (33 / 32, B * Lp * 3 * C * es) if self.activation_bits == 8 else (es, 0)
+        lite = B * Lp * C * (es + es8) + B * self.num_heads * Lp * 4
+        full = B * Lp * (C * es + ((4 if qkv else 7) * C + self.ffn_dim) * es8) + B * self.num_heads * Lp * 4
         budget = self.activation_budget_gb
         if budget is None:
             if dev.type == "cuda":
@@ -1077,6 +1078,7 @@ class WanTransformer4DModel(nn.Module):
         nb = len(self.blocks)
         n_lite = int(min(nb, budget // max(lite, 1)))
         n_full = int(min(n_lite, max(0.0, budget - n_lite * lite) // max(full - lite, 1))) if n_lite == nb else 0
+        n_qkv = int(min(nb, (budget - nb * full) // qkv)) if qkv and n_full == nb else 0
         self.last_stored_blocks = n_lite
         self.last_full_blocks = n_full
         # ---- spatial guidance (:1126-1156): SiLU'd [B, h*w, 768] table shared by every block, T-periodic over the tokens
@@ -1091,7 +1093,7 @@ class WanTransformer4DModel(nn.Module):
                 gfeat, period, glen = self._guidance_tables(first_frame_features, (h, w), x.shape[2] // pt)
                 gmeta = (period, glen)
         for i, blk in enumerate(self.blocks):
-            store = 2 if i < n_full else (1 if i < n_lite else 0)
+            store = 3 if i < n_qkv else 2 if i < n_full else (1 if i < n_lite else 0)
             xres = BlockFn.apply(xres, e0, ctx_txt, ctx_img, gfeat, blk, c, self.text_len, img_len, (store, self.activation_bits),
                                  gmeta, *blk.parameters())
         # ---- head (:708-721) + unpatchify (:1343-1366)
