@@ -312,12 +312,14 @@ def block_backward(blk, x0, e0, c, txt, txt_len, img, img_len, dres, saved=None,
     `saved` (STORE_KEYS -> tensor): outputs of the six big GEMMs and of the self-attention that the forward kept in
     HBM ("stored" blocks, see BlockFn); they are used instead of being recomputed — only the HBM-bound LayerNorm /
     RMSNorm / GELU passes and the small cross-attention run again.  An entry may be an ops.Act8 (8-bit form, half the memory of bf16):
-    the GELU input is then read as codes by the two passes that use it, the others are expanded when they are needed.  forward_only=True runs just the forward half and
+    the GELU input is then read as codes by the two passes that use it, the others are expanded when they are needed.  `saved` is emptied: each
+    entry is let go of where it is used.  forward_only=True runs just the forward half and
     returns (x3, {STORE_KEYS}) — the same code path produces the stored tensors, so both modes are bit-identical."""
-    saved = dict(saved) if saved else {}
+    if saved is None:
+        saved = {}
 
     def take(key):
-        """the stored tensor (None: recompute), expanded from its 8-bit form; the stash lets go of it"""
+        """the stored tensor (None: recompute), expanded from its 8-bit form"""
         t = saved.pop(key, None)
         return ops.act_dequant8(t) if isinstance(t, ops.Act8) else t
 
@@ -539,7 +541,8 @@ class BlockFn(Function):
     best recompute time per byte).  `WanTransformer4DModel.activation_budget_gb` decides how many blocks get which.
     bits=8 (`WanTransformer4DModel.activation_bits`) keeps what is stored in 8 bits (ops.act_quant8), but for what the self-attention's backward
     works on (STORE_EXACT); store=2 then recomputes q, k, v, which save the least time per byte now (1.0 GB per block instead of 2.4), store=3 keeps
-    them too (1.7 GB).  The block's output and its loss are those of bits=16, the gradients come from the rounded activations."""
+    them too (1.7 GB).  The block's output and its loss are those of bits=16, the gradients come from the rounded activations.  (The backward empties
+    the stash; a second one over a retained graph recomputes everything, without roundings.)"""
 
     @staticmethod
     def forward(ctx, x, e0, txt, img, gfeat, blk, c, txt_len, img_len, store, gmeta, *params):

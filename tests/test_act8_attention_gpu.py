@@ -73,3 +73,38 @@ def test_gradients_at_large_logits(dtype):
     off = {n: float((got[1][n].double() - b.double()).norm() / (b.double().norm() + 1e-12)) for n, b in ref[1].items()}
     bad = {n: (v, own[n]) for n, v in off.items() if v > 0.08 + 2 * own[n]}
     assert not bad, bad
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_the_backward_lets_go_of_what_it_has_used(bits, monkeypatch):
+    """By the time a block's backward has come to its self-attention, the codes of that block are gone, and with 16 bits the tensors of its feed-forward."""
+    import weakref
+    from more4d_amd import autograd, ops
+    m, kw = _tiny(torch.bfloat16)
+    m.activation_budget_gb, m.activation_bits = 1e6, bits
+    kept, alive, real, quant = [], [], ops.attention_bwd, ops.act_quant8
+    forward = autograd.block_backward
+
+    def forward_half(*a, **k):
+        out = forward(*a, **k)
+        if k.get("forward_only") and bits == 16:
+            kept.append([weakref.ref(out[1][n]) for n in ("pre", "y2")])
+        elif k.get("forward_only"):
+            kept.append([])
+        return out
+
+    def quantized(t):
+        a8 = quant(t)
+        kept[-1].append(weakref.ref(a8.buf))
+        return a8
+
+    def spy(q, k, *a, Lq, Lk_rows, **kws):
+        if Lq == Lk_rows:
+            alive.append(sum(r() is not None for r in kept.pop()))
+        return real(q, k, *a, Lq=Lq, Lk_rows=Lk_rows, **kws)
+
+    monkeypatch.setattr(autograd, "block_backward", forward_half)
+    monkeypatch.setattr(ops, "act_quant8", quantized)
+    monkeypatch.setattr(ops, "attention_bwd", spy)
+    _grads(m, kw)
+    assert len(alive) == len(m.blocks) and not any(alive), alive
