@@ -1438,6 +1438,8 @@ def adapter_grad(vt, x, plan, bank, *, transposed=False):
     x8 = isinstance(x, Act8)
     if plan.n_adapters > G:
         raise ValueError(f"adapter_grad: the plan names adapter {plan.n_adapters - 1}, the bank has {G}")
+    if vt.dtype != bank.buf.dtype:
+        raise TypeError(f"adapter_grad: vt {vt.dtype} vs adapters {bank.buf.dtype}")
     if vt.shape != _slots_shape(bank, plan) or not vt.is_contiguous():
         raise ValueError("adapter_grad: vt must be adapter_down's slots")
     rows, ldx = (x.rows, 0) if x8 else _rows_of(x, C)

@@ -119,3 +119,14 @@ def test_adapter_numbers_have_a_limit():
     a, b = torch.empty(1).expand(65536, 1, 1), torch.empty(1).expand(65536, 1, 1)
     with pytest.raises(ValueError):
         ops.AdapterBank(a, b, [1.0] * 65536)
+
+
+def test_slots_of_another_type_than_the_bank_are_refused():
+    """bfloat16 slots hold two parts per value, float32 slots one: read as the other type they would end before the kernel does."""
+    bank = ops.AdapterBank.__new__(ops.AdapterBank)
+    plan = ops.AdapterPlan([3], [0], "cpu")
+    bank.G, bank.rank, bank.R = 1, 4, 16
+    for own, other in ((torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)):
+        bank.buf = torch.empty(0, dtype=own)
+        with pytest.raises(TypeError):
+            ops.adapter_grad(torch.zeros(ops._slots_shape(bank, plan), dtype=other), torch.zeros(3, 64, dtype=other), plan, bank)
