@@ -352,3 +352,21 @@ def test_rows_far_apart():
     assert o.launch_counts()["gemm_wide"] == 1
     del far
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("rows,K,per", [(300, 8960, 9), (1600, 8192, 13), (21800, 5120, 27)])
+def test_codes_of_slices_that_begin_on_odd_chunks(rows, K, per, dt):
+    """Slices of K of an odd number of 64-channel chunks: the exponents of a row, two bytes a chunk, meet in one dword from two workgroups."""
+    from more4d_amd import _lib
+    o = ops()
+    x, w, bias, a, b, scale, _ = on_gpu(*problem([rows], [0], K, 64, 16, dt))
+    x *= torch.exp(3 * torch.randn(1, K, generator=torch.Generator().manual_seed(4))).to(dt).to(DEV)
+    x[5, 3], x[rows - 1, K - 1] = float("inf"), float("nan")
+    plan, bank = o.AdapterPlan([rows], [0], DEV), o.AdapterBank(a, b, scale)
+    slices = _lib.load().m4d_adapter_down_workspace(plan.args, K, bank.R, 1) // (plan.n_pieces * 32 * 64)
+    assert -(-(K // 64) // slices) == per and per % 2 == 1
+    _, ut, x8 = o.linear_adapters(x, w, bias, bank, plan, keep8=True)
+    ref = o.act_quant8(x)
+    assert torch.equal(x8.codes, ref.codes) and torch.equal(x8.exps, ref.exps)
+    assert torch.equal(ut.nan_to_num(0), o.adapter_down(x, bank, plan, slots=True)[1].nan_to_num(0))
