@@ -11,6 +11,7 @@ remaining backward.
 """
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .ops import (ACT_GELU_TANH, EPI_STORE, EPI_STORE_F32, KV)
@@ -111,6 +112,7 @@ class AdapterLinearFn(Function):
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
+    @once_differentiable        # (its gradients leave no graph: a second derivative raises)
     def backward(ctx, dy):
         kept, weight, ut, _ = ctx.saved_tensors
         bank, plan, bits, xshape, xdt = ctx.meta

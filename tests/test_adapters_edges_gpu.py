@@ -354,6 +354,19 @@ def test_rows_far_apart():
     torch.cuda.empty_cache()
 
 
+def test_a_second_derivative_is_refused():
+    """The backward's kernels leave no graph: a gradient of a gradient raises, it does not come out without their part."""
+    from more4d_amd.autograd import AdapterLinearFn
+    o = ops()
+    lengths, ids = [30, 3, 40], [1, -1, 0]
+    x, w, bias, a, b, scale, _ = on_gpu(*problem(lengths, ids, 64, 72, 4, BF))
+    x = x.requires_grad_(True)
+    y = AdapterLinearFn.apply(x, w, bias, a.requires_grad_(True), b, scale, o.AdapterPlan(lengths, ids, DEV), 16)
+    (dx,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|differentiat"):
+        (dx.float().square().sum() + x.float().square().sum()).backward()
+
+
 @pytest.mark.parametrize("dt", [BF, F32])
 @pytest.mark.parametrize("rows,K,per", [(300, 8960, 9), (1600, 8192, 13), (21800, 5120, 27)])
 def test_codes_of_slices_that_begin_on_odd_chunks(rows, K, per, dt):
