@@ -1094,8 +1094,8 @@ class Act8:
         self.shape, self.dtype, self.nb = torch.Size(shape), dtype, (C + 31) // 32
         self.rows = self.shape.numel() // C if C else 0
         n = self.rows * self.nb * 33
-        if buf is not None and buf.numel() != n:
-            raise ValueError(f"Act8: a buffer of {n} bytes expected, got {buf.numel()}")
+        if buf is not None and (buf.numel() != n or buf.dtype != torch.uint8 or not buf.is_contiguous()):
+            raise ValueError(f"Act8: a contiguous uint8 buffer of {n} bytes expected, got {buf.numel()} of {buf.dtype}")
         self.buf = torch.empty(n, device=device, dtype=torch.uint8) if buf is None else buf
 
     @property

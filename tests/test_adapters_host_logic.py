@@ -130,3 +130,13 @@ def test_slots_of_another_type_than_the_bank_are_refused():
         bank.buf = torch.empty(0, dtype=own)
         with pytest.raises(TypeError):
             ops.adapter_grad(torch.zeros(ops._slots_shape(bank, plan), dtype=other), torch.zeros(3, 64, dtype=other), plan, bank)
+
+
+def test_a_buffer_that_is_not_whole_is_refused():
+    """Act8's kernels address its buffer as n bytes one behind the other."""
+    n = 2 * 33
+    assert ops.Act8((2, 32), torch.float32, buf=torch.empty(n, dtype=torch.uint8)).rows == 2
+    for buf in (torch.empty(n + 1, dtype=torch.uint8), torch.empty(1, dtype=torch.uint8).expand(n), torch.empty(2 * n, dtype=torch.uint8)[::2],
+                torch.empty(n, dtype=torch.int8)):
+        with pytest.raises(ValueError):
+            ops.Act8((2, 32), torch.float32, buf=buf)
