@@ -140,3 +140,18 @@ def test_a_buffer_that_is_not_whole_is_refused():
                 torch.empty(n, dtype=torch.int8)):
         with pytest.raises(ValueError):
             ops.Act8((2, 32), torch.float32, buf=buf)
+
+
+def test_side_libraries_are_built_with_the_flags_of_the_library(tmp_path):
+    """tools/side_lib.sh compiles one source to stand in for the library's: with another flag list (packed float32 instructions on) it would not."""
+    import os
+    import subprocess
+    from more4d_amd.build import FLAGS
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    stub, log = tmp_path / "hipcc", tmp_path / "log"
+    stub.write_text(f'#!/bin/bash\nprintf "%s\\n" "$*" >> {log}\n')
+    stub.chmod(0o755)
+    subprocess.run(["bash", os.path.join(root, "tools", "side_lib.sh"), "x", "act8.hip", "-DY=1"], check=True, env={**os.environ, "HIPCC": str(stub)},
+                   capture_output=True)
+    line = log.read_text().splitlines()[0].split()
+    assert set(FLAGS) <= set(line) and "-DY=1" in line and "-DM4D_ABLATIONS" in line

@@ -3,7 +3,7 @@
 // dq[head][q][d] (32 wave-instructions, each 2 rows x 128 B).  Heads are pinned per XCD (block b runs on XCD b % 8), so the
 // updates of one head stay in one XCD's L2 — compared across memory scopes: SCOPE 0 = workgroup (plain L2 atomic), 1 = agent
 // (device scope), 2 = plain load+add+store (no atomicity, upper bound of the RMW traffic itself).
-// hipcc --offload-arch=gfx950 -O3 tools/probes/atomic_dq.hip -o tools/probes/atomic_dq.bin && tools/probes/atomic_dq.bin
+// hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/probes/atomic_dq.hip -o tools/probes/atomic_dq.bin && tools/probes/atomic_dq.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

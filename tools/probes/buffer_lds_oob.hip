@@ -1,5 +1,5 @@
 // Probe: does `buffer_load_dwordx4 ... lds` write ZEROS for lanes whose offset is past num_records (raw buffer, stride 0)?
-// hipcc --offload-arch=gfx950 -O2 tools/probes/buffer_lds_oob.hip -o /tmp/probe && /tmp/probe
+// hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 tools/probes/buffer_lds_oob.hip -o /tmp/probe && /tmp/probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -4,7 +4,7 @@
 //   ACC   0 = accumulators in arch VGPRs, 1 = AGPRs
 //   GAP   instructions between MFMAs: 0 none, 1 = s_waitcnt lgkmcnt(7) (satisfied), 2 = s_waitcnt + ds_read_b128
 //   OTHER what the other wave of the SIMD does: 0 = waits at the barrier, 1 = v_exp_f32 loop, 2 = v_fma_f32 loop
-// hipcc --offload-arch=gfx950 -O3 tools/probes/mfma_rate.hip -o tools/probes/mfma_rate.bin && tools/probes/mfma_rate.bin
+// hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/probes/mfma_rate.hip -o tools/probes/mfma_rate.bin && tools/probes/mfma_rate.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
