@@ -598,15 +598,14 @@ __global__ __launch_bounds__(256, 1) void gemm_bt256w_kernel(std::conditional_t<
 #undef W_MMA
 #undef W_READ
     W_LGKM0();
-    if constexpr (AD) {
-        // the fragments read ahead by the last phases are not used: keep their registers taken until the wait above, so that nothing computed
-        // for the extension can be put into one that an LDS read in flight still writes
+    // the fragments read ahead by the last phases are not used: keep their registers taken until the wait above, so that nothing computed
+    // for what follows can be put into one that an LDS read in flight still writes
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
+    for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) asm volatile("" :: "v"(fa0[h][kk]), "v"(fa1[h][kk]), "v"(fbx[h][kk]), "v"(fby[h][kk]));
+        for (int h = 0; h < 2; ++h) asm volatile("" :: "v"(fa0[h][kk]), "v"(fa1[h][kk]), "v"(fbx[h][kk]), "v"(fby[h][kk]));
+    if constexpr (AD)
         adapters_extend<T, 4, 4>(p, acc, ad_tile, n0 + wn * 128, lane, 1, (nkt - nk) * 32);      // (its loads fly with the last stagings)
-    }
     if constexpr (ABL & 64) ts[2] = __builtin_readcyclecounter();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the redundant tail stagings must land before the LDS is re-used
     __builtin_amdgcn_s_barrier();
