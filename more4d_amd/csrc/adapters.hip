@@ -134,7 +134,7 @@ M4D_DEV void down_store(const DownArgs& p, int64_t piece, int g, int slot, int r
 // chunks cannot also store: loads and stores share one counter, only loads return in order, so a wait that must not pass too early has to
 // wait for the stores as well, and little stays in flight: 128 us instead of 75 + 40 at 21840 x 5120.)
 // DEEP: fewer workgroups than CUs, each with the LDS of a whole CU: up to twelve chunks in flight, because alone a workgroup waits for memory (0.5
-// us a chunk with four stages).  21840 x 5120, rank 64: 60 - 68 us (3.7 TB/s of x), with codes 97 - 107 (floors 46 and 69).
+// us a chunk with four stages).  21840 x 5120, rank 64: 60 - 68 us (3.7 TB/s of x), with codes 96 - 107 (floors 46 and 69), and 7 - 13 more for the join.
 template <typename T, int RT, bool DEEP> struct DownShape {
     static constexpr int XB = 64 * 64 * sizeof(T), AB = RT * 64 * 32 * sizeof(T), STAGE = XB + AB;
     static constexpr int NST = DEEP ? (STAGE * 12 <= 144 * 1024 ? 12 : 144 * 1024 / STAGE) : STAGE * 4 <= 80 * 1024 ? 4 : STAGE * 3 <= 80 * 1024 ? 3 : 2;
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(QUANT ? 512 : 256, 2) void adapter_down_kernel(Down
 
 // The same for at most 16 rows (single tokens): a workgroup takes 16 ranks of one adapter, its eight waves the chunks of K in turn, straight from
 // memory into the 16 x 16 x 32 MFMA; all rows are multiplied by every adapter and only its own are kept.  One launch instead of slices and
-// their join: K = 5120, six adapters 12 us -> 5.
+// their join (12 us): K = 5120, rank 32, six adapters 9 us; K = 1536, rank 16, two adapters 4.
 template <typename T>
 __global__ __launch_bounds__(64 * SKINNY_WAVES) void adapter_down16_kernel(DownArgs p, const int* row_adapter, const int* adapters, int rows) {
     typedef typename Frag8<T>::type frag_t;
@@ -585,12 +585,13 @@ struct Choice { int kind, S; int64_t head; };      // head rows on the 256 x 256
 
 double wide_round_us(int64_t K, double wide_ad) { return (double)(K / 64) * 1.03 + 10.0 + wide_ad; }
 // Which kernel, and into how many slices of K: the least estimated time.  A CU runs its workgroups in rounds; a round costs a fixed part (filling
-// the ring, epilogue) and c per 128-byte K tile.  c is what the tile moves from L2 at the 60 - 80 bytes/ns that a CU gets (fp32: the MFMA
-// rate), so larger tiles are cheaper per product and smaller ones waste less of a round; slices pay for writing and joining float32 partial
+// the ring, epilogue) and c per 128-byte K tile.  c is what the tile stages from L2 at the 55 - 64 bytes/ns that a CU's K loop gets (fp32: the
+// MFMA rate), so larger tiles are cheaper per product and smaller ones waste less of a round; slices pay for writing and joining float32 partial
 // tiles.  Measured c (us, bf16 / fp32): 64 x 64 0.30 / 0.70 alone on a CU and 0.42 / 1.25 as one of two, 64 x 128 0.36 / 1.16, 128 x 128
-// 0.55 / 2.1, 128 x 192 0.66 / -, 256 x 128 0.78 / 4.0, 256 x 256 (gemm_wide.h) 1.03.  Measured against each other at 40 shapes (M 2 .. 21840): the
-// choice is within 10 % of the best of all kinds and slices, e.g. 64 x 5120 x 4096: 64 x 64 in 3 slices 14.2 us, whole 21.4, 128 x 128 whole 32;
-// 986 x 5120 x 4096: 128 x 192 47 us, 256 x 128 54, 256 x 256 67, 128 x 128 72.
+// 0.55 / 2.1, 128 x 192 0.66 / -, 256 x 128 0.78 / 4.0, 256 x 256 (gemm_wide.h) 1.03.  These are of runs too short for the board's power limit: many
+// rounds take longer than they say, whichever the tile (256 x 256, 21840 x 5120 x 5120: 650 us by them, 870 - 990 measured), and there the 256 x 256 tiles
+// are ahead by a quarter.  Against every kind and number of slices (profiles/adapters_gemm_sweep.log): within 8 % of the best at 33 bf16 and 5 % at 11 float32
+// shapes, e.g. 64 x 5120 x 4096 64 x 64 in 3 slices, 986 x 5120 x 4096 128 x 192 whole (63 us; 256 x 128 74).
 Choice choose_whole(bool bf16, int64_t M, int64_t N, int64_t K, bool wide_ok, double wide_ad, int ncu, double& t_best) {
     t_best = 1e30;
 #ifdef M4D_ABLATIONS
@@ -784,8 +785,8 @@ static int launch_gemm(AdGemmArgs& p, hipStream_t st) {
 
 static bool wide_shape(m4d_dtype dt, int64_t M, int64_t N, int64_t K) { return dt == M4D_BF16 && K % 64 == 0 && M >= 512 && N >= 512; }
 // what the adapters of a 256 x 256 tile add to its time, us (its direct loads take 32 consecutive rows each: it does not see row_order).  Measured
-// per adapter: rank 16 0.8, rank 64 3.8.  The other tiles take interleaved rows in order and have one or two adapters each.
-static double wide_adapters_us(const m4d_adapter_plan* plan, int R) { return plan->row_order ? 0.06 * R * plan->n_wide / (double)((plan->rows + 255) / 256) : 0.0; }
+// per adapter: rank 16 0.7, rank 32 1.5, rank 64 3.0, rank 128 5.5.  The other tiles take interleaved rows in order and have one or two adapters each.
+static double wide_adapters_us(const m4d_adapter_plan* plan, int R) { return plan->row_order ? 0.045 * R * plan->n_wide / (double)((plan->rows + 255) / 256) : 0.0; }
 
 static int u_parts(m4d_dtype dt) { return dt == M4D_BF16 ? Parts<bf16_t>::N : Parts<float>::N; }
 // the down projection's slices and the GEMM's run one after the other: one workspace, the larger of the two
