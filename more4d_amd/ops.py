@@ -1249,10 +1249,11 @@ class AdapterBank:
 class AdapterPlan:
     """Which adapter each row of a batch uses: request j owns the next lengths[j] rows (0 allowed) and names adapter adapters[j] (-1: none).
     Host numbers; the tables (include/more4d_hip.h: m4d_adapter_plan) are built here and copied to `device` once per batch composition, then
-    shared by every projection of the model (not inside a graph capture).  Any order of the requests is right, requests of one adapter side
-    by side are a little faster: a tile of the projection adds the adapters of all its rows, so where requests interleave them (twice the
-    (tile, adapter) pairs or more) the smaller tiles take the rows in order of their adapters (row_order).  1024 one-row requests of 64 adapters,
-    rank 16 / 64, 5120 x 5120: 95 / 108 us, 90 / 103 sorted by the caller (120 / 346 without row_order)."""
+    shared by every projection of the model (not inside a graph capture).  That is host time, so a plan is kept as long as the composition lasts: 0.14 ms
+    for 2 rows, 0.17 for 7 requests of 986 rows, 0.3 for 2 x 21840 rows, 1.3 for 4096 one-row requests of 64 adapters.  Any order of the requests is
+    right, requests of one adapter side by side are a little faster: a tile of the projection adds the adapters of all its rows, so where
+    requests interleave them (twice the (tile, adapter) pairs or more) the smaller tiles take the rows in order of their adapters
+    (row_order).  1024 one-row requests of 64 adapters, rank 16 / 64, 5120 x 5120: 83 / 91 us, 84 / 89 sorted by the caller."""
     PIECE, CHUNK_PIECES, MAX_ADAPTERS = 64, 64, 65535
 
     def __init__(self, lengths, adapters, device):
