@@ -87,3 +87,20 @@ def test_what_is_left_of_products_that_cancel(M):
     want, tol = oracle2(x, w, None, a, b, [1.0], torch.zeros(M, device=DEV))
     check(y, want, tol)
     # (of the bound 264 2^-23 2 * 256 * 0.64 = 0.01 is the accumulation's; two ranks of size 16 rounded to bf16 would be off by up to 2^-8 16 = 0.06 each)
+
+
+@pytest.mark.parametrize("r", [16, 32, 48, 72, 144, 256])
+@pytest.mark.parametrize("K", [1984, 2048])
+def test_a_row_that_two_tiles_write_gets_the_same_bits_from_both(r, K):
+    """The last 256 x 256 tile is shifted inwards: rows 3844 .. 4095 are also the one's before.  Ranks in the K loop (all rows name one adapter) and behind it
+    (the last rows name another) have to add up in the same order."""
+    o = ops()
+    M, N = 4100, 2056
+    x, w, bias, a, b, scale, _ = (t.to(DEV) if isinstance(t, torch.Tensor) else t for t in problem([M], [0], K, N, r, BF, G=2))
+    bank = o.AdapterBank(a, b, scale)
+    o.launch_counts(reset=True)
+    whole = o.linear_adapters(x, w, bias, bank, o.AdapterPlan([M], [0], DEV))
+    assert o.launch_counts()["gemm_wide"] == 1
+    mixed = o.AdapterPlan([M - 2, 2], [0, 1], DEV)
+    for _ in range(4):
+        assert torch.equal(o.linear_adapters(x, w, bias, bank, mixed)[:M - 2], whole[:M - 2])
